@@ -366,6 +366,130 @@ int lik_hidden_scatter_rows(const void* compact_rows, int64_t row_bytes, int32_t
                             const uint32_t* bitmap, const int32_t* prefix, void* grad_h, lik_stream_t stream);
 
 /* ------------------------------------------------------------------------- */
+/* Layers between an encoder's hidden states and the document head: layer norm, */
+/* a linear layer with bias, activation and residual, a gated feed-forward      */
+/* block; forward and backward.  (No counterpart in the reference, which starts */
+/* at the hidden states.)  dtype is LIK_F32, LIK_F16 or LIK_BF16 for all of a   */
+/* call's matrices; sums, statistics and activations are fp32.  Matrices are    */
+/* row-major with unit stride inside a row; *_stride are elements between rows, */
+/* and what has none is contiguous.  Gradients of parameters are written as     */
+/* param_dtype (dtype or LIK_F32).  Results do not depend on the order in which */
+/* blocks run.                                                                  */
+/* ------------------------------------------------------------------------- */
+enum lik_activation {
+  LIK_ACT_NONE = 0,
+  LIK_ACT_RELU = 1,
+  LIK_ACT_SILU = 2,      /* z * sigmoid(z) */
+  LIK_ACT_GELU = 3,      /* z * Phi(z), Phi the normal distribution */
+  LIK_ACT_GELU_TANH = 4, /* z/2 * (1 + tanh(sqrt(2/pi) * (z + 0.044715 z^3))) */
+  LIK_ACT_TANH = 5,
+  LIK_ACT_SIGMOID = 6
+};
+
+/* y = (x - mean) * rstd * weight + bias, rstd = 1 / sqrt(var + eps), over each row */
+typedef struct lik_norm_args {
+  const void* x;       /* [rows, width] */
+  int64_t x_stride;
+  int64_t rows;
+  int32_t width;
+  int32_t dtype;
+  const void* weight;  /* [width] of param_dtype, or NULL: 1 */
+  const void* bias;    /* [width] of param_dtype, or NULL: 0 */
+  int32_t param_dtype;
+  float eps;
+  void* y;             /* forward: [rows, width] */
+  float* mean;         /* [rows]: written by the forward (may be NULL there, with rstd), read by the backward */
+  float* rstd;
+  const void* dy;      /* backward: [rows, width] */
+  void* dx;            /* backward: [rows, width], or NULL */
+  void* dweight;       /* backward: [width] of param_dtype, or NULL */
+  void* dbias;
+  void* workspace;
+  size_t workspace_bytes;
+} lik_norm_args;
+int lik_layer_norm_fwd(const lik_norm_args* args, lik_stream_t stream);
+size_t lik_layer_norm_bwd_workspace(const lik_norm_args* args);
+int lik_layer_norm_bwd(const lik_norm_args* args, lik_stream_t stream);
+
+/* y = act(x w^T + bias) + residual */
+typedef struct lik_linear_args {
+  const void* x;         /* [rows, in] */
+  int64_t x_stride;
+  const void* w;         /* [out, in] */
+  int64_t w_stride;
+  const void* bias;      /* [out] or NULL */
+  const void* residual;  /* [rows, out] or NULL */
+  int64_t residual_stride;
+  int64_t rows;
+  int32_t in;
+  int32_t out;
+  int32_t dtype;
+  int32_t activation;
+  void* y;               /* forward: [rows, out] */
+  void* z;               /* x w^T + bias for the backward: written by the forward unless NULL; only an activation needs it */
+  int64_t z_stride;      /* a multiple of 16 bytes, as z itself */
+  const void* dy;        /* backward: [rows, out] */
+  int64_t dy_stride;
+  void* dx;              /* backward: [rows, in] or NULL */
+  void* dw;              /* backward: [out, in] of param_dtype or NULL */
+  void* dbias;           /* backward: [out] of param_dtype or NULL */
+  int32_t param_dtype;
+  int32_t reserved;
+  void* workspace;
+  size_t workspace_bytes;
+  int32_t* status;
+} lik_linear_args;
+size_t lik_linear_fwd_workspace(const lik_linear_args* args);
+int lik_linear_fwd(const lik_linear_args* args, lik_stream_t stream);
+size_t lik_linear_bwd_workspace(const lik_linear_args* args);
+int lik_linear_bwd(const lik_linear_args* args, lik_stream_t stream);
+
+/* g = x w_gate^T + b_gate, u = x w_up^T + b_up, h = act(g) * u, y = h w_down^T + b_down + residual */
+typedef struct lik_gated_args {
+  const void* x;         /* [rows, in] */
+  int64_t x_stride;
+  const void* w_gate;    /* [hidden, in] */
+  int64_t w_gate_stride;
+  const void* w_up;      /* [hidden, in] */
+  int64_t w_up_stride;
+  const void* w_down;    /* [out, hidden] */
+  int64_t w_down_stride;
+  const void* b_gate;    /* [hidden] or NULL */
+  const void* b_up;
+  const void* b_down;    /* [out] or NULL */
+  const void* residual;  /* [rows, out] or NULL */
+  int64_t residual_stride;
+  int64_t rows;
+  int32_t in;
+  int32_t hidden;
+  int32_t out;
+  int32_t dtype;
+  int32_t activation;
+  int32_t param_dtype;
+  void* y;               /* forward: [rows, out] */
+  void* gate;            /* g, u and h for the backward, [rows, hidden] with kept_stride (a multiple of 16 bytes): written by */
+  void* up;              /* the forward unless NULL (all three or none), read by the backward */
+  void* h;
+  int64_t kept_stride;
+  const void* dy;        /* backward: [rows, out] */
+  int64_t dy_stride;
+  void* dx;              /* backward: [rows, in] or NULL; the parameters' gradients or NULL */
+  void* dw_gate;
+  void* dw_up;
+  void* dw_down;
+  void* db_gate;
+  void* db_up;
+  void* db_down;
+  void* workspace;
+  size_t workspace_bytes;
+  int32_t* status;
+} lik_gated_args;
+size_t lik_gated_fwd_workspace(const lik_gated_args* args);
+int lik_gated_fwd(const lik_gated_args* args, lik_stream_t stream);
+size_t lik_gated_bwd_workspace(const lik_gated_args* args);
+int lik_gated_bwd(const lik_gated_args* args, lik_stream_t stream);
+
+/* ------------------------------------------------------------------------- */
 /* Utilities                                                                    */
 /* ------------------------------------------------------------------------- */
 /* out[r] = 1 / max(||x_r||, eps) for every row; the fused-normalise kernels take these. */

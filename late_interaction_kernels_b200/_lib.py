@@ -98,6 +98,40 @@ class PlaidIndex(C.Structure):
     ]
 
 
+class NormArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("x_stride", C.c_int64), ("rows", C.c_int64), ("width", C.c_int32), ("dtype", C.c_int32),
+        ("weight", C.c_void_p), ("bias", C.c_void_p), ("param_dtype", C.c_int32), ("eps", C.c_float),
+        ("y", C.c_void_p), ("mean", C.c_void_p), ("rstd", C.c_void_p), ("dy", C.c_void_p), ("dx", C.c_void_p),
+        ("dweight", C.c_void_p), ("dbias", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class LinearArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("x_stride", C.c_int64), ("w", C.c_void_p), ("w_stride", C.c_int64), ("bias", C.c_void_p),
+        ("residual", C.c_void_p), ("residual_stride", C.c_int64), ("rows", C.c_int64), ("in", C.c_int32),
+        ("out", C.c_int32), ("dtype", C.c_int32), ("activation", C.c_int32), ("y", C.c_void_p), ("z", C.c_void_p),
+        ("z_stride", C.c_int64), ("dy", C.c_void_p), ("dy_stride", C.c_int64), ("dx", C.c_void_p), ("dw", C.c_void_p),
+        ("dbias", C.c_void_p), ("param_dtype", C.c_int32), ("reserved", C.c_int32), ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_size_t), ("status", C.c_void_p),
+    ]
+
+
+class GatedArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("x_stride", C.c_int64), ("w_gate", C.c_void_p), ("w_gate_stride", C.c_int64),
+        ("w_up", C.c_void_p), ("w_up_stride", C.c_int64), ("w_down", C.c_void_p), ("w_down_stride", C.c_int64),
+        ("b_gate", C.c_void_p), ("b_up", C.c_void_p), ("b_down", C.c_void_p), ("residual", C.c_void_p),
+        ("residual_stride", C.c_int64), ("rows", C.c_int64), ("in", C.c_int32), ("hidden", C.c_int32),
+        ("out", C.c_int32), ("dtype", C.c_int32), ("activation", C.c_int32), ("param_dtype", C.c_int32),
+        ("y", C.c_void_p), ("gate", C.c_void_p), ("up", C.c_void_p), ("h", C.c_void_p), ("kept_stride", C.c_int64),
+        ("dy", C.c_void_p), ("dy_stride", C.c_int64), ("dx", C.c_void_p), ("dw_gate", C.c_void_p),
+        ("dw_up", C.c_void_p), ("dw_down", C.c_void_p), ("db_gate", C.c_void_p), ("db_up", C.c_void_p),
+        ("db_down", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("status", C.c_void_p),
+    ]
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -138,6 +172,11 @@ def _declare(lib):
     lib.lik_hidden_winners.restype = i32
     lib.lik_hidden_scatter_rows.argtypes = [vp, i64, i32, i32, i32, vp, vp, vp, vp]
     lib.lik_hidden_scatter_rows.restype = i32
+    for name, args in (("layer_norm", NormArgs), ("linear", LinearArgs), ("gated", GatedArgs)):
+        for entry in (f"lik_{name}_fwd", f"lik_{name}_bwd"):
+            getattr(lib, entry).argtypes, getattr(lib, entry).restype = [C.POINTER(args), vp], i32
+            if entry != "lik_layer_norm_fwd":
+                getattr(lib, entry + "_workspace").argtypes, getattr(lib, entry + "_workspace").restype = [C.POINTER(args)], sz
     lib.lik_selftest_wait_timeout.argtypes = [i64, vp, vp, vp]
     lib.lik_selftest_wait_timeout.restype = i32
     lib.lik_selftest_other_waits.argtypes = [i64, vp, vp, vp]
@@ -169,6 +208,8 @@ EXPORTED_SYMBOLS = (
     "lik_maxsim_fwd_kernel", "lik_maxsim_fwd_topk_supported", "lik_maxsim_fwd_topk_workspace", "lik_maxsim_fwd_topk",
     "lik_maxsim_hidden_fwd_supported", "lik_maxsim_hidden_fwd_workspace", "lik_maxsim_hidden_fwd",
     "lik_hidden_winners", "lik_hidden_scatter_rows",
+    "lik_layer_norm_fwd", "lik_layer_norm_bwd_workspace", "lik_layer_norm_bwd", "lik_linear_fwd_workspace", "lik_linear_fwd",
+    "lik_linear_bwd_workspace", "lik_linear_bwd", "lik_gated_fwd_workspace", "lik_gated_fwd", "lik_gated_bwd_workspace", "lik_gated_bwd",
     "lik_plaid_fwd_supported", "lik_plaid_fwd_workspace", "lik_plaid_fwd", "lik_launch_count", "lik_selftest_wait_timeout",
     "lik_selftest_other_waits", "lik_selftest_all_lanes_wait",
     "lik_topk_merge", "lik_plaid_decompress", "lik_plaid_approx", "lik_plaid_bwd_dq", "lik_row_inv_norm",

@@ -464,5 +464,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("backward", torch::wrap_pybind_function(&backward_py));
   bind_head(m);
   bind_search(m);
+  bind_layers(m);
   m.def("status_word", torch::wrap_pybind_function_no_gil(&status_tensor));
 }

@@ -63,5 +63,6 @@ Side side_of(const pybind11::tuple& t);
 
 void bind_head(pybind11::module_& m);
 void bind_search(pybind11::module_& m);
+void bind_layers(pybind11::module_& m);
 
 }  // namespace lik_host

@@ -1,0 +1,461 @@
+// The layers' C entry points: which products and passes a call is made of, and the passes that are not products.
+#include "lik_layers.cuh"
+
+namespace lik {
+namespace {
+
+// ---------------------------------------------------------------------------------------------
+// out[i] = sum over parts of partial[part][i], in the order of the parts
+// ---------------------------------------------------------------------------------------------
+constexpr int SUM_LANES = 8;
+template <typename T>
+__global__ void __launch_bounds__(256) sum_parts_kernel(const float* __restrict__ partial, int parts, long long n, long long split, T* __restrict__ out,
+                                                        T* __restrict__ out2) {
+  __shared__ float s[SUM_LANES][33];
+  const int col = threadIdx.x % 32, lane = threadIdx.x / 32;
+  const long long i = blockIdx.x * 32ll + col;
+  float v = 0.0f;
+  if (i < n) {
+#pragma unroll 4
+    for (int q = lane; q < parts; q += SUM_LANES) v += partial[q * n + i];
+  }
+  s[lane][col] = v;
+  __syncthreads();
+  if (lane == 0 && i < n) {
+#pragma unroll
+    for (int l = 1; l < SUM_LANES; ++l) v += s[l][col];
+    T* o = i < split ? out : out2;
+    if (o) o[i < split ? i : i - split] = from_f32<T>(v);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// dz = dy * act'(z), and the sums of dz's columns per block of rows.  Memory-bound: each element read once, dz written once.
+// A block takes 32 vectors of columns (a lane's V columns) and ROWS_PER rows, eight at a time.
+// ---------------------------------------------------------------------------------------------
+constexpr int SLOPE_LANES = 8;
+struct SlopeParams {
+  const void *dy, *z;
+  long long dy_stride, z_stride, rows, rows_per;
+  int n;
+  void* dz;  // or NULL: sums only
+  long long dz_stride;
+  float* partial;  // [gridDim.y][n] or NULL
+};
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(32 * SLOPE_LANES) slope_kernel(const SlopeParams p) {
+  __shared__ float s[SLOPE_LANES][32 * V + 1];
+  const int lane = threadIdx.x % 32, row = threadIdx.x / 32;
+  const int c = (blockIdx.x * 32 + lane) * V;
+  float sum[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) sum[j] = 0.0f;
+  if (c < p.n) {
+    const long long r0 = blockIdx.y * p.rows_per, r1 = r0 + p.rows_per < p.rows ? r0 + p.rows_per : p.rows;
+#pragma unroll 2
+    for (long long r = r0 + row; r < r1; r += SLOPE_LANES) {
+      float g[V], z[V];
+      load_vec<T, V>((const T*)p.dy + r * p.dy_stride + c, g);
+      if constexpr (ACT != LIK_ACT_NONE) {
+        load_vec<T, V>((const T*)p.z + r * p.z_stride + c, z);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          float a;
+          g[j] *= act_slope<ACT, sizeof(T) == 4>(z[j], a);
+        }
+      }
+      if (p.dz) store_vec<T, V>((T*)p.dz + r * p.dz_stride + c, g);
+#pragma unroll
+      for (int j = 0; j < V; ++j) sum[j] += g[j];
+    }
+  }
+  if (!p.partial) return;
+#pragma unroll
+  for (int j = 0; j < V; ++j) s[row][j * 32 + lane] = sum[j];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 32 * V; i += 32 * SLOPE_LANES) {
+    float v = 0.0f;
+#pragma unroll
+    for (int q = 0; q < SLOPE_LANES; ++q) v += s[q][i];
+    const int col = (blockIdx.x * 32 + i % 32) * V + i / 32;
+    if (col < p.n) p.partial[(long long)blockIdx.y * p.n + col] = v;
+  }
+}
+int slope_parts(long long rows, int n, int dtype) {
+  const long long cols = ceil_div(n, 32 * (16 / (int)dtype_size(dtype)));
+  long long want = ceil_div(4ll * sm_count(), cols);
+  if (want > ceil_div(rows, SLOPE_LANES)) want = ceil_div(rows, SLOPE_LANES);
+  if (want > 65535) want = 65535;
+  return want < 1 ? 1 : (int)want;
+}
+template <typename T>
+int run_slope(const SlopeParams& p, int act, bool vec, int parts, cudaStream_t st) {
+  constexpr int V = vec_elems<T>();
+  with_activation(act, [&](auto a) {
+    if (vec) slope_kernel<T, V, decltype(a)::value><<<dim3((unsigned)ceil_div(p.n, 32 * V), parts), 32 * SLOPE_LANES, 0, st>>>(p), count_launch();
+    else slope_kernel<T, 1, decltype(a)::value><<<dim3((unsigned)ceil_div(p.n, 32), parts), 32 * SLOPE_LANES, 0, st>>>(p), count_launch();
+  });
+  LIK_CUDA_OK(cudaGetLastError());
+  return LIK_OK;
+}
+// dz (or NULL) and the columns' sums (sums != NULL: param_dtype [n], with `partial` as scratch)
+size_t slope_workspace(long long rows, int n, int dtype) { return align_up((size_t)slope_parts(rows, n, dtype) * n * sizeof(float), 256); }
+int launch_slope(SlopeParams p, int act, int dtype, void* sums, int sums_dtype, cudaStream_t st) {
+  const int item = (int)dtype_size(dtype), parts = slope_parts(p.rows, p.n, dtype);
+  p.rows_per = ceil_div(p.rows, parts);
+  if (!sums) p.partial = nullptr;
+  const bool vec = vec_ok(p.dy, p.dy_stride, p.n, item) && (act == LIK_ACT_NONE || vec_ok(p.z, p.z_stride, p.n, item)) &&
+                   (!p.dz || vec_ok(p.dz, p.dz_stride, p.n, item));
+  int rc = dtype == LIK_F32 ? run_slope<float>(p, act, vec, parts, st)
+                            : (dtype == LIK_F16 ? run_slope<__half>(p, act, vec, parts, st) : run_slope<__nv_bfloat16>(p, act, vec, parts, st));
+  if (rc || !sums) return rc;
+  return launch_sum_parts(p.partial, parts, p.n, p.n, sums_dtype, sums, nullptr, st);
+}
+
+bool act_known(int a) { return a >= LIK_ACT_NONE && a <= LIK_ACT_SIGMOID; }
+bool dtype_known(int d) { return d == LIK_F32 || d == LIK_F16 || d == LIK_BF16; }
+// rows of kept and internal matrices start on 16 bytes
+long long pad_cols(long long n, int dtype) {
+  const long long v = 16 / (long long)dtype_size(dtype);
+  return (n + v - 1) / v * v;
+}
+
+// workspace, taken piece by piece: with a NULL base only the sizes are added up
+struct Carve {
+  char* base;
+  size_t off = 0;
+  template <typename P = void>
+  P* take(size_t bytes) {
+    P* p = base ? (P*)(base + off) : nullptr;
+    off += align_up(bytes, 256);
+    return p;
+  }
+};
+
+int check_linear(const lik_linear_args* a) {
+  LIK_REQUIRE(a != nullptr, "args is NULL");
+  LIK_REQUIRE(dtype_known(a->dtype), "dtype must be fp32, fp16 or bf16");
+  LIK_REQUIRE(a->param_dtype == a->dtype || a->param_dtype == LIK_F32, "param_dtype must be dtype or fp32");
+  LIK_REQUIRE(act_known(a->activation), "unknown activation");
+  LIK_REQUIRE(a->rows >= 0 && a->rows < (1ll << 31) && a->in > 0 && a->out > 0, "sizes must be positive, rows below 2^31");
+  LIK_REQUIRE(a->x_stride >= a->in && a->w_stride >= a->in, "x_stride and w_stride must be at least in");
+  return LIK_OK;
+}
+GemmDesc linear_fwd_desc(const lik_linear_args& a) {
+  GemmDesc d;
+  d.act = a.activation;
+  d.dtype = d.out_dtype = a.dtype;
+  d.m = a.rows;
+  d.n = a.out;
+  d.k[0] = a.in;
+  d.a[0] = {a.x, a.x_stride, 1};
+  d.b[0] = {a.w, a.w_stride, 1};
+  d.bias[0] = a.bias;
+  d.residual = a.residual;
+  d.residual_stride = a.residual_stride;
+  d.out = a.y;
+  d.out_stride = a.out;
+  d.z = a.activation == LIK_ACT_NONE ? nullptr : a.z;
+  d.z_stride = a.z_stride;
+  return d;
+}
+// dx = dz w and dw = dz^T x
+GemmDesc grad_x_desc(int dtype, long long rows, int out, int in, const void* dz, long long dz_stride, const void* w, long long w_stride, void* dx) {
+  GemmDesc d;
+  d.dtype = d.out_dtype = dtype;
+  d.m = rows;
+  d.n = in;
+  d.k[0] = out;
+  d.a[0] = {dz, dz_stride, 1};
+  d.b[0] = {w, 1, w_stride};
+  d.out = dx;
+  d.out_stride = in;
+  return d;
+}
+GemmDesc grad_w_desc(int dtype, int param_dtype, long long rows, int out, int in, const void* dz, long long dz_stride, const void* x, long long x_stride,
+                     void* dw) {
+  GemmDesc d;
+  d.dtype = dtype;
+  d.out_dtype = param_dtype;
+  d.m = out;
+  d.n = in;
+  d.k[0] = rows;
+  d.a[0] = {dz, 1, dz_stride};
+  d.b[0] = {x, 1, x_stride};
+  d.out = dw;
+  d.out_stride = in;
+  return d;
+}
+
+struct LinearBwd {
+  void* dz;
+  long long dz_stride;
+  float* partial;
+  void* gemm;
+  size_t gemm_bytes, total;
+};
+LinearBwd linear_bwd_layout(const lik_linear_args& a, void* ws) {
+  LinearBwd l{};
+  Carve c{(char*)ws};
+  l.dz = nullptr;
+  if (a.activation != LIK_ACT_NONE) {
+    l.dz_stride = pad_cols(a.out, a.dtype);
+    l.dz = c.take((size_t)a.rows * l.dz_stride * dtype_size(a.dtype));
+  }
+  if (a.dbias) l.partial = c.take<float>(slope_workspace(a.rows, a.out, a.dtype));
+  const void* dz = a.activation != LIK_ACT_NONE ? l.dz : a.dy;
+  const long long st = a.activation != LIK_ACT_NONE ? l.dz_stride : a.dy_stride;
+  if (a.dx) l.gemm_bytes = gemm_workspace(grad_x_desc(a.dtype, a.rows, a.out, a.in, dz, st, a.w, a.w_stride, a.dx));
+  if (a.dw) {
+    const size_t b = gemm_workspace(grad_w_desc(a.dtype, a.param_dtype, a.rows, a.out, a.in, dz, st, a.x, a.x_stride, a.dw));
+    l.gemm_bytes = b > l.gemm_bytes ? b : l.gemm_bytes;
+  }
+  l.gemm = c.take(l.gemm_bytes);
+  l.total = c.off;
+  return l;
+}
+int too_small(const char* what) {
+  set_error("%s: workspace too small", what);
+  return LIK_ERR_WORKSPACE;
+}
+int zero(void* p, size_t bytes, cudaStream_t st) {
+  if (p) LIK_CUDA_OK(cudaMemsetAsync(p, 0, bytes, st));
+  return LIK_OK;
+}
+
+int check_gated(const lik_gated_args* a) {
+  LIK_REQUIRE(a != nullptr, "args is NULL");
+  LIK_REQUIRE(dtype_known(a->dtype), "dtype must be fp32, fp16 or bf16");
+  LIK_REQUIRE(a->param_dtype == a->dtype || a->param_dtype == LIK_F32, "param_dtype must be dtype or fp32");
+  LIK_REQUIRE(act_known(a->activation), "unknown activation");
+  LIK_REQUIRE(a->rows >= 0 && a->rows < (1ll << 31) && a->in > 0 && a->hidden > 0 && a->out > 0, "sizes must be positive, rows below 2^31");
+  LIK_REQUIRE(a->x_stride >= a->in && a->w_gate_stride >= a->in && a->w_up_stride >= a->in && a->w_down_stride >= a->hidden, "a stride is below its row");
+  return LIK_OK;
+}
+struct GatedFwd {
+  GemmDesc up, down;
+  void* gemm;
+  size_t gemm_bytes, total;
+};
+GatedFwd gated_fwd_layout(const lik_gated_args& a, void* ws) {
+  GatedFwd l{};
+  Carve c{(char*)ws};
+  void* h = a.h;
+  long long h_stride = a.kept_stride;
+  if (!a.gate) {
+    h_stride = pad_cols(a.hidden, a.dtype);
+    h = c.take((size_t)a.rows * h_stride * dtype_size(a.dtype));
+  }
+  GemmDesc& u = l.up;
+  u.kind = GEMM_GATED;
+  u.act = a.activation;
+  u.dtype = u.out_dtype = a.dtype;
+  u.m = a.rows;
+  u.n = a.hidden;
+  u.k[0] = a.in;
+  u.a[0] = {a.x, a.x_stride, 1};
+  u.b[0] = {a.w_gate, a.w_gate_stride, 1};
+  u.b[1] = {a.w_up, a.w_up_stride, 1};
+  u.bias[0] = a.b_gate;
+  u.bias[1] = a.b_up;
+  u.out = h;
+  u.out_stride = h_stride;
+  u.z = a.gate;
+  u.z2 = a.up;
+  u.z_stride = a.kept_stride;
+  GemmDesc& d = l.down;
+  d.dtype = d.out_dtype = a.dtype;
+  d.m = a.rows;
+  d.n = a.out;
+  d.k[0] = a.hidden;
+  d.a[0] = {h, h_stride, 1};
+  d.b[0] = {a.w_down, a.w_down_stride, 1};
+  d.bias[0] = a.b_down;
+  d.residual = a.residual;
+  d.residual_stride = a.residual_stride;
+  d.out = a.y;
+  d.out_stride = a.out;
+  const size_t b1 = gemm_workspace(u), b2 = gemm_workspace(d);
+  l.gemm_bytes = b1 > b2 ? b1 : b2;
+  l.gemm = c.take(l.gemm_bytes);
+  l.total = c.off;
+  return l;
+}
+struct GatedBwd {
+  GemmDesc dh, dx, dwg, dwu, dwd;  // products that are not asked for have no out
+  void *dg, *du;
+  long long stride;
+  float* partial;
+  void* gemm;
+  size_t gemm_bytes, total;
+};
+GatedBwd gated_bwd_layout(const lik_gated_args& a, void* ws) {
+  GatedBwd l{};
+  Carve c{(char*)ws};
+  l.stride = pad_cols(a.hidden, a.dtype);
+  const bool inner = a.dx || a.dw_gate || a.dw_up || a.db_gate || a.db_up;
+  if (inner) {
+    l.dg = c.take((size_t)a.rows * l.stride * dtype_size(a.dtype));
+    l.du = c.take((size_t)a.rows * l.stride * dtype_size(a.dtype));
+    GemmDesc& h = l.dh;
+    h.kind = GEMM_GATED_BWD;
+    h.act = a.activation;
+    h.dtype = h.out_dtype = a.dtype;
+    h.m = a.rows;
+    h.n = a.hidden;
+    h.k[0] = a.out;
+    h.a[0] = {a.dy, a.dy_stride, 1};
+    h.b[0] = {a.w_down, 1, a.w_down_stride};
+    h.out = l.dg;
+    h.out2 = l.du;
+    h.out_stride = l.stride;
+    h.z = a.gate;
+    h.z2 = a.up;
+    h.z_stride = a.kept_stride;
+    l.gemm_bytes = gemm_workspace(h);
+  }
+  auto want = [&](const GemmDesc& d) {
+    const size_t b = gemm_workspace(d);
+    l.gemm_bytes = b > l.gemm_bytes ? b : l.gemm_bytes;
+  };
+  if (a.dx) {
+    l.dx = grad_x_desc(a.dtype, a.rows, a.hidden, a.in, l.dg, l.stride, a.w_gate, a.w_gate_stride, a.dx);
+    l.dx.n_seg = 2;
+    l.dx.k[1] = a.hidden;
+    l.dx.a[1] = {l.du, l.stride, 1};
+    l.dx.b[1] = {a.w_up, 1, a.w_up_stride};
+    want(l.dx);
+  }
+  if (a.dw_gate) want(l.dwg = grad_w_desc(a.dtype, a.param_dtype, a.rows, a.hidden, a.in, l.dg, l.stride, a.x, a.x_stride, a.dw_gate));
+  if (a.dw_up) want(l.dwu = grad_w_desc(a.dtype, a.param_dtype, a.rows, a.hidden, a.in, l.du, l.stride, a.x, a.x_stride, a.dw_up));
+  if (a.dw_down) want(l.dwd = grad_w_desc(a.dtype, a.param_dtype, a.rows, a.out, a.hidden, a.dy, a.dy_stride, a.h, a.kept_stride, a.dw_down));
+  if (a.db_gate || a.db_up || a.db_down) l.partial = c.take<float>(slope_workspace(a.rows, a.hidden > a.out ? a.hidden : a.out, a.dtype) * 2);
+  l.gemm = c.take(l.gemm_bytes);
+  l.total = c.off;
+  return l;
+}
+
+}  // namespace
+
+int launch_sum_parts(const float* partial, int parts, long long n, long long split, int dtype, void* out, void* out2, cudaStream_t st) {
+  const long long grid = ceil_div(n, 32);
+  LIK_REQUIRE(grid < (1ll << 31), "too many sums");
+  if (dtype == LIK_F32) sum_parts_kernel<float><<<(unsigned)grid, 256, 0, st>>>(partial, parts, n, split, (float*)out, (float*)out2), count_launch();
+  else if (dtype == LIK_F16) sum_parts_kernel<__half><<<(unsigned)grid, 256, 0, st>>>(partial, parts, n, split, (__half*)out, (__half*)out2), count_launch();
+  else sum_parts_kernel<__nv_bfloat16><<<(unsigned)grid, 256, 0, st>>>(partial, parts, n, split, (__nv_bfloat16*)out, (__nv_bfloat16*)out2), count_launch();
+  LIK_CUDA_OK(cudaGetLastError());
+  return LIK_OK;
+}
+
+}  // namespace lik
+
+extern "C" size_t lik_linear_fwd_workspace(const lik_linear_args* a) {
+  using namespace lik;
+  if (check_linear(a) || a->rows == 0) return 0;
+  return gemm_workspace(linear_fwd_desc(*a));
+}
+extern "C" int lik_linear_fwd(const lik_linear_args* args, lik_stream_t stream) {
+  using namespace lik;
+  if (int rc = check_linear(args)) return rc;
+  const lik_linear_args& a = *args;
+  if (a.rows == 0) return LIK_OK;
+  LIK_REQUIRE(a.x && a.w && a.y, "x, w and y must not be NULL");
+  LIK_REQUIRE(!a.z || (a.z_stride >= a.out && a.z_stride * dtype_size(a.dtype) % 16 == 0 && ((uintptr_t)a.z & 15) == 0), "z must have 16-byte rows");
+  LIK_REQUIRE(!a.residual || a.residual_stride >= a.out, "residual_stride must be at least out");
+  const GemmDesc d = linear_fwd_desc(a);
+  if (a.workspace_bytes < gemm_workspace(d)) return too_small("lik_linear_fwd");
+  return launch_gemm(d, a.workspace, a.workspace_bytes, a.status, (cudaStream_t)stream);
+}
+
+extern "C" size_t lik_linear_bwd_workspace(const lik_linear_args* a) {
+  using namespace lik;
+  if (check_linear(a) || a->rows == 0) return 0;
+  return linear_bwd_layout(*a, nullptr).total;
+}
+extern "C" int lik_linear_bwd(const lik_linear_args* args, lik_stream_t stream) {
+  using namespace lik;
+  if (int rc = check_linear(args)) return rc;
+  const lik_linear_args& a = *args;
+  cudaStream_t st = (cudaStream_t)stream;
+  const size_t pi = dtype_size(a.param_dtype);
+  if (a.rows == 0) {
+    if (int rc = zero(a.dw, pi * a.out * a.in, st)) return rc;
+    return zero(a.dbias, pi * a.out, st);
+  }
+  if (!a.dx && !a.dw && !a.dbias) return LIK_OK;
+  LIK_REQUIRE(a.x && a.w && a.dy && a.dy_stride >= a.out, "x, w and dy must not be NULL, dy_stride at least out");
+  const bool act = a.activation != LIK_ACT_NONE;
+  LIK_REQUIRE(!act || (a.z && a.z_stride >= a.out && a.z_stride * dtype_size(a.dtype) % 16 == 0 && ((uintptr_t)a.z & 15) == 0), "z must have 16-byte rows");
+  const LinearBwd l = linear_bwd_layout(a, a.workspace);
+  if (a.workspace_bytes < l.total || (l.total && !a.workspace)) return too_small("lik_linear_bwd");
+  const void* dz = act ? l.dz : a.dy;
+  const long long dz_stride = act ? l.dz_stride : a.dy_stride;
+  if (act || a.dbias) {
+    SlopeParams p{a.dy, a.z, a.dy_stride, a.z_stride, a.rows, 0, a.out, l.dz, l.dz_stride, l.partial};
+    if (int rc = launch_slope(p, a.activation, a.dtype, a.dbias, a.param_dtype, st)) return rc;
+  }
+  if (a.dx)
+    if (int rc = launch_gemm(grad_x_desc(a.dtype, a.rows, a.out, a.in, dz, dz_stride, a.w, a.w_stride, a.dx), l.gemm, l.gemm_bytes, a.status, st)) return rc;
+  if (a.dw)
+    return launch_gemm(grad_w_desc(a.dtype, a.param_dtype, a.rows, a.out, a.in, dz, dz_stride, a.x, a.x_stride, a.dw), l.gemm, l.gemm_bytes, a.status, st);
+  return LIK_OK;
+}
+
+extern "C" size_t lik_gated_fwd_workspace(const lik_gated_args* a) {
+  using namespace lik;
+  if (check_gated(a) || a->rows == 0) return 0;
+  return gated_fwd_layout(*a, nullptr).total;
+}
+extern "C" int lik_gated_fwd(const lik_gated_args* args, lik_stream_t stream) {
+  using namespace lik;
+  if (int rc = check_gated(args)) return rc;
+  const lik_gated_args& a = *args;
+  if (a.rows == 0) return LIK_OK;
+  LIK_REQUIRE(a.x && a.w_gate && a.w_up && a.w_down && a.y, "x, the weights and y must not be NULL");
+  LIK_REQUIRE(!a.gate == !a.up && !a.gate == !a.h, "gate, up and h are kept together");
+  LIK_REQUIRE(!a.gate || (a.kept_stride >= a.hidden && a.kept_stride * dtype_size(a.dtype) % 16 == 0 &&
+                          (((uintptr_t)a.gate | (uintptr_t)a.up | (uintptr_t)a.h) & 15) == 0), "gate, up and h must have 16-byte rows");
+  LIK_REQUIRE(!a.residual || a.residual_stride >= a.out, "residual_stride must be at least out");
+  const GatedFwd l = gated_fwd_layout(a, a.workspace);
+  if (a.workspace_bytes < l.total || (l.total && !a.workspace)) return too_small("lik_gated_fwd");
+  if (int rc = launch_gemm(l.up, l.gemm, l.gemm_bytes, a.status, (cudaStream_t)stream)) return rc;
+  return launch_gemm(l.down, l.gemm, l.gemm_bytes, a.status, (cudaStream_t)stream);
+}
+
+extern "C" size_t lik_gated_bwd_workspace(const lik_gated_args* a) {
+  using namespace lik;
+  if (check_gated(a) || a->rows == 0) return 0;
+  return gated_bwd_layout(*a, nullptr).total;
+}
+extern "C" int lik_gated_bwd(const lik_gated_args* args, lik_stream_t stream) {
+  using namespace lik;
+  if (int rc = check_gated(args)) return rc;
+  const lik_gated_args& a = *args;
+  cudaStream_t st = (cudaStream_t)stream;
+  const size_t pi = dtype_size(a.param_dtype);
+  if (a.rows == 0) {
+    void* const ptrs[] = {a.dw_gate, a.dw_up, a.dw_down, a.db_gate, a.db_up, a.db_down};
+    const size_t sizes[] = {pi * a.hidden * a.in, pi * a.hidden * a.in, pi * a.hidden * a.out, pi * a.hidden, pi * a.hidden, pi * a.out};
+    for (int i = 0; i < 6; ++i)
+      if (int rc = zero(ptrs[i], sizes[i], st)) return rc;
+    return LIK_OK;
+  }
+  LIK_REQUIRE(a.x && a.w_gate && a.w_up && a.w_down && a.dy && a.dy_stride >= a.out, "x, the weights and dy must not be NULL, dy_stride at least out");
+  LIK_REQUIRE(a.gate && a.up && a.h && a.kept_stride >= a.hidden && a.kept_stride * dtype_size(a.dtype) % 16 == 0 &&
+                  (((uintptr_t)a.gate | (uintptr_t)a.up | (uintptr_t)a.h) & 15) == 0, "gate, up and h must be there, with 16-byte rows");
+  const GatedBwd l = gated_bwd_layout(a, a.workspace);
+  if (a.workspace_bytes < l.total || (l.total && !a.workspace)) return too_small("lik_gated_bwd");
+  if (l.dg)
+    if (int rc = launch_gemm(l.dh, l.gemm, l.gemm_bytes, a.status, st)) return rc;
+  for (const GemmDesc* d : {&l.dx, &l.dwg, &l.dwu, &l.dwd})
+    if (d->out)
+      if (int rc = launch_gemm(*d, l.gemm, l.gemm_bytes, a.status, st)) return rc;
+  auto sums = [&](const void* g, long long stride, int n, void* out) {
+    if (!out) return (int)LIK_OK;
+    SlopeParams p{g, nullptr, stride, 0, a.rows, 0, n, nullptr, 0, l.partial};
+    return launch_slope(p, LIK_ACT_NONE, a.dtype, out, a.param_dtype, st);
+  };
+  if (int rc = sums(l.dg, l.stride, a.hidden, a.db_gate)) return rc;
+  if (int rc = sums(l.du, l.stride, a.hidden, a.db_up)) return rc;
+  return sums(a.dy, a.dy_stride, a.out, a.db_down);
+}

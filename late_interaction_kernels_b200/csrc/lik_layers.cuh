@@ -1,0 +1,218 @@
+// What the kernels of the layers between an encoder and the document head share: activations with their slopes, the
+// description of a matrix product with what is done to its elements, vector loads and stores.
+#pragma once
+
+#include "lik_common.cuh"
+
+namespace lik {
+
+// ---------------------------------------------------------------------------------------------
+// Activations.  PRECISE (fp32 operands): CUDA's own functions.  Otherwise what is stored has 11 or 8 bits, and the two
+// hardware approximations (2^x and the reciprocal, each good to 2^-22) are enough.
+// ---------------------------------------------------------------------------------------------
+template <bool PRECISE>
+__device__ __forceinline__ float sigmoid_f(float z) {
+  return PRECISE ? 1.0f / (1.0f + expf(-z)) : __fdividef(1.0f, 1.0f + __expf(-z));
+}
+template <bool PRECISE>
+__device__ __forceinline__ float tanh_f(float z) {
+  if (PRECISE) return tanhf(z);
+  // below 1/8 the difference would cancel: three terms of the series, the first one left out is 17/315 z^7
+  const float q = z * z;
+  return fabsf(z) < 0.125f ? z * fmaf(q, fmaf(q, 2.0f / 15.0f, -1.0f / 3.0f), 1.0f) : fmaf(2.0f, sigmoid_f<false>(2.0f * z), -1.0f);
+}
+// Phi(-|z|), the lower tail of the normal distribution, and exp(-z^2 / 2).  With t = 1 / (1 + 0.3 |z|) the ratio
+// exp(z^2 / 2) Phi(-|z|) is a smooth function on (0, 1]; six coefficients (least squares, reweighted towards the largest relative
+// error; our own fit) give it to 8.5e-6 relative for all |z| <= 14, a fiftieth of half a step of fp16.
+__device__ __forceinline__ float normal_tail(float z, float& e) {
+  const float a = fabsf(z), t = __fdividef(1.0f, fmaf(0.3f, a, 1.0f));
+  e = exp2f(-0.72134752f * z * z);
+  float r = fmaf(-0.0770966218f, t, 0.216034401f);
+  r = fmaf(r, t, -0.0169447843f);
+  r = fmaf(r, t, 0.144194491f);
+  r = fmaf(r, t, 0.113742429f);
+  r = fmaf(r, t, 0.120074183f);
+  return r * t * e;
+}
+constexpr float GELU_C = 1.5957691216057308f;  // 2 sqrt(2 / pi): (1 + tanh(y)) / 2 = sigmoid(2 y)
+
+template <int ACT, bool PRECISE>
+__device__ __forceinline__ float act_value(float z) {
+  if constexpr (ACT == LIK_ACT_RELU) return z < 0.0f ? 0.0f : z;  // (a NaN stays one)
+  if constexpr (ACT == LIK_ACT_SILU) return z * sigmoid_f<PRECISE>(z);
+  if constexpr (ACT == LIK_ACT_GELU) {
+    if constexpr (PRECISE) return 0.5f * z * erfcf(-0.70710678118654752f * z);
+    float e;
+    const float tail = z * normal_tail(z, e);
+    return z < 0.0f ? tail : z - tail;
+  }
+  if constexpr (ACT == LIK_ACT_GELU_TANH) return z * sigmoid_f<PRECISE>(GELU_C * fmaf(0.044715f * z * z, z, z));
+  if constexpr (ACT == LIK_ACT_TANH) return tanh_f<PRECISE>(z);
+  if constexpr (ACT == LIK_ACT_SIGMOID) return sigmoid_f<PRECISE>(z);
+  return z;
+}
+// the value and the derivative
+template <int ACT, bool PRECISE>
+__device__ __forceinline__ float act_slope(float z, float& value) {
+  if constexpr (ACT == LIK_ACT_RELU) {
+    value = z < 0.0f ? 0.0f : z;
+    return z > 0.0f ? 1.0f : 0.0f;
+  }
+  if constexpr (ACT == LIK_ACT_SILU) {
+    const float s = sigmoid_f<PRECISE>(z);
+    value = z * s;
+    return s * fmaf(z, 1.0f - s, 1.0f);
+  }
+  if constexpr (ACT == LIK_ACT_GELU) {
+    float cdf, e;
+    if constexpr (PRECISE) {
+      cdf = 0.5f * erfcf(-0.70710678118654752f * z);
+      e = expf(-0.5f * z * z);
+    } else {
+      const float tail = normal_tail(z, e);
+      cdf = z < 0.0f ? tail : 1.0f - tail;
+    }
+    value = z * cdf;
+    return fmaf(0.3989422804014327f * z, e, cdf);
+  }
+  if constexpr (ACT == LIK_ACT_GELU_TANH) {
+    const float q = 0.044715f * z * z, s = sigmoid_f<PRECISE>(GELU_C * fmaf(q, z, z));
+    value = z * s;
+    return s * fmaf(GELU_C * z * fmaf(3.0f, q, 1.0f), 1.0f - s, 1.0f);
+  }
+  if constexpr (ACT == LIK_ACT_TANH) {
+    value = tanh_f<PRECISE>(z);
+    return fmaf(-value, value, 1.0f);
+  }
+  if constexpr (ACT == LIK_ACT_SIGMOID) {
+    value = sigmoid_f<PRECISE>(z);
+    return value * (1.0f - value);
+  }
+  value = z;
+  return 1.0f;
+}
+
+// f(ActConst<activation>): the activation as a compile-time constant, on the host (which kernel) and on the device (which epilogue)
+template <int V>
+struct ActConst {
+  static constexpr int value = V;
+};
+#define LIK_WITH_ACTIVATION(NAME, SPACE)                                             \
+  template <typename F>                                                              \
+  SPACE inline void NAME(int act, F&& f) {                                           \
+    switch (act) {                                                                   \
+      case LIK_ACT_RELU: f(ActConst<LIK_ACT_RELU>{}); break;                         \
+      case LIK_ACT_SILU: f(ActConst<LIK_ACT_SILU>{}); break;                         \
+      case LIK_ACT_GELU: f(ActConst<LIK_ACT_GELU>{}); break;                         \
+      case LIK_ACT_GELU_TANH: f(ActConst<LIK_ACT_GELU_TANH>{}); break;               \
+      case LIK_ACT_TANH: f(ActConst<LIK_ACT_TANH>{}); break;                         \
+      case LIK_ACT_SIGMOID: f(ActConst<LIK_ACT_SIGMOID>{}); break;                   \
+      default: f(ActConst<LIK_ACT_NONE>{}); break;                                   \
+    }                                                                                \
+  }
+LIK_WITH_ACTIVATION(with_activation, __host__)
+LIK_WITH_ACTIVATION(with_activation_dev, __device__)
+#undef LIK_WITH_ACTIVATION
+
+// ---------------------------------------------------------------------------------------------
+// Vectors of V elements, V * sizeof(T) = 16 bytes or one element, as fp32
+// ---------------------------------------------------------------------------------------------
+template <typename T>
+constexpr int vec_elems() {
+  return 16 / (int)sizeof(T);
+}
+__device__ __forceinline__ void unpack2(uint32_t w, float& lo, float& hi, __nv_bfloat16) {
+  lo = __uint_as_float(w << 16);
+  hi = __uint_as_float(w & 0xffff0000u);
+}
+__device__ __forceinline__ void unpack2(uint32_t w, float& lo, float& hi, __half) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  lo = f.x;
+  hi = f.y;
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <typename T, int V>
+__device__ __forceinline__ void load_vec(const T* p, float (&v)[V]) {
+  if constexpr (V == 1) {
+    v[0] = to_f32(*p);
+  } else if constexpr (sizeof(T) == 4) {
+    static_assert(V % 4 == 0, "whole 16-byte vectors");
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+      const float4 f = *reinterpret_cast<const float4*>(p + i);
+      v[i] = f.x, v[i + 1] = f.y, v[i + 2] = f.z, v[i + 3] = f.w;
+    }
+  } else {
+    static_assert(V % 8 == 0, "whole 16-byte vectors");
+#pragma unroll
+    for (int i = 0; i < V; i += 8) {
+      const uint4 u = *reinterpret_cast<const uint4*>(p + i);
+      unpack2(u.x, v[i + 0], v[i + 1], T());
+      unpack2(u.y, v[i + 2], v[i + 3], T());
+      unpack2(u.z, v[i + 4], v[i + 5], T());
+      unpack2(u.w, v[i + 6], v[i + 7], T());
+    }
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_vec(T* p, const float (&v)[V]) {
+  if constexpr (V == 1) {
+    *p = from_f32<T>(v[0]);
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < V; i += 4) *reinterpret_cast<float4*>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 8)
+      *reinterpret_cast<uint4*>(p + i) = make_uint4(pack2(v[i], v[i + 1], T()), pack2(v[i + 2], v[i + 3], T()), pack2(v[i + 4], v[i + 5], T()),
+                                                    pack2(v[i + 6], v[i + 7], T()));
+  }
+}
+inline bool vec_ok(const void* p, long long stride, int width, int item) {
+  return ((uintptr_t)p & 15) == 0 && stride * item % 16 == 0 && (long long)width * item % 16 == 0;
+}
+
+// ---------------------------------------------------------------------------------------------
+// A matrix product and what is done to its elements: c[m, n] = sum over segments and k of a(m, k) b(n, k)
+// ---------------------------------------------------------------------------------------------
+enum GemmKind {
+  GEMM_LINEAR = 0,     // out = act(c + bias) + residual; z = c + bias where it is asked for
+  GEMM_GATED = 1,      // two products of the same a: z = c0 + bias0, z2 = c1 + bias1, out = act(z) * z2
+  GEMM_GATED_BWD = 2,  // c = gradient of act(z) * z2: out = gradient of z, out2 = gradient of z2
+};
+struct GemmOperand {
+  const void* p = nullptr;
+  long long row = 0, k = 0;  // elements from one row (m or n) to the next, and from one k to the next; one of the two is 1
+};
+struct GemmDesc {
+  int kind = GEMM_LINEAR, act = LIK_ACT_NONE, dtype = 0;
+  long long m = 0;
+  int n = 0;
+  int n_seg = 1;              // segments of the sum (GEMM_LINEAR) ...
+  long long k[2] = {0, 0};
+  GemmOperand a[2], b[2];     // ... GEMM_GATED: a[0] with b[0] and b[1], k[0]
+  const void* bias[2] = {nullptr, nullptr};
+  const void* residual = nullptr;
+  long long residual_stride = 0;
+  void* out = nullptr;
+  long long out_stride = 0;
+  int out_dtype = 0;          // dtype, or LIK_F32 for products without anything else to them
+  void* out2 = nullptr;       // (with out_stride)
+  void* z = nullptr;          // written (GEMM_LINEAR, GEMM_GATED) or read (GEMM_GATED_BWD)
+  void* z2 = nullptr;
+  long long z_stride = 0;
+};
+size_t gemm_workspace(const GemmDesc& d);
+int launch_gemm(const GemmDesc& d, void* ws, size_t ws_bytes, int* status, cudaStream_t st);
+
+// sum over `parts` of partial[part][i], i < n, as dtype: out[i], the second half (i >= split) to out2
+int launch_sum_parts(const float* partial, int parts, long long n, long long split, int dtype, void* out, void* out2, cudaStream_t st);
+
+}  // namespace lik

@@ -1,0 +1,405 @@
+// Layer norm over rows, forward and backward.
+//
+//   mean = sum x / N, rstd = 1 / sqrt(sum (x - mean)^2 / N + eps), h = (x - mean) rstd, y = h w + b
+//   g = dy w, dx = rstd (g - sum g / N - h sum(g h) / N), dw = sum over rows of dy h, db = sum over rows of dy
+//
+// Everything is bound by memory: a row is read once into registers (a warp's or a block's), and all that is done to it
+// happens there, the variance as a second pass over the registers.  The backward keeps its columns' sums for dw and db in
+// registers from row to row; each block writes them once and a small kernel adds the blocks' sums in their order.
+#include "lik_layers.cuh"
+
+namespace lik {
+namespace {
+
+struct NormParams {
+  const void* x;
+  long long x_stride, rows;
+  int width;
+  const void *w, *b;
+  float eps;
+  void* y;
+  float *mean, *rstd;
+  const void* dy;
+  void* dx;
+  float* partial;  // [blocks][2][width]
+};
+
+constexpr int NORM_THREADS = 256;
+
+// sums of two numbers over the threads of a row: a warp, or the block
+template <int TPR>
+__device__ __forceinline__ float2 row_sum(float a, float b, float2 (&buf)[2][32], int& turn) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    a += __shfl_xor_sync(0xffffffffu, a, o);
+    b += __shfl_xor_sync(0xffffffffu, b, o);
+  }
+  if (TPR == 32) return make_float2(a, b);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // two buffers in turn: nobody is more than one barrier ahead of who still reads
+  turn ^= 1;
+  if (lane == 0) buf[turn][warp] = make_float2(a, b);
+  __syncthreads();
+  a = b = 0.0f;
+#pragma unroll
+  for (int w = 0; w < TPR / 32; ++w) {
+    const float2 f = buf[turn][w];
+    a += f.x;
+    b += f.y;
+  }
+  return make_float2(a, b);
+}
+
+template <typename T, typename P, int V, int NV, int TPR>
+__global__ void __launch_bounds__(NORM_THREADS) norm_fwd_kernel(const NormParams p) {
+  __shared__ float2 buf[2][32];
+  int turn = 0;
+  constexpr int PER_BLOCK = NORM_THREADS / TPR;
+  const int lane = threadIdx.x % TPR;
+  const float inv_n = 1.0f / (float)p.width;
+  for (long long r = (long long)blockIdx.x * PER_BLOCK + threadIdx.x / TPR; r < p.rows; r += (long long)gridDim.x * PER_BLOCK) {
+    const T* x = (const T*)p.x + r * p.x_stride;
+    float v[NV][V];
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + lane) * V;
+      if (c < p.width) {
+        load_vec<T, V>(x + c, v[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[i][j] = 0.0f;
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) s += v[i][j];
+    }
+    const float mean = row_sum<TPR>(s, 0.0f, buf, turn).x * inv_n;
+    float q = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if ((i * TPR + lane) * V < p.width) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          v[i][j] -= mean;
+          q = fmaf(v[i][j], v[i][j], q);
+        }
+      }
+    const float rstd = 1.0f / sqrtf(row_sum<TPR>(q, 0.0f, buf, turn).x * inv_n + p.eps);
+    if (lane == 0 && p.mean) {
+      p.mean[r] = mean;
+      p.rstd[r] = rstd;
+    }
+    T* y = (T*)p.y + r * p.width;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + lane) * V;
+      if (c < p.width) {
+        float w[V], b[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) w[j] = 1.0f, b[j] = 0.0f;
+        if (p.w) load_vec<P, V>((const P*)p.w + c, w);
+        if (p.b) load_vec<P, V>((const P*)p.b + c, b);
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[i][j] = fmaf(v[i][j] * rstd, w[j], b[j]);
+        store_vec<T, V>(y + c, v[i]);
+      }
+    }
+  }
+}
+
+template <typename T, typename P, int V, int NV, int TPR, bool PARAMS>
+__global__ void __launch_bounds__(NORM_THREADS) norm_bwd_kernel(const NormParams p) {
+  __shared__ float2 buf[2][32];
+  int turn = 0;
+  constexpr int PER_BLOCK = NORM_THREADS / TPR;
+  const int lane = threadIdx.x % TPR;
+  const float inv_n = 1.0f / (float)p.width;
+  float dw[PARAMS ? NV : 1][V], db[PARAMS ? NV : 1][V];
+#pragma unroll
+  for (int i = 0; i < (PARAMS ? NV : 1); ++i)
+#pragma unroll
+    for (int j = 0; j < V; ++j) dw[i][j] = db[i][j] = 0.0f;
+  for (long long r = (long long)blockIdx.x * PER_BLOCK + threadIdx.x / TPR; r < p.rows; r += (long long)gridDim.x * PER_BLOCK) {
+    const T* x = (const T*)p.x + r * p.x_stride;
+    const T* dy = (const T*)p.dy + r * p.width;
+    const float mean = p.mean[r], rstd = p.rstd[r];
+    float h[NV][V], g[NV][V];
+    float s = 0.0f, t = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + lane) * V;
+      if (c < p.width) {
+        load_vec<T, V>(x + c, h[i]);
+        load_vec<T, V>(dy + c, g[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + lane) * V;
+      if (c < p.width) {
+        float w[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) w[j] = 1.0f;
+        if (p.w) load_vec<P, V>((const P*)p.w + c, w);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          h[i][j] = (h[i][j] - mean) * rstd;
+          if (PARAMS) {
+            dw[i][j] = fmaf(g[i][j], h[i][j], dw[i][j]);
+            db[i][j] += g[i][j];
+          }
+          g[i][j] *= w[j];
+          s += g[i][j];
+          t = fmaf(g[i][j], h[i][j], t);
+        }
+      }
+    }
+    if (p.dx) {
+      const float2 m = row_sum<TPR>(s, t, buf, turn);
+      const float c1 = m.x * inv_n, c2 = m.y * inv_n;
+      T* dx = (T*)p.dx + r * p.width;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (i * TPR + lane) * V;
+        if (c < p.width) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) g[i][j] = rstd * (g[i][j] - c1 - h[i][j] * c2);
+          store_vec<T, V>(dx + c, g[i]);
+        }
+      }
+    }
+  }
+  if constexpr (PARAMS) {
+    float* out = p.partial + (long long)blockIdx.x * 2 * p.width;
+    if constexpr (TPR == NORM_THREADS) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (i * TPR + lane) * V;
+        if (c < p.width)
+#pragma unroll
+          for (int j = 0; j < V; ++j) out[c + j] = dw[i][j], out[p.width + c + j] = db[i][j];
+      }
+    } else {
+      // the block's warps in their order, each adding to what is in shared memory
+      extern __shared__ float acc[];  // [2][NV * TPR * V]
+      constexpr int COLS = NV * TPR * V;
+      for (int w = 0; w < PER_BLOCK; ++w) {
+        if (threadIdx.x / TPR == w) {
+#pragma unroll
+          for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+              const int c = (i * V + j) * TPR + lane;  // (one bank per lane)
+              acc[c] = w ? acc[c] + dw[i][j] : dw[i][j];
+              acc[COLS + c] = w ? acc[COLS + c] + db[i][j] : db[i][j];
+            }
+        }
+        __syncthreads();
+      }
+      for (int c = threadIdx.x; c < COLS; c += NORM_THREADS) {
+        // (i, lane, j) of a column
+        const int i = c / (TPR * V), l = c / V % TPR, j = c % V, at = (i * V + j) * TPR + l;
+        if (c < p.width) out[c] = acc[at], out[p.width + c] = acc[COLS + at];
+      }
+    }
+  }
+}
+
+// Rows that no block holds in registers: a block goes through its row three times, the later ones out of L2.
+template <typename T, typename P>
+__global__ void __launch_bounds__(NORM_THREADS) norm_fwd_wide_kernel(const NormParams p) {
+  __shared__ float2 buf[2][32];
+  int turn = 0;
+  const float inv_n = 1.0f / (float)p.width;
+  for (long long r = blockIdx.x; r < p.rows; r += gridDim.x) {
+    const T* x = (const T*)p.x + r * p.x_stride;
+    float s = 0.0f, q = 0.0f;
+    for (int c = threadIdx.x; c < p.width; c += NORM_THREADS) s += to_f32(x[c]);
+    const float mean = row_sum<NORM_THREADS>(s, 0.0f, buf, turn).x * inv_n;
+    for (int c = threadIdx.x; c < p.width; c += NORM_THREADS) {
+      const float d = to_f32(x[c]) - mean;
+      q = fmaf(d, d, q);
+    }
+    const float rstd = 1.0f / sqrtf(row_sum<NORM_THREADS>(q, 0.0f, buf, turn).x * inv_n + p.eps);
+    if (threadIdx.x == 0 && p.mean) p.mean[r] = mean, p.rstd[r] = rstd;
+    for (int c = threadIdx.x; c < p.width; c += NORM_THREADS)
+      ((T*)p.y)[r * p.width + c] =
+          from_f32<T>(fmaf((to_f32(x[c]) - mean) * rstd, p.w ? to_f32(((const P*)p.w)[c]) : 1.0f, p.b ? to_f32(((const P*)p.b)[c]) : 0.0f));
+  }
+}
+template <typename T, typename P>
+__global__ void __launch_bounds__(NORM_THREADS) norm_dx_wide_kernel(const NormParams p) {
+  __shared__ float2 buf[2][32];
+  int turn = 0;
+  const float inv_n = 1.0f / (float)p.width;
+  for (long long r = blockIdx.x; r < p.rows; r += gridDim.x) {
+    const T *x = (const T*)p.x + r * p.x_stride, *dy = (const T*)p.dy + r * p.width;
+    const float mean = p.mean[r], rstd = p.rstd[r];
+    float s = 0.0f, t = 0.0f;
+    for (int c = threadIdx.x; c < p.width; c += NORM_THREADS) {
+      const float g = to_f32(dy[c]) * (p.w ? to_f32(((const P*)p.w)[c]) : 1.0f);
+      s += g;
+      t = fmaf(g, (to_f32(x[c]) - mean) * rstd, t);
+    }
+    const float2 m = row_sum<NORM_THREADS>(s, t, buf, turn);
+    const float c1 = m.x * inv_n, c2 = m.y * inv_n;
+    for (int c = threadIdx.x; c < p.width; c += NORM_THREADS) {
+      const float g = to_f32(dy[c]) * (p.w ? to_f32(((const P*)p.w)[c]) : 1.0f);
+      ((T*)p.dx)[r * p.width + c] = from_f32<T>(rstd * (g - c1 - (to_f32(x[c]) - mean) * rstd * c2));
+    }
+  }
+}
+// a thread's column over every gridDim.y-th row
+template <typename T>
+__global__ void __launch_bounds__(NORM_THREADS) norm_dparam_wide_kernel(const NormParams p) {
+  const int c = blockIdx.x * NORM_THREADS + threadIdx.x;
+  if (c >= p.width) return;
+  float dw = 0.0f, db = 0.0f;
+  for (long long r = blockIdx.y; r < p.rows; r += gridDim.y) {
+    const float g = to_f32(((const T*)p.dy)[r * p.width + c]);
+    dw = fmaf(g, (to_f32(((const T*)p.x)[r * p.x_stride + c]) - p.mean[r]) * p.rstd[r], dw);
+    db += g;
+  }
+  float* out = p.partial + (long long)blockIdx.y * 2 * p.width;
+  out[c] = dw;
+  out[p.width + c] = db;
+}
+
+constexpr int NORM_WIDE_PARTS = 64;
+
+// Which kernel a width goes to: a warp per row as long as its lanes hold the row in 32 (16-bit) or 16 (fp32) registers each, then a
+// block of 256 threads; vectors of 16 bytes where rows and parameters are aligned, else single elements.
+struct NormPlan {
+  bool wide, vec;
+  int nv, tpr;
+};
+NormPlan norm_plan(const lik_norm_args& a) {
+  const int item = (int)dtype_size(a.dtype), v = 16 / item;
+  NormPlan pl{};
+  pl.vec = vec_ok(a.x, a.x_stride, a.width, item) && vec_ok(a.y, a.width, a.width, item) && vec_ok(a.dy, a.width, a.width, item) &&
+           vec_ok(a.dx, a.width, a.width, item) && ((uintptr_t)a.weight & 15) == 0 && ((uintptr_t)a.bias & 15) == 0;
+  const int per = pl.vec ? v : 1;
+  const long long vecs = ceil_div(a.width, per);
+  const int warp_most = pl.vec ? 4 : 8, block_most = pl.vec ? 4 : 16;
+  pl.tpr = vecs <= 32 * warp_most ? 32 : 256;
+  pl.nv = (int)ceil_div(vecs, pl.tpr);
+  pl.wide = pl.tpr == 256 && pl.nv > block_most;
+  if (!pl.vec && pl.nv > 1) pl.nv = pl.nv <= 4 ? 4 : (pl.nv <= 8 ? 8 : 16);
+  else if (pl.vec && pl.tpr == 256 && pl.nv == 3) pl.nv = 4;
+  return pl;
+}
+int norm_bwd_blocks(const lik_norm_args& a, const NormPlan& pl) {
+  if (pl.wide) return (int)(a.rows < NORM_WIDE_PARTS ? (a.rows ? a.rows : 1) : NORM_WIDE_PARTS);
+  const long long need = ceil_div(a.rows, NORM_THREADS / pl.tpr), most = 2ll * sm_count();
+  return (int)(need < most ? (need ? need : 1) : most);
+}
+
+template <typename T, typename P, int V, int NV, int TPR>
+int run_norm(const NormParams& p, bool bwd, bool params, int blocks, cudaStream_t st) {
+  if (!bwd) {
+    norm_fwd_kernel<T, P, V, NV, TPR><<<blocks, NORM_THREADS, 0, st>>>(p), count_launch();
+  } else if (params) {
+    const size_t smem = TPR == 32 ? sizeof(float) * 2 * NV * TPR * V : 0;
+    norm_bwd_kernel<T, P, V, NV, TPR, true><<<blocks, NORM_THREADS, smem, st>>>(p), count_launch();
+  } else {
+    norm_bwd_kernel<T, P, V, NV, TPR, false><<<blocks, NORM_THREADS, 0, st>>>(p), count_launch();
+  }
+  LIK_CUDA_OK(cudaGetLastError());
+  return LIK_OK;
+}
+template <typename T, typename P>
+int run_norm(const NormPlan& pl, const NormParams& p, bool bwd, bool params, int blocks, cudaStream_t st) {
+  constexpr int V = vec_elems<T>();
+  if (pl.wide) {
+    if (!bwd) {
+      norm_fwd_wide_kernel<T, P><<<blocks, NORM_THREADS, 0, st>>>(p), count_launch();
+    } else {
+      if (p.dx) norm_dx_wide_kernel<T, P><<<(unsigned)(p.rows < 8ll * sm_count() ? p.rows : 8ll * sm_count()), NORM_THREADS, 0, st>>>(p), count_launch();
+      if (params) norm_dparam_wide_kernel<T><<<dim3((unsigned)ceil_div(p.width, NORM_THREADS), blocks), NORM_THREADS, 0, st>>>(p), count_launch();
+    }
+    LIK_CUDA_OK(cudaGetLastError());
+    return LIK_OK;
+  }
+#define LIK_NORM_CASE(VV, NN, TT) \
+  if ((pl.vec ? V : 1) == VV && pl.nv == NN && pl.tpr == TT) return run_norm<T, P, VV, NN, TT>(p, bwd, params, blocks, st)
+  LIK_NORM_CASE(V, 1, 32);
+  LIK_NORM_CASE(V, 2, 32);
+  LIK_NORM_CASE(V, 3, 32);
+  LIK_NORM_CASE(V, 4, 32);
+  LIK_NORM_CASE(V, 1, 256);
+  LIK_NORM_CASE(V, 2, 256);
+  LIK_NORM_CASE(V, 4, 256);
+  LIK_NORM_CASE(1, 1, 32);
+  LIK_NORM_CASE(1, 4, 32);
+  LIK_NORM_CASE(1, 8, 32);
+  LIK_NORM_CASE(1, 4, 256);
+  LIK_NORM_CASE(1, 8, 256);
+  LIK_NORM_CASE(1, 16, 256);
+#undef LIK_NORM_CASE
+  set_error("layer norm: no kernel for width %d", p.width);
+  return LIK_ERR_UNSUPPORTED;
+}
+int run_norm(const lik_norm_args& a, const NormPlan& pl, const NormParams& p, bool bwd, bool params, int blocks, cudaStream_t st) {
+  if (a.dtype == LIK_F32) return run_norm<float, float>(pl, p, bwd, params, blocks, st);
+  if (a.dtype == LIK_F16)
+    return a.param_dtype == LIK_F32 ? run_norm<__half, float>(pl, p, bwd, params, blocks, st) : run_norm<__half, __half>(pl, p, bwd, params, blocks, st);
+  return a.param_dtype == LIK_F32 ? run_norm<__nv_bfloat16, float>(pl, p, bwd, params, blocks, st)
+                                  : run_norm<__nv_bfloat16, __nv_bfloat16>(pl, p, bwd, params, blocks, st);
+}
+NormParams norm_params(const lik_norm_args& a) {
+  return NormParams{a.x, a.x_stride, a.rows, a.width, a.weight, a.bias, a.eps, a.y, a.mean, a.rstd, a.dy, a.dx, nullptr};
+}
+int check_norm(const lik_norm_args* a) {
+  LIK_REQUIRE(a != nullptr, "args is NULL");
+  LIK_REQUIRE(a->dtype == LIK_F32 || a->dtype == LIK_F16 || a->dtype == LIK_BF16, "dtype must be fp32, fp16 or bf16");
+  LIK_REQUIRE(a->param_dtype == a->dtype || a->param_dtype == LIK_F32, "param_dtype must be dtype or fp32");
+  LIK_REQUIRE(a->rows >= 0 && a->width > 0 && a->x_stride >= a->width, "sizes must be positive, x_stride at least width");
+  LIK_REQUIRE(a->eps >= 0.0f, "eps must not be negative");
+  return LIK_OK;
+}
+
+}  // namespace
+}  // namespace lik
+
+extern "C" int lik_layer_norm_fwd(const lik_norm_args* args, lik_stream_t stream) {
+  using namespace lik;
+  if (int rc = check_norm(args)) return rc;
+  const lik_norm_args& a = *args;
+  if (a.rows == 0) return LIK_OK;
+  LIK_REQUIRE(a.x && a.y && !a.mean == !a.rstd, "x and y must not be NULL; mean and rstd go together");
+  const NormPlan pl = norm_plan(a);
+  const long long need = ceil_div(a.rows, pl.wide ? 1 : NORM_THREADS / pl.tpr), most = 8ll * sm_count();
+  return run_norm(a, pl, norm_params(a), false, false, (int)(need < most ? need : most), (cudaStream_t)stream);
+}
+
+extern "C" size_t lik_layer_norm_bwd_workspace(const lik_norm_args* a) {
+  using namespace lik;
+  if (check_norm(a) || a->rows == 0 || (!a->dweight && !a->dbias)) return 0;
+  return (size_t)norm_bwd_blocks(*a, norm_plan(*a)) * 2 * a->width * sizeof(float);
+}
+
+extern "C" int lik_layer_norm_bwd(const lik_norm_args* args, lik_stream_t stream) {
+  using namespace lik;
+  if (int rc = check_norm(args)) return rc;
+  const lik_norm_args& a = *args;
+  cudaStream_t st = (cudaStream_t)stream;
+  const bool params = a.dweight || a.dbias;
+  if (a.rows == 0) {
+    const size_t bytes = (size_t)a.width * dtype_size(a.param_dtype);
+    if (a.dweight) LIK_CUDA_OK(cudaMemsetAsync(a.dweight, 0, bytes, st));
+    if (a.dbias) LIK_CUDA_OK(cudaMemsetAsync(a.dbias, 0, bytes, st));
+    return LIK_OK;
+  }
+  if (!a.dx && !params) return LIK_OK;
+  LIK_REQUIRE(a.x && a.dy && a.mean && a.rstd, "x, dy, mean and rstd must not be NULL");
+  if (params && (!a.workspace || a.workspace_bytes < lik_layer_norm_bwd_workspace(args))) {
+    set_error("lik_layer_norm_bwd: workspace too small");
+    return LIK_ERR_WORKSPACE;
+  }
+  const NormPlan pl = norm_plan(a);
+  NormParams p = norm_params(a);
+  p.partial = (float*)a.workspace;
+  const int blocks = norm_bwd_blocks(a, pl);
+  if (int rc = run_norm(a, pl, p, true, params, blocks, st)) return rc;
+  return params ? launch_sum_parts(p.partial, blocks, 2ll * a.width, a.width, a.param_dtype, a.dweight, a.dbias, st) : LIK_OK;
+}

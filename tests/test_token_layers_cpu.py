@@ -1,0 +1,60 @@
+"""The layers in front of the document head, without a GPU: refusals, argument checks of the C entry points, struct layout."""
+
+import ctypes as C
+import os
+import subprocess
+
+import pytest
+import torch
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+@pytest.fixture(scope="module")
+def layers():
+    from late_interaction_kernels_b200 import _build, token_layers
+
+    _build.build()
+    return token_layers
+
+
+def test_no_cpu_path(layers):
+    x, w = torch.zeros(2, 8), torch.zeros(8, 8)
+    for fn in (lambda: layers.layer_norm(x), lambda: layers.linear(x, w), lambda: layers.gated_feed_forward(x, w, w, w)):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            fn()
+
+
+def test_struct_sizes_are_the_compilers(layers, tmp_path):
+    from late_interaction_kernels_b200 import _lib
+
+    src = tmp_path / "sizes.c"
+    src.write_text('#include <stdio.h>\n#include "lik_b200.h"\nint main(void) { printf("%zu %zu %zu", sizeof(lik_norm_args), sizeof(lik_linear_args), '
+                   "sizeof(lik_gated_args)); return 0; }\n")
+    subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(tmp_path / "sizes")], check=True)
+    out = subprocess.run([str(tmp_path / "sizes")], check=True, capture_output=True, text=True).stdout
+    assert out == " ".join(str(C.sizeof(t)) for t in (_lib.NormArgs, _lib.LinearArgs, _lib.GatedArgs))
+
+
+def test_c_entries_refuse_before_any_launch(layers):
+    from late_interaction_kernels_b200 import _lib
+
+    lib = _lib.load()
+    for name, args in (("layer_norm", _lib.NormArgs), ("linear", _lib.LinearArgs), ("gated", _lib.GatedArgs)):
+        for way in ("fwd", "bwd"):
+            fn = getattr(lib, f"lik_{name}_{way}")
+            assert fn(None, None) == -1
+            a = args()
+            a.dtype = a.param_dtype = _lib.LIK_BF16
+            assert fn(C.byref(a), None) == -1 and b"positive" in lib.lik_last_error()
+            a.dtype = _lib.LIK_E4M3
+            assert fn(C.byref(a), None) == -1 and b"dtype must be" in lib.lik_last_error()
+    a = _lib.LinearArgs(dtype=2, param_dtype=2, x_stride=8, w_stride=8, rows=4, out=8, activation=9)
+    setattr(a, "in", 8)
+    assert lib.lik_linear_fwd(C.byref(a), None) == -1 and b"activation" in lib.lik_last_error()
+    a.activation = 3
+    assert lib.lik_linear_fwd(C.byref(a), None) == -1 and b"must not be NULL" in lib.lik_last_error()
+    a.param_dtype = _lib.LIK_F16
+    assert lib.lik_linear_bwd(C.byref(a), None) == -1 and b"param_dtype" in lib.lik_last_error()
+    n = _lib.NormArgs(dtype=2, param_dtype=0, x_stride=8, rows=4, width=8, eps=-1.0)
+    assert lib.lik_layer_norm_fwd(C.byref(n), None) == -1 and b"eps" in lib.lik_last_error()
