@@ -125,7 +125,7 @@ class GatedArgs(C.Structure):
         ("b_gate", C.c_void_p), ("b_up", C.c_void_p), ("b_down", C.c_void_p), ("residual", C.c_void_p),
         ("residual_stride", C.c_int64), ("rows", C.c_int64), ("in", C.c_int32), ("hidden", C.c_int32),
         ("out", C.c_int32), ("dtype", C.c_int32), ("activation", C.c_int32), ("param_dtype", C.c_int32),
-        ("y", C.c_void_p), ("gate", C.c_void_p), ("up", C.c_void_p), ("h", C.c_void_p), ("kept_stride", C.c_int64),
+        ("y", C.c_void_p), ("gate_factor", C.c_void_p), ("up_factor", C.c_void_p), ("h", C.c_void_p), ("kept_stride", C.c_int64),
         ("dy", C.c_void_p), ("dy_stride", C.c_int64), ("dx", C.c_void_p), ("dw_gate", C.c_void_p),
         ("dw_up", C.c_void_p), ("dw_down", C.c_void_p), ("db_gate", C.c_void_p), ("db_up", C.c_void_p),
         ("db_down", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("status", C.c_void_p),

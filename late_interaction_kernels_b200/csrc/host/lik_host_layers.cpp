@@ -440,8 +440,8 @@ struct GatedFeedForwardBackward : public torch::autograd::Node {
       lik_gated_args a = gated_args(X, WG, WU, WD, act);
       a.param_dtype = grad_type;
       const auto popt = X.options().dtype(scalar_of(grad_type));
-      a.gate = ptr(G);
-      a.up = ptr(U);
+      a.gate_factor = ptr(G);
+      a.up_factor = ptr(U);
       a.h = ptr(H);
       a.kept_stride = G.size(1);
       a.dy = ptr(dy);
@@ -510,8 +510,8 @@ Tensor gated_feed_forward(const Tensor& x_, const Tensor& wg, const Tensor& wu, 
       g = kept_rows(x.size(0), f, x);
       u = kept_rows(x.size(0), f, x);
       h = kept_rows(x.size(0), f, x);
-      a.gate = ptr(g);
-      a.up = ptr(u);
+      a.gate_factor = ptr(g);
+      a.up_factor = ptr(u);
       a.h = ptr(h);
       a.kept_stride = g.size(1);
     }

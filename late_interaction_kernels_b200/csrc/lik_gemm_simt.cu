@@ -60,25 +60,28 @@ __device__ __forceinline__ void slab_store(const GemmOperand& o, const float (&v
 template <typename T, typename O, int KIND, int ACT>
 __device__ __forceinline__ void simt_element(const GemmDesc& d, long long m, int n, float c0, float c1) {
   constexpr bool PRECISE = sizeof(T) == 4;
-  const long long zi = m * d.z_stride + n, oi = m * d.out_stride + n;
+  const long long ki = m * d.kept_stride + n, oi = m * d.out_stride + n;
   if constexpr (KIND == GEMM_GATED_BWD) {
-    float a;
-    const float s = act_slope<ACT, PRECISE>(to_f32(((const T*)d.z)[zi]), a);
-    ((T*)d.out)[oi] = from_f32<T>(c0 * to_f32(((const T*)d.z2)[zi]) * s);
-    ((T*)d.out2)[oi] = from_f32<T>(c0 * a);
+    ((T*)d.out[0])[oi] = from_f32<T>(c0 * to_f32(((const T*)d.kept[0])[ki]));
+    ((T*)d.out[1])[oi] = from_f32<T>(c0 * to_f32(((const T*)d.kept[1])[ki]));
     return;
   }
   if (d.bias[0]) c0 += to_f32(((const T*)d.bias[0])[n]);
-  if (d.z) ((T*)d.z)[zi] = from_f32<T>(c0);
-  float v = act_value<ACT, PRECISE>(c0);
+  float v;
   if constexpr (KIND == GEMM_GATED) {
+    const float slope = act_slope<ACT, PRECISE>(c0, v);
     if (d.bias[1]) c1 += to_f32(((const T*)d.bias[1])[n]);
-    if (d.z2) ((T*)d.z2)[zi] = from_f32<T>(c1);
+    if (d.kept[0]) {
+      ((T*)d.kept[0])[ki] = from_f32<T>(c1 * slope);
+      ((T*)d.kept[1])[ki] = from_f32<T>(v);
+    }
     v *= c1;
-  } else if (d.residual) {
-    v += to_f32(((const T*)d.residual)[m * d.residual_stride + n]);
+  } else {
+    v = act_value<ACT, PRECISE>(c0);
+    if (d.kept[0]) ((T*)d.kept[0])[ki] = from_f32<T>(c0);
+    if (d.residual) v += to_f32(((const T*)d.residual)[m * d.residual_stride + n]);
   }
-  ((O*)d.out)[oi] = from_f32<O>(v);
+  ((O*)d.out[0])[oi] = from_f32<O>(v);
 }
 
 template <typename T, typename O, int KIND, int BM, int BN, int TM, int TN>
@@ -173,7 +176,7 @@ SimtPlan simt_plan(const GemmDesc& d) {
   pl.tiles = ceil_div(d.m, b) * pl.tiles_n;
   pl.splits = 1;
   pl.per_split = 0;
-  const bool plain = d.kind == GEMM_LINEAR && d.n_seg == 1 && d.act == LIK_ACT_NONE && !d.bias[0] && !d.residual && !d.z && d.out_stride == d.n;
+  const bool plain = d.kind == GEMM_LINEAR && d.n_seg == 1 && d.act == LIK_ACT_NONE && !d.bias[0] && !d.residual && !d.kept[0] && d.out_stride == d.n;
   if (plain && pl.tiles < sm_count() && d.k[0] >= 512) {
     long long want = ceil_div(2ll * sm_count(), pl.tiles);
     if (want > d.k[0] / 256) want = d.k[0] / 256;
@@ -209,23 +212,22 @@ int run_simt(const SimtParams& p, const SimtPlan& pl, cudaStream_t st) {
 
 }  // namespace
 
-size_t gemm_workspace(const GemmDesc& d) {
+size_t gemm_simt_workspace(const GemmDesc& d) {
   const SimtPlan pl = simt_plan(d);
   return pl.splits > 1 ? align_up((size_t)pl.splits * d.m * d.n * sizeof(float), 256) : 0;
 }
 
-int launch_gemm(const GemmDesc& d, void* ws, size_t ws_bytes, int* status, cudaStream_t st) {
-  (void)status;
+int launch_gemm_simt(const GemmDesc& d, void* ws, size_t ws_bytes, cudaStream_t st) {
   const SimtPlan pl = simt_plan(d);
   LIK_REQUIRE(pl.tiles < (1ll << 31), "the product has too many tiles");
   SimtParams p{d, pl.tiles_n, pl.splits, pl.per_split, (float*)ws};
-  if (pl.splits > 1 && (!ws || ws_bytes < gemm_workspace(d))) {
+  if (pl.splits > 1 && (!ws || ws_bytes < gemm_simt_workspace(d))) {
     set_error("workspace too small");
     return LIK_ERR_WORKSPACE;
   }
   int rc = d.dtype == LIK_F32 ? run_simt<float>(p, pl, st) : (d.dtype == LIK_F16 ? run_simt<__half>(p, pl, st) : run_simt<__nv_bfloat16>(p, pl, st));
   if (rc || pl.splits == 1) return rc;
-  return launch_sum_parts((const float*)ws, pl.splits, d.m * d.n, d.m * d.n, d.out_dtype, d.out, nullptr, st);
+  return launch_sum_parts((const float*)ws, pl.splits, d.m * d.n, d.m * d.n, d.out_dtype, d.out[0], nullptr, st);
 }
 
 }  // namespace lik

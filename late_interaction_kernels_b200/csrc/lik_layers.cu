@@ -59,10 +59,7 @@ __global__ void __launch_bounds__(32 * SLOPE_LANES) slope_kernel(const SlopePara
       if constexpr (ACT != LIK_ACT_NONE) {
         load_vec<T, V>((const T*)p.z + r * p.z_stride + c, z);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          float a;
-          g[j] *= act_slope<ACT, sizeof(T) == 4>(z[j], a);
-        }
+        for (int j = 0; j < V; ++j) g[j] *= act_slope<ACT, sizeof(T) == 4>(z[j], z[j]);
       }
       if (p.dz) store_vec<T, V>((T*)p.dz + r * p.dz_stride + c, g);
 #pragma unroll
@@ -112,6 +109,13 @@ int launch_slope(SlopeParams p, int act, int dtype, void* sums, int sums_dtype, 
   return launch_sum_parts(p.partial, parts, p.n, p.n, sums_dtype, sums, nullptr, st);
 }
 
+// which kernel a product goes to
+bool on_tensor_cores(const GemmDesc& d) { return gemm_tc_supported(d); }
+size_t gemm_workspace(const GemmDesc& d) { return on_tensor_cores(d) ? gemm_tc_workspace(d) : gemm_simt_workspace(d); }
+int launch_gemm(const GemmDesc& d, void* ws, size_t ws_bytes, int* status, cudaStream_t st) {
+  return on_tensor_cores(d) ? launch_gemm_tc(d, ws, ws_bytes, status, st) : launch_gemm_simt(d, ws, ws_bytes, st);
+}
+
 bool act_known(int a) { return a >= LIK_ACT_NONE && a <= LIK_ACT_SIGMOID; }
 bool dtype_known(int d) { return d == LIK_F32 || d == LIK_F16 || d == LIK_BF16; }
 // rows of kept and internal matrices start on 16 bytes
@@ -153,10 +157,10 @@ GemmDesc linear_fwd_desc(const lik_linear_args& a) {
   d.bias[0] = a.bias;
   d.residual = a.residual;
   d.residual_stride = a.residual_stride;
-  d.out = a.y;
+  d.out[0] = a.y;
   d.out_stride = a.out;
-  d.z = a.activation == LIK_ACT_NONE ? nullptr : a.z;
-  d.z_stride = a.z_stride;
+  d.kept[0] = a.activation == LIK_ACT_NONE ? nullptr : a.z;
+  d.kept_stride = a.z_stride;
   return d;
 }
 // dx = dz w and dw = dz^T x
@@ -168,7 +172,7 @@ GemmDesc grad_x_desc(int dtype, long long rows, int out, int in, const void* dz,
   d.k[0] = out;
   d.a[0] = {dz, dz_stride, 1};
   d.b[0] = {w, 1, w_stride};
-  d.out = dx;
+  d.out[0] = dx;
   d.out_stride = in;
   return d;
 }
@@ -182,7 +186,7 @@ GemmDesc grad_w_desc(int dtype, int param_dtype, long long rows, int out, int in
   d.k[0] = rows;
   d.a[0] = {dz, 1, dz_stride};
   d.b[0] = {x, 1, x_stride};
-  d.out = dw;
+  d.out[0] = dw;
   d.out_stride = in;
   return d;
 }
@@ -242,7 +246,7 @@ GatedFwd gated_fwd_layout(const lik_gated_args& a, void* ws) {
   Carve c{(char*)ws};
   void* h = a.h;
   long long h_stride = a.kept_stride;
-  if (!a.gate) {
+  if (!a.gate_factor) {
     h_stride = pad_cols(a.hidden, a.dtype);
     h = c.take((size_t)a.rows * h_stride * dtype_size(a.dtype));
   }
@@ -258,11 +262,11 @@ GatedFwd gated_fwd_layout(const lik_gated_args& a, void* ws) {
   u.b[1] = {a.w_up, a.w_up_stride, 1};
   u.bias[0] = a.b_gate;
   u.bias[1] = a.b_up;
-  u.out = h;
+  u.out[0] = h;
   u.out_stride = h_stride;
-  u.z = a.gate;
-  u.z2 = a.up;
-  u.z_stride = a.kept_stride;
+  u.kept[0] = a.gate_factor;
+  u.kept[1] = a.up_factor;
+  u.kept_stride = a.kept_stride;
   GemmDesc& d = l.down;
   d.dtype = d.out_dtype = a.dtype;
   d.m = a.rows;
@@ -273,7 +277,7 @@ GatedFwd gated_fwd_layout(const lik_gated_args& a, void* ws) {
   d.bias[0] = a.b_down;
   d.residual = a.residual;
   d.residual_stride = a.residual_stride;
-  d.out = a.y;
+  d.out[0] = a.y;
   d.out_stride = a.out;
   const size_t b1 = gemm_workspace(u), b2 = gemm_workspace(d);
   l.gemm_bytes = b1 > b2 ? b1 : b2;
@@ -299,19 +303,18 @@ GatedBwd gated_bwd_layout(const lik_gated_args& a, void* ws) {
     l.du = c.take((size_t)a.rows * l.stride * dtype_size(a.dtype));
     GemmDesc& h = l.dh;
     h.kind = GEMM_GATED_BWD;
-    h.act = a.activation;
     h.dtype = h.out_dtype = a.dtype;
     h.m = a.rows;
     h.n = a.hidden;
     h.k[0] = a.out;
     h.a[0] = {a.dy, a.dy_stride, 1};
     h.b[0] = {a.w_down, 1, a.w_down_stride};
-    h.out = l.dg;
-    h.out2 = l.du;
+    h.out[0] = l.dg;
+    h.out[1] = l.du;
     h.out_stride = l.stride;
-    h.z = a.gate;
-    h.z2 = a.up;
-    h.z_stride = a.kept_stride;
+    h.kept[0] = a.gate_factor;
+    h.kept[1] = a.up_factor;
+    h.kept_stride = a.kept_stride;
     l.gemm_bytes = gemm_workspace(h);
   }
   auto want = [&](const GemmDesc& d) {
@@ -385,7 +388,8 @@ extern "C" int lik_linear_bwd(const lik_linear_args* args, lik_stream_t stream) 
   if (!a.dx && !a.dw && !a.dbias) return LIK_OK;
   LIK_REQUIRE(a.x && a.w && a.dy && a.dy_stride >= a.out, "x, w and dy must not be NULL, dy_stride at least out");
   const bool act = a.activation != LIK_ACT_NONE;
-  LIK_REQUIRE(!act || (a.z && a.z_stride >= a.out && a.z_stride * dtype_size(a.dtype) % 16 == 0 && ((uintptr_t)a.z & 15) == 0), "z must have 16-byte rows");
+  LIK_REQUIRE(!act || (a.z && a.z_stride >= a.out && a.z_stride * dtype_size(a.dtype) % 16 == 0 && ((uintptr_t)a.z & 15) == 0),
+              "z must be there, with 16-byte rows");
   const LinearBwd l = linear_bwd_layout(a, a.workspace);
   if (a.workspace_bytes < l.total || (l.total && !a.workspace)) return too_small("lik_linear_bwd");
   const void* dz = act ? l.dz : a.dy;
@@ -412,9 +416,9 @@ extern "C" int lik_gated_fwd(const lik_gated_args* args, lik_stream_t stream) {
   const lik_gated_args& a = *args;
   if (a.rows == 0) return LIK_OK;
   LIK_REQUIRE(a.x && a.w_gate && a.w_up && a.w_down && a.y, "x, the weights and y must not be NULL");
-  LIK_REQUIRE(!a.gate == !a.up && !a.gate == !a.h, "gate, up and h are kept together");
-  LIK_REQUIRE(!a.gate || (a.kept_stride >= a.hidden && a.kept_stride * dtype_size(a.dtype) % 16 == 0 &&
-                          (((uintptr_t)a.gate | (uintptr_t)a.up | (uintptr_t)a.h) & 15) == 0), "gate, up and h must have 16-byte rows");
+  LIK_REQUIRE(!a.gate_factor == !a.up_factor && !a.gate_factor == !a.h, "gate_factor, up_factor and h are kept together");
+  LIK_REQUIRE(!a.gate_factor || (a.kept_stride >= a.hidden && a.kept_stride * dtype_size(a.dtype) % 16 == 0 &&
+                          (((uintptr_t)a.gate_factor | (uintptr_t)a.up_factor | (uintptr_t)a.h) & 15) == 0), "gate_factor, up_factor and h must have 16-byte rows");
   LIK_REQUIRE(!a.residual || a.residual_stride >= a.out, "residual_stride must be at least out");
   const GatedFwd l = gated_fwd_layout(a, a.workspace);
   if (a.workspace_bytes < l.total || (l.total && !a.workspace)) return too_small("lik_gated_fwd");
@@ -441,14 +445,14 @@ extern "C" int lik_gated_bwd(const lik_gated_args* args, lik_stream_t stream) {
     return LIK_OK;
   }
   LIK_REQUIRE(a.x && a.w_gate && a.w_up && a.w_down && a.dy && a.dy_stride >= a.out, "x, the weights and dy must not be NULL, dy_stride at least out");
-  LIK_REQUIRE(a.gate && a.up && a.h && a.kept_stride >= a.hidden && a.kept_stride * dtype_size(a.dtype) % 16 == 0 &&
-                  (((uintptr_t)a.gate | (uintptr_t)a.up | (uintptr_t)a.h) & 15) == 0, "gate, up and h must be there, with 16-byte rows");
+  LIK_REQUIRE(a.gate_factor && a.up_factor && a.h && a.kept_stride >= a.hidden && a.kept_stride * dtype_size(a.dtype) % 16 == 0 &&
+                  (((uintptr_t)a.gate_factor | (uintptr_t)a.up_factor | (uintptr_t)a.h) & 15) == 0, "gate_factor, up_factor and h must be there, with 16-byte rows");
   const GatedBwd l = gated_bwd_layout(a, a.workspace);
   if (a.workspace_bytes < l.total || (l.total && !a.workspace)) return too_small("lik_gated_bwd");
   if (l.dg)
     if (int rc = launch_gemm(l.dh, l.gemm, l.gemm_bytes, a.status, st)) return rc;
   for (const GemmDesc* d : {&l.dx, &l.dwg, &l.dwu, &l.dwd})
-    if (d->out)
+    if (d->out[0])
       if (int rc = launch_gemm(*d, l.gemm, l.gemm_bytes, a.status, st)) return rc;
   auto sums = [&](const void* g, long long stride, int n, void* out) {
     if (!out) return (int)LIK_OK;

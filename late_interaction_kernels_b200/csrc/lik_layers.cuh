@@ -43,8 +43,8 @@ __device__ __forceinline__ float act_value(float z) {
   if constexpr (ACT == LIK_ACT_GELU) {
     if constexpr (PRECISE) return 0.5f * z * erfcf(-0.70710678118654752f * z);
     float e;
-    const float tail = z * normal_tail(z, e);
-    return z < 0.0f ? tail : z - tail;
+    const float tail = normal_tail(z, e), zt = z * tail;
+    return z < 0.0f ? zt : z - zt;
   }
   if constexpr (ACT == LIK_ACT_GELU_TANH) return z * sigmoid_f<PRECISE>(GELU_C * fmaf(0.044715f * z * z, z, z));
   if constexpr (ACT == LIK_ACT_TANH) return tanh_f<PRECISE>(z);
@@ -68,11 +68,12 @@ __device__ __forceinline__ float act_slope(float z, float& value) {
     if constexpr (PRECISE) {
       cdf = 0.5f * erfcf(-0.70710678118654752f * z);
       e = expf(-0.5f * z * z);
+      value = z * cdf;
     } else {
-      const float tail = normal_tail(z, e);
+      const float tail = normal_tail(z, e), zt = z * tail;
       cdf = z < 0.0f ? tail : 1.0f - tail;
+      value = z < 0.0f ? zt : z - zt;  // (the bits of act_value)
     }
-    value = z * cdf;
     return fmaf(0.3989422804014327f * z, e, cdf);
   }
   if constexpr (ACT == LIK_ACT_GELU_TANH) {
@@ -183,9 +184,9 @@ inline bool vec_ok(const void* p, long long stride, int width, int item) {
 // A matrix product and what is done to its elements: c[m, n] = sum over segments and k of a(m, k) b(n, k)
 // ---------------------------------------------------------------------------------------------
 enum GemmKind {
-  GEMM_LINEAR = 0,     // out = act(c + bias) + residual; z = c + bias where it is asked for
-  GEMM_GATED = 1,      // two products of the same a: z = c0 + bias0, z2 = c1 + bias1, out = act(z) * z2
-  GEMM_GATED_BWD = 2,  // c = gradient of act(z) * z2: out = gradient of z, out2 = gradient of z2
+  GEMM_LINEAR = 0,     // z = c + bias, out = act(z) + residual; kept[0] = z where it is asked for
+  GEMM_GATED = 1,      // two products of the same a: g = c0 + bias0, u = c1 + bias1, out = act(g) u; kept = u act'(g), act(g)
+  GEMM_GATED_BWD = 2,  // c = gradient of act(g) u: out[i] = c kept[i], the gradients of g and u
 };
 struct GemmOperand {
   const void* p = nullptr;
@@ -201,16 +202,19 @@ struct GemmDesc {
   const void* bias[2] = {nullptr, nullptr};
   const void* residual = nullptr;
   long long residual_stride = 0;
-  void* out = nullptr;
+  void* out[2] = {nullptr, nullptr};
   long long out_stride = 0;
-  int out_dtype = 0;          // dtype, or LIK_F32 for products without anything else to them
-  void* out2 = nullptr;       // (with out_stride)
-  void* z = nullptr;          // written (GEMM_LINEAR, GEMM_GATED) or read (GEMM_GATED_BWD)
-  void* z2 = nullptr;
-  long long z_stride = 0;
+  int out_dtype = 0;                   // dtype, or LIK_F32 for products without anything else to them
+  void* kept[2] = {nullptr, nullptr};  // the factors of the backward: written, or read by GEMM_GATED_BWD; rows of 16 bytes
+  long long kept_stride = 0;
 };
-size_t gemm_workspace(const GemmDesc& d);
-int launch_gemm(const GemmDesc& d, void* ws, size_t ws_bytes, int* status, cudaStream_t st);
+// fp32 multiply-add (lik_gemm_simt.cu): any type, stride and size
+size_t gemm_simt_workspace(const GemmDesc& d);
+int launch_gemm_simt(const GemmDesc& d, void* ws, size_t ws_bytes, cudaStream_t st);
+// tensor cores (lik_gemm_tc.cu): 16-bit operands
+bool gemm_tc_supported(const GemmDesc& d);
+size_t gemm_tc_workspace(const GemmDesc& d);
+int launch_gemm_tc(const GemmDesc& d, void* ws, size_t ws_bytes, int* status, cudaStream_t st);
 
 // sum over `parts` of partial[part][i], i < n, as dtype: out[i], the second half (i >= split) to out2
 int launch_sum_parts(const float* partial, int parts, long long n, long long split, int dtype, void* out, void* out2, cudaStream_t st);

@@ -5,8 +5,8 @@ u = eps / 2 of the type (a rounding's largest relative error), e = 2^-24 (fp32) 
 
   product         n terms added in fp32 in any order, by an adder that may truncate:     2 n e S
   activation      fp32 functions within a few steps (fp32), 2^-16 of the value's scale (16-bit types, far below their u)
-  what is kept    z, gate, up and h in the type: u of each, carried through the activation's largest slope (1.13 for all of them) or
-                  curvature (at most 0.9)
+  what is kept    z, and of a gated block u act'(g), act(g) and h, in the type: u of each; an error of z goes through the
+                  activation's largest slope (1.13 for all of them) or curvature (at most 0.9)
 """
 
 import pytest
@@ -198,7 +198,7 @@ def check_linear(x, w, b, r, dy, act, y, grads, dt):
     u = unit(dt)
     dz = dy * slope64(z, act)
     # z is kept rounded; dz is rounded before the products
-    err = dy.abs() * (CURVE * (u * z.abs() + dz_err) + act_err(z, dt)) if act and act != "relu" else torch.zeros_like(dz)
+    err = dy.abs() * (CURVE * (u * (z.abs() + dz_err) + dz_err + floor(dt)) + act_err(z, dt)) if act and act != "relu" else torch.zeros_like(dz)
     if act == "relu":
         err = torch.where(z.abs() <= dz_err + floor(dt), dy.abs(), err)  # the kink: either side
     if act:
@@ -350,15 +350,16 @@ def gated_case(m, k, f, o, dt, act, bias, residual, wdt=None):
     d = dy.double()
     dh, dh_err = product(d, v["wd"].t())
     s = slope64(z, act)
-    z_kept, p_kept = z_err + u * z.abs() + floor(dt), p_err + u * p.abs() + floor(dt)  # the rounded values that the backward reads
-    s_err = CURVE * z_kept + act_err(z, dt) if act and act != "relu" else torch.zeros_like(z)
+    s_err = CURVE * z_err + act_err(z, dt) if act and act != "relu" else torch.zeros_like(z)
     if act == "relu":
-        s_err = torch.where(z.abs() <= z_err + floor(dt), torch.ones_like(z), s_err)
+        s_err = torch.where(z.abs() <= z_err, torch.ones_like(z), s_err)
     dg, du = dh * p * s, dh * a
-    dg_err = dh_err * (p.abs() + p_kept) * (s.abs() + s_err) + dh.abs() * (p_kept * (s.abs() + s_err) + p.abs() * s_err) + 3 * E * dg.abs()
+    fg, fu = (p * s).abs(), a.abs()  # the factors that are kept
+    fg_err = p_err * (s.abs() + s_err) + p.abs() * s_err + E * fg
+    fg_err, fu_err = fg_err + u * (fg + fg_err) + floor(dt), a_err + u * (fu + a_err) + floor(dt)
+    dg_err = dh_err * (fg + fg_err) + dh.abs() * fg_err + E * dg.abs()
+    du_err = dh_err * (fu + fu_err) + dh.abs() * fu_err + E * du.abs()
     dg_err = dg_err + u * (dg.abs() + dg_err) + floor(dt)
-    du_a = SLOPE * z_kept + (act_err(z, dt) if act else 0)
-    du_err = dh_err * (a.abs() + du_a) + dh.abs() * du_a + 2 * E * du.abs()
     du_err = du_err + u * (du.abs() + du_err) + floor(dt)
     dx1, e1 = product(dg, v["wg"].t())
     dx2, e2 = product(du, v["wu"].t())
