@@ -23,30 +23,35 @@ namespace {
 
 constexpr int GT_EPI_WARPS = 8, GT_PRODUCER = 8, GT_ISSUER = 9, GT_THREADS = 320;
 constexpr int GT_BK = 64, GT_BOX = 64, GT_BOX_BYTES = GT_BOX * GT_BK * 2;
-constexpr int GT_STAGE_BYTES = 4 * GT_BOX_BYTES, GT_STAGES = 5;
-constexpr int GT_SLOTS_BYTES = 8192;  // per epilogue warp: slots of 32 rows x 32 columns on their way out
+constexpr int GT_STAGE_BYTES = 4 * GT_BOX_BYTES, GT_MAX_STAGES = 5;
+// Shared memory: stages of the operands, and per epilogue warp slots of 32 rows x 32 columns on their way in and out.  Kernels whose
+// epilogue reads matrices give a stage for the slots of those.
+template <bool READS>
+struct GtShape {
+  static constexpr int STAGES = READS ? 4 : 5, SLOTS_BYTES = READS ? 12288 : 8192;
+  static constexpr size_t SLOTS_AT = (size_t)STAGES * GT_STAGE_BYTES, CTL_AT = SLOTS_AT + GT_EPI_WARPS * SLOTS_BYTES;
+};
 
 struct GtMaps {
-  CUtensorMap a[2], b[2], out[2], kept[2];
+  CUtensorMap a[2], b[2], out[2], kept[2], residual;
 };
 struct GtParams {
   int m, n, n_seg;
   int kb0, kb_total, kb_per, tiles, tiles_n, units;
-  bool a_mn, b_mn, bf16, bias_vec, residual_vec;
+  bool a_mn, b_mn, bf16, bias_vec, residual_tma;
   int act;
-  const void *bias[2], *residual, *kept[2];
-  long long residual_stride, kept_stride;
+  const void *bias[2], *residual;
+  long long residual_stride;
   bool keep;      // factors are written
   void* direct;   // not NULL: out is written by plain stores, rows of out_stride
   long long out_stride;
   int* status;
 };
 struct GtCtl {
-  unsigned long long full[GT_STAGES], empty[GT_STAGES], acc_full[2], acc_empty[2];
+  unsigned long long full[GT_MAX_STAGES], empty[GT_MAX_STAGES], acc_full[2], acc_empty[2], in_full[GT_EPI_WARPS][2];
   uint32_t tmem;
   WaitCtl wait;
 };
-constexpr size_t GT_SMEM = 1024 + (size_t)GT_STAGES * GT_STAGE_BYTES + GT_EPI_WARPS * GT_SLOTS_BYTES + sizeof(GtCtl);
 
 __device__ __forceinline__ uint32_t cta_rank() {
   uint32_t r;
@@ -73,6 +78,11 @@ __device__ __forceinline__ void gt_load(uint32_t dst, const CUtensorMap* map, in
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map),
                  "r"(x), "r"(y), "r"(bar)
                  : "memory");
+}
+__device__ __forceinline__ void gt_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map), "r"(x),
+               "r"(y), "r"(0), "r"(bar)
+               : "memory");
 }
 __device__ __forceinline__ void gt_store(const CUtensorMap* map, uint32_t src, int x, int y, int z) {
   asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map), "r"(src), "r"(x), "r"(y), "r"(z) : "memory");
@@ -127,73 +137,98 @@ __device__ __forceinline__ GtUnit gt_unit(const GtParams& p, int u) {
   return t;
 }
 
-// 32 consecutive elements, the first n of them there
-template <typename T>
-__device__ __forceinline__ void load_32(const T* p, int n, bool vec, float (&v)[32]) {
-  if (vec) {
-#pragma unroll
-    for (int i = 0; i < 32; i += 8) {
-      uint4 u = make_uint4(0u, 0u, 0u, 0u);
-      if (i < n) u = __ldg(reinterpret_cast<const uint4*>(p + i));
-      unpack2(u.x, v[i + 0], v[i + 1], T());
-      unpack2(u.y, v[i + 2], v[i + 3], T());
-      unpack2(u.z, v[i + 4], v[i + 5], T());
-      unpack2(u.w, v[i + 6], v[i + 7], T());
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = i < n ? to_f32(p[i]) : 0.0f;
-  }
+// 32 lanes x 16 columns of tensor memory; the registers may be read after tmem_wait16
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]),
+                 "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_wait16(float (&v)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]),
+                 "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])::"memory");
 }
 
-// The way out of an epilogue warp: slots of 32 rows x 32 columns, written by the lanes (a row each), read by TMA.
-template <typename O>
-struct GtOut {
-  static constexpr int ROW = 32 * (int)sizeof(O), BYTES = 32 * ROW, SLOTS = GT_SLOTS_BYTES / BYTES;
-  uint32_t base;
-  uint8_t* gen;
-  int at = 0;
-  // 16-byte piece c of row r: the 64-byte or 128-byte swizzle of the store's tensor map, which also keeps the lanes' stores apart
-  __device__ __forceinline__ static int offset(int r, int c) {
-    return ROW == 64 ? r * 64 + ((c ^ ((r >> 1) & 3)) << 4) : r * 128 + ((c ^ (r & 7)) << 4);
-  }
-  __device__ __forceinline__ void put(int lane, const float (&v)[32], const CUtensorMap* map, int x, int y, int z, const GtParams& p, O* direct) {
-    // (the slot's last store has been read out of it)
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(SLOTS - 1) : "memory");
-    __syncwarp();
-    uint8_t* s = gen + at * BYTES;
+// 16 consecutive elements, the first n of them there: fetched early, unpacked when they are wanted
+template <typename T>
+struct Raw16 {
+  uint4 u[2];
+  __device__ __forceinline__ void load(const T* p, int n, bool vec) {
+    if (vec) {
 #pragma unroll
-    for (int c = 0; c < ROW / 16; ++c) {
-      uint4 u;
-      if constexpr (sizeof(O) == 4)
-        u = make_uint4(__float_as_uint(v[4 * c]), __float_as_uint(v[4 * c + 1]), __float_as_uint(v[4 * c + 2]), __float_as_uint(v[4 * c + 3]));
-      else
-        u = make_uint4(pack2(v[8 * c], v[8 * c + 1], O()), pack2(v[8 * c + 2], v[8 * c + 3], O()), pack2(v[8 * c + 4], v[8 * c + 5], O()),
-                       pack2(v[8 * c + 6], v[8 * c + 7], O()));
-      *reinterpret_cast<uint4*>(s + offset(lane, c)) = u;
-    }
-    if (!direct) {
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) {
-        gt_store(map, base + at * BYTES, x, y, z);
-        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-      }
+      for (int i = 0; i < 2; ++i) u[i] = 8 * i < n ? __ldg(reinterpret_cast<const uint4*>(p) + i) : make_uint4(0u, 0u, 0u, 0u);
     } else {
-      __syncwarp();
-      constexpr int PER = 16 / (int)sizeof(O);
-      const int rows = min(32, p.m - y);
-      if (x + lane < p.n)
-        for (int r = 0; r < rows; ++r)
-          direct[(y + r) * p.out_stride + x + lane] = *reinterpret_cast<const O*>(s + offset(r, lane / PER) + (lane % PER) * sizeof(O));
-      __syncwarp();
+      const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
+      uint32_t w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = (2 * i < n ? (uint32_t)q[2 * i] : 0u) | (2 * i + 1 < n ? (uint32_t)q[2 * i + 1] << 16 : 0u);
+      u[0] = make_uint4(w[0], w[1], w[2], w[3]);
+      u[1] = make_uint4(w[4], w[5], w[6], w[7]);
     }
-    at = at + 1 == SLOTS ? 0 : at + 1;
+  }
+  __device__ __forceinline__ void add_to(float (&v)[16]) const {
+    float f[16];
+    get(f);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] += f[i];
+  }
+  __device__ __forceinline__ void get(float (&f)[16]) const {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      unpack2(u[i].x, f[8 * i + 0], f[8 * i + 1], T());
+      unpack2(u[i].y, f[8 * i + 2], f[8 * i + 3], T());
+      unpack2(u[i].z, f[8 * i + 4], f[8 * i + 5], T());
+      unpack2(u[i].w, f[8 * i + 6], f[8 * i + 7], T());
+    }
   }
 };
 
-template <int CG, int KIND, typename T, typename O>
+// 16-byte piece c of row r in a slot of 32 rows of ROW bytes: the 64-byte or 128-byte swizzle of the slot's tensor map, which also keeps
+// the lanes' accesses, a row each, apart
+template <int ROW>
+__device__ __forceinline__ int slot_offset(int r, int c) {
+  return ROW == 64 ? r * 64 + ((c ^ ((r >> 1) & 3)) << 4) : r * 128 + ((c ^ (r & 7)) << 4);
+}
+// columns [16 h, 16 h + 16) of the lane's row
+template <typename O>
+__device__ __forceinline__ void slot_put(uint8_t* s, int lane, int h, const float (&v)[16]) {
+  constexpr int ROW = 32 * (int)sizeof(O);
+  if constexpr (sizeof(O) == 4) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      *reinterpret_cast<float4*>(s + slot_offset<ROW>(lane, h * 4 + c)) = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+  } else {
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+      *reinterpret_cast<uint4*>(s + slot_offset<ROW>(lane, h * 2 + c)) =
+          make_uint4(pack2(v[8 * c], v[8 * c + 1], O()), pack2(v[8 * c + 2], v[8 * c + 3], O()), pack2(v[8 * c + 4], v[8 * c + 5], O()),
+                     pack2(v[8 * c + 6], v[8 * c + 7], O()));
+  }
+}
+template <typename T>
+__device__ __forceinline__ void slot_get(const uint8_t* s, int lane, int h, float (&f)[16]) {
+  Raw16<T> r;
+#pragma unroll
+  for (int c = 0; c < 2; ++c) r.u[c] = *reinterpret_cast<const uint4*>(s + slot_offset<64>(lane, h * 2 + c));
+  r.get(f);
+}
+
+// the chunks of a warp that have anything in them, in the order in which it comes to them
+template <int CG, int OUT_N>
+__device__ __forceinline__ bool gt_chunk(const GtParams& p, int u, int c, int rank, int quad, int half, int& col, int& row0) {
+  const GtUnit t = gt_unit(p, u);
+  row0 = t.tm * (128 * CG) + rank * 128 + quad * 32;
+  col = t.tn * OUT_N + half * (OUT_N / 2) + c * 32;
+  return row0 < p.m && col < p.n;
+}
+
+// RES: a residual that comes by TMA (GEMM_LINEAR)
+template <int CG, int KIND, bool RES, typename T, typename O>
 __global__ void __launch_bounds__(GT_THREADS, 1) gemm_tc_kernel(const __grid_constant__ GtMaps maps, const __grid_constant__ GtParams p) {
+  using Shape = GtShape<RES || KIND == GEMM_GATED_BWD>;
+  constexpr int STAGES = Shape::STAGES;
   constexpr bool DUAL = KIND == GEMM_GATED;
   constexpr int BN = CG == 2 ? 256 : 128;          // columns of an accumulator
   constexpr int OUT_N = DUAL ? BN / 2 : BN;        // columns of the result in a unit
@@ -201,17 +236,18 @@ __global__ void __launch_bounds__(GT_THREADS, 1) gemm_tc_kernel(const __grid_con
   extern __shared__ uint8_t raw[];
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
   uint8_t* gen = raw + (base - smem_u32(raw));
-  GtCtl* ctl = reinterpret_cast<GtCtl*>(gen + GT_STAGES * GT_STAGE_BYTES + GT_EPI_WARPS * GT_SLOTS_BYTES);
+  GtCtl* ctl = reinterpret_cast<GtCtl*>(gen + Shape::CTL_AT);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = CG == 2 ? (int)cta_rank() : 0;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < GT_STAGES; ++s) {
+    for (int s = 0; s < STAGES; ++s) {
       mbar_init(smem_u32(&ctl->full[s]), 1);
       mbar_init(smem_u32(&ctl->empty[s]), 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(smem_u32(&ctl->acc_full[b]), 1);
       mbar_init(smem_u32(&ctl->acc_empty[b]), CG * GT_EPI_WARPS);
+      for (int w = 0; w < GT_EPI_WARPS; ++w) mbar_init(smem_u32(&ctl->in_full[w][b]), 1);
     }
     ctl->wait.init();
     fence_barrier_init();
@@ -257,19 +293,19 @@ __global__ void __launch_bounds__(GT_THREADS, 1) gemm_tc_kernel(const __grid_con
         }
         __syncwarp();
         ++issued;
-        if (++s == GT_STAGES) s = 0, phase ^= 1;
+        if (++s == STAGES) s = 0, phase ^= 1;
       }
     }
     // the last stages' releases arrive here, perhaps from the other CTA: not after this one is gone
-    for (int i = 0; i < GT_STAGES && i < issued && ok; ++i) {
+    for (int i = 0; i < STAGES && i < issued && ok; ++i) {
       const int back = issued - 1 - i;
-      ok = wait_bar_all(&ctl->empty[back % GT_STAGES], (back / GT_STAGES) & 1, &ctl->wait, p.status);
+      ok = wait_bar_all(&ctl->empty[back % STAGES], (back / STAGES) & 1, &ctl->wait, p.status);
     }
     if (!ok && rank == 0) {  // copies in flight land before the shared memory goes away
       const long long t0 = clock64();
-      for (int i = 0; i < GT_STAGES && i < issued; ++i) {
+      for (int i = 0; i < STAGES && i < issued; ++i) {
         const int back = issued - 1 - i;
-        while (!mbar_try_wait(smem_u32(&ctl->full[back % GT_STAGES]), (back / GT_STAGES) & 1) && clock64() - t0 < ctl->wait.limit) {
+        while (!mbar_try_wait(smem_u32(&ctl->full[back % STAGES]), (back / STAGES) & 1) && clock64() - t0 < ctl->wait.limit) {
         }
       }
     }
@@ -304,17 +340,47 @@ __global__ void __launch_bounds__(GT_THREADS, 1) gemm_tc_kernel(const __grid_con
             if (kb + 1 == t.kb_hi) gt_commit<CG>(smem_u32(&ctl->acc_full[buf]));
           }
           __syncwarp();
-          if (++s == GT_STAGES) s = 0, phase ^= 1;
+          if (++s == STAGES) s = 0, phase ^= 1;
         }
       }
     }
   } else {
     const int quad = warp & 3, half = warp >> 2;
-    GtOut<O> out;
-    out.base = base + GT_STAGES * GT_STAGE_BYTES + warp * GT_SLOTS_BYTES;
-    out.gen = gen + GT_STAGES * GT_STAGE_BYTES + warp * GT_SLOTS_BYTES;
+    // What a chunk of 32 rows x 32 columns is added to or multiplied with comes by TMA, two chunks ahead, and what becomes of it leaves by
+    // TMA: IN matrices in and OUT matrices out, a slot each.
+    constexpr int IN = KIND == GEMM_GATED_BWD ? 2 : (RES ? 1 : 0);
+    constexpr int OUT = KIND == GEMM_GATED ? 3 : (KIND == GEMM_GATED_BWD || std::is_same<T, O>::value ? 2 : 1);
+    constexpr int SLOT = 32 * 32 * (int)sizeof(O), OUT_SETS = (Shape::SLOTS_BYTES - 2 * IN * SLOT) / (OUT * SLOT);
+    static_assert(OUT_SETS >= 1, "room for a chunk's results");
+    const uint32_t in_base = base + STAGES * GT_STAGE_BYTES + warp * Shape::SLOTS_BYTES, out_base = in_base + 2 * IN * SLOT;
+    uint8_t* const in_gen = gen + (in_base - base);
+    uint8_t* const out_gen = gen + (out_base - base);
+    int in_unit = IN ? first : p.units, in_chunk = 0, issued = 0, taken = 0, set = 0;
+    // fetches for the next chunk that has anything in it, into the slots that were emptied last
+    auto fetch = [&] {
+      int col = 0, row0 = 0;
+      bool there = false;
+      while (in_unit < p.units && !there) {
+        there = gt_chunk<CG, OUT_N>(p, in_unit, in_chunk, rank, quad, half, col, row0);
+        if (++in_chunk == CHUNKS) in_chunk = 0, in_unit += step;
+      }
+      if (!there) return;
+      const int slot = issued & 1;
+      if (lane == 0) {
+        const uint32_t bar = smem_u32(&ctl->in_full[warp][slot]);
+        mbar_arrive_expect_tx(bar, IN * SLOT);
+#pragma unroll
+        for (int q = 0; q < IN; ++q) gt_load_3d(in_base + (slot * IN + q) * SLOT, KIND == GEMM_GATED_BWD ? &maps.kept[q] : &maps.residual, col, row0, bar);
+      }
+      ++issued;
+    };
+    if constexpr (IN > 0) {
+      fetch();
+      fetch();
+    }
+    bool ok = true;
     int it = 0;
-    for (int u = first; u < p.units; u += step, ++it) {
+    for (int u = first; u < p.units && ok; u += step, ++it) {
       const GtUnit t = gt_unit(p, u);
       const int buf = it & 1;
       if (!wait_bar_all(&ctl->acc_full[buf], (it >> 1) & 1, &ctl->wait, p.status)) break;
@@ -326,75 +392,115 @@ __global__ void __launch_bounds__(GT_THREADS, 1) gemm_tc_kernel(const __grid_con
       for (int c = 0; c < CHUNKS; ++c) {
         const int in_tile = half * (OUT_N / 2) + c * 32, col = t.tn * OUT_N + in_tile, left = p.n - col;
         const bool live = row0 < p.m && left > 0;
-        float v[32], w[32];
-        if (live) {
-          tmem_ld32_issue(acc + in_tile, v);
-          if constexpr (DUAL) tmem_ld32_issue(acc + BN / 2 + in_tile, w);
-          tmem_ld_wait(v);
-          if constexpr (DUAL) tmem_ld_wait(w);
+        if (!live) {
+          if (c + 1 == CHUNKS) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) CG == 2 ? arrive_remote(release) : mbar_arrive(release);
+          }
+          continue;
         }
-        if (c + 1 == CHUNKS) {
-          tc_fence_before();
+        uint8_t* const to = out_gen + set * OUT * SLOT;
+        const uint8_t* from = in_gen + (taken & 1) * IN * SLOT;
+        if (IN > 0 && !(ok = wait_bar_all(&ctl->in_full[warp][taken & 1], (taken >> 1) & 1, &ctl->wait, p.status))) break;
+        // (the slots' last stores have been read out of them)
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(OUT_SETS - 1) : "memory");
+        __syncwarp();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float v[16], w[16];
+          Raw16<T> bias[2], res;
+          tmem_ld16(acc + in_tile + 16 * h, v);
+          if constexpr (DUAL) tmem_ld16(acc + BN / 2 + in_tile + 16 * h, w);
+          if constexpr (KIND != GEMM_GATED_BWD) {
+            if (p.bias[0]) bias[0].load((const T*)p.bias[0] + col + 16 * h, left - 16 * h, p.bias_vec);
+            if (DUAL && p.bias[1]) bias[1].load((const T*)p.bias[1] + col + 16 * h, left - 16 * h, p.bias_vec);
+            if (!DUAL && !RES && p.residual)  // rows that TMA cannot address
+              res.load((const T*)p.residual + (row < p.m ? row * p.residual_stride + col + 16 * h : 0), row < p.m ? left - 16 * h : 0, false);
+          }
+          tmem_wait16(v);
+          if constexpr (DUAL) tmem_wait16(w);
+          if (h == 1 && c + 1 == CHUNKS) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) CG == 2 ? arrive_remote(release) : mbar_arrive(release);
+          }
+          if constexpr (KIND == GEMM_GATED_BWD) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              float f[16];
+              slot_get<T>(from + q * SLOT, lane, h, f);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) f[i] *= v[i];
+              slot_put<O>(to + q * SLOT, lane, h, f);
+            }
+          } else {
+            if (p.bias[0]) bias[0].add_to(v);
+            if constexpr (DUAL) {
+              if (p.bias[1]) bias[1].add_to(w);
+            }
+            if constexpr (std::is_same<T, O>::value) {
+              if (DUAL && p.keep) {
+                float f[16];
+                with_activation_dev(p.act, [&](auto act) {
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) f[i] = w[i] * act_slope<decltype(act)::value, false>(v[i], v[i]);
+                });
+                slot_put<O>(to + SLOT, lane, h, f);
+                slot_put<O>(to + (OUT - 1) * SLOT, lane, h, v);
+              } else if (p.act != LIK_ACT_NONE) {
+                if (!DUAL && p.keep) slot_put<O>(to + (OUT - 1) * SLOT, lane, h, v);
+                with_activation_dev(p.act, [&](auto act) {
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) v[i] = act_value<decltype(act)::value, false>(v[i]);
+                });
+              }
+            }
+            if constexpr (DUAL) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) v[i] *= w[i];
+            } else if constexpr (RES) {
+              float f[16];
+              slot_get<T>(from, lane, h, f);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) v[i] += f[i];
+            } else if (p.residual) {
+              res.add_to(v);
+            }
+            slot_put<O>(to, lane, h, v);
+          }
+        }
+        if constexpr (IN > 0) ++taken;
+        fence_proxy_async();
+        __syncwarp();
+        if constexpr (IN > 0) fetch();
+        if (lane == 0) {
+          const uint32_t src = out_base + set * OUT * SLOT;
+          if (KIND == GEMM_GATED_BWD || !p.direct) gt_store(&maps.out[0], src, col, row0, t.split);
+          if (KIND == GEMM_GATED_BWD) gt_store(&maps.out[1], src + SLOT, col, row0, 0);
+          if (KIND != GEMM_GATED_BWD && OUT > 1 && p.keep) {
+            gt_store(&maps.kept[0], src + SLOT, col, row0, 0);
+            if (DUAL) gt_store(&maps.kept[1], src + (OUT - 1) * SLOT, col, row0, 0);
+          }
+          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
+        if (KIND == GEMM_LINEAR && p.direct) {
+          constexpr int PIECE = 16 / (int)sizeof(O);
+          const int rows = min(32, p.m - row0);
+          if (lane < left)
+            for (int r = 0; r < rows; ++r)
+              ((O*)p.direct)[(row0 + r) * p.out_stride + col + lane] =
+                  *reinterpret_cast<const O*>(to + slot_offset<32 * (int)sizeof(O)>(r, lane / PIECE) + (lane % PIECE) * sizeof(O));
           __syncwarp();
-          if (lane == 0) CG == 2 ? arrive_remote(release) : mbar_arrive(release);
         }
-        if (!live) continue;
-        if constexpr (KIND == GEMM_GATED_BWD) {
-          float f[32];
-          const bool there = row < p.m;
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            load_32((const T*)p.kept[q] + (there ? row * p.kept_stride + col : 0), there ? left : 0, true, f);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) f[i] *= v[i];
-            out.put(lane, f, &maps.out[q], col, row0, 0, p, nullptr);
-          }
-        } else {
-          if (p.bias[0]) {
-            float b[32];
-            load_32((const T*)p.bias[0] + col, left, p.bias_vec, b);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] += b[i];
-          }
-          if constexpr (DUAL) {
-            if (p.bias[1]) {
-              float b[32];
-              load_32((const T*)p.bias[1] + col, left, p.bias_vec, b);
-#pragma unroll
-              for (int i = 0; i < 32; ++i) w[i] += b[i];
-            }
-          }
-          if constexpr (std::is_same<T, O>::value) {
-            if (DUAL && p.keep) {
-              float f[32];
-              with_activation_dev(p.act, [&](auto act) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) f[i] = w[i] * act_slope<decltype(act)::value, false>(v[i], v[i]);
-              });
-              out.put(lane, f, &maps.kept[0], col, row0, 0, p, nullptr);
-              out.put(lane, v, &maps.kept[1], col, row0, 0, p, nullptr);
-            } else if (p.act != LIK_ACT_NONE) {
-              if (!DUAL && p.keep) out.put(lane, v, &maps.kept[0], col, row0, 0, p, nullptr);
-              with_activation_dev(p.act, [&](auto act) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = act_value<decltype(act)::value, false>(v[i]);
-              });
-            }
-          }
-          if constexpr (DUAL) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] *= w[i];
-          } else if (p.residual) {
-            float r[32];
-            const bool there = row < p.m;
-            load_32((const T*)p.residual + (there ? row * p.residual_stride + col : 0), there ? left : 0, p.residual_vec, r);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] += r[i];
-          }
-          out.put(lane, v, &maps.out[0], col, row0, t.split, p, (O*)p.direct);
-        }
+        set = set + 1 == OUT_SETS ? 0 : set + 1;
       }
     }
+    // (after an expired wait: what was fetched and not taken lands before the shared memory goes away)
+    const long long t0 = clock64();
+    for (; taken < issued; ++taken)
+      while (!mbar_try_wait(smem_u32(&ctl->in_full[warp][taken & 1]), (taken >> 1) & 1) && clock64() - t0 < ctl->wait.limit) {
+      }
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   __syncwarp();
@@ -451,7 +557,7 @@ EncodeFn encode_fn() {
   }();
   return fn;
 }
-// [splits][rows][cols] for stores of 32 x 32
+// [splits][rows][cols] in pieces of 32 x 32, for the way in or out
 int store_map(CUtensorMap* map, void* p, int dtype, long long cols, long long rows, long long splits, long long stride) {
   const long long item = (long long)dtype_size(dtype);
   const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)splits};
@@ -527,14 +633,14 @@ GtPlan gt_plan(const GemmDesc& d) {
   return pl;
 }
 
-template <int CG, int KIND, typename T, typename O>
+template <int CG, int KIND, bool RES, typename T, typename O>
 int run_tc(const GtMaps& maps, const GtParams& p, cudaStream_t st) {
-  LIK_CUDA_OK((allow_smem<gemm_tc_kernel<CG, KIND, T, O>>()));
+  LIK_CUDA_OK((allow_smem<gemm_tc_kernel<CG, KIND, RES, T, O>>()));
   const int slots = sm_count() / CG;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)((p.units < slots ? p.units : slots) * CG));
   cfg.blockDim = dim3(GT_THREADS);
-  cfg.dynamicSmemBytes = GT_SMEM;
+  cfg.dynamicSmemBytes = 1024 + GtShape<RES || KIND == GEMM_GATED_BWD>::CTL_AT + sizeof(GtCtl);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -542,19 +648,20 @@ int run_tc(const GtMaps& maps, const GtParams& p, cudaStream_t st) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  LIK_CUDA_OK(cudaLaunchKernelEx(&cfg, gemm_tc_kernel<CG, KIND, T, O>, maps, p));
+  LIK_CUDA_OK(cudaLaunchKernelEx(&cfg, gemm_tc_kernel<CG, KIND, RES, T, O>, maps, p));
   count_launch();
   return LIK_OK;
 }
-template <int KIND, typename T, typename O>
+template <int KIND, bool RES, typename T, typename O>
 int run_tc(int cg, const GtMaps& maps, const GtParams& p, cudaStream_t st) {
-  return cg == 2 ? run_tc<2, KIND, T, O>(maps, p, st) : run_tc<1, KIND, T, O>(maps, p, st);
+  return cg == 2 ? run_tc<2, KIND, RES, T, O>(maps, p, st) : run_tc<1, KIND, RES, T, O>(maps, p, st);
 }
 template <typename T>
 int run_tc(int kind, bool f32_out, int cg, const GtMaps& maps, const GtParams& p, cudaStream_t st) {
-  if (kind == GEMM_GATED) return run_tc<GEMM_GATED, T, T>(cg, maps, p, st);
-  if (kind == GEMM_GATED_BWD) return run_tc<GEMM_GATED_BWD, T, T>(cg, maps, p, st);
-  return f32_out ? run_tc<GEMM_LINEAR, T, float>(cg, maps, p, st) : run_tc<GEMM_LINEAR, T, T>(cg, maps, p, st);
+  if (kind == GEMM_GATED) return run_tc<GEMM_GATED, false, T, T>(cg, maps, p, st);
+  if (kind == GEMM_GATED_BWD) return run_tc<GEMM_GATED_BWD, false, T, T>(cg, maps, p, st);
+  if (f32_out) return run_tc<GEMM_LINEAR, false, T, float>(cg, maps, p, st);
+  return p.residual_tma ? run_tc<GEMM_LINEAR, true, T, T>(cg, maps, p, st) : run_tc<GEMM_LINEAR, false, T, T>(cg, maps, p, st);
 }
 
 }  // namespace
@@ -611,7 +718,7 @@ int launch_gemm_tc(const GemmDesc& d, void* ws, size_t ws_bytes, int* status, cu
     }
   }
   p.keep = d.kind != GEMM_GATED_BWD && d.kept[0];
-  for (int i = 0; p.keep && i < (dual ? 2 : 1); ++i)
+  for (int i = 0; d.kept[0] && i < (d.kind == GEMM_LINEAR ? 1 : 2); ++i)
     if (int rc = store_map(&maps.kept[i], d.kept[i], d.dtype, d.n, d.m, 1, d.kept_stride)) return rc;
   p.m = (int)d.m;
   p.n = d.n;
@@ -627,13 +734,13 @@ int launch_gemm_tc(const GemmDesc& d, void* ws, size_t ws_bytes, int* status, cu
   p.bias_vec = d.n % 8 == 0;
   for (int i = 0; i < 2; ++i) {
     p.bias[i] = d.bias[i];
-    p.kept[i] = d.kept[i];
     if (d.bias[i] && ((uintptr_t)d.bias[i] & 15)) p.bias_vec = false;
   }
   p.residual = d.residual;
   p.residual_stride = d.residual_stride;
-  p.residual_vec = vec_ok(d.residual, d.residual_stride, d.n, 2);
-  p.kept_stride = d.kept_stride;
+  p.residual_tma = d.residual && tma_out(d.residual, d.residual_stride, d.dtype);
+  if (p.residual_tma)
+    if (int rc = store_map(&maps.residual, const_cast<void*>(d.residual), d.dtype, d.n, d.m, 1, d.residual_stride)) return rc;
   p.out_stride = d.out_stride;
   p.status = status;
   int rc = d.dtype == LIK_F16 ? run_tc<__half>(d.kind, f32_out, pl.cg, maps, p, st) : run_tc<__nv_bfloat16>(d.kind, f32_out, pl.cg, maps, p, st);

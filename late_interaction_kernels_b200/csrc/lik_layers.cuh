@@ -10,9 +10,20 @@ namespace lik {
 // Activations.  PRECISE (fp32 operands): CUDA's own functions.  Otherwise what is stored has 11 or 8 bits, and the two
 // hardware approximations (2^x and the reciprocal, each good to 2^-22) are enough.
 // ---------------------------------------------------------------------------------------------
+// (the two instructions themselves, without the rescaling that keeps results below 2^-126)
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float fast_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 template <bool PRECISE>
 __device__ __forceinline__ float sigmoid_f(float z) {
-  return PRECISE ? 1.0f / (1.0f + expf(-z)) : __fdividef(1.0f, 1.0f + __expf(-z));
+  return PRECISE ? 1.0f / (1.0f + expf(-z)) : fast_rcp(1.0f + fast_exp2(-1.4426950408889634f * z));
 }
 template <bool PRECISE>
 __device__ __forceinline__ float tanh_f(float z) {
@@ -25,8 +36,8 @@ __device__ __forceinline__ float tanh_f(float z) {
 // exp(z^2 / 2) Phi(-|z|) is a smooth function on (0, 1]; six coefficients (least squares, reweighted towards the largest relative
 // error; our own fit) give it to 8.5e-6 relative for all |z| <= 14, a fiftieth of half a step of fp16.
 __device__ __forceinline__ float normal_tail(float z, float& e) {
-  const float a = fabsf(z), t = __fdividef(1.0f, fmaf(0.3f, a, 1.0f));
-  e = exp2f(-0.72134752f * z * z);
+  const float a = fabsf(z), t = fast_rcp(fmaf(0.3f, a, 1.0f));
+  e = fast_exp2(-0.72134752f * z * z);
   float r = fmaf(-0.0770966218f, t, 0.216034401f);
   r = fmaf(r, t, -0.0169447843f);
   r = fmaf(r, t, 0.144194491f);
@@ -43,8 +54,8 @@ __device__ __forceinline__ float act_value(float z) {
   if constexpr (ACT == LIK_ACT_GELU) {
     if constexpr (PRECISE) return 0.5f * z * erfcf(-0.70710678118654752f * z);
     float e;
-    const float tail = normal_tail(z, e), zt = z * tail;
-    return z < 0.0f ? zt : z - zt;
+    const float tail = normal_tail(z, e);
+    return fmaf(-fabsf(z), tail, fmaxf(z, 0.0f));  // z - z tail above 0, z tail below
   }
   if constexpr (ACT == LIK_ACT_GELU_TANH) return z * sigmoid_f<PRECISE>(GELU_C * fmaf(0.044715f * z * z, z, z));
   if constexpr (ACT == LIK_ACT_TANH) return tanh_f<PRECISE>(z);
@@ -70,9 +81,9 @@ __device__ __forceinline__ float act_slope(float z, float& value) {
       e = expf(-0.5f * z * z);
       value = z * cdf;
     } else {
-      const float tail = normal_tail(z, e), zt = z * tail;
+      const float tail = normal_tail(z, e);
       cdf = z < 0.0f ? tail : 1.0f - tail;
-      value = z < 0.0f ? zt : z - zt;  // (the bits of act_value)
+      value = fmaf(-fabsf(z), tail, fmaxf(z, 0.0f));
     }
     return fmaf(0.3989422804014327f * z, e, cdf);
   }
