@@ -1,0 +1,425 @@
+// Matrix products of fp32 operands on the tensor cores: c[m, n] = sum over k of a(m, k) b(n, k), with what the layers do to c.
+//
+// A value is cut into three bf16 parts, a = a0 + a1 + a2 to 2^-26 of itself, in a pass over the operand, and of the nine products of
+// parts the six largest are taken (what is left out is at most 2^-25 of |a b|).  The tensor core adds into fp32 but cuts the sum off
+// instead of rounding it, a shift of some 0.3 last places towards zero per 16 products; so a0 b0 and the five small products have
+// an accumulator each - cutting off the small one's sums is 2^-8 as bad - and after 128 k both are added to sums in registers, which are
+// rounded.  What remains is below 2e-7 of a sum of 768 Gaussian products, less than fp32 multiply-adds in a row leave.
+// An operand that is infinite gives NaN or infinities, as inf * 0 is among its products of parts.
+//
+// Roles as in the 16-bit kernel: a persistent CTA per SM, tiles of 128 x 128; a stage is 64 k of three parts of either operand (96 KB,
+// 24 MMAs), and there are two.  Bound by shared memory, which the MMAs read at 128 bytes per cycle while TMA writes half as much.
+#include "lik_gemm.cuh"
+
+namespace lik {
+namespace {
+
+constexpr int GF_EPI = 8, GF_PRODUCER = 8, GF_ISSUER = 9, GF_THREADS = 320;
+constexpr int GF_PARTS = 3, GF_STAGES = 2, GF_OPERAND = 2 * GT_BOX_BYTES, GF_STAGE_BYTES = 2 * GF_PARTS * GF_OPERAND;
+constexpr int GF_BN = 128, GF_DRAIN = 2;  // slabs of 64 k between two visits to the accumulators
+constexpr int GF_SLOT = 32 * 32 * 4;
+constexpr size_t GF_CTL_AT = (size_t)GF_STAGES * GF_STAGE_BYTES + GF_EPI * GF_SLOT;
+
+struct GfMaps {
+  CUtensorMap a[2][GF_PARTS], b[2][GF_PARTS];
+};
+struct GfParams {
+  int m, n;
+  int kb0, kb_total, kb_per, tiles, tiles_n, units;
+  bool a_mn, b_mn;
+  int act;
+  const float *bias[2], *residual;
+  float *out[2], *kept[2];
+  long long residual_stride, out_stride, kept_stride, split_stride;
+  bool residual_vec, out_vec, keep;
+  int* status;
+};
+struct GfCtl {
+  unsigned long long full[GF_STAGES], empty[GF_STAGES], acc_full[2], acc_empty[2];
+  uint32_t tmem;
+  WaitCtl wait;
+};
+
+template <int KIND>
+__global__ void __launch_bounds__(GF_THREADS, 1) gemm_f32_kernel(const __grid_constant__ GfMaps maps, const __grid_constant__ GfParams p) {
+  constexpr bool DUAL = KIND == GEMM_GATED;
+  constexpr int OUT_N = DUAL ? GF_BN / 2 : GF_BN;
+  extern __shared__ uint8_t raw[];
+  const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+  uint8_t* gen = raw + (base - smem_u32(raw));
+  GfCtl* ctl = reinterpret_cast<GfCtl*>(gen + GF_CTL_AT);
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < GF_STAGES; ++s) {
+      mbar_init(smem_u32(&ctl->full[s]), 1);
+      mbar_init(smem_u32(&ctl->empty[s]), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(smem_u32(&ctl->acc_full[b]), 1);
+      mbar_init(smem_u32(&ctl->acc_empty[b]), GF_EPI);
+    }
+    ctl->wait.init();
+    fence_barrier_init();
+  }
+  __syncthreads();
+  if (warp == GF_ISSUER) {
+    tmem_alloc(smem_u32(&ctl->tmem), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ctl->tmem;  // accumulator pair b: a0 b0 in columns [256 b, 256 b + 128), the small products behind
+
+  if (warp == GF_PRODUCER) {
+    int s = 0, issued = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int u = blockIdx.x; u < p.units && ok; u += gridDim.x) {
+      const int split = u / p.tiles, i = u - split * p.tiles, tm = i / p.tiles_n, tn = i - tm * p.tiles_n;
+      const int kb_lo = split * p.kb_per, kb_hi = min(kb_lo + p.kb_per, p.kb_total);
+      for (int kb = kb_lo; kb < kb_hi; ++kb) {
+        if (!wait_bar_all(&ctl->empty[s], phase ^ 1, &ctl->wait, p.status)) {
+          ok = false;
+          break;
+        }
+        const int seg = kb < p.kb0 ? 0 : 1, k = (kb - (seg ? p.kb0 : 0)) * GT_BK;
+        if (elect_one()) {
+          const uint32_t bar = smem_u32(&ctl->full[s]);
+          mbar_arrive_expect_tx(bar, GF_STAGE_BYTES);
+          const uint32_t dst = base + s * GF_STAGE_BYTES;
+#pragma unroll
+          for (int q = 0; q < GF_PARTS; ++q)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int ra = tm * 128 + h * GT_BOX, rb = tn * OUT_N + (DUAL ? 0 : h * GT_BOX);
+              tma_load_2d(dst + q * GF_OPERAND + h * GT_BOX_BYTES, &maps.a[seg][q], p.a_mn ? ra : k, p.a_mn ? k : ra, bar);
+              tma_load_2d(dst + (GF_PARTS + q) * GF_OPERAND + h * GT_BOX_BYTES, &maps.b[DUAL ? h : seg][q], p.b_mn ? rb : k, p.b_mn ? k : rb, bar);
+            }
+        }
+        __syncwarp();
+        ++issued;
+        if (++s == GF_STAGES) s = 0, phase ^= 1;
+      }
+    }
+    // the last stages' releases arrive here: not after this CTA is gone
+    for (int i = 0; i < GF_STAGES && i < issued && ok; ++i) {
+      const int back = issued - 1 - i;
+      ok = wait_bar_all(&ctl->empty[back % GF_STAGES], (back / GF_STAGES) & 1, &ctl->wait, p.status);
+    }
+    if (!ok) {  // copies in flight land before the shared memory goes away
+      const long long t0 = clock64();
+      for (int i = 0; i < GF_STAGES && i < issued; ++i) {
+        const int back = issued - 1 - i;
+        while (!mbar_try_wait(smem_u32(&ctl->full[back % GF_STAGES]), (back / GF_STAGES) & 1) && clock64() - t0 < ctl->wait.limit) {
+        }
+      }
+    }
+  } else if (warp == GF_ISSUER) {
+    int s = 0, it = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    const uint32_t hi = (uint32_t)(smem_desc_sw128(0) >> 32);
+    const uint32_t a_lbo = (p.a_mn ? GT_BOX_BYTES >> 4 : 1) << 16, b_lbo = (p.b_mn ? GT_BOX_BYTES >> 4 : 1) << 16;
+    const uint32_t a_step = p.a_mn ? 128 : 2, b_step = p.b_mn ? 128 : 2;
+    const uint32_t idesc = instr_desc(1, GF_BN) | ((p.a_mn ? 1u : 0u) << 15) | ((p.b_mn ? 1u : 0u) << 16);
+    for (int u = blockIdx.x; u < p.units && ok; u += gridDim.x) {
+      const int split = u / p.tiles, kb_lo = split * p.kb_per, kb_hi = min(kb_lo + p.kb_per, p.kb_total);
+      for (int kb = kb_lo; kb < kb_hi && ok; ++it) {
+        const int buf = it & 1, end = min(kb + GF_DRAIN, kb_hi);
+        if (!(ok = wait_bar_all(&ctl->acc_empty[buf], ((it >> 1) & 1) ^ 1, &ctl->wait, p.status))) break;
+        tc_fence_after();
+        for (int first = kb; kb < end; ++kb) {
+          if (!(ok = wait_bar_all(&ctl->full[s], phase, &ctl->wait, p.status))) break;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint32_t at = ((base + s * GF_STAGE_BYTES) & 0x3FFFFu) >> 4;
+            const uint32_t a = at | a_lbo, b = (at + (GF_PARTS * GF_OPERAND >> 4)) | b_lbo;
+            constexpr uint32_t PART = GF_OPERAND >> 4;
+            const uint32_t big = tmem + buf * 256, small = big + 128;
+            // (products of parts, the sums of the same accumulator apart from one another)
+            constexpr int PA[6] = {0, 2, 1, 0, 1, 0}, PB[6] = {0, 0, 1, 2, 0, 1};
+#pragma unroll
+            for (int k = 0; k < GT_BK / 16; ++k)
+#pragma unroll
+              for (int q = 0; q < 6; ++q)
+                tc_mma<false>(q ? small : big, a + PA[q] * PART + k * a_step, b + PB[q] * PART + k * b_step, hi, idesc, kb > first || k > 0 || q > 1);
+            tc_commit(smem_u32(&ctl->empty[s]));
+            if (kb + 1 == end) tc_commit(smem_u32(&ctl->acc_full[buf]));
+          }
+          __syncwarp();
+          if (++s == GF_STAGES) s = 0, phase ^= 1;
+        }
+      }
+    }
+  } else {
+    const int quad = warp & 3, part = warp >> 2;
+    uint8_t* const slot = gen + GF_STAGES * GF_STAGE_BYTES + warp * GF_SLOT;
+    int it = 0;
+    bool ok = true;
+    for (int u = blockIdx.x; u < p.units && ok; u += gridDim.x) {
+      const int split = u / p.tiles, i = u - split * p.tiles, tm = i / p.tiles_n, tn = i - tm * p.tiles_n;
+      const int kb_lo = split * p.kb_per, kb_hi = min(kb_lo + p.kb_per, p.kb_total);
+      // the warp's 64 columns: two chunks of 32, of the result or (DUAL) one of the gate and the same one of up
+      float sum[2][2][16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) sum[0][0][j] = sum[0][1][j] = sum[1][0][j] = sum[1][1][j] = 0.0f;
+      for (int kb = kb_lo; kb < kb_hi; kb += GF_DRAIN, ++it) {
+        const int buf = it & 1;
+        if (!(ok = wait_bar_all(&ctl->acc_full[buf], (it >> 1) & 1, &ctl->wait, p.status))) break;
+        tc_fence_after();
+        const uint32_t acc = tmem + buf * 256 + ((uint32_t)(quad * 32) << 16);
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int col = DUAL ? c * 64 + part * 32 + h * 16 : part * 64 + c * 32 + h * 16;
+            float big[16], small[16];
+            tmem_ld16(acc + col, big);
+            tmem_ld16(acc + 128 + col, small);
+            tmem_wait16(big);
+            tmem_wait16(small);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) sum[c][h][j] += big[j] + small[j];
+          }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&ctl->acc_empty[buf]));
+      }
+      if (!ok) break;
+      const int row0 = tm * 128 + quad * 32, rows = p.m - row0;
+      if (rows <= 0) continue;
+      // 32 x 32 of a matrix between memory and the lanes' rows, by way of the slot
+      auto in = [&](const float* src, long long stride, int cols, bool vec, float (&f)[2][16]) {
+        slot_fetch<float>(slot, lane, src, stride, rows, cols, vec);
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncwarp();
+        slot_get<float>(slot, lane, 0, f[0]);
+        slot_get<float>(slot, lane, 1, f[1]);
+        __syncwarp();
+      };
+      auto out = [&](float* dst, long long stride, int cols, bool vec, const float (&f)[2][16]) {
+        slot_put<float>(slot, lane, 0, f[0]);
+        slot_put<float>(slot, lane, 1, f[1]);
+        __syncwarp();
+        slot_store<float>(slot, lane, dst, stride, rows, cols, vec);
+        __syncwarp();
+      };
+#pragma unroll
+      for (int c = 0; c < (DUAL ? 1 : 2); ++c) {
+        const int col = tn * OUT_N + (DUAL ? part * 32 : part * 64 + c * 32), left = p.n - col;
+        if (left <= 0) continue;
+        float* const to = p.out[0] + split * p.split_stride + row0 * p.out_stride + col;
+        float* const keep0 = p.kept[0] + row0 * p.kept_stride + col;
+        float* const keep1 = p.kept[1] + row0 * p.kept_stride + col;
+        float(&v)[2][16] = sum[c];
+        if constexpr (KIND == GEMM_GATED_BWD) {
+          float f[2][16];
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            in(q ? keep1 : keep0, p.kept_stride, left, true, f);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) f[j / 16][j % 16] *= v[j / 16][j % 16];
+            out(q ? p.out[1] + row0 * p.out_stride + col : to, p.out_stride, left, true, f);
+          }
+        } else {
+          if (p.bias[0]) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j / 16][j % 16] += j < left ? __ldg(p.bias[0] + col + j) : 0.0f;
+          }
+          if constexpr (DUAL) {
+            float(&w)[2][16] = sum[1];
+            if (p.bias[1]) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) w[j / 16][j % 16] += j < left ? __ldg(p.bias[1] + col + j) : 0.0f;
+            }
+            float f[2][16];
+            with_activation_dev(p.act, [&](auto act) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) f[j / 16][j % 16] = w[j / 16][j % 16] * act_slope<decltype(act)::value, true>(v[j / 16][j % 16], v[j / 16][j % 16]);
+            });
+            if (p.keep) {
+              out(keep0, p.kept_stride, left, true, f);
+              out(keep1, p.kept_stride, left, true, v);
+            }
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j / 16][j % 16] *= w[j / 16][j % 16];
+          } else {
+            if (p.keep) out(keep0, p.kept_stride, left, true, v);
+            if (p.act != LIK_ACT_NONE)
+              with_activation_dev(p.act, [&](auto act) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j / 16][j % 16] = act_value<decltype(act)::value, true>(v[j / 16][j % 16]);
+              });
+            if (p.residual) {
+              float f[2][16];
+              in(p.residual + row0 * p.residual_stride + col, p.residual_stride, left, p.residual_vec, f);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j / 16][j % 16] += f[j / 16][j % 16];
+            }
+          }
+          out(to, p.out_stride, left, p.out_vec, v);
+        }
+      }
+    }
+  }
+  __syncwarp();
+  __syncthreads();
+  if (warp == GF_ISSUER) tmem_dealloc(tmem, 512);
+}
+
+// x = p0 + p1 + p2 in bf16, each the nearest to what the ones before leave.  A value that bf16 would round to infinity is cut off instead,
+// and one that is not finite has no further parts.
+__device__ __forceinline__ void cut3(float x, uint32_t (&p)[3]) {
+  __nv_bfloat16 h = __float2bfloat16_rn(x);
+  if (fabsf(x) > 3.3895e38f) h = __float2bfloat16_rz(x);
+  const bool finite = fabsf(x) <= 3.402823466e38f;
+  p[0] = __bfloat16_as_ushort(h);
+  float r = finite ? x - __bfloat162float(h) : 0.0f;
+  h = __float2bfloat16_rn(r);
+  p[1] = __bfloat16_as_ushort(h);
+  r -= __bfloat162float(h);
+  p[2] = __bfloat16_as_ushort(__float2bfloat16_rn(r));
+}
+// a matrix in its three parts, rows of whole 16-byte pieces (zeros behind the columns)
+__global__ void __launch_bounds__(256) cut_kernel(const float* __restrict__ src, long long src_stride, long long rows, int cols, uint4* __restrict__ dst, int vecs,
+                                                  bool vec) {
+  const long long total = rows * vecs;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
+    const long long r = i / vecs;
+    const int c = (int)(i - r * vecs) * 8;
+    const float* s = src + r * src_stride + c;
+    float x[8];
+    if (vec && c + 8 <= cols) {
+      load_vec<float, 8>(s, x);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = c + j < cols ? s[j] : 0.0f;
+    }
+    uint32_t w[3][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t lo[3], hi[3];
+      cut3(x[2 * j], lo);
+      cut3(x[2 * j + 1], hi);
+#pragma unroll
+      for (int q = 0; q < 3; ++q) w[q][j] = lo[q] | hi[q] << 16;
+    }
+#pragma unroll
+    for (int q = 0; q < 3; ++q) dst[q * total + i] = make_uint4(w[q][0], w[q][1], w[q][2], w[q][3]);
+  }
+}
+
+struct GfPlan {
+  int tiles_m, tiles_n, kb[2], kb_total, kb_per, splits, partial_stride;
+  size_t parts[4], partial, total;  // offsets: the parts of a[0], a[1], b[0], b[1]
+};
+// whether operand i (a[0], a[1], b[0], b[1]) is there
+bool operand_there(const GemmDesc& d, int i) { return (i & 1) < (i >= 2 && d.kind == GEMM_GATED ? 2 : d.n_seg); }
+Stored operand_stored(const GemmDesc& d, int i) {
+  return stored(i >= 2 ? d.b[i & 1] : d.a[i & 1], i >= 2 ? d.n : d.m, d.k[d.kind == GEMM_GATED ? 0 : i & 1]);
+}
+GfPlan gf_plan(const GemmDesc& d) {
+  GfPlan pl{};
+  for (int s = 0; s < d.n_seg; ++s) pl.kb_total += pl.kb[s] = (int)ceil_div(d.k[s], GT_BK);
+  pl.tiles_m = (int)ceil_div(d.m, 128);
+  pl.tiles_n = (int)ceil_div(d.n, d.kind == GEMM_GATED ? 64 : 128);
+  const long long t = (long long)pl.tiles_m * pl.tiles_n, sms = sm_count();
+  pl.splits = 1;
+  if (gemm_plain(d) && t < sms) {
+    long long want = sms / t;
+    if (want > pl.kb_total / 4) want = pl.kb_total / 4;
+    if (want > 1) pl.splits = (int)want;
+  }
+  pl.kb_per = (int)ceil_div(pl.kb_total, pl.splits);
+  pl.splits = (int)ceil_div(pl.kb_total, pl.kb_per);
+  size_t off = 0;
+  for (int i = 0; i < 4; ++i) {
+    if (!operand_there(d, i)) continue;
+    const Stored o = operand_stored(d, i);
+    pl.parts[i] = off;
+    off += align_up((size_t)o.rows * o.padded() * 2 * GF_PARTS, 256);
+  }
+  if (pl.splits > 1) {
+    pl.partial = off;
+    pl.partial_stride = (d.n + 3) / 4 * 4;
+    off += align_up((size_t)pl.splits * d.m * pl.partial_stride * sizeof(float), 256);
+  }
+  pl.total = off;
+  return pl;
+}
+template <int KIND>
+int run_f32(const GfMaps& maps, const GfParams& p, cudaStream_t st) {
+  LIK_CUDA_OK(allow_smem<gemm_f32_kernel<KIND>>());
+  gemm_f32_kernel<KIND><<<p.units < sm_count() ? p.units : sm_count(), GF_THREADS, 1024 + GF_CTL_AT + sizeof(GfCtl), st>>>(maps, p), count_launch();
+  LIK_CUDA_OK(cudaGetLastError());
+  return LIK_OK;
+}
+
+}  // namespace
+
+bool gemm_f32_supported(const GemmDesc& d) {
+  if (d.dtype != LIK_F32 || !tmap_available()) return false;
+  if (d.m >= (1ll << 31) || d.k[0] >= (1ll << 31) || d.k[1] >= (1ll << 31)) return false;
+  return ceil_div(d.m, 128) * ceil_div(d.n, 64) < (1ll << 30);
+}
+size_t gemm_f32_workspace(const GemmDesc& d) { return gf_plan(d).total; }
+
+int launch_gemm_f32(const GemmDesc& d, void* ws, size_t ws_bytes, int* status, cudaStream_t st) {
+  const GfPlan pl = gf_plan(d);
+  if (ws_bytes < pl.total || !ws) {
+    set_error("workspace too small");
+    return LIK_ERR_WORKSPACE;
+  }
+  if (int rc = make_context_current()) return rc;
+  GfMaps maps{};
+  GfParams p{};
+  for (int i = 0; i < 4; ++i) {
+    if (!operand_there(d, i)) continue;
+    const Stored o = operand_stored(d, i);
+    (i >= 2 ? p.b_mn : p.a_mn) = o.mn;
+    uint8_t* to = (uint8_t*)ws + pl.parts[i];
+    const long long vecs = o.padded() / 8, total = o.rows * vecs, blocks = ceil_div(total, 256), most = 16ll * sm_count();
+    cut_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, st>>>((const float*)o.p, o.stride, o.rows, (int)o.cols, (uint4*)to, (int)vecs,
+                                                                          ((uintptr_t)o.p & 15) == 0 && o.stride % 4 == 0), count_launch();
+    LIK_CUDA_OK(cudaGetLastError());
+    for (int q = 0; q < GF_PARTS; ++q) {
+      CUtensorMap* map = i >= 2 ? &maps.b[i & 1][q] : &maps.a[i & 1][q];
+      if (int rc = make_tmap_rows(map, to + q * total * 16, LIK_BF16, o.cols, o.rows, o.padded(), GT_BOX)) return rc;
+    }
+  }
+  if (pl.splits > 1) {
+    p.out[0] = (float*)((char*)ws + pl.partial);
+    p.out_stride = pl.partial_stride;
+    p.split_stride = d.m * pl.partial_stride;
+    p.out_vec = true;
+  } else {
+    for (int i = 0; i < 2; ++i) p.out[i] = (float*)d.out[i];
+    p.out_stride = d.out_stride;
+    p.out_vec = rows_of_pieces(d.out[0], d.out_stride, LIK_F32);
+  }
+  p.m = (int)d.m;
+  p.n = d.n;
+  p.kb0 = pl.kb[0];
+  p.kb_total = pl.kb_total;
+  p.kb_per = pl.kb_per;
+  p.tiles_n = pl.tiles_n;
+  p.tiles = pl.tiles_m * pl.tiles_n;
+  p.units = p.tiles * pl.splits;
+  p.act = d.act;
+  for (int i = 0; i < 2; ++i) {
+    p.bias[i] = (const float*)d.bias[i];
+    p.kept[i] = (float*)d.kept[i];
+  }
+  p.keep = d.kind != GEMM_GATED_BWD && d.kept[0];
+  p.kept_stride = d.kept_stride;
+  p.residual = (const float*)d.residual;
+  p.residual_stride = d.residual_stride;
+  p.residual_vec = d.n % 4 == 0 && rows_of_pieces(d.residual, d.residual_stride, LIK_F32);
+  p.status = status;
+  const int rc = d.kind == GEMM_GATED ? run_f32<GEMM_GATED>(maps, p, st) : (d.kind == GEMM_GATED_BWD ? run_f32<GEMM_GATED_BWD>(maps, p, st) : run_f32<GEMM_LINEAR>(maps, p, st));
+  if (rc || pl.splits == 1) return rc;
+  return launch_sum_splits((const float*)((char*)ws + pl.partial), pl.splits, d, pl.partial_stride, st);
+}
+
+}  // namespace lik

@@ -176,7 +176,7 @@ SimtPlan simt_plan(const GemmDesc& d) {
   pl.tiles = ceil_div(d.m, b) * pl.tiles_n;
   pl.splits = 1;
   pl.per_split = 0;
-  const bool plain = d.kind == GEMM_LINEAR && d.n_seg == 1 && d.act == LIK_ACT_NONE && !d.bias[0] && !d.residual && !d.kept[0] && d.out_stride == d.n;
+  const bool plain = gemm_plain(d) && d.n_seg == 1 && d.out_stride == d.n;
   if (plain && pl.tiles < sm_count() && d.k[0] >= 512) {
     long long want = ceil_div(2ll * sm_count(), pl.tiles);
     if (want > d.k[0] / 256) want = d.k[0] / 256;

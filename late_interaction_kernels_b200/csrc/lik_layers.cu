@@ -110,10 +110,24 @@ int launch_slope(SlopeParams p, int act, int dtype, void* sums, int sums_dtype, 
 }
 
 // which kernel a product goes to
-bool on_tensor_cores(const GemmDesc& d) { return gemm_tc_supported(d); }
-size_t gemm_workspace(const GemmDesc& d) { return on_tensor_cores(d) ? gemm_tc_workspace(d) : gemm_simt_workspace(d); }
+enum GemmEngine { ENGINE_SIMT, ENGINE_TC, ENGINE_F32 };
+GemmEngine gemm_engine(const GemmDesc& d) {
+  if (d.dtype == LIK_F32) return (d.kind == GEMM_GATED ? 4.0 : 2.0) * d.m * d.n * (d.k[0] + d.k[1]) >= 4e8 && gemm_f32_supported(d) ? ENGINE_F32 : ENGINE_SIMT;
+  return gemm_tc_supported(d) ? ENGINE_TC : ENGINE_SIMT;
+}
+size_t gemm_workspace(const GemmDesc& d) {
+  switch (gemm_engine(d)) {
+    case ENGINE_TC: return gemm_tc_workspace(d);
+    case ENGINE_F32: return gemm_f32_workspace(d);
+    default: return gemm_simt_workspace(d);
+  }
+}
 int launch_gemm(const GemmDesc& d, void* ws, size_t ws_bytes, int* status, cudaStream_t st) {
-  return on_tensor_cores(d) ? launch_gemm_tc(d, ws, ws_bytes, status, st) : launch_gemm_simt(d, ws, ws_bytes, st);
+  switch (gemm_engine(d)) {
+    case ENGINE_TC: return launch_gemm_tc(d, ws, ws_bytes, status, st);
+    case ENGINE_F32: return launch_gemm_f32(d, ws, ws_bytes, status, st);
+    default: return launch_gemm_simt(d, ws, ws_bytes, st);
+  }
 }
 
 bool act_known(int a) { return a >= LIK_ACT_NONE && a <= LIK_ACT_SIGMOID; }

@@ -219,6 +219,10 @@ struct GemmDesc {
   void* kept[2] = {nullptr, nullptr};  // the factors of the backward: written, or read by GEMM_GATED_BWD; rows of 16 bytes
   long long kept_stride = 0;
 };
+// nothing but the product: its sum may be cut along k
+inline bool gemm_plain(const GemmDesc& d) {
+  return d.kind == GEMM_LINEAR && d.act == LIK_ACT_NONE && !d.bias[0] && !d.residual && !d.kept[0];
+}
 // fp32 multiply-add (lik_gemm_simt.cu): any type, stride and size
 size_t gemm_simt_workspace(const GemmDesc& d);
 int launch_gemm_simt(const GemmDesc& d, void* ws, size_t ws_bytes, cudaStream_t st);
@@ -226,6 +230,10 @@ int launch_gemm_simt(const GemmDesc& d, void* ws, size_t ws_bytes, cudaStream_t 
 bool gemm_tc_supported(const GemmDesc& d);
 size_t gemm_tc_workspace(const GemmDesc& d);
 int launch_gemm_tc(const GemmDesc& d, void* ws, size_t ws_bytes, int* status, cudaStream_t st);
+// tensor cores (lik_gemm_f32.cu): fp32 operands in three bf16 parts
+bool gemm_f32_supported(const GemmDesc& d);
+size_t gemm_f32_workspace(const GemmDesc& d);
+int launch_gemm_f32(const GemmDesc& d, void* ws, size_t ws_bytes, int* status, cudaStream_t st);
 
 // sum over `parts` of partial[part][i], i < n, as dtype: out[i], the second half (i >= split) to out2
 int launch_sum_parts(const float* partial, int parts, long long n, long long split, int dtype, void* out, void* out2, cudaStream_t st);

@@ -234,7 +234,8 @@ def linear_case(m, k, n, dt, act, bias, residual, wdt=None):
 
 
 SHAPES = [(1, 1, 1), (1, 7, 3), (2, 64, 5), (5, 16, 16), (8, 768, 768), (9, 768, 130), (16, 512, 1024), (17, 512, 1000), (32, 768, 128), (33, 100, 65), (64, 72, 264),
-          (128, 128, 128), (129, 255, 257), (255, 264, 248), (300, 768, 520), (700, 1001, 333), (2050, 192, 72), (4096, 64, 64), (20000, 40, 24), (1000, 2048, 136)]
+          (128, 128, 128), (129, 255, 257), (255, 264, 248), (300, 768, 520), (700, 1001, 333), (2050, 192, 72), (4096, 64, 64), (20000, 40, 24), (1000, 2048, 136),
+          (2500, 520, 392), (4100, 260, 1030), (30000, 96, 200)]
 
 
 @pytest.mark.parametrize("dt", [BF16, FP16, FP32])
@@ -379,7 +380,8 @@ def gated_case(m, k, f, o, dt, act, bias, residual, wdt=None):
 
 
 GATED = [(1, 1, 1, 1), (1, 16, 40, 8), (3, 5, 7, 9), (8, 768, 512, 768), (16, 64, 2048, 64), (17, 384, 1100, 384), (40, 128, 96, 136), (128, 256, 128, 256), (130, 264, 200, 72),
-         (257, 65, 129, 33), (600, 768, 512, 768), (2050, 128, 320, 128), (9000, 64, 40, 64)]
+         (257, 65, 129, 33), (600, 768, 512, 768), (2050, 128, 320, 128), (9000, 64, 40, 64),
+         (1500, 300, 700, 260), (3001, 257, 515, 129)]
 
 
 @pytest.mark.parametrize("dt", [BF16, FP16, FP32])
