@@ -56,34 +56,6 @@ __device__ __forceinline__ void slab_store(const GemmOperand& o, const float (&v
   }
 }
 
-// one element of the result
-template <typename T, typename O, int KIND, int ACT>
-__device__ __forceinline__ void simt_element(const GemmDesc& d, long long m, int n, float c0, float c1) {
-  constexpr bool PRECISE = sizeof(T) == 4;
-  const long long ki = m * d.kept_stride + n, oi = m * d.out_stride + n;
-  if constexpr (KIND == GEMM_GATED_BWD) {
-    ((T*)d.out[0])[oi] = from_f32<T>(c0 * to_f32(((const T*)d.kept[0])[ki]));
-    ((T*)d.out[1])[oi] = from_f32<T>(c0 * to_f32(((const T*)d.kept[1])[ki]));
-    return;
-  }
-  if (d.bias[0]) c0 += to_f32(((const T*)d.bias[0])[n]);
-  float v;
-  if constexpr (KIND == GEMM_GATED) {
-    const float slope = act_slope<ACT, PRECISE>(c0, v);
-    if (d.bias[1]) c1 += to_f32(((const T*)d.bias[1])[n]);
-    if (d.kept[0]) {
-      ((T*)d.kept[0])[ki] = from_f32<T>(c1 * slope);
-      ((T*)d.kept[1])[ki] = from_f32<T>(v);
-    }
-    v *= c1;
-  } else {
-    v = act_value<ACT, PRECISE>(c0);
-    if (d.kept[0]) ((T*)d.kept[0])[ki] = from_f32<T>(c0);
-    if (d.residual) v += to_f32(((const T*)d.residual)[m * d.residual_stride + n]);
-  }
-  ((O*)d.out[0])[oi] = from_f32<O>(v);
-}
-
 template <typename T, typename O, int KIND, int BM, int BN, int TM, int TN>
 __global__ void __launch_bounds__(SIMT_THREADS) gemm_simt_kernel(const __grid_constant__ SimtParams p) {
   constexpr bool DUAL = KIND == GEMM_GATED;
@@ -154,7 +126,7 @@ __global__ void __launch_bounds__(SIMT_THREADS) gemm_simt_kernel(const __grid_co
       for (int j = 0; j < TN; ++j) {
         const long long m = m0 + ty * TM + i;
         const int n = n0 + tx * TN + j;
-        if (m < d.m && n < d.n) simt_element<T, O, KIND, decltype(act)::value>(d, m, n, acc[0][i][j], DUAL ? acc[DUAL ? 1 : 0][i][j] : 0.0f);
+        if (m < d.m && n < d.n) gemm_element<T, O, KIND, decltype(act)::value>(d, m, n, acc[0][i][j], DUAL ? acc[DUAL ? 1 : 0][i][j] : 0.0f);
       }
   });
 }

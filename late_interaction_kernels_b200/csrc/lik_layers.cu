@@ -110,8 +110,9 @@ int launch_slope(SlopeParams p, int act, int dtype, void* sums, int sums_dtype, 
 }
 
 // which kernel a product goes to
-enum GemmEngine { ENGINE_SIMT, ENGINE_TC, ENGINE_F32 };
+enum GemmEngine { ENGINE_SIMT, ENGINE_FEW, ENGINE_TC, ENGINE_F32 };
 GemmEngine gemm_engine(const GemmDesc& d) {
+  if (gemm_few_supported(d)) return ENGINE_FEW;
   if (d.dtype == LIK_F32) return (d.kind == GEMM_GATED ? 4.0 : 2.0) * d.m * d.n * (d.k[0] + d.k[1]) >= 4e8 && gemm_f32_supported(d) ? ENGINE_F32 : ENGINE_SIMT;
   return gemm_tc_supported(d) ? ENGINE_TC : ENGINE_SIMT;
 }
@@ -119,6 +120,7 @@ size_t gemm_workspace(const GemmDesc& d) {
   switch (gemm_engine(d)) {
     case ENGINE_TC: return gemm_tc_workspace(d);
     case ENGINE_F32: return gemm_f32_workspace(d);
+    case ENGINE_FEW: return 0;
     default: return gemm_simt_workspace(d);
   }
 }
@@ -126,6 +128,7 @@ int launch_gemm(const GemmDesc& d, void* ws, size_t ws_bytes, int* status, cudaS
   switch (gemm_engine(d)) {
     case ENGINE_TC: return launch_gemm_tc(d, ws, ws_bytes, status, st);
     case ENGINE_F32: return launch_gemm_f32(d, ws, ws_bytes, status, st);
+    case ENGINE_FEW: return launch_gemm_few(d, st);
     default: return launch_gemm_simt(d, ws, ws_bytes, st);
   }
 }

@@ -219,6 +219,34 @@ struct GemmDesc {
   void* kept[2] = {nullptr, nullptr};  // the factors of the backward: written, or read by GEMM_GATED_BWD; rows of 16 bytes
   long long kept_stride = 0;
 };
+// one element of the result, from the sums c0 and (GEMM_GATED) c1
+template <typename T, typename O, int KIND, int ACT>
+__device__ __forceinline__ void gemm_element(const GemmDesc& d, long long m, int n, float c0, float c1) {
+  constexpr bool PRECISE = sizeof(T) == 4;
+  const long long ki = m * d.kept_stride + n, oi = m * d.out_stride + n;
+  if constexpr (KIND == GEMM_GATED_BWD) {
+    ((T*)d.out[0])[oi] = from_f32<T>(c0 * to_f32(((const T*)d.kept[0])[ki]));
+    ((T*)d.out[1])[oi] = from_f32<T>(c0 * to_f32(((const T*)d.kept[1])[ki]));
+    return;
+  }
+  if (d.bias[0]) c0 += to_f32(((const T*)d.bias[0])[n]);
+  float v;
+  if constexpr (KIND == GEMM_GATED) {
+    const float slope = act_slope<ACT, PRECISE>(c0, v);
+    if (d.bias[1]) c1 += to_f32(((const T*)d.bias[1])[n]);
+    if (d.kept[0]) {
+      ((T*)d.kept[0])[ki] = from_f32<T>(c1 * slope);
+      ((T*)d.kept[1])[ki] = from_f32<T>(v);
+    }
+    v *= c1;
+  } else {
+    v = act_value<ACT, PRECISE>(c0);
+    if (d.kept[0]) ((T*)d.kept[0])[ki] = from_f32<T>(c0);
+    if (d.residual) v += to_f32(((const T*)d.residual)[m * d.residual_stride + n]);
+  }
+  ((O*)d.out[0])[oi] = from_f32<O>(v);
+}
+
 // nothing but the product: its sum may be cut along k
 inline bool gemm_plain(const GemmDesc& d) {
   return d.kind == GEMM_LINEAR && d.act == LIK_ACT_NONE && !d.bias[0] && !d.residual && !d.kept[0];
@@ -226,6 +254,9 @@ inline bool gemm_plain(const GemmDesc& d) {
 // fp32 multiply-add (lik_gemm_simt.cu): any type, stride and size
 size_t gemm_simt_workspace(const GemmDesc& d);
 int launch_gemm_simt(const GemmDesc& d, void* ws, size_t ws_bytes, cudaStream_t st);
+// few rows of a (lik_gemm_few.cu): any type, both operands with their k contiguous
+bool gemm_few_supported(const GemmDesc& d);
+int launch_gemm_few(const GemmDesc& d, cudaStream_t st);
 // tensor cores (lik_gemm_tc.cu): 16-bit operands
 bool gemm_tc_supported(const GemmDesc& d);
 size_t gemm_tc_workspace(const GemmDesc& d);
