@@ -158,13 +158,14 @@ struct Stored {
   const void* p;
   long long rows, cols, stride;
   bool mn;  // rows are k
+  const void* parts = nullptr;
   // as TMA wants 16-bit rows
   bool aligned() const { return ((uintptr_t)p & 15) == 0 && (rows == 1 || stride % 8 == 0); }
   long long padded() const { return (cols + 7) / 8 * 8; }
 };
 Stored stored(const GemmOperand& o, long long rows, long long k) {
-  if (o.k == 1) return {o.p, rows, k, o.row, false};
-  return {o.p, k, rows, o.k, true};
+  if (o.k == 1) return {o.p, rows, k, o.row, false, o.parts};
+  return {o.p, k, rows, o.k, true, o.parts};
 }
 bool rows_of_pieces(const void* p, long long stride, int dtype) { return ((uintptr_t)p & 15) == 0 && stride * (long long)dtype_size(dtype) % 16 == 0; }
 

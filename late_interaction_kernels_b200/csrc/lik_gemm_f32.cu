@@ -281,16 +281,26 @@ __device__ __forceinline__ void cut3(float x, uint32_t (&p)[3]) {
   r -= __bfloat162float(h);
   p[2] = __bfloat16_as_ushort(__float2bfloat16_rn(r));
 }
-// a matrix in its three parts, rows of whole 16-byte pieces (zeros behind the columns)
-__global__ void __launch_bounds__(256) cut_kernel(const float* __restrict__ src, long long src_stride, long long rows, int cols, uint4* __restrict__ dst, int vecs,
-                                                  bool vec) {
-  const long long total = rows * vecs;
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
+// matrices in their three parts, rows of whole 16-byte pieces (zeros behind the columns).  Bound by memory: 4 bytes in and 6 out per value.
+struct CutJobs {
+  CutMatrix m[CUT_MOST];
+  long long end[CUT_MOST];  // pieces up to and with this matrix
+  int vecs[CUT_MOST];
+  bool vec[CUT_MOST];
+  int n;
+};
+__global__ void __launch_bounds__(256) cut_kernel(const __grid_constant__ CutJobs p) {
+  const long long total = p.end[p.n - 1];
+  for (long long g = blockIdx.x * 256ll + threadIdx.x; g < total; g += gridDim.x * 256ll) {
+    int q = 0;
+    while (g >= p.end[q]) ++q;
+    const long long i = q ? g - p.end[q - 1] : g;
+    const int vecs = p.vecs[q], cols = (int)p.m[q].cols;
     const long long r = i / vecs;
     const int c = (int)(i - r * vecs) * 8;
-    const float* s = src + r * src_stride + c;
+    const float* s = (const float*)p.m[q].src + r * p.m[q].stride + c;
     float x[8];
-    if (vec && c + 8 <= cols) {
+    if (p.vec[q] && c + 8 <= cols) {
       load_vec<float, 8>(s, x);
     } else {
 #pragma unroll
@@ -303,10 +313,12 @@ __global__ void __launch_bounds__(256) cut_kernel(const float* __restrict__ src,
       cut3(x[2 * j], lo);
       cut3(x[2 * j + 1], hi);
 #pragma unroll
-      for (int q = 0; q < 3; ++q) w[q][j] = lo[q] | hi[q] << 16;
+      for (int k = 0; k < 3; ++k) w[k][j] = lo[k] | hi[k] << 16;
     }
+    uint4* dst = (uint4*)p.m[q].parts + i;
+    const long long part = p.m[q].rows * vecs;
 #pragma unroll
-    for (int q = 0; q < 3; ++q) dst[q * total + i] = make_uint4(w[q][0], w[q][1], w[q][2], w[q][3]);
+    for (int k = 0; k < 3; ++k) dst[k * part] = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
   }
 }
 
@@ -337,8 +349,9 @@ GfPlan gf_plan(const GemmDesc& d) {
   for (int i = 0; i < 4; ++i) {
     if (!operand_there(d, i)) continue;
     const Stored o = operand_stored(d, i);
+    if (o.parts) continue;
     pl.parts[i] = off;
-    off += align_up((size_t)o.rows * o.padded() * 2 * GF_PARTS, 256);
+    off += cut_bytes(o.rows, o.cols);
   }
   if (pl.splits > 1) {
     pl.partial = off;
@@ -358,36 +371,52 @@ int run_f32(const GfMaps& maps, const GfParams& p, cudaStream_t st) {
 
 }  // namespace
 
-bool gemm_f32_supported(const GemmDesc& d) {
-  if (d.dtype != LIK_F32 || !tmap_available()) return false;
-  if (d.m >= (1ll << 31) || d.k[0] >= (1ll << 31) || d.k[1] >= (1ll << 31)) return false;
-  return ceil_div(d.m, 128) * ceil_div(d.n, 64) < (1ll << 30);
-}
 size_t gemm_f32_workspace(const GemmDesc& d) { return gf_plan(d).total; }
+
+size_t cut_bytes(long long rows, long long cols) { return align_up((size_t)rows * ((cols + 7) / 8) * 16 * GF_PARTS, 256); }
+int launch_cut(const CutMatrix* m, int n, cudaStream_t st) {
+  if (!n) return LIK_OK;
+  CutJobs p{};
+  long long total = 0;
+  for (int i = 0; i < n; ++i) {
+    p.m[i] = m[i];
+    p.vecs[i] = (int)((m[i].cols + 7) / 8);
+    p.vec[i] = ((uintptr_t)m[i].src & 15) == 0 && m[i].stride % 4 == 0;
+    p.end[i] = total += m[i].rows * p.vecs[i];
+  }
+  p.n = n;
+  const long long blocks = ceil_div(total, 256), most = 16ll * sm_count();
+  cut_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, st>>>(p), count_launch();
+  LIK_CUDA_OK(cudaGetLastError());
+  return LIK_OK;
+}
 
 int launch_gemm_f32(const GemmDesc& d, void* ws, size_t ws_bytes, int* status, cudaStream_t st) {
   const GfPlan pl = gf_plan(d);
-  if (ws_bytes < pl.total || !ws) {
+  if (ws_bytes < pl.total || (pl.total && !ws)) {
     set_error("workspace too small");
     return LIK_ERR_WORKSPACE;
   }
   if (int rc = make_context_current()) return rc;
   GfMaps maps{};
   GfParams p{};
+  CutMatrix cuts[4];
+  int n_cuts = 0;
   for (int i = 0; i < 4; ++i) {
     if (!operand_there(d, i)) continue;
     const Stored o = operand_stored(d, i);
     (i >= 2 ? p.b_mn : p.a_mn) = o.mn;
-    uint8_t* to = (uint8_t*)ws + pl.parts[i];
-    const long long vecs = o.padded() / 8, total = o.rows * vecs, blocks = ceil_div(total, 256), most = 16ll * sm_count();
-    cut_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, st>>>((const float*)o.p, o.stride, o.rows, (int)o.cols, (uint4*)to, (int)vecs,
-                                                                          ((uintptr_t)o.p & 15) == 0 && o.stride % 4 == 0), count_launch();
-    LIK_CUDA_OK(cudaGetLastError());
+    const uint8_t* parts = (const uint8_t*)o.parts;
+    if (!parts) {
+      cuts[n_cuts++] = {o.p, o.rows, o.cols, o.stride, (uint8_t*)ws + pl.parts[i]};
+      parts = (const uint8_t*)ws + pl.parts[i];
+    }
     for (int q = 0; q < GF_PARTS; ++q) {
       CUtensorMap* map = i >= 2 ? &maps.b[i & 1][q] : &maps.a[i & 1][q];
-      if (int rc = make_tmap_rows(map, to + q * total * 16, LIK_BF16, o.cols, o.rows, o.padded(), GT_BOX)) return rc;
+      if (int rc = make_tmap_rows(map, parts + q * o.rows * o.padded() * 2, LIK_BF16, o.cols, o.rows, o.padded(), GT_BOX)) return rc;
     }
   }
+  if (int rc = launch_cut(cuts, n_cuts, st)) return rc;
   if (pl.splits > 1) {
     p.out[0] = (float*)((char*)ws + pl.partial);
     p.out_stride = pl.partial_stride;

@@ -13,7 +13,7 @@
 namespace lik {
 namespace {
 
-constexpr int FEW_WARPS = 8, FEW_THREADS = 32 * FEW_WARPS, FEW_MOST = 32;
+constexpr int FEW_WARPS = 8, FEW_THREADS = 32 * FEW_WARPS;  // of the multiply-add kernel, and of the other one unless k is long
 
 struct FewParams {
   GemmDesc d;
@@ -32,15 +32,15 @@ __device__ __forceinline__ void mma_16x8x16(float (&c)[4], const uint32_t (&a)[4
 }
 
 // NT: tiles of eight rows of a
-template <typename T, int KIND, int NT>
-__global__ void __launch_bounds__(FEW_THREADS) few_mma_kernel(const __grid_constant__ FewParams p) {
+template <typename T, int KIND, int NT, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) few_mma_kernel(const __grid_constant__ FewParams p) {
   constexpr int DUAL = KIND == GEMM_GATED ? 2 : 1;
-  __shared__ float part[FEW_WARPS][DUAL][NT][32][4];
+  __shared__ float part[WARPS][DUAL][NT][32][4];
   const GemmDesc& d = p.d;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int n0 = blockIdx.x * 16;
+  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 8 * NT;
   // blocks of 32 k (64 bytes of a row): this warp's share
-  const int blocks = (int)((d.k[0] + 31) / 32), per = (blocks + FEW_WARPS - 1) / FEW_WARPS;
+  const int blocks = (int)((d.k[0] + 31) / 32), per = (blocks + WARPS - 1) / WARPS;
   const int kb_lo = warp * per, kb_hi = min(kb_lo + per, blocks);
   const int k_left = (int)d.k[0];
   float c[DUAL][NT][4];
@@ -62,8 +62,8 @@ __global__ void __launch_bounds__(FEW_THREADS) few_mma_kernel(const __grid_const
   bool x_there[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
-    x_there[i] = i * 8 + g < d.m;
-    x[i] = (const T*)d.a[0].p + (x_there[i] ? (i * 8 + g) * d.a[0].row : 0) + t * 8;
+    x_there[i] = m0 + i * 8 + g < d.m;
+    x[i] = (const T*)d.a[0].p + (x_there[i] ? (m0 + i * 8 + g) * d.a[0].row : 0) + t * 8;
   }
   const uint4 none = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll 4
@@ -95,14 +95,14 @@ __global__ void __launch_bounds__(FEW_THREADS) few_mma_kernel(const __grid_const
   __syncthreads();
   with_activation_dev(d.act, [&](auto act) {
     // neighbouring threads: neighbouring rows of b, which are neighbours in the result
-    for (int e = threadIdx.x; e < NT * 128; e += FEW_THREADS) {
-      const int r = e % 16, m = e / 16, i = m / 8, col = m % 8;
+    for (int e = threadIdx.x; e < NT * 128; e += 32 * WARPS) {
+      const int r = e % 16, in = e / 16, i = in / 8, col = in % 8, m = m0 + in;
       if (m < d.m && n0 + r < d.n) {
         float v[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int q = 0; q < DUAL; ++q)
 #pragma unroll
-          for (int s = 0; s < FEW_WARPS; ++s) v[q] += part[s][q][i][(r % 8) * 4 + col / 2][(r / 8) * 2 + col % 2];
+          for (int s = 0; s < WARPS; ++s) v[q] += part[s][q][i][(r % 8) * 4 + col / 2][(r / 8) * 2 + col % 2];
         gemm_element<T, T, KIND, decltype(act)::value>(d, m, n0 + r, v[0], v[1]);
       }
     }
@@ -180,19 +180,28 @@ bool few_vec(const GemmDesc& d) {
     if (((uintptr_t)d.b[q].p & 15) || (d.n > 1 && d.b[q].row * item % 16)) return false;
   return d.k[0] * item % 16 == 0 && ((uintptr_t)d.a[0].p & 15) == 0 && (d.m == 1 || d.a[0].row * item % 16 == 0);
 }
+template <typename T, int KIND, int NT>
+int run_mma(const FewParams& p, cudaStream_t st) {
+  const GemmDesc& d = p.d;
+  const dim3 grid((unsigned)ceil_div(d.n, 16), (unsigned)ceil_div(d.m, 8 * NT));
+  // a long k: twice the warps, half the loads one after another (32 rows, 2048 x 768: 8.4 us against 6.2)
+  if constexpr (KIND == GEMM_LINEAR) {
+    if (d.k[0] >= 1024) {
+      few_mma_kernel<T, KIND, NT, 2 * FEW_WARPS><<<grid, 64 * FEW_WARPS, 0, st>>>(p), count_launch();
+      LIK_CUDA_OK(cudaGetLastError());
+      return LIK_OK;
+    }
+  }
+  few_mma_kernel<T, KIND, NT, FEW_WARPS><<<grid, FEW_THREADS, 0, st>>>(p), count_launch();
+  LIK_CUDA_OK(cudaGetLastError());
+  return LIK_OK;
+}
 template <typename T, int KIND>
 int run_few(const FewParams& p, cudaStream_t st) {
   const GemmDesc& d = p.d;
   const bool vec = few_vec(d);
   if constexpr (sizeof(T) == 2) {
-    if (vec) {
-      const unsigned grid = (unsigned)ceil_div(d.n, 16);
-      if (d.m <= 8) few_mma_kernel<T, KIND, 1><<<grid, FEW_THREADS, 0, st>>>(p), count_launch();
-      else if (d.m <= 16) few_mma_kernel<T, KIND, 2><<<grid, FEW_THREADS, 0, st>>>(p), count_launch();
-      else few_mma_kernel<T, KIND, 4><<<grid, FEW_THREADS, 0, st>>>(p), count_launch();
-      LIK_CUDA_OK(cudaGetLastError());
-      return LIK_OK;
-    }
+    if (vec) return d.m <= 8 ? run_mma<T, KIND, 1>(p, st) : (d.m <= 16 ? run_mma<T, KIND, 2>(p, st) : run_mma<T, KIND, 4>(p, st));
   }
   const dim3 grid((unsigned)ceil_div(d.n, FMA_ROWS), (unsigned)ceil_div(d.m, FMA_COLS));
   if constexpr (sizeof(T) == 4) {
@@ -213,8 +222,18 @@ int run_few(const FewParams& p, cudaStream_t st) {
 
 }  // namespace
 
-bool gemm_few_supported(const GemmDesc& d) {
-  return d.kind != GEMM_GATED_BWD && d.n_seg == 1 && d.m <= FEW_MOST && d.a[0].k == 1 && d.b[0].k == 1 && d.out_dtype == d.dtype && d.k[0] < (1ll << 31) - 4096;
+// By the blocks that there are for an SM.  A block's time grows little with k; the tensor-core kernels have a start of their own of 6 us
+// (fp32: 10 with the cuts) and one CTA's loads per 128 columns.  Measured on both sides of either limit, few rows against tensor cores in
+// us, by blocks per SM: 16-bit 768 x 2048, 96 rows (2.6) 6.2 / 8.2, 128 rows (3.5) 9.8 / 8.4; 2048 x 2048, 96 rows (2.6) 10.1 / 12.3, 128 rows
+// (3.5) 17 / 12.5; fp32 768 x 768, 32 rows (5.2) 9.0 / 13.1, 64 rows (10.4) 16 / 13.4.
+bool gemm_few_pays(const GemmDesc& d) {
+  if (d.kind == GEMM_GATED_BWD || d.n_seg != 1 || d.a[0].k != 1 || d.b[0].k != 1 || d.out_dtype != d.dtype || d.k[0] >= (1ll << 31) - 4096) return false;
+  const long long sms = sm_count(), dual = d.kind == GEMM_GATED ? 2 : 1;
+  if (d.dtype != LIK_F32 && few_vec(d)) {
+    const long long rows = d.m <= 8 ? 8 : (d.m <= 16 ? 16 : 32);
+    return dual * ceil_div(d.n, 16) * ceil_div(d.m, rows) * 5 <= 13 * sms * (32 / rows);
+  }
+  return dual * ceil_div(d.n, FMA_ROWS) * ceil_div(d.m, FMA_COLS) <= 8 * sms;
 }
 int launch_gemm_few(const GemmDesc& d, cudaStream_t st) {
   const FewParams p{d};

@@ -485,12 +485,6 @@ int run_tc(int kind, bool f32_out, int cg, const GtMaps& maps, const GtParams& p
 
 }  // namespace
 
-bool gemm_tc_supported(const GemmDesc& d) {
-  if ((d.dtype != LIK_F16 && d.dtype != LIK_BF16) || !tmap_available()) return false;
-  if (d.m >= (1ll << 31) || d.k[0] >= (1ll << 31) || d.k[1] >= (1ll << 31)) return false;
-  const long long tiles = ceil_div(d.m, 128) * ceil_div(d.n, 64);
-  return tiles < (1ll << 30);
-}
 size_t gemm_tc_workspace(const GemmDesc& d) { return gt_plan(d).total; }
 
 int launch_gemm_tc(const GemmDesc& d, void* ws, size_t ws_bytes, int* status, cudaStream_t st) {

@@ -1,4 +1,6 @@
 // The layers' C entry points: which products and passes a call is made of, and the passes that are not products.
+#include <initializer_list>
+
 #include "lik_layers.cuh"
 
 namespace lik {
@@ -110,26 +112,20 @@ int launch_slope(SlopeParams p, int act, int dtype, void* sums, int sums_dtype, 
 }
 
 // which kernel a product goes to
-enum GemmEngine { ENGINE_SIMT, ENGINE_FEW, ENGINE_TC, ENGINE_F32 };
-GemmEngine gemm_engine(const GemmDesc& d) {
-  if (gemm_few_supported(d)) return ENGINE_FEW;
-  if (d.dtype == LIK_F32) return (d.kind == GEMM_GATED ? 4.0 : 2.0) * d.m * d.n * (d.k[0] + d.k[1]) >= 4e8 && gemm_f32_supported(d) ? ENGINE_F32 : ENGINE_SIMT;
-  return gemm_tc_supported(d) ? ENGINE_TC : ENGINE_SIMT;
-}
+enum GemmEngine { ENGINE_FEW, ENGINE_TC, ENGINE_F32 };
+GemmEngine gemm_engine(const GemmDesc& d) { return gemm_few_pays(d) ? ENGINE_FEW : (d.dtype == LIK_F32 ? ENGINE_F32 : ENGINE_TC); }
 size_t gemm_workspace(const GemmDesc& d) {
   switch (gemm_engine(d)) {
     case ENGINE_TC: return gemm_tc_workspace(d);
     case ENGINE_F32: return gemm_f32_workspace(d);
-    case ENGINE_FEW: return 0;
-    default: return gemm_simt_workspace(d);
+    default: return 0;
   }
 }
 int launch_gemm(const GemmDesc& d, void* ws, size_t ws_bytes, int* status, cudaStream_t st) {
   switch (gemm_engine(d)) {
     case ENGINE_TC: return launch_gemm_tc(d, ws, ws_bytes, status, st);
     case ENGINE_F32: return launch_gemm_f32(d, ws, ws_bytes, status, st);
-    case ENGINE_FEW: return launch_gemm_few(d, st);
-    default: return launch_gemm_simt(d, ws, ws_bytes, st);
+    default: return launch_gemm_few(d, st);
   }
 }
 
@@ -153,12 +149,17 @@ struct Carve {
   }
 };
 
+// units of the products are counted in 32 bits, shares of k included
+bool tiles_fit(long long m, long long n) { return ceil_div(m, 128) * ceil_div(n, 64) < (1ll << 30); }
+
 int check_linear(const lik_linear_args* a) {
   LIK_REQUIRE(a != nullptr, "args is NULL");
   LIK_REQUIRE(dtype_known(a->dtype), "dtype must be fp32, fp16 or bf16");
   LIK_REQUIRE(a->param_dtype == a->dtype || a->param_dtype == LIK_F32, "param_dtype must be dtype or fp32");
   LIK_REQUIRE(act_known(a->activation), "unknown activation");
   LIK_REQUIRE(a->rows >= 0 && a->rows < (1ll << 31) && a->in > 0 && a->out > 0, "sizes must be positive, rows below 2^31");
+  LIK_REQUIRE(tiles_fit(a->rows, a->out) && tiles_fit(a->rows, a->in) && tiles_fit(a->out, a->in), "the matrices are too large");
+  LIK_REQUIRE(((uintptr_t)a->workspace & 15) == 0, "the workspace must be 16-byte aligned");
   LIK_REQUIRE(a->x_stride >= a->in && a->w_stride >= a->in, "x_stride and w_stride must be at least in");
   return LIK_OK;
 }
@@ -208,7 +209,21 @@ GemmDesc grad_w_desc(int dtype, int param_dtype, long long rows, int out, int in
   return d;
 }
 
+// fp32 matrices that several products of a pass on the tensor cores read: cut once, in one launch with the others of the pass
+struct Cuts {
+  CutMatrix m[CUT_MOST];
+  int n = 0;
+  void add(Carve& c, std::initializer_list<GemmOperand*> users, const void* src, long long rows, long long cols, long long stride) {
+    void* parts = c.take(cut_bytes(rows, cols));
+    m[n++] = {src, rows, cols, stride, parts};
+    // (when only sizes are added up there is no address yet; the product still must not ask for room of its own)
+    for (GemmOperand* u : users) u->parts = parts ? parts : (const void*)16;
+  }
+};
+
 struct LinearBwd {
+  GemmDesc dx, dw;  // products that are not asked for have no out
+  Cuts cuts;
   void* dz;
   long long dz_stride;
   float* partial;
@@ -226,11 +241,18 @@ LinearBwd linear_bwd_layout(const lik_linear_args& a, void* ws) {
   if (a.dbias) l.partial = c.take<float>(slope_workspace(a.rows, a.out, a.dtype));
   const void* dz = a.activation != LIK_ACT_NONE ? l.dz : a.dy;
   const long long st = a.activation != LIK_ACT_NONE ? l.dz_stride : a.dy_stride;
-  if (a.dx) l.gemm_bytes = gemm_workspace(grad_x_desc(a.dtype, a.rows, a.out, a.in, dz, st, a.w, a.w_stride, a.dx));
-  if (a.dw) {
-    const size_t b = gemm_workspace(grad_w_desc(a.dtype, a.param_dtype, a.rows, a.out, a.in, dz, st, a.x, a.x_stride, a.dw));
-    l.gemm_bytes = b > l.gemm_bytes ? b : l.gemm_bytes;
+  if (a.dx) l.dx = grad_x_desc(a.dtype, a.rows, a.out, a.in, dz, st, a.w, a.w_stride, a.dx);
+  if (a.dw) l.dw = grad_w_desc(a.dtype, a.param_dtype, a.rows, a.out, a.in, dz, st, a.x, a.x_stride, a.dw);
+  if (a.dx && a.dw && gemm_engine(l.dx) == ENGINE_F32 && gemm_engine(l.dw) == ENGINE_F32) {
+    l.cuts.add(c, {&l.dx.a[0], &l.dw.a[0]}, dz, a.rows, a.out, st);
+    l.cuts.add(c, {&l.dx.b[0]}, a.w, a.out, a.in, a.w_stride);
+    l.cuts.add(c, {&l.dw.b[0]}, a.x, a.rows, a.in, a.x_stride);
   }
+  for (const GemmDesc* d : {&l.dx, &l.dw})
+    if (d->m) {
+      const size_t b = gemm_workspace(*d);
+      l.gemm_bytes = b > l.gemm_bytes ? b : l.gemm_bytes;
+    }
   l.gemm = c.take(l.gemm_bytes);
   l.total = c.off;
   return l;
@@ -250,6 +272,9 @@ int check_gated(const lik_gated_args* a) {
   LIK_REQUIRE(a->param_dtype == a->dtype || a->param_dtype == LIK_F32, "param_dtype must be dtype or fp32");
   LIK_REQUIRE(act_known(a->activation), "unknown activation");
   LIK_REQUIRE(a->rows >= 0 && a->rows < (1ll << 31) && a->in > 0 && a->hidden > 0 && a->out > 0, "sizes must be positive, rows below 2^31");
+  LIK_REQUIRE(tiles_fit(a->rows, a->hidden) && tiles_fit(a->rows, a->in) && tiles_fit(a->rows, a->out) && tiles_fit(a->hidden, a->in) &&
+                  tiles_fit(a->hidden, a->out), "the matrices are too large");
+  LIK_REQUIRE(((uintptr_t)a->workspace & 15) == 0, "the workspace must be 16-byte aligned");
   LIK_REQUIRE(a->x_stride >= a->in && a->w_gate_stride >= a->in && a->w_up_stride >= a->in && a->w_down_stride >= a->hidden, "a stride is below its row");
   return LIK_OK;
 }
@@ -304,6 +329,7 @@ GatedFwd gated_fwd_layout(const lik_gated_args& a, void* ws) {
 }
 struct GatedBwd {
   GemmDesc dh, dx, dwg, dwu, dwd;  // products that are not asked for have no out
+  Cuts first, second;              // before dh and after it
   void *dg, *du;
   long long stride;
   float* partial;
@@ -332,23 +358,33 @@ GatedBwd gated_bwd_layout(const lik_gated_args& a, void* ws) {
     h.kept[0] = a.gate_factor;
     h.kept[1] = a.up_factor;
     h.kept_stride = a.kept_stride;
-    l.gemm_bytes = gemm_workspace(h);
   }
-  auto want = [&](const GemmDesc& d) {
-    const size_t b = gemm_workspace(d);
-    l.gemm_bytes = b > l.gemm_bytes ? b : l.gemm_bytes;
-  };
   if (a.dx) {
     l.dx = grad_x_desc(a.dtype, a.rows, a.hidden, a.in, l.dg, l.stride, a.w_gate, a.w_gate_stride, a.dx);
     l.dx.n_seg = 2;
     l.dx.k[1] = a.hidden;
     l.dx.a[1] = {l.du, l.stride, 1};
     l.dx.b[1] = {a.w_up, 1, a.w_up_stride};
-    want(l.dx);
   }
-  if (a.dw_gate) want(l.dwg = grad_w_desc(a.dtype, a.param_dtype, a.rows, a.hidden, a.in, l.dg, l.stride, a.x, a.x_stride, a.dw_gate));
-  if (a.dw_up) want(l.dwu = grad_w_desc(a.dtype, a.param_dtype, a.rows, a.hidden, a.in, l.du, l.stride, a.x, a.x_stride, a.dw_up));
-  if (a.dw_down) want(l.dwd = grad_w_desc(a.dtype, a.param_dtype, a.rows, a.out, a.hidden, a.dy, a.dy_stride, a.h, a.kept_stride, a.dw_down));
+  if (a.dw_gate) l.dwg = grad_w_desc(a.dtype, a.param_dtype, a.rows, a.hidden, a.in, l.dg, l.stride, a.x, a.x_stride, a.dw_gate);
+  if (a.dw_up) l.dwu = grad_w_desc(a.dtype, a.param_dtype, a.rows, a.hidden, a.in, l.du, l.stride, a.x, a.x_stride, a.dw_up);
+  if (a.dw_down) l.dwd = grad_w_desc(a.dtype, a.param_dtype, a.rows, a.out, a.hidden, a.dy, a.dy_stride, a.h, a.kept_stride, a.dw_down);
+  if (a.dx && a.dw_gate && a.dw_up && a.dw_down && gemm_engine(l.dh) == ENGINE_F32 && gemm_engine(l.dx) == ENGINE_F32 && gemm_engine(l.dwg) == ENGINE_F32 &&
+      gemm_engine(l.dwd) == ENGINE_F32) {
+    l.first.add(c, {&l.dh.a[0], &l.dwd.a[0]}, a.dy, a.rows, a.out, a.dy_stride);
+    l.first.add(c, {&l.dh.b[0]}, a.w_down, a.out, a.hidden, a.w_down_stride);
+    l.first.add(c, {&l.dwd.b[0]}, a.h, a.rows, a.hidden, a.kept_stride);
+    l.first.add(c, {&l.dwg.b[0], &l.dwu.b[0]}, a.x, a.rows, a.in, a.x_stride);
+    l.first.add(c, {&l.dx.b[0]}, a.w_gate, a.hidden, a.in, a.w_gate_stride);
+    l.first.add(c, {&l.dx.b[1]}, a.w_up, a.hidden, a.in, a.w_up_stride);
+    l.second.add(c, {&l.dx.a[0], &l.dwg.a[0]}, l.dg, a.rows, a.hidden, l.stride);
+    l.second.add(c, {&l.dx.a[1], &l.dwu.a[0]}, l.du, a.rows, a.hidden, l.stride);
+  }
+  for (const GemmDesc* d : {&l.dh, &l.dx, &l.dwg, &l.dwu, &l.dwd})
+    if (d->m) {
+      const size_t b = gemm_workspace(*d);
+      l.gemm_bytes = b > l.gemm_bytes ? b : l.gemm_bytes;
+    }
   if (a.db_gate || a.db_up || a.db_down) l.partial = c.take<float>(slope_workspace(a.rows, a.hidden > a.out ? a.hidden : a.out, a.dtype) * 2);
   l.gemm = c.take(l.gemm_bytes);
   l.total = c.off;
@@ -409,16 +445,14 @@ extern "C" int lik_linear_bwd(const lik_linear_args* args, lik_stream_t stream) 
               "z must be there, with 16-byte rows");
   const LinearBwd l = linear_bwd_layout(a, a.workspace);
   if (a.workspace_bytes < l.total || (l.total && !a.workspace)) return too_small("lik_linear_bwd");
-  const void* dz = act ? l.dz : a.dy;
-  const long long dz_stride = act ? l.dz_stride : a.dy_stride;
   if (act || a.dbias) {
     SlopeParams p{a.dy, a.z, a.dy_stride, a.z_stride, a.rows, 0, a.out, l.dz, l.dz_stride, l.partial};
     if (int rc = launch_slope(p, a.activation, a.dtype, a.dbias, a.param_dtype, st)) return rc;
   }
-  if (a.dx)
-    if (int rc = launch_gemm(grad_x_desc(a.dtype, a.rows, a.out, a.in, dz, dz_stride, a.w, a.w_stride, a.dx), l.gemm, l.gemm_bytes, a.status, st)) return rc;
-  if (a.dw)
-    return launch_gemm(grad_w_desc(a.dtype, a.param_dtype, a.rows, a.out, a.in, dz, dz_stride, a.x, a.x_stride, a.dw), l.gemm, l.gemm_bytes, a.status, st);
+  if (int rc = launch_cut(l.cuts.m, l.cuts.n, st)) return rc;
+  for (const GemmDesc* d : {&l.dx, &l.dw})
+    if (d->out[0])
+      if (int rc = launch_gemm(*d, l.gemm, l.gemm_bytes, a.status, st)) return rc;
   return LIK_OK;
 }
 
@@ -466,8 +500,10 @@ extern "C" int lik_gated_bwd(const lik_gated_args* args, lik_stream_t stream) {
                   (((uintptr_t)a.gate_factor | (uintptr_t)a.up_factor | (uintptr_t)a.h) & 15) == 0, "gate_factor, up_factor and h must be there, with 16-byte rows");
   const GatedBwd l = gated_bwd_layout(a, a.workspace);
   if (a.workspace_bytes < l.total || (l.total && !a.workspace)) return too_small("lik_gated_bwd");
+  if (int rc = launch_cut(l.first.m, l.first.n, st)) return rc;
   if (l.dg)
     if (int rc = launch_gemm(l.dh, l.gemm, l.gemm_bytes, a.status, st)) return rc;
+  if (int rc = launch_cut(l.second.m, l.second.n, st)) return rc;
   for (const GemmDesc* d : {&l.dx, &l.dwg, &l.dwu, &l.dwd})
     if (d->out[0])
       if (int rc = launch_gemm(*d, l.gemm, l.gemm_bytes, a.status, st)) return rc;

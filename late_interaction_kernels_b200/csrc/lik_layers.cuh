@@ -202,6 +202,7 @@ enum GemmKind {
 struct GemmOperand {
   const void* p = nullptr;
   long long row = 0, k = 0;  // elements from one row (m or n) to the next, and from one k to the next; one of the two is 1
+  const void* parts = nullptr;  // fp32 on the tensor cores: the matrix as launch_cut left it, or NULL: the product cuts it itself
 };
 struct GemmDesc {
   int kind = GEMM_LINEAR, act = LIK_ACT_NONE, dtype = 0;
@@ -251,20 +252,24 @@ __device__ __forceinline__ void gemm_element(const GemmDesc& d, long long m, int
 inline bool gemm_plain(const GemmDesc& d) {
   return d.kind == GEMM_LINEAR && d.act == LIK_ACT_NONE && !d.bias[0] && !d.residual && !d.kept[0];
 }
-// fp32 multiply-add (lik_gemm_simt.cu): any type, stride and size
-size_t gemm_simt_workspace(const GemmDesc& d);
-int launch_gemm_simt(const GemmDesc& d, void* ws, size_t ws_bytes, cudaStream_t st);
-// few rows of a (lik_gemm_few.cu): any type, both operands with their k contiguous
-bool gemm_few_supported(const GemmDesc& d);
+// few rows of a (lik_gemm_few.cu): any type, both operands with their k contiguous; whether it is the faster one
+bool gemm_few_pays(const GemmDesc& d);
 int launch_gemm_few(const GemmDesc& d, cudaStream_t st);
 // tensor cores (lik_gemm_tc.cu): 16-bit operands
-bool gemm_tc_supported(const GemmDesc& d);
 size_t gemm_tc_workspace(const GemmDesc& d);
 int launch_gemm_tc(const GemmDesc& d, void* ws, size_t ws_bytes, int* status, cudaStream_t st);
 // tensor cores (lik_gemm_f32.cu): fp32 operands in three bf16 parts
-bool gemm_f32_supported(const GemmDesc& d);
 size_t gemm_f32_workspace(const GemmDesc& d);
 int launch_gemm_f32(const GemmDesc& d, void* ws, size_t ws_bytes, int* status, cudaStream_t st);
+// fp32 matrices cut into their bf16 parts, in one launch: what several products read is cut once
+struct CutMatrix {
+  const void* src;
+  long long rows, cols, stride;
+  void* parts;  // cut_bytes(rows, cols)
+};
+constexpr int CUT_MOST = 6;
+size_t cut_bytes(long long rows, long long cols);
+int launch_cut(const CutMatrix* m, int n, cudaStream_t st);
 
 // sum over `parts` of partial[part][i], i < n, as dtype: out[i], the second half (i >= split) to out2
 int launch_sum_parts(const float* partial, int parts, long long n, long long split, int dtype, void* out, void* out2, cudaStream_t st);

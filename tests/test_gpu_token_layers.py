@@ -280,21 +280,20 @@ def test_activations_over_their_range():
 
 
 def test_linear_strides():
+    """Rows that do not follow one another, start off 16 bytes, overlap or lie across: the kernels differ, the numbers are held to the same bounds."""
     from late_interaction_kernels_b200.token_layers import linear
 
     big, W = rand(40, 40, 512, dt=BF16), rand(96, 512, dt=BF16)
-    base = rand(40, 40, 96, dt=BF16)
+    base = rand(40, 40, 97, dt=BF16)
     for x in (big[..., :256], big[..., 1:257], big[::2, :, 256:], big[..., ::2], big.transpose(0, 1)[..., :256], big[:1, :1, :256].expand(3, 5, 256)):
         for w in (W[:, :256], W[:, 3:259], W[:, ::2], W.t().contiguous().t()[:, :256]):
-            x1, w1 = x.detach().requires_grad_(), w.detach().requires_grad_()
-            r = base[: x.shape[0], : x.shape[1]]
-            y = linear(x1, w1, activation="silu", residual=r)
-            x2, w2 = x.contiguous().detach().requires_grad_(), w.contiguous().detach().requires_grad_()
-            want = linear(x2, w2, activation="silu", residual=r.contiguous())
-            assert torch.equal(y, want)
-            dy = rand(1, 1, 96, dt=BF16).expand(y.shape)  # a broadcast gradient, rows that overlap
-            for a, c in zip(torch.autograd.grad(y, (x1, w1), dy), torch.autograd.grad(want, (x2, w2), dy.contiguous())):
-                assert torch.equal(a, c)
+            for r in (base[: x.shape[0], : x.shape[1], :96], base[: x.shape[0], : x.shape[1], 1:]):
+                leaves = [t.detach().requires_grad_() for t in (x, w, r)]
+                y = linear(leaves[0], leaves[1], activation="silu", residual=leaves[2])
+                dy = rand(1, 1, 96, dt=BF16).expand(y.shape)  # a broadcast gradient, rows that overlap
+                grads = dict(zip("xwr", torch.autograd.grad(y, leaves, dy)))
+                flat = lambda t: t.reshape(-1, t.shape[-1])
+                check_linear(flat(x), w, None, flat(r), flat(dy), "silu", flat(y), {"x": flat(grads["x"]), "w": grads["w"], "r": flat(grads["r"])}, BF16)
 
 
 def test_linear_nan_and_infinity_stay_in_their_rows():
