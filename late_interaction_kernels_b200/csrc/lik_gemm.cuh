@@ -60,8 +60,8 @@ struct Raw16 {
   }
 };
 
-// 16-byte piece c of row r in a slot of 32 rows of ROW bytes: the 64-byte or 128-byte swizzle of the slot's tensor map, which also keeps
-// the lanes' accesses, a row each, apart
+// 16-byte piece c of row r in a slot of 32 rows of ROW bytes: shuffled within its row so that
+// the lanes' accesses, a row each, keep apart
 template <int ROW>
 __device__ __forceinline__ int slot_offset(int r, int c) {
   return ROW == 64 ? r * 64 + ((c ^ ((r >> 1) & 3)) << 4) : r * 128 + ((c ^ (r & 7)) << 4);
@@ -130,27 +130,112 @@ __device__ __forceinline__ void slot_fetch(uint8_t* s, int lane, const T* p, lon
   }
 }
 
-// out[i][j] = sum over splits of partial[split][i][j], in their order
-template <typename O>
-__global__ void __launch_bounds__(256) sum_splits_kernel(const float* __restrict__ partial, int splits, long long m, int n, int stride, O* __restrict__ out,
-                                                         long long out_stride) {
-  const int per_row = (n + 3) / 4;
-  const long long total = m * per_row;
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
+// a slot of fp32 written as another type
+template <typename T>
+__device__ __forceinline__ void slot_store_as(const uint8_t* s, int lane, T* p, long long stride, int rows, int cols, bool vec) {
+  if (vec) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = lane + 32 * j, r = i / 4, c = i % 4;
+      const float4 x = *reinterpret_cast<const float4*>(s + slot_offset<128>(r, 2 * c)), y = *reinterpret_cast<const float4*>(s + slot_offset<128>(r, 2 * c + 1));
+      if (r < rows && c * 8 < cols)
+        *reinterpret_cast<uint4*>(p + r * stride + c * 8) = make_uint4(pack2(x.x, x.y, T()), pack2(x.z, x.w, T()), pack2(y.x, y.y, T()), pack2(y.z, y.w, T()));
+    }
+  } else if (lane < cols) {
+    for (int r = 0; r < rows && r < 32; ++r) p[r * stride + lane] = from_f32<T>(*reinterpret_cast<const float*>(s + slot_offset<128>(r, lane / 4) + (lane % 4) * 4));
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// One launch computes up to four products.  A problem's tiles, each cut along k into `splits` shares, are its units; units are numbered
+// through the problems and dealt to the CTAs (or pairs) in turn.
+// ---------------------------------------------------------------------------------------------
+constexpr int GT_PROBLEMS = 4, GT_MATRICES = 8;
+struct GtProblem {
+  int m, n;
+  int kb0, kb_total, kb_per, tiles, tiles_n, unit0;  // slabs of 64 k: of the first segment, of both, of a share
+  bool a_mn, b_mn, out_vec, out_f32;
+  unsigned char a[2], b[2];                          // which matrices, per segment (GEMM_GATED: b of the gate and of up)
+  void* out;
+  long long out_stride, split_stride;
+};
+struct GtUnit {
+  int q, tm, tn, split, kb_lo, kb_hi;
+};
+template <bool MULTI>
+__device__ __forceinline__ GtUnit gt_unit(const GtProblem (&q)[GT_PROBLEMS], int n, int u) {
+  GtUnit t;
+  t.q = 0;
+  if constexpr (MULTI)
+    while (t.q + 1 < n && u >= q[t.q + 1].unit0) ++t.q;
+  const GtProblem& p = q[t.q];
+  const int v = u - p.unit0;
+  t.split = v / p.tiles;
+  const int i = v - t.split * p.tiles;
+  t.tm = i / p.tiles_n;
+  t.tn = i - t.tm * p.tiles_n;
+  t.kb_lo = t.split * p.kb_per;
+  t.kb_hi = min(t.kb_lo + p.kb_per, p.kb_total);
+  return t;
+}
+
+// the shares of products that were cut along k, added in their order and rounded
+struct SumJob {
+  const float* partial;
+  int splits, n, stride;
+  long long m, end, out_stride;  // end: pieces of four columns up to and with this job
+  void* out;
+  bool out_f32;
+};
+struct SumJobs {
+  SumJob q[GT_PROBLEMS];
+  int n;
+};
+__device__ __forceinline__ float4 sum_shares(const SumJob& j, long long r, int c) {
+  const float* src = j.partial + r * j.stride + c;
+  float4 v = *reinterpret_cast<const float4*>(src);
+  for (int s = 1; s < j.splits; ++s) {
+    const float4 w = *reinterpret_cast<const float4*>(src + s * j.m * j.stride);
+    v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+  }
+  return v;
+}
+template <typename T>
+__global__ void __launch_bounds__(256) sum_splits_kernel(const __grid_constant__ SumJobs p) {
+  const long long total = p.q[p.n - 1].end;
+  for (long long g = blockIdx.x * 256ll + threadIdx.x; g < total; g += gridDim.x * 256ll) {
+    int q = 0;
+    while (g >= p.q[q].end) ++q;
+    const SumJob& j = p.q[q];
+    const long long i = q ? g - p.q[q - 1].end : g;
+    const int per_row = (j.n + 3) / 4;
     const long long r = i / per_row;
     const int c = (int)(i - r * per_row) * 4;
-    const float* src = partial + r * stride + c;
-    float4 v = *reinterpret_cast<const float4*>(src);
-    for (int s = 1; s < splits; ++s) {
-      const float4 w = *reinterpret_cast<const float4*>(src + s * m * stride);
-      v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
-    }
-    O* o = out + r * out_stride + c;
+    const float4 v = sum_shares(j, r, c);
     const float f[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (c + j < n) o[j] = from_f32<O>(f[j]);
+    for (int k = 0; k < 4; ++k)
+      if (c + k < j.n) {
+        if (j.out_f32) ((float*)j.out)[r * j.out_stride + c + k] = f[k];
+        else ((T*)j.out)[r * j.out_stride + c + k] = from_f32<T>(f[k]);
+      }
   }
+}
+// ... and what GEMM_LINEAR does to them
+template <typename T>
+__global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ SumJob j, const __grid_constant__ GemmDesc d) {
+  const int per_row = (j.n + 3) / 4;
+  with_activation_dev(d.act, [&](auto act) {
+    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < j.end; i += gridDim.x * 256ll) {
+      const long long r = i / per_row;
+      const int c = (int)(i - r * per_row) * 4;
+      const float4 v = sum_shares(j, r, c);
+      const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (c + k < j.n) gemm_element<T, T, GEMM_LINEAR, decltype(act)::value>(d, r, c + k, f[k], 0.0f);
+    }
+  });
 }
 
 // an operand as it lies in memory
@@ -158,29 +243,134 @@ struct Stored {
   const void* p;
   long long rows, cols, stride;
   bool mn;  // rows are k
-  const void* parts = nullptr;
   // as TMA wants 16-bit rows
   bool aligned() const { return ((uintptr_t)p & 15) == 0 && (rows == 1 || stride % 8 == 0); }
   long long padded() const { return (cols + 7) / 8 * 8; }
 };
-Stored stored(const GemmOperand& o, long long rows, long long k) {
-  if (o.k == 1) return {o.p, rows, k, o.row, false, o.parts};
-  return {o.p, k, rows, o.k, true, o.parts};
+inline Stored stored(const GemmOperand& o, long long rows, long long k) {
+  if (o.k == 1) return {o.p, rows, k, o.row, false};
+  return {o.p, k, rows, o.k, true};
 }
-bool rows_of_pieces(const void* p, long long stride, int dtype) { return ((uintptr_t)p & 15) == 0 && stride * (long long)dtype_size(dtype) % 16 == 0; }
+inline bool rows_of_pieces(const void* p, long long stride, int dtype) { return ((uintptr_t)p & 15) == 0 && stride * (long long)dtype_size(dtype) % 16 == 0; }
 
-int launch_sum_splits(const float* partial, int splits, const GemmDesc& d, int stride, cudaStream_t st) {
-  const long long blocks = ceil_div(d.m * ((d.n + 3) / 4), 256), most = 16ll * sm_count();
+// What a launch is made of: the problems, the matrices that they read (each once, whoever reads it), the workspace.
+struct GtPlan {
+  int cg, n, n_mat, units;
+  GtProblem q[GT_PROBLEMS];  // without addresses
+  int splits[GT_PROBLEMS];
+  Stored mat[GT_MATRICES];
+  bool copied[GT_MATRICES];
+  size_t copy[GT_MATRICES], partial[GT_PROBLEMS], total;  // offsets
+  bool any_split() const {
+    for (int i = 0; i < n; ++i)
+      if (splits[i] > 1) return true;
+    return false;
+  }
+};
+// tile_m, tile_n: of a unit; slots: units that run side by side; share: slabs of k that a share has at least (a product with more to it than the
+// sum: twice that); copy_bytes: of a matrix that is not read as it lies in memory, 0 otherwise
+template <typename CopyBytes>
+GtPlan gt_plan(const GemmDesc* d, int n, int tile_m, int tile_n, int slots, int share, CopyBytes&& copy_bytes) {
+  GtPlan pl{};
+  pl.n = n;
+  long long work = 0;
+  for (int i = 0; i < n; ++i) {
+    const bool dual = d[i].kind == GEMM_GATED;
+    GtProblem& q = pl.q[i];
+    q.m = (int)d[i].m;
+    q.n = d[i].n;
+    q.tiles_n = (int)ceil_div(q.n, tile_n / (dual ? 2 : 1));
+    q.tiles = (int)ceil_div(q.m, tile_m) * q.tiles_n;
+    for (int s = 0; s < d[i].n_seg; ++s) {
+      const int kb = (int)ceil_div(d[i].k[s], GT_BK);
+      q.kb_total += kb;
+      if (s == 0) q.kb0 = kb;
+    }
+    work += (long long)q.tiles * q.kb_total;
+    for (int s = 0; s < 2; ++s)
+      for (int is_b = 0; is_b < 2; ++is_b) {
+        if (s >= (is_b && dual ? 2 : d[i].n_seg)) continue;
+        const Stored o = stored(is_b ? d[i].b[s] : d[i].a[s], is_b ? d[i].n : d[i].m, d[i].k[dual ? 0 : s]);
+        (is_b ? q.b_mn : q.a_mn) = o.mn;
+        int at = 0;
+        while (at < pl.n_mat && !(pl.mat[at].p == o.p && o.p && pl.mat[at].rows == o.rows && pl.mat[at].cols == o.cols && pl.mat[at].stride == o.stride)) ++at;
+        if (at == pl.n_mat) pl.mat[pl.n_mat++] = o;
+        (is_b ? q.b : q.a)[s] = (unsigned char)at;
+      }
+  }
+  // A share of k for every slot, where that leaves a share worth its start and the pass that adds the shares up.
+  long long ideal = ceil_div(work, slots);
+  if (ideal < share) ideal = share;
+  size_t off = 0;
+  for (int i = 0; i < n; ++i) {
+    GtProblem& q = pl.q[i];
+    const bool plain = gemm_plain(d[i]);
+    const long long least = plain ? ideal : 2 * ideal;
+    long long s = (plain || (n == 1 && d[i].kind == GEMM_LINEAR)) && q.kb_total >= 2 * least ? q.kb_total / least : 1;
+    q.kb_per = (int)ceil_div(q.kb_total, s);
+    pl.splits[i] = (int)ceil_div(q.kb_total, q.kb_per);
+    q.unit0 = pl.units;
+    pl.units += q.tiles * pl.splits[i];
+    if (pl.splits[i] > 1) {
+      pl.partial[i] = off;
+      off += align_up((size_t)pl.splits[i] * q.m * ((q.n + 3) / 4 * 4) * sizeof(float), 256);
+    }
+  }
+  for (int i = 0; i < pl.n_mat; ++i) {
+    const size_t bytes = copy_bytes(pl.mat[i]);
+    pl.copied[i] = bytes > 0;
+    pl.copy[i] = off;
+    off += bytes;
+  }
+  pl.total = off;
+  return pl;
+}
+// the addresses: where each problem's sums go
+inline void gt_outputs(GtPlan& pl, const GemmDesc* d, void* ws, int operand_dtype) {
+  for (int i = 0; i < pl.n; ++i) {
+    GtProblem& q = pl.q[i];
+    if (pl.splits[i] > 1) {
+      q.out = (char*)ws + pl.partial[i];
+      q.out_stride = (q.n + 3) / 4 * 4;
+      q.split_stride = q.m * q.out_stride;
+      q.out_vec = q.out_f32 = true;
+    } else {
+      q.out = d[i].out[0];
+      q.out_stride = d[i].out_stride;
+      q.out_f32 = d[i].out_dtype == LIK_F32;
+      q.out_vec = rows_of_pieces(q.out, q.out_stride, d[i].out_dtype);
+    }
+  }
+}
+template <typename T>
+int launch_sum_splits(const GtPlan& pl, const GemmDesc* d, cudaStream_t st) {
+  SumJobs jobs{};
+  long long total = 0;
+  for (int i = 0; i < pl.n; ++i) {
+    if (pl.splits[i] == 1) continue;
+    const GtProblem& q = pl.q[i];
+    SumJob& j = jobs.q[jobs.n++];
+    j.partial = (const float*)q.out;
+    j.splits = pl.splits[i];
+    j.n = q.n;
+    j.stride = (int)q.out_stride;
+    j.m = q.m;
+    j.end = total += (long long)q.m * ((q.n + 3) / 4);
+    j.out_stride = d[i].out_stride;
+    j.out = d[i].out[0];
+    j.out_f32 = d[i].out_dtype == LIK_F32;
+  }
+  if (!jobs.n) return LIK_OK;
+  const long long blocks = ceil_div(total, 256), most = 16ll * sm_count();
   const unsigned grid = (unsigned)(blocks < most ? blocks : most);
-  if (d.out_dtype == LIK_F32) sum_splits_kernel<float><<<grid, 256, 0, st>>>(partial, splits, d.m, d.n, stride, (float*)d.out[0], d.out_stride), count_launch();
-  else if (d.out_dtype == LIK_F16) sum_splits_kernel<__half><<<grid, 256, 0, st>>>(partial, splits, d.m, d.n, stride, (__half*)d.out[0], d.out_stride), count_launch();
-  else sum_splits_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(partial, splits, d.m, d.n, stride, (__nv_bfloat16*)d.out[0], d.out_stride), count_launch();
+  if (gemm_plain(d[0])) sum_splits_kernel<T><<<grid, 256, 0, st>>>(jobs), count_launch();
+  else finish_kernel<T><<<grid, 256, 0, st>>>(jobs.q[0], d[0]), count_launch();
   LIK_CUDA_OK(cudaGetLastError());
   return LIK_OK;
 }
 // Tensor maps are made by the driver, which wants the device's context to be current: a thread that has made no call of the runtime's
 // yet (autograd's, on the first backward of a process) has none until it says which device it is on.
-int make_context_current() {
+inline int make_context_current() {
   int dev = 0;
   LIK_CUDA_OK(cudaGetDevice(&dev));
   LIK_CUDA_OK(cudaSetDevice(dev));

@@ -21,17 +21,18 @@ constexpr int GF_SLOT = 32 * 32 * 4;
 constexpr size_t GF_CTL_AT = (size_t)GF_STAGES * GF_STAGE_BYTES + GF_EPI * GF_SLOT;
 
 struct GfMaps {
-  CUtensorMap a[2][GF_PARTS], b[2][GF_PARTS];
+  CUtensorMap m[GT_MATRICES][GF_PARTS];
 };
 struct GfParams {
-  int m, n;
-  int kb0, kb_total, kb_per, tiles, tiles_n, units;
-  bool a_mn, b_mn;
+  GtProblem q[GT_PROBLEMS];
+  int n_prob, units;
+  bool raw;  // products only: several of them, or shares of one
+  // what follows is for a single problem
   int act;
   const float *bias[2], *residual;
-  float *out[2], *kept[2];
-  long long residual_stride, out_stride, kept_stride, split_stride;
-  bool residual_vec, out_vec, keep;
+  float *out2, *kept[2];
+  long long residual_stride, kept_stride;
+  bool residual_vec, keep;
   int* status;
 };
 struct GfCtl {
@@ -76,14 +77,14 @@ __global__ void __launch_bounds__(GF_THREADS, 1) gemm_f32_kernel(const __grid_co
     uint32_t phase = 0;
     bool ok = true;
     for (int u = blockIdx.x; u < p.units && ok; u += gridDim.x) {
-      const int split = u / p.tiles, i = u - split * p.tiles, tm = i / p.tiles_n, tn = i - tm * p.tiles_n;
-      const int kb_lo = split * p.kb_per, kb_hi = min(kb_lo + p.kb_per, p.kb_total);
-      for (int kb = kb_lo; kb < kb_hi; ++kb) {
+      const GtUnit t = gt_unit<KIND == GEMM_LINEAR>(p.q, p.n_prob, u);
+      const GtProblem& pr = p.q[t.q];
+      for (int kb = t.kb_lo; kb < t.kb_hi; ++kb) {
         if (!wait_bar_all(&ctl->empty[s], phase ^ 1, &ctl->wait, p.status)) {
           ok = false;
           break;
         }
-        const int seg = kb < p.kb0 ? 0 : 1, k = (kb - (seg ? p.kb0 : 0)) * GT_BK;
+        const int seg = kb < pr.kb0 ? 0 : 1, k = (kb - (seg ? pr.kb0 : 0)) * GT_BK;
         if (elect_one()) {
           const uint32_t bar = smem_u32(&ctl->full[s]);
           mbar_arrive_expect_tx(bar, GF_STAGE_BYTES);
@@ -92,9 +93,9 @@ __global__ void __launch_bounds__(GF_THREADS, 1) gemm_f32_kernel(const __grid_co
           for (int q = 0; q < GF_PARTS; ++q)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const int ra = tm * 128 + h * GT_BOX, rb = tn * OUT_N + (DUAL ? 0 : h * GT_BOX);
-              tma_load_2d(dst + q * GF_OPERAND + h * GT_BOX_BYTES, &maps.a[seg][q], p.a_mn ? ra : k, p.a_mn ? k : ra, bar);
-              tma_load_2d(dst + (GF_PARTS + q) * GF_OPERAND + h * GT_BOX_BYTES, &maps.b[DUAL ? h : seg][q], p.b_mn ? rb : k, p.b_mn ? k : rb, bar);
+              const int ra = t.tm * 128 + h * GT_BOX, rb = t.tn * OUT_N + (DUAL ? 0 : h * GT_BOX);
+              tma_load_2d(dst + q * GF_OPERAND + h * GT_BOX_BYTES, &maps.m[pr.a[seg]][q], pr.a_mn ? ra : k, pr.a_mn ? k : ra, bar);
+              tma_load_2d(dst + (GF_PARTS + q) * GF_OPERAND + h * GT_BOX_BYTES, &maps.m[pr.b[DUAL ? h : seg]][q], pr.b_mn ? rb : k, pr.b_mn ? k : rb, bar);
             }
         }
         __syncwarp();
@@ -120,13 +121,14 @@ __global__ void __launch_bounds__(GF_THREADS, 1) gemm_f32_kernel(const __grid_co
     uint32_t phase = 0;
     bool ok = true;
     const uint32_t hi = (uint32_t)(smem_desc_sw128(0) >> 32);
-    const uint32_t a_lbo = (p.a_mn ? GT_BOX_BYTES >> 4 : 1) << 16, b_lbo = (p.b_mn ? GT_BOX_BYTES >> 4 : 1) << 16;
-    const uint32_t a_step = p.a_mn ? 128 : 2, b_step = p.b_mn ? 128 : 2;
-    const uint32_t idesc = instr_desc(1, GF_BN) | ((p.a_mn ? 1u : 0u) << 15) | ((p.b_mn ? 1u : 0u) << 16);
     for (int u = blockIdx.x; u < p.units && ok; u += gridDim.x) {
-      const int split = u / p.tiles, kb_lo = split * p.kb_per, kb_hi = min(kb_lo + p.kb_per, p.kb_total);
-      for (int kb = kb_lo; kb < kb_hi && ok; ++it) {
-        const int buf = it & 1, end = min(kb + GF_DRAIN, kb_hi);
+      const GtUnit t = gt_unit<KIND == GEMM_LINEAR>(p.q, p.n_prob, u);
+      const GtProblem& pr = p.q[t.q];
+      const uint32_t a_lbo = (pr.a_mn ? GT_BOX_BYTES >> 4 : 1) << 16, b_lbo = (pr.b_mn ? GT_BOX_BYTES >> 4 : 1) << 16;
+      const uint32_t a_step = pr.a_mn ? 128 : 2, b_step = pr.b_mn ? 128 : 2;
+      const uint32_t idesc = instr_desc(1, GF_BN) | ((pr.a_mn ? 1u : 0u) << 15) | ((pr.b_mn ? 1u : 0u) << 16);
+      for (int kb = t.kb_lo; kb < t.kb_hi && ok; ++it) {
+        const int buf = it & 1, end = min(kb + GF_DRAIN, t.kb_hi);
         if (!(ok = wait_bar_all(&ctl->acc_empty[buf], ((it >> 1) & 1) ^ 1, &ctl->wait, p.status))) break;
         tc_fence_after();
         for (int first = kb; kb < end; ++kb) {
@@ -158,13 +160,13 @@ __global__ void __launch_bounds__(GF_THREADS, 1) gemm_f32_kernel(const __grid_co
     int it = 0;
     bool ok = true;
     for (int u = blockIdx.x; u < p.units && ok; u += gridDim.x) {
-      const int split = u / p.tiles, i = u - split * p.tiles, tm = i / p.tiles_n, tn = i - tm * p.tiles_n;
-      const int kb_lo = split * p.kb_per, kb_hi = min(kb_lo + p.kb_per, p.kb_total);
+      const GtUnit t = gt_unit<KIND == GEMM_LINEAR>(p.q, p.n_prob, u);
+      const GtProblem& pr = p.q[t.q];
       // the warp's 64 columns: two chunks of 32, of the result or (DUAL) one of the gate and the same one of up
       float sum[2][2][16];
 #pragma unroll
       for (int j = 0; j < 16; ++j) sum[0][0][j] = sum[0][1][j] = sum[1][0][j] = sum[1][1][j] = 0.0f;
-      for (int kb = kb_lo; kb < kb_hi; kb += GF_DRAIN, ++it) {
+      for (int kb = t.kb_lo; kb < t.kb_hi; kb += GF_DRAIN, ++it) {
         const int buf = it & 1;
         if (!(ok = wait_bar_all(&ctl->acc_full[buf], (it >> 1) & 1, &ctl->wait, p.status))) break;
         tc_fence_after();
@@ -187,7 +189,7 @@ __global__ void __launch_bounds__(GF_THREADS, 1) gemm_f32_kernel(const __grid_co
         if (lane == 0) mbar_arrive(smem_u32(&ctl->acc_empty[buf]));
       }
       if (!ok) break;
-      const int row0 = tm * 128 + quad * 32, rows = p.m - row0;
+      const int row0 = t.tm * 128 + quad * 32, rows = pr.m - row0;
       if (rows <= 0) continue;
       // 32 x 32 of a matrix between memory and the lanes' rows, by way of the slot
       auto in = [&](const float* src, long long stride, int cols, bool vec, float (&f)[2][16]) {
@@ -207,9 +209,9 @@ __global__ void __launch_bounds__(GF_THREADS, 1) gemm_f32_kernel(const __grid_co
       };
 #pragma unroll
       for (int c = 0; c < (DUAL ? 1 : 2); ++c) {
-        const int col = tn * OUT_N + (DUAL ? part * 32 : part * 64 + c * 32), left = p.n - col;
+        const int col = t.tn * OUT_N + (DUAL ? part * 32 : part * 64 + c * 32), left = pr.n - col;
         if (left <= 0) continue;
-        float* const to = p.out[0] + split * p.split_stride + row0 * p.out_stride + col;
+        float* const to = (float*)pr.out + t.split * pr.split_stride + row0 * pr.out_stride + col;
         float* const keep0 = p.kept[0] + row0 * p.kept_stride + col;
         float* const keep1 = p.kept[1] + row0 * p.kept_stride + col;
         float(&v)[2][16] = sum[c];
@@ -220,9 +222,13 @@ __global__ void __launch_bounds__(GF_THREADS, 1) gemm_f32_kernel(const __grid_co
             in(q ? keep1 : keep0, p.kept_stride, left, true, f);
 #pragma unroll
             for (int j = 0; j < 32; ++j) f[j / 16][j % 16] *= v[j / 16][j % 16];
-            out(q ? p.out[1] + row0 * p.out_stride + col : to, p.out_stride, left, true, f);
+            out(q ? p.out2 + row0 * pr.out_stride + col : to, pr.out_stride, left, true, f);
           }
         } else {
+          if (KIND == GEMM_LINEAR && p.raw) {
+            out(to, pr.out_stride, left, pr.out_vec, v);
+            continue;
+          }
           if (p.bias[0]) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j / 16][j % 16] += j < left ? __ldg(p.bias[0] + col + j) : 0.0f;
@@ -258,7 +264,7 @@ __global__ void __launch_bounds__(GF_THREADS, 1) gemm_f32_kernel(const __grid_co
               for (int j = 0; j < 32; ++j) v[j / 16][j % 16] += f[j / 16][j % 16];
             }
           }
-          out(to, p.out_stride, left, p.out_vec, v);
+          out(to, pr.out_stride, left, pr.out_vec, v);
         }
       }
     }
@@ -283,10 +289,9 @@ __device__ __forceinline__ void cut3(float x, uint32_t (&p)[3]) {
 }
 // matrices in their three parts, rows of whole 16-byte pieces (zeros behind the columns).  Bound by memory: 4 bytes in and 6 out per value.
 struct CutJobs {
-  CutMatrix m[CUT_MOST];
-  long long end[CUT_MOST];  // pieces up to and with this matrix
-  int vecs[CUT_MOST];
-  bool vec[CUT_MOST];
+  Stored m[GT_MATRICES];
+  void* parts[GT_MATRICES];
+  long long end[GT_MATRICES];  // pieces up to and with this matrix
   int n;
 };
 __global__ void __launch_bounds__(256) cut_kernel(const __grid_constant__ CutJobs p) {
@@ -295,12 +300,12 @@ __global__ void __launch_bounds__(256) cut_kernel(const __grid_constant__ CutJob
     int q = 0;
     while (g >= p.end[q]) ++q;
     const long long i = q ? g - p.end[q - 1] : g;
-    const int vecs = p.vecs[q], cols = (int)p.m[q].cols;
+    const int cols = (int)p.m[q].cols, vecs = (cols + 7) / 8;
     const long long r = i / vecs;
     const int c = (int)(i - r * vecs) * 8;
-    const float* s = (const float*)p.m[q].src + r * p.m[q].stride + c;
+    const float* s = (const float*)p.m[q].p + r * p.m[q].stride + c;
     float x[8];
-    if (p.vec[q] && c + 8 <= cols) {
+    if (((uintptr_t)s & 15) == 0 && c + 8 <= cols) {
       load_vec<float, 8>(s, x);
     } else {
 #pragma unroll
@@ -315,51 +320,15 @@ __global__ void __launch_bounds__(256) cut_kernel(const __grid_constant__ CutJob
 #pragma unroll
       for (int k = 0; k < 3; ++k) w[k][j] = lo[k] | hi[k] << 16;
     }
-    uint4* dst = (uint4*)p.m[q].parts + i;
+    uint4* dst = (uint4*)p.parts[q] + i;
     const long long part = p.m[q].rows * vecs;
 #pragma unroll
     for (int k = 0; k < 3; ++k) dst[k * part] = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
   }
 }
 
-struct GfPlan {
-  int tiles_m, tiles_n, kb[2], kb_total, kb_per, splits, partial_stride;
-  size_t parts[4], partial, total;  // offsets: the parts of a[0], a[1], b[0], b[1]
-};
-// whether operand i (a[0], a[1], b[0], b[1]) is there
-bool operand_there(const GemmDesc& d, int i) { return (i & 1) < (i >= 2 && d.kind == GEMM_GATED ? 2 : d.n_seg); }
-Stored operand_stored(const GemmDesc& d, int i) {
-  return stored(i >= 2 ? d.b[i & 1] : d.a[i & 1], i >= 2 ? d.n : d.m, d.k[d.kind == GEMM_GATED ? 0 : i & 1]);
-}
-GfPlan gf_plan(const GemmDesc& d) {
-  GfPlan pl{};
-  for (int s = 0; s < d.n_seg; ++s) pl.kb_total += pl.kb[s] = (int)ceil_div(d.k[s], GT_BK);
-  pl.tiles_m = (int)ceil_div(d.m, 128);
-  pl.tiles_n = (int)ceil_div(d.n, d.kind == GEMM_GATED ? 64 : 128);
-  const long long t = (long long)pl.tiles_m * pl.tiles_n, sms = sm_count();
-  pl.splits = 1;
-  if (gemm_plain(d) && t < sms) {
-    long long want = sms / t;
-    if (want > pl.kb_total / 4) want = pl.kb_total / 4;
-    if (want > 1) pl.splits = (int)want;
-  }
-  pl.kb_per = (int)ceil_div(pl.kb_total, pl.splits);
-  pl.splits = (int)ceil_div(pl.kb_total, pl.kb_per);
-  size_t off = 0;
-  for (int i = 0; i < 4; ++i) {
-    if (!operand_there(d, i)) continue;
-    const Stored o = operand_stored(d, i);
-    if (o.parts) continue;
-    pl.parts[i] = off;
-    off += cut_bytes(o.rows, o.cols);
-  }
-  if (pl.splits > 1) {
-    pl.partial = off;
-    pl.partial_stride = (d.n + 3) / 4 * 4;
-    off += align_up((size_t)pl.splits * d.m * pl.partial_stride * sizeof(float), 256);
-  }
-  pl.total = off;
-  return pl;
+GtPlan f32_plan(const GemmDesc* d, int n) {
+  return gt_plan(d, n, 128, GF_BN, sm_count(), 4, [](const Stored& o) { return align_up((size_t)o.rows * o.padded() * 2 * GF_PARTS, 256); });
 }
 template <int KIND>
 int run_f32(const GfMaps& maps, const GfParams& p, cudaStream_t st) {
@@ -371,28 +340,10 @@ int run_f32(const GfMaps& maps, const GfParams& p, cudaStream_t st) {
 
 }  // namespace
 
-size_t gemm_f32_workspace(const GemmDesc& d) { return gf_plan(d).total; }
+size_t gemm_f32_workspace(const GemmDesc* d, int n) { return f32_plan(d, n).total; }
 
-size_t cut_bytes(long long rows, long long cols) { return align_up((size_t)rows * ((cols + 7) / 8) * 16 * GF_PARTS, 256); }
-int launch_cut(const CutMatrix* m, int n, cudaStream_t st) {
-  if (!n) return LIK_OK;
-  CutJobs p{};
-  long long total = 0;
-  for (int i = 0; i < n; ++i) {
-    p.m[i] = m[i];
-    p.vecs[i] = (int)((m[i].cols + 7) / 8);
-    p.vec[i] = ((uintptr_t)m[i].src & 15) == 0 && m[i].stride % 4 == 0;
-    p.end[i] = total += m[i].rows * p.vecs[i];
-  }
-  p.n = n;
-  const long long blocks = ceil_div(total, 256), most = 16ll * sm_count();
-  cut_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, st>>>(p), count_launch();
-  LIK_CUDA_OK(cudaGetLastError());
-  return LIK_OK;
-}
-
-int launch_gemm_f32(const GemmDesc& d, void* ws, size_t ws_bytes, int* status, cudaStream_t st) {
-  const GfPlan pl = gf_plan(d);
+int launch_gemm_f32(const GemmDesc* d, int n, void* ws, size_t ws_bytes, int* status, cudaStream_t st) {
+  GtPlan pl = f32_plan(d, n);
   if (ws_bytes < pl.total || (pl.total && !ws)) {
     set_error("workspace too small");
     return LIK_ERR_WORKSPACE;
@@ -400,55 +351,41 @@ int launch_gemm_f32(const GemmDesc& d, void* ws, size_t ws_bytes, int* status, c
   if (int rc = make_context_current()) return rc;
   GfMaps maps{};
   GfParams p{};
-  CutMatrix cuts[4];
-  int n_cuts = 0;
-  for (int i = 0; i < 4; ++i) {
-    if (!operand_there(d, i)) continue;
-    const Stored o = operand_stored(d, i);
-    (i >= 2 ? p.b_mn : p.a_mn) = o.mn;
-    const uint8_t* parts = (const uint8_t*)o.parts;
-    if (!parts) {
-      cuts[n_cuts++] = {o.p, o.rows, o.cols, o.stride, (uint8_t*)ws + pl.parts[i]};
-      parts = (const uint8_t*)ws + pl.parts[i];
-    }
-    for (int q = 0; q < GF_PARTS; ++q) {
-      CUtensorMap* map = i >= 2 ? &maps.b[i & 1][q] : &maps.a[i & 1][q];
-      if (int rc = make_tmap_rows(map, parts + q * o.rows * o.padded() * 2, LIK_BF16, o.cols, o.rows, o.padded(), GT_BOX)) return rc;
-    }
+  CutJobs cuts{};
+  long long total = 0;
+  for (int i = 0; i < pl.n_mat; ++i) {
+    const Stored& o = pl.mat[i];
+    uint8_t* parts = (uint8_t*)ws + pl.copy[i];
+    cuts.m[i] = o;
+    cuts.parts[i] = parts;
+    cuts.end[i] = total += o.rows * (o.padded() / 8);
+    for (int q = 0; q < GF_PARTS; ++q)
+      if (int rc = make_tmap_rows(&maps.m[i][q], parts + q * o.rows * o.padded() * 2, LIK_BF16, o.cols, o.rows, o.padded(), GT_BOX)) return rc;
   }
-  if (int rc = launch_cut(cuts, n_cuts, st)) return rc;
-  if (pl.splits > 1) {
-    p.out[0] = (float*)((char*)ws + pl.partial);
-    p.out_stride = pl.partial_stride;
-    p.split_stride = d.m * pl.partial_stride;
-    p.out_vec = true;
-  } else {
-    for (int i = 0; i < 2; ++i) p.out[i] = (float*)d.out[i];
-    p.out_stride = d.out_stride;
-    p.out_vec = rows_of_pieces(d.out[0], d.out_stride, LIK_F32);
-  }
-  p.m = (int)d.m;
-  p.n = d.n;
-  p.kb0 = pl.kb[0];
-  p.kb_total = pl.kb_total;
-  p.kb_per = pl.kb_per;
-  p.tiles_n = pl.tiles_n;
-  p.tiles = pl.tiles_m * pl.tiles_n;
-  p.units = p.tiles * pl.splits;
-  p.act = d.act;
+  cuts.n = pl.n_mat;
+  const long long blocks = ceil_div(total, 256), most = 16ll * sm_count();
+  cut_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, st>>>(cuts), count_launch();
+  LIK_CUDA_OK(cudaGetLastError());
+  gt_outputs(pl, d, ws, LIK_F32);
+  for (int i = 0; i < n; ++i) p.q[i] = pl.q[i];
+  p.n_prob = n;
+  p.units = pl.units;
+  p.raw = n > 1 || pl.any_split();
+  p.act = d->act;
   for (int i = 0; i < 2; ++i) {
-    p.bias[i] = (const float*)d.bias[i];
-    p.kept[i] = (float*)d.kept[i];
+    p.bias[i] = (const float*)d->bias[i];
+    p.kept[i] = (float*)d->kept[i];
   }
-  p.keep = d.kind != GEMM_GATED_BWD && d.kept[0];
-  p.kept_stride = d.kept_stride;
-  p.residual = (const float*)d.residual;
-  p.residual_stride = d.residual_stride;
-  p.residual_vec = d.n % 4 == 0 && rows_of_pieces(d.residual, d.residual_stride, LIK_F32);
+  p.out2 = (float*)d->out[1];
+  p.keep = d->kind != GEMM_GATED_BWD && d->kept[0];
+  p.kept_stride = d->kept_stride;
+  p.residual = (const float*)d->residual;
+  p.residual_stride = d->residual_stride;
+  p.residual_vec = d->n % 4 == 0 && rows_of_pieces(d->residual, d->residual_stride, LIK_F32);
   p.status = status;
-  const int rc = d.kind == GEMM_GATED ? run_f32<GEMM_GATED>(maps, p, st) : (d.kind == GEMM_GATED_BWD ? run_f32<GEMM_GATED_BWD>(maps, p, st) : run_f32<GEMM_LINEAR>(maps, p, st));
-  if (rc || pl.splits == 1) return rc;
-  return launch_sum_splits((const float*)((char*)ws + pl.partial), pl.splits, d, pl.partial_stride, st);
+  if (int rc = d->kind == GEMM_GATED ? run_f32<GEMM_GATED>(maps, p, st) : (d->kind == GEMM_GATED_BWD ? run_f32<GEMM_GATED_BWD>(maps, p, st) : run_f32<GEMM_LINEAR>(maps, p, st)))
+    return rc;
+  return launch_sum_splits<float>(pl, d, st);
 }
 
 }  // namespace lik

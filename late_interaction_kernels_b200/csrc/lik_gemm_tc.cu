@@ -29,17 +29,18 @@ struct GtWarps {
 };
 
 struct GtMaps {
-  CUtensorMap a[2], b[2];
+  CUtensorMap m[GT_MATRICES];
 };
 struct GtParams {
-  int m, n, n_seg;
-  int kb0, kb_total, kb_per, tiles, tiles_n, units;
-  bool a_mn, b_mn, bf16;
+  GtProblem q[GT_PROBLEMS];
+  int n_prob, units;
+  bool bf16;
+  // what follows is for a single problem
   int act;
   const void *bias[2], *residual;
-  void *out[2], *kept[2];  // kept: written, or read by GEMM_GATED_BWD
-  long long residual_stride, out_stride, kept_stride, split_stride;
-  bool bias_vec, residual_vec, out_vec, keep;  // *_vec: rows of whole 16-byte pieces
+  void *out2, *kept[2];  // kept: written, or read by GEMM_GATED_BWD
+  long long residual_stride, kept_stride;
+  bool bias_vec, residual_vec, keep;  // *_vec: rows of whole 16-byte pieces
   int* status;
 };
 struct GtCtl {
@@ -110,36 +111,22 @@ __device__ __forceinline__ void gt_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
 }
 
-struct GtUnit {
-  int tm, tn, split, kb_lo, kb_hi;
-};
-__device__ __forceinline__ GtUnit gt_unit(const GtParams& p, int u) {
-  GtUnit t;
-  t.split = u / p.tiles;
-  const int i = u - t.split * p.tiles;
-  t.tm = i / p.tiles_n;
-  t.tn = i - t.tm * p.tiles_n;
-  t.kb_lo = t.split * p.kb_per;
-  t.kb_hi = min(t.kb_lo + p.kb_per, p.kb_total);
-  return t;
-}
-
 // the chunks of a warp that have anything in them, in the order in which it comes to them
 template <int CG, int OUT_N, int WARP_N>
 __device__ __forceinline__ bool gt_chunk(const GtParams& p, int u, int c, int rank, int quad, int part, int& col, int& row0) {
-  const GtUnit t = gt_unit(p, u);
+  const GtUnit t = gt_unit<false>(p.q, 1, u);
   row0 = t.tm * (128 * CG) + rank * 128 + quad * 32;
   col = t.tn * OUT_N + part * WARP_N + c * 32;
-  return row0 < p.m && col < p.n;
+  return row0 < p.q[0].m && col < p.q[0].n;
 }
 
-// RES: with a residual (GEMM_LINEAR)
+// RES: with a residual (GEMM_LINEAR).  O fp32: plain products, several of them, in fp32 or T, or shares of one.
 template <int CG, int KIND, bool RES, typename T, typename O>
 __global__ void __launch_bounds__(GtWarps<KIND, !std::is_same<T, O>::value>::THREADS, 1) gemm_tc_kernel(const __grid_constant__ GtMaps maps,
                                                                                                        const __grid_constant__ GtParams p) {
   using Warps = GtWarps<KIND, !std::is_same<T, O>::value>;
   constexpr int STAGES = GT_STAGES, EPI = Warps::EPI;
-  constexpr bool DUAL = KIND == GEMM_GATED;
+  constexpr bool DUAL = KIND == GEMM_GATED, MULTI = !std::is_same<T, O>::value;
   constexpr int BN = CG == 2 ? 256 : 128;          // columns of an accumulator
   constexpr int OUT_N = DUAL ? BN / 2 : BN;        // columns of the result in a unit
   constexpr int WARP_N = OUT_N / (EPI / 4), CHUNKS = WARP_N / 32;  // columns of an epilogue warp, 32 at a time
@@ -175,7 +162,8 @@ __global__ void __launch_bounds__(GtWarps<KIND, !std::is_same<T, O>::value>::THR
     uint32_t phase = 0;
     bool ok = true;
     for (int u = first; u < p.units && ok; u += step) {
-      const GtUnit t = gt_unit(p, u);
+      const GtUnit t = gt_unit<MULTI>(p.q, p.n_prob, u);
+      const GtProblem& q = p.q[t.q];
       const int row_a = t.tm * (128 * CG) + rank * 128;
       const int row_b = DUAL ? t.tn * OUT_N : t.tn * BN + rank * (BN / CG);
       for (int kb = t.kb_lo; kb < t.kb_hi; ++kb) {
@@ -183,7 +171,7 @@ __global__ void __launch_bounds__(GtWarps<KIND, !std::is_same<T, O>::value>::THR
           ok = false;
           break;
         }
-        const int seg = kb < p.kb0 ? 0 : 1, k = (kb - (seg ? p.kb0 : 0)) * GT_BK;
+        const int seg = kb < q.kb0 ? 0 : 1, k = (kb - (seg ? q.kb0 : 0)) * GT_BK;
         if (elect_one()) {
           const uint32_t local = smem_u32(&ctl->full[s]), bar = CG == 2 ? leader_addr(local) : local;
           if (rank == 0) mbar_arrive_expect_tx(local, CG * GT_STAGE_BYTES);
@@ -191,13 +179,13 @@ __global__ void __launch_bounds__(GtWarps<KIND, !std::is_same<T, O>::value>::THR
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const int r = row_a + i * GT_BOX;
-            gt_load<CG>(dst + i * GT_BOX_BYTES, &maps.a[seg], p.a_mn ? r : k, p.a_mn ? k : r, bar);
+            gt_load<CG>(dst + i * GT_BOX_BYTES, &maps.m[q.a[seg]], q.a_mn ? r : k, q.a_mn ? k : r, bar);
           }
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const int r = row_b + (DUAL && CG == 1 ? 0 : i * GT_BOX);
-            const CUtensorMap* map = DUAL ? (CG == 2 ? &maps.b[rank] : &maps.b[i]) : &maps.b[seg];
-            gt_load<CG>(dst + (2 + i) * GT_BOX_BYTES, map, p.b_mn ? r : k, p.b_mn ? k : r, bar);
+            const CUtensorMap* map = &maps.m[q.b[DUAL ? (CG == 2 ? rank : i) : seg]];
+            gt_load<CG>(dst + (2 + i) * GT_BOX_BYTES, map, q.b_mn ? r : k, q.b_mn ? k : r, bar);
           }
         }
         __syncwarp();
@@ -225,12 +213,13 @@ __global__ void __launch_bounds__(GtWarps<KIND, !std::is_same<T, O>::value>::THR
       bool ok = true;
       // (leading dimension: the next 64 rows of an MN-major operand; k steps of 16: 32 bytes along a row, or 16 rows of 128 bytes)
       const uint32_t hi = (uint32_t)(smem_desc_sw128(0) >> 32);
-      const uint32_t a_lbo = (p.a_mn ? GT_BOX_BYTES >> 4 : 1) << 16, b_lbo = (p.b_mn ? GT_BOX_BYTES >> 4 : 1) << 16;
-      const uint32_t a_step = p.a_mn ? 128 : 2, b_step = p.b_mn ? 128 : 2;
-      const uint32_t idesc = (1u << 4) | ((p.bf16 ? 1u : 0u) << 7) | ((p.bf16 ? 1u : 0u) << 10) | ((p.a_mn ? 1u : 0u) << 15) | ((p.b_mn ? 1u : 0u) << 16) |
-                             ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(128 * CG >> 4) << 24);
       for (int u = first; u < p.units && ok; u += step, ++it) {
-        const GtUnit t = gt_unit(p, u);
+        const GtUnit t = gt_unit<MULTI>(p.q, p.n_prob, u);
+      const GtProblem& q = p.q[t.q];
+        const uint32_t a_lbo = (q.a_mn ? GT_BOX_BYTES >> 4 : 1) << 16, b_lbo = (q.b_mn ? GT_BOX_BYTES >> 4 : 1) << 16;
+        const uint32_t a_step = q.a_mn ? 128 : 2, b_step = q.b_mn ? 128 : 2;
+        const uint32_t idesc = (1u << 4) | ((p.bf16 ? 1u : 0u) << 7) | ((p.bf16 ? 1u : 0u) << 10) | ((q.a_mn ? 1u : 0u) << 15) | ((q.b_mn ? 1u : 0u) << 16) |
+                               ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(128 * CG >> 4) << 24);
         const int buf = it & 1;
         if (!wait_bar_all(&ctl->acc_empty[buf], ((it >> 1) & 1) ^ 1, &ctl->wait, p.status)) break;
         tc_fence_after();
@@ -275,17 +264,18 @@ __global__ void __launch_bounds__(GtWarps<KIND, !std::is_same<T, O>::value>::THR
       if (!there) return;
       if constexpr (KIND == GEMM_GATED_BWD) {
 #pragma unroll
-        for (int q = 0; q < 2; ++q)
-          slot_fetch<T>(to + q * SLOT, lane, (const T*)p.kept[q] + row0 * p.kept_stride + col, p.kept_stride, p.m - row0, p.n - col, true);
+        for (int i = 0; i < 2; ++i)
+          slot_fetch<T>(to + i * SLOT, lane, (const T*)p.kept[i] + row0 * p.kept_stride + col, p.kept_stride, p.q[0].m - row0, p.q[0].n - col, true);
       } else if constexpr (RES) {
-        slot_fetch<T>(to, lane, (const T*)p.residual + row0 * p.residual_stride + col, p.residual_stride, p.m - row0, p.n - col, p.residual_vec);
+        slot_fetch<T>(to, lane, (const T*)p.residual + row0 * p.residual_stride + col, p.residual_stride, p.q[0].m - row0, p.q[0].n - col, p.residual_vec);
       }
     };
     if constexpr (IN > 0) fetch();
     bool ok = true;
     int it = 0;
     for (int u = first; u < p.units && ok; u += step, ++it) {
-      const GtUnit t = gt_unit(p, u);
+      const GtUnit t = gt_unit<MULTI>(p.q, p.n_prob, u);
+      const GtProblem& q = p.q[t.q];
       const int buf = it & 1;
       if (!wait_bar_all(&ctl->acc_full[buf], (it >> 1) & 1, &ctl->wait, p.status)) break;
       tc_fence_after();
@@ -294,8 +284,8 @@ __global__ void __launch_bounds__(GtWarps<KIND, !std::is_same<T, O>::value>::THR
       const uint32_t release = CG == 2 ? leader_addr(smem_u32(&ctl->acc_empty[buf])) : smem_u32(&ctl->acc_empty[buf]);
 #pragma unroll 1
       for (int c = 0; c < CHUNKS; ++c) {
-        const int in_tile = part * WARP_N + c * 32, col = t.tn * OUT_N + in_tile, left = p.n - col;
-        const bool live = row0 < p.m && left > 0;
+        const int in_tile = part * WARP_N + c * 32, col = t.tn * OUT_N + in_tile, left = q.n - col;
+        const bool live = row0 < q.m && left > 0;
         if (!live) {
           if (c + 1 == CHUNKS) {
             tc_fence_before();
@@ -314,7 +304,7 @@ __global__ void __launch_bounds__(GtWarps<KIND, !std::is_same<T, O>::value>::THR
           Raw16<T> bias[2];
           tmem_ld16(acc + in_tile + 16 * h, v);
           if constexpr (DUAL) tmem_ld16(acc + BN / 2 + in_tile + 16 * h, w);
-          if constexpr (KIND != GEMM_GATED_BWD) {
+          if constexpr (KIND != GEMM_GATED_BWD && !MULTI) {
             if (p.bias[0]) bias[0].load((const T*)p.bias[0] + col + 16 * h, left - 16 * h, p.bias_vec);
             if (DUAL && p.bias[1]) bias[1].load((const T*)p.bias[1] + col + 16 * h, left - 16 * h, p.bias_vec);
           }
@@ -327,19 +317,21 @@ __global__ void __launch_bounds__(GtWarps<KIND, !std::is_same<T, O>::value>::THR
           }
           if constexpr (KIND == GEMM_GATED_BWD) {
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
+            for (int j = 0; j < 2; ++j) {
               float f[16];
-              slot_get<T>(to + q * SLOT, lane, h, f);
+              slot_get<T>(to + j * SLOT, lane, h, f);
 #pragma unroll
               for (int i = 0; i < 16; ++i) f[i] *= v[i];
-              slot_put<O>(to + q * SLOT, lane, h, f);
+              slot_put<O>(to + j * SLOT, lane, h, f);
             }
           } else {
-            if (p.bias[0]) bias[0].add_to(v);
+            if constexpr (!MULTI) {
+              if (p.bias[0]) bias[0].add_to(v);
+            }
             if constexpr (DUAL) {
               if (p.bias[1]) bias[1].add_to(w);
             }
-            if constexpr (std::is_same<T, O>::value) {
+            if constexpr (!MULTI) {
               if (DUAL && p.keep) {
                 float f[16];
                 with_activation_dev(p.act, [&](auto act) {
@@ -369,10 +361,16 @@ __global__ void __launch_bounds__(GtWarps<KIND, !std::is_same<T, O>::value>::THR
           }
         }
         __syncwarp();
-        const int rows = p.m - row0;
-        slot_store<O>(to, lane, (O*)p.out[0] + t.split * p.split_stride + row0 * p.out_stride + col, p.out_stride, rows, left, p.out_vec);
+        const int rows = q.m - row0;
+        const long long at = t.split * q.split_stride + row0 * q.out_stride + col;
+        if constexpr (MULTI) {
+          if (q.out_f32) slot_store<float>(to, lane, (float*)q.out + at, q.out_stride, rows, left, q.out_vec);
+          else slot_store_as<T>(to, lane, (T*)q.out + at, q.out_stride, rows, left, q.out_vec);
+        } else {
+          slot_store<O>(to, lane, (O*)q.out + at, q.out_stride, rows, left, q.out_vec);
+        }
         if constexpr (KIND == GEMM_GATED_BWD) {
-          slot_store<O>(to + SLOT, lane, (O*)p.out[1] + row0 * p.out_stride + col, p.out_stride, rows, left, true);
+          slot_store<O>(to + SLOT, lane, (O*)p.out2 + row0 * q.out_stride + col, q.out_stride, rows, left, true);
         } else if constexpr (OUT > 1) {
           if (p.keep) {
             slot_store<O>(to + SLOT, lane, (O*)p.kept[0] + row0 * p.kept_stride + col, p.kept_stride, rows, left, true);
@@ -406,49 +404,21 @@ __global__ void __launch_bounds__(256) repack_kernel(const uint16_t* __restrict_
   }
 }
 
-struct GtPlan {
-  int cg, tiles_m, tiles_n, kb[2], kb_total, kb_per, splits;
-  size_t copy[4], partial, total;  // offsets; copies of a[0], a[1], b[0], b[1] where they are needed
-  bool copies[4];
-  int partial_stride;
-};
-GtPlan gt_plan(const GemmDesc& d) {
-  GtPlan pl{};
-  const bool dual = d.kind == GEMM_GATED;
+// Pairs of CTAs take tiles of 256 x 256 where there are enough of them, or enough k to cut into shares, for every pair; else single CTAs
+// tiles of 128 x 128.
+GtPlan tc_plan(const GemmDesc* d, int n) {
   const int sms = sm_count();
-  for (int s = 0; s < d.n_seg; ++s) pl.kb_total += pl.kb[s] = (int)ceil_div(d.k[s], GT_BK);
-  auto tiles = [&](int cg) { return ceil_div(d.m, 128 * cg) * ceil_div(d.n, (cg == 2 ? 256 : 128) / (dual ? 2 : 1)); };
-  const bool plain = gemm_plain(d);
-  pl.cg = tiles(2) * 2 >= sms || (plain && pl.kb_total >= 64 && d.m > 128 && d.n > 128) ? 2 : 1;
-  pl.tiles_m = (int)ceil_div(d.m, 128 * pl.cg);
-  pl.tiles_n = (int)ceil_div(d.n, (pl.cg == 2 ? 256 : 128) / (dual ? 2 : 1));
-  const long long t = (long long)pl.tiles_m * pl.tiles_n, slots = sms / pl.cg;
-  pl.splits = 1;
-  if (plain && t < slots && pl.kb_total >= 8) {
-    long long want = slots / t;
-    if (want > pl.kb_total / 4) want = pl.kb_total / 4;
-    if (want > 1) pl.splits = (int)want;
+  long long tiles = 0, work = 0;
+  bool cuttable = true;
+  for (int i = 0; i < n; ++i) {
+    const long long t = ceil_div(d[i].m, 256) * ceil_div(d[i].n, d[i].kind == GEMM_GATED ? 128 : 256);
+    tiles += t;
+    work += t * ceil_div(d[i].k[0] + d[i].k[1], GT_BK);
+    cuttable = cuttable && gemm_plain(d[i]) && d[i].m > 128 && d[i].n > 128;
   }
-  pl.kb_per = (int)ceil_div(pl.kb_total, pl.splits);
-  pl.splits = (int)ceil_div(pl.kb_total, pl.kb_per);
-  size_t off = 0;
-  for (int i = 0; i < 4; ++i) {
-    const bool is_b = i >= 2;
-    const int s = i & 1;
-    if (is_b ? s >= (dual ? 2 : d.n_seg) : s >= d.n_seg) continue;
-    const Stored o = stored(is_b ? d.b[s] : d.a[s], is_b ? d.n : d.m, d.k[dual ? 0 : s]);
-    pl.copies[i] = !o.aligned();
-    if (pl.copies[i]) {
-      pl.copy[i] = off;
-      off += align_up((size_t)o.rows * o.padded() * 2, 256);
-    }
-  }
-  if (pl.splits > 1) {
-    pl.partial = off;
-    pl.partial_stride = (d.n + 3) / 4 * 4;
-    off += align_up((size_t)pl.splits * d.m * pl.partial_stride * sizeof(float), 256);
-  }
-  pl.total = off;
+  const int cg = tiles * 2 >= sms || (cuttable && work >= 16 * (sms / 2)) ? 2 : 1;
+  GtPlan pl = gt_plan(d, n, 128 * cg, 128 * cg, sms / cg, 16, [](const Stored& o) { return o.aligned() ? (size_t)0 : align_up((size_t)o.rows * o.padded() * 2, 256); });
+  pl.cg = cg;
   return pl;
 }
 
@@ -476,34 +446,29 @@ int run_tc(int cg, const GtMaps& maps, const GtParams& p, cudaStream_t st) {
   return cg == 2 ? run_tc<2, KIND, RES, T, O>(maps, p, st) : run_tc<1, KIND, RES, T, O>(maps, p, st);
 }
 template <typename T>
-int run_tc(int kind, bool f32_out, int cg, const GtMaps& maps, const GtParams& p, cudaStream_t st) {
+int run_tc(int kind, bool multi, int cg, const GtMaps& maps, const GtParams& p, cudaStream_t st) {
   if (kind == GEMM_GATED) return run_tc<GEMM_GATED, false, T, T>(cg, maps, p, st);
   if (kind == GEMM_GATED_BWD) return run_tc<GEMM_GATED_BWD, false, T, T>(cg, maps, p, st);
-  if (f32_out) return run_tc<GEMM_LINEAR, false, T, float>(cg, maps, p, st);
+  if (multi) return run_tc<GEMM_LINEAR, false, T, float>(cg, maps, p, st);
   return p.residual ? run_tc<GEMM_LINEAR, true, T, T>(cg, maps, p, st) : run_tc<GEMM_LINEAR, false, T, T>(cg, maps, p, st);
 }
 
 }  // namespace
 
-size_t gemm_tc_workspace(const GemmDesc& d) { return gt_plan(d).total; }
+size_t gemm_tc_workspace(const GemmDesc* d, int n) { return tc_plan(d, n).total; }
 
-int launch_gemm_tc(const GemmDesc& d, void* ws, size_t ws_bytes, int* status, cudaStream_t st) {
-  const GtPlan pl = gt_plan(d);
+int launch_gemm_tc(const GemmDesc* d, int n, void* ws, size_t ws_bytes, int* status, cudaStream_t st) {
+  GtPlan pl = tc_plan(d, n);
   if (ws_bytes < pl.total || (pl.total && !ws)) {
     set_error("workspace too small");
     return LIK_ERR_WORKSPACE;
   }
   if (int rc = make_context_current()) return rc;
-  const bool dual = d.kind == GEMM_GATED;
   GtMaps maps{};
   GtParams p{};
-  for (int i = 0; i < 4; ++i) {
-    const bool is_b = i >= 2;
-    const int s = i & 1;
-    if (is_b ? s >= (dual ? 2 : d.n_seg) : s >= d.n_seg) continue;
-    Stored o = stored(is_b ? d.b[s] : d.a[s], is_b ? d.n : d.m, d.k[dual ? 0 : s]);
-    (is_b ? p.b_mn : p.a_mn) = o.mn;
-    if (pl.copies[i]) {
+  for (int i = 0; i < pl.n_mat; ++i) {
+    Stored o = pl.mat[i];
+    if (pl.copied[i]) {
       void* to = (char*)ws + pl.copy[i];
       const long long vecs = o.padded() / 8, blocks = ceil_div(o.rows * vecs, 256), most = 16ll * sm_count();
       repack_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, st>>>((const uint16_t*)o.p, o.stride, o.rows, (int)o.cols, (uint4*)to, (int)vecs), count_launch();
@@ -512,46 +477,34 @@ int launch_gemm_tc(const GemmDesc& d, void* ws, size_t ws_bytes, int* status, cu
       o.stride = o.padded();
     }
     if (o.rows == 1) o.stride = o.padded();
-    if (int rc = make_tmap_rows(is_b ? &maps.b[s] : &maps.a[s], o.p, d.dtype, o.cols, o.rows, o.stride, GT_BOX)) return rc;
+    if (int rc = make_tmap_rows(&maps.m[i], o.p, d->dtype, o.cols, o.rows, o.stride, GT_BOX)) return rc;
   }
-  const bool f32_out = pl.splits > 1 || d.out_dtype == LIK_F32;
-  if (pl.splits > 1) {
-    p.out[0] = (char*)ws + pl.partial;
-    p.out_stride = pl.partial_stride;
-    p.split_stride = d.m * pl.partial_stride;
-    p.out_vec = true;
-  } else {
-    p.out[0] = d.out[0];
-    p.out[1] = d.out[1];
-    p.out_stride = d.out_stride;
-    p.out_vec = rows_of_pieces(d.out[0], d.out_stride, d.out_dtype);
-  }
-  p.keep = d.kind != GEMM_GATED_BWD && d.kept[0];
-  p.m = (int)d.m;
-  p.n = d.n;
-  p.n_seg = d.n_seg;
-  p.kb0 = pl.kb[0];
-  p.kb_total = pl.kb_total;
-  p.kb_per = pl.kb_per;
-  p.tiles_n = pl.tiles_n;
-  p.tiles = pl.tiles_m * pl.tiles_n;
-  p.units = p.tiles * pl.splits;
-  p.bf16 = d.dtype == LIK_BF16;
-  p.act = d.act;
-  p.bias_vec = d.n % 8 == 0;
+  gt_outputs(pl, d, ws, d->dtype);
+  for (int i = 0; i < n; ++i) p.q[i] = pl.q[i];
+  p.n_prob = n;
+  p.units = pl.units;
+  p.bf16 = d->dtype == LIK_BF16;
+  p.act = d->act;
+  p.bias_vec = d->n % 8 == 0;
   for (int i = 0; i < 2; ++i) {
-    p.bias[i] = d.bias[i];
-    p.kept[i] = d.kept[i];
-    if (d.bias[i] && ((uintptr_t)d.bias[i] & 15)) p.bias_vec = false;
+    p.bias[i] = d->bias[i];
+    p.kept[i] = d->kept[i];
+    if (d->bias[i] && ((uintptr_t)d->bias[i] & 15)) p.bias_vec = false;
   }
-  p.kept_stride = d.kept_stride;
-  p.residual = d.residual;
-  p.residual_stride = d.residual_stride;
-  p.residual_vec = d.n % 8 == 0 && rows_of_pieces(d.residual, d.residual_stride, d.dtype);
+  p.out2 = d->out[1];
+  p.keep = d->kind != GEMM_GATED_BWD && d->kept[0];
+  p.kept_stride = d->kept_stride;
+  p.residual = d->residual;
+  p.residual_stride = d->residual_stride;
+  p.residual_vec = d->n % 8 == 0 && rows_of_pieces(d->residual, d->residual_stride, d->dtype);
   p.status = status;
-  int rc = d.dtype == LIK_F16 ? run_tc<__half>(d.kind, f32_out, pl.cg, maps, p, st) : run_tc<__nv_bfloat16>(d.kind, f32_out, pl.cg, maps, p, st);
-  if (rc || pl.splits == 1) return rc;
-  return launch_sum_splits((const float*)((char*)ws + pl.partial), pl.splits, d, pl.partial_stride, st);
+  const bool multi = n > 1 || pl.any_split() || d->out_dtype == LIK_F32;
+  if (d->dtype == LIK_F16) {
+    if (int rc = run_tc<__half>(d->kind, multi, pl.cg, maps, p, st)) return rc;
+    return launch_sum_splits<__half>(pl, d, st);
+  }
+  if (int rc = run_tc<__nv_bfloat16>(d->kind, multi, pl.cg, maps, p, st)) return rc;
+  return launch_sum_splits<__nv_bfloat16>(pl, d, st);
 }
 
 }  // namespace lik

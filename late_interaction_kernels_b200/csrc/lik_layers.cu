@@ -1,6 +1,4 @@
 // The layers' C entry points: which products and passes a call is made of, and the passes that are not products.
-#include <initializer_list>
-
 #include "lik_layers.cuh"
 
 namespace lik {
@@ -111,22 +109,15 @@ int launch_slope(SlopeParams p, int act, int dtype, void* sums, int sums_dtype, 
   return launch_sum_parts(p.partial, parts, p.n, p.n, sums_dtype, sums, nullptr, st);
 }
 
-// which kernel a product goes to
-enum GemmEngine { ENGINE_FEW, ENGINE_TC, ENGINE_F32 };
-GemmEngine gemm_engine(const GemmDesc& d) { return gemm_few_pays(d) ? ENGINE_FEW : (d.dtype == LIK_F32 ? ENGINE_F32 : ENGINE_TC); }
-size_t gemm_workspace(const GemmDesc& d) {
-  switch (gemm_engine(d)) {
-    case ENGINE_TC: return gemm_tc_workspace(d);
-    case ENGINE_F32: return gemm_f32_workspace(d);
-    default: return 0;
-  }
+// Which kernel a product goes to.  Several products of a pass are plain ones and go to the tensor cores together.
+size_t gemm_workspace(const GemmDesc* d, int n = 1) {
+  if (n == 0 || (n == 1 && gemm_few_pays(*d))) return 0;
+  return d->dtype == LIK_F32 ? gemm_f32_workspace(d, n) : gemm_tc_workspace(d, n);
 }
-int launch_gemm(const GemmDesc& d, void* ws, size_t ws_bytes, int* status, cudaStream_t st) {
-  switch (gemm_engine(d)) {
-    case ENGINE_TC: return launch_gemm_tc(d, ws, ws_bytes, status, st);
-    case ENGINE_F32: return launch_gemm_f32(d, ws, ws_bytes, status, st);
-    default: return launch_gemm_few(d, st);
-  }
+int launch_gemm(const GemmDesc* d, int n, void* ws, size_t ws_bytes, int* status, cudaStream_t st) {
+  if (n == 0) return LIK_OK;
+  if (n == 1 && gemm_few_pays(*d)) return launch_gemm_few(*d, st);
+  return d->dtype == LIK_F32 ? launch_gemm_f32(d, n, ws, ws_bytes, status, st) : launch_gemm_tc(d, n, ws, ws_bytes, status, st);
 }
 
 bool act_known(int a) { return a >= LIK_ACT_NONE && a <= LIK_ACT_SIGMOID; }
@@ -137,13 +128,15 @@ long long pad_cols(long long n, int dtype) {
   return (n + v - 1) / v * v;
 }
 
-// workspace, taken piece by piece: with a NULL base only the sizes are added up
+// Workspace, taken piece by piece.  Without a base only the sizes are added up; the addresses are then made up, but as far apart and as
+// aligned as the real ones, since a plan looks at both.
 struct Carve {
   char* base;
   size_t off = 0;
+  explicit Carve(void* ws) : base(ws ? (char*)ws : (char*)256) {}
   template <typename P = void>
   P* take(size_t bytes) {
-    P* p = base ? (P*)(base + off) : nullptr;
+    P* p = (P*)(base + off);
     off += align_up(bytes, 256);
     return p;
   }
@@ -209,21 +202,9 @@ GemmDesc grad_w_desc(int dtype, int param_dtype, long long rows, int out, int in
   return d;
 }
 
-// fp32 matrices that several products of a pass on the tensor cores read: cut once, in one launch with the others of the pass
-struct Cuts {
-  CutMatrix m[CUT_MOST];
-  int n = 0;
-  void add(Carve& c, std::initializer_list<GemmOperand*> users, const void* src, long long rows, long long cols, long long stride) {
-    void* parts = c.take(cut_bytes(rows, cols));
-    m[n++] = {src, rows, cols, stride, parts};
-    // (when only sizes are added up there is no address yet; the product still must not ask for room of its own)
-    for (GemmOperand* u : users) u->parts = parts ? parts : (const void*)16;
-  }
-};
-
 struct LinearBwd {
-  GemmDesc dx, dw;  // products that are not asked for have no out
-  Cuts cuts;
+  GemmDesc grads[2];  // dx and dw, as far as they are asked for
+  int n_grads = 0;
   void* dz;
   long long dz_stride;
   float* partial;
@@ -232,27 +213,18 @@ struct LinearBwd {
 };
 LinearBwd linear_bwd_layout(const lik_linear_args& a, void* ws) {
   LinearBwd l{};
-  Carve c{(char*)ws};
-  l.dz = nullptr;
-  if (a.activation != LIK_ACT_NONE) {
+  Carve c(ws);
+  const bool act = a.activation != LIK_ACT_NONE;
+  if (act) {
     l.dz_stride = pad_cols(a.out, a.dtype);
     l.dz = c.take((size_t)a.rows * l.dz_stride * dtype_size(a.dtype));
   }
   if (a.dbias) l.partial = c.take<float>(slope_workspace(a.rows, a.out, a.dtype));
-  const void* dz = a.activation != LIK_ACT_NONE ? l.dz : a.dy;
-  const long long st = a.activation != LIK_ACT_NONE ? l.dz_stride : a.dy_stride;
-  if (a.dx) l.dx = grad_x_desc(a.dtype, a.rows, a.out, a.in, dz, st, a.w, a.w_stride, a.dx);
-  if (a.dw) l.dw = grad_w_desc(a.dtype, a.param_dtype, a.rows, a.out, a.in, dz, st, a.x, a.x_stride, a.dw);
-  if (a.dx && a.dw && gemm_engine(l.dx) == ENGINE_F32 && gemm_engine(l.dw) == ENGINE_F32) {
-    l.cuts.add(c, {&l.dx.a[0], &l.dw.a[0]}, dz, a.rows, a.out, st);
-    l.cuts.add(c, {&l.dx.b[0]}, a.w, a.out, a.in, a.w_stride);
-    l.cuts.add(c, {&l.dw.b[0]}, a.x, a.rows, a.in, a.x_stride);
-  }
-  for (const GemmDesc* d : {&l.dx, &l.dw})
-    if (d->m) {
-      const size_t b = gemm_workspace(*d);
-      l.gemm_bytes = b > l.gemm_bytes ? b : l.gemm_bytes;
-    }
+  const void* dz = act ? l.dz : a.dy;
+  const long long st = act ? l.dz_stride : a.dy_stride;
+  if (a.dw) l.grads[l.n_grads++] = grad_w_desc(a.dtype, a.param_dtype, a.rows, a.out, a.in, dz, st, a.x, a.x_stride, a.dw);
+  if (a.dx) l.grads[l.n_grads++] = grad_x_desc(a.dtype, a.rows, a.out, a.in, dz, st, a.w, a.w_stride, a.dx);
+  l.gemm_bytes = gemm_workspace(l.grads, l.n_grads);
   l.gemm = c.take(l.gemm_bytes);
   l.total = c.off;
   return l;
@@ -285,7 +257,7 @@ struct GatedFwd {
 };
 GatedFwd gated_fwd_layout(const lik_gated_args& a, void* ws) {
   GatedFwd l{};
-  Carve c{(char*)ws};
+  Carve c(ws);
   void* h = a.h;
   long long h_stride = a.kept_stride;
   if (!a.gate_factor) {
@@ -321,15 +293,15 @@ GatedFwd gated_fwd_layout(const lik_gated_args& a, void* ws) {
   d.residual_stride = a.residual_stride;
   d.out[0] = a.y;
   d.out_stride = a.out;
-  const size_t b1 = gemm_workspace(u), b2 = gemm_workspace(d);
+  const size_t b1 = gemm_workspace(&u), b2 = gemm_workspace(&d);
   l.gemm_bytes = b1 > b2 ? b1 : b2;
   l.gemm = c.take(l.gemm_bytes);
   l.total = c.off;
   return l;
 }
 struct GatedBwd {
-  GemmDesc dh, dx, dwg, dwu, dwd;  // products that are not asked for have no out
-  Cuts first, second;              // before dh and after it
+  GemmDesc dh, grads[4];  // dh for the gradients behind it; dx and the weights' gradients, as far as they are asked for
+  int n_grads = 0;
   void *dg, *du;
   long long stride;
   float* partial;
@@ -338,7 +310,7 @@ struct GatedBwd {
 };
 GatedBwd gated_bwd_layout(const lik_gated_args& a, void* ws) {
   GatedBwd l{};
-  Carve c{(char*)ws};
+  Carve c(ws);
   l.stride = pad_cols(a.hidden, a.dtype);
   const bool inner = a.dx || a.dw_gate || a.dw_up || a.db_gate || a.db_up;
   if (inner) {
@@ -359,32 +331,21 @@ GatedBwd gated_bwd_layout(const lik_gated_args& a, void* ws) {
     h.kept[1] = a.up_factor;
     h.kept_stride = a.kept_stride;
   }
+  if (a.dw_gate) l.grads[l.n_grads++] = grad_w_desc(a.dtype, a.param_dtype, a.rows, a.hidden, a.in, l.dg, l.stride, a.x, a.x_stride, a.dw_gate);
+  if (a.dw_up) l.grads[l.n_grads++] = grad_w_desc(a.dtype, a.param_dtype, a.rows, a.hidden, a.in, l.du, l.stride, a.x, a.x_stride, a.dw_up);
+  if (a.dw_down) l.grads[l.n_grads++] = grad_w_desc(a.dtype, a.param_dtype, a.rows, a.out, a.hidden, a.dy, a.dy_stride, a.h, a.kept_stride, a.dw_down);
   if (a.dx) {
-    l.dx = grad_x_desc(a.dtype, a.rows, a.hidden, a.in, l.dg, l.stride, a.w_gate, a.w_gate_stride, a.dx);
-    l.dx.n_seg = 2;
-    l.dx.k[1] = a.hidden;
-    l.dx.a[1] = {l.du, l.stride, 1};
-    l.dx.b[1] = {a.w_up, 1, a.w_up_stride};
+    GemmDesc& d = l.grads[l.n_grads++] = grad_x_desc(a.dtype, a.rows, a.hidden, a.in, l.dg, l.stride, a.w_gate, a.w_gate_stride, a.dx);
+    d.n_seg = 2;
+    d.k[1] = a.hidden;
+    d.a[1] = {l.du, l.stride, 1};
+    d.b[1] = {a.w_up, 1, a.w_up_stride};
   }
-  if (a.dw_gate) l.dwg = grad_w_desc(a.dtype, a.param_dtype, a.rows, a.hidden, a.in, l.dg, l.stride, a.x, a.x_stride, a.dw_gate);
-  if (a.dw_up) l.dwu = grad_w_desc(a.dtype, a.param_dtype, a.rows, a.hidden, a.in, l.du, l.stride, a.x, a.x_stride, a.dw_up);
-  if (a.dw_down) l.dwd = grad_w_desc(a.dtype, a.param_dtype, a.rows, a.out, a.hidden, a.dy, a.dy_stride, a.h, a.kept_stride, a.dw_down);
-  if (a.dx && a.dw_gate && a.dw_up && a.dw_down && gemm_engine(l.dh) == ENGINE_F32 && gemm_engine(l.dx) == ENGINE_F32 && gemm_engine(l.dwg) == ENGINE_F32 &&
-      gemm_engine(l.dwd) == ENGINE_F32) {
-    l.first.add(c, {&l.dh.a[0], &l.dwd.a[0]}, a.dy, a.rows, a.out, a.dy_stride);
-    l.first.add(c, {&l.dh.b[0]}, a.w_down, a.out, a.hidden, a.w_down_stride);
-    l.first.add(c, {&l.dwd.b[0]}, a.h, a.rows, a.hidden, a.kept_stride);
-    l.first.add(c, {&l.dwg.b[0], &l.dwu.b[0]}, a.x, a.rows, a.in, a.x_stride);
-    l.first.add(c, {&l.dx.b[0]}, a.w_gate, a.hidden, a.in, a.w_gate_stride);
-    l.first.add(c, {&l.dx.b[1]}, a.w_up, a.hidden, a.in, a.w_up_stride);
-    l.second.add(c, {&l.dx.a[0], &l.dwg.a[0]}, l.dg, a.rows, a.hidden, l.stride);
-    l.second.add(c, {&l.dx.a[1], &l.dwu.a[0]}, l.du, a.rows, a.hidden, l.stride);
+  l.gemm_bytes = gemm_workspace(l.grads, l.n_grads);
+  if (inner) {
+    const size_t b = gemm_workspace(&l.dh);
+    l.gemm_bytes = b > l.gemm_bytes ? b : l.gemm_bytes;
   }
-  for (const GemmDesc* d : {&l.dh, &l.dx, &l.dwg, &l.dwu, &l.dwd})
-    if (d->m) {
-      const size_t b = gemm_workspace(*d);
-      l.gemm_bytes = b > l.gemm_bytes ? b : l.gemm_bytes;
-    }
   if (a.db_gate || a.db_up || a.db_down) l.partial = c.take<float>(slope_workspace(a.rows, a.hidden > a.out ? a.hidden : a.out, a.dtype) * 2);
   l.gemm = c.take(l.gemm_bytes);
   l.total = c.off;
@@ -408,7 +369,8 @@ int launch_sum_parts(const float* partial, int parts, long long n, long long spl
 extern "C" size_t lik_linear_fwd_workspace(const lik_linear_args* a) {
   using namespace lik;
   if (check_linear(a) || a->rows == 0) return 0;
-  return gemm_workspace(linear_fwd_desc(*a));
+  const GemmDesc d = linear_fwd_desc(*a);
+  return gemm_workspace(&d);
 }
 extern "C" int lik_linear_fwd(const lik_linear_args* args, lik_stream_t stream) {
   using namespace lik;
@@ -419,8 +381,8 @@ extern "C" int lik_linear_fwd(const lik_linear_args* args, lik_stream_t stream) 
   LIK_REQUIRE(!a.z || (a.z_stride >= a.out && a.z_stride * dtype_size(a.dtype) % 16 == 0 && ((uintptr_t)a.z & 15) == 0), "z must have 16-byte rows");
   LIK_REQUIRE(!a.residual || a.residual_stride >= a.out, "residual_stride must be at least out");
   const GemmDesc d = linear_fwd_desc(a);
-  if (a.workspace_bytes < gemm_workspace(d)) return too_small("lik_linear_fwd");
-  return launch_gemm(d, a.workspace, a.workspace_bytes, a.status, (cudaStream_t)stream);
+  if (a.workspace_bytes < gemm_workspace(&d)) return too_small("lik_linear_fwd");
+  return launch_gemm(&d, 1, a.workspace, a.workspace_bytes, a.status, (cudaStream_t)stream);
 }
 
 extern "C" size_t lik_linear_bwd_workspace(const lik_linear_args* a) {
@@ -449,11 +411,7 @@ extern "C" int lik_linear_bwd(const lik_linear_args* args, lik_stream_t stream) 
     SlopeParams p{a.dy, a.z, a.dy_stride, a.z_stride, a.rows, 0, a.out, l.dz, l.dz_stride, l.partial};
     if (int rc = launch_slope(p, a.activation, a.dtype, a.dbias, a.param_dtype, st)) return rc;
   }
-  if (int rc = launch_cut(l.cuts.m, l.cuts.n, st)) return rc;
-  for (const GemmDesc* d : {&l.dx, &l.dw})
-    if (d->out[0])
-      if (int rc = launch_gemm(*d, l.gemm, l.gemm_bytes, a.status, st)) return rc;
-  return LIK_OK;
+  return launch_gemm(l.grads, l.n_grads, l.gemm, l.gemm_bytes, a.status, st);
 }
 
 extern "C" size_t lik_gated_fwd_workspace(const lik_gated_args* a) {
@@ -473,8 +431,8 @@ extern "C" int lik_gated_fwd(const lik_gated_args* args, lik_stream_t stream) {
   LIK_REQUIRE(!a.residual || a.residual_stride >= a.out, "residual_stride must be at least out");
   const GatedFwd l = gated_fwd_layout(a, a.workspace);
   if (a.workspace_bytes < l.total || (l.total && !a.workspace)) return too_small("lik_gated_fwd");
-  if (int rc = launch_gemm(l.up, l.gemm, l.gemm_bytes, a.status, (cudaStream_t)stream)) return rc;
-  return launch_gemm(l.down, l.gemm, l.gemm_bytes, a.status, (cudaStream_t)stream);
+  if (int rc = launch_gemm(&l.up, 1, l.gemm, l.gemm_bytes, a.status, (cudaStream_t)stream)) return rc;
+  return launch_gemm(&l.down, 1, l.gemm, l.gemm_bytes, a.status, (cudaStream_t)stream);
 }
 
 extern "C" size_t lik_gated_bwd_workspace(const lik_gated_args* a) {
@@ -500,13 +458,9 @@ extern "C" int lik_gated_bwd(const lik_gated_args* args, lik_stream_t stream) {
                   (((uintptr_t)a.gate_factor | (uintptr_t)a.up_factor | (uintptr_t)a.h) & 15) == 0, "gate_factor, up_factor and h must be there, with 16-byte rows");
   const GatedBwd l = gated_bwd_layout(a, a.workspace);
   if (a.workspace_bytes < l.total || (l.total && !a.workspace)) return too_small("lik_gated_bwd");
-  if (int rc = launch_cut(l.first.m, l.first.n, st)) return rc;
   if (l.dg)
-    if (int rc = launch_gemm(l.dh, l.gemm, l.gemm_bytes, a.status, st)) return rc;
-  if (int rc = launch_cut(l.second.m, l.second.n, st)) return rc;
-  for (const GemmDesc* d : {&l.dx, &l.dwg, &l.dwu, &l.dwd})
-    if (d->out[0])
-      if (int rc = launch_gemm(*d, l.gemm, l.gemm_bytes, a.status, st)) return rc;
+    if (int rc = launch_gemm(&l.dh, 1, l.gemm, l.gemm_bytes, a.status, st)) return rc;
+  if (int rc = launch_gemm(l.grads, l.n_grads, l.gemm, l.gemm_bytes, a.status, st)) return rc;
   auto sums = [&](const void* g, long long stride, int n, void* out) {
     if (!out) return (int)LIK_OK;
     SlopeParams p{g, nullptr, stride, 0, a.rows, 0, n, nullptr, 0, l.partial};

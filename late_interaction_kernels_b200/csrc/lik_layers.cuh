@@ -202,7 +202,6 @@ enum GemmKind {
 struct GemmOperand {
   const void* p = nullptr;
   long long row = 0, k = 0;  // elements from one row (m or n) to the next, and from one k to the next; one of the two is 1
-  const void* parts = nullptr;  // fp32 on the tensor cores: the matrix as launch_cut left it, or NULL: the product cuts it itself
 };
 struct GemmDesc {
   int kind = GEMM_LINEAR, act = LIK_ACT_NONE, dtype = 0;
@@ -255,21 +254,12 @@ inline bool gemm_plain(const GemmDesc& d) {
 // few rows of a (lik_gemm_few.cu): any type, both operands with their k contiguous; whether it is the faster one
 bool gemm_few_pays(const GemmDesc& d);
 int launch_gemm_few(const GemmDesc& d, cudaStream_t st);
-// tensor cores (lik_gemm_tc.cu): 16-bit operands
-size_t gemm_tc_workspace(const GemmDesc& d);
-int launch_gemm_tc(const GemmDesc& d, void* ws, size_t ws_bytes, int* status, cudaStream_t st);
-// tensor cores (lik_gemm_f32.cu): fp32 operands in three bf16 parts
-size_t gemm_f32_workspace(const GemmDesc& d);
-int launch_gemm_f32(const GemmDesc& d, void* ws, size_t ws_bytes, int* status, cudaStream_t st);
-// fp32 matrices cut into their bf16 parts, in one launch: what several products read is cut once
-struct CutMatrix {
-  const void* src;
-  long long rows, cols, stride;
-  void* parts;  // cut_bytes(rows, cols)
-};
-constexpr int CUT_MOST = 6;
-size_t cut_bytes(long long rows, long long cols);
-int launch_cut(const CutMatrix* m, int n, cudaStream_t st);
+// Tensor cores: 16-bit operands (lik_gemm_tc.cu), and fp32 operands in three bf16 parts (lik_gemm_f32.cu).  One product, or up to four plain
+// ones of one type in one launch.
+size_t gemm_tc_workspace(const GemmDesc* d, int n);
+int launch_gemm_tc(const GemmDesc* d, int n, void* ws, size_t ws_bytes, int* status, cudaStream_t st);
+size_t gemm_f32_workspace(const GemmDesc* d, int n);
+int launch_gemm_f32(const GemmDesc* d, int n, void* ws, size_t ws_bytes, int* status, cudaStream_t st);
 
 // sum over `parts` of partial[part][i], i < n, as dtype: out[i], the second half (i >= split) to out2
 int launch_sum_parts(const float* partial, int parts, long long n, long long split, int dtype, void* out, void* out2, cudaStream_t st);
