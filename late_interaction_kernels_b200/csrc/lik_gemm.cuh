@@ -147,8 +147,8 @@ __device__ __forceinline__ void slot_store_as(const uint8_t* s, int lane, T* p, 
 }
 
 // ---------------------------------------------------------------------------------------------
-// One launch computes up to four products.  A problem's tiles, each cut along k into `splits` shares, are its units; units are numbered
-// through the problems and dealt to the CTAs (or pairs) in turn.
+// A product's tiles, each cut along k into `splits` shares, are its units.  One launch computes one product, its units dealt to the CTAs (or
+// pairs) in turn, or up to four whose units all run side by side.
 // ---------------------------------------------------------------------------------------------
 constexpr int GT_PROBLEMS = 4, GT_MATRICES = 8;
 struct GtProblem {
@@ -253,64 +253,60 @@ inline Stored stored(const GemmOperand& o, long long rows, long long k) {
 }
 inline bool rows_of_pieces(const void* p, long long stride, int dtype) { return ((uintptr_t)p & 15) == 0 && stride * (long long)dtype_size(dtype) % 16 == 0; }
 
-// What a launch is made of: the problems, the matrices that they read (each once, whoever reads it), the workspace.
+// What a call is made of: the problems, the matrices that they read (each brought to its layout once, whoever reads it), the workspace.
 struct GtPlan {
-  int cg, n, n_mat, units;
-  GtProblem q[GT_PROBLEMS];  // without addresses
-  int splits[GT_PROBLEMS];
+  int n, n_mat;
+  GtProblem q[GT_PROBLEMS];  // without addresses; unit0 as if alone
+  int cg[GT_PROBLEMS], splits[GT_PROBLEMS], units[GT_PROBLEMS];
   Stored mat[GT_MATRICES];
   bool copied[GT_MATRICES];
   size_t copy[GT_MATRICES], partial[GT_PROBLEMS], total;  // offsets
-  bool any_split() const {
-    for (int i = 0; i < n; ++i)
-      if (splits[i] > 1) return true;
-    return false;
+  // problems [i, end) that a launch takes together
+  int group_end(int i) const {
+    int end = i + 1;
+    long long sum = units[i];
+    while (end < n && cg[end] == cg[i] && sum + units[end] <= sm_count() / cg[i]) sum += units[end++];
+    return end;
   }
 };
-// tile_m, tile_n: of a unit; slots: units that run side by side; share: slabs of k that a share has at least (a product with more to it than the
-// sum: twice that); copy_bytes: of a matrix that is not read as it lies in memory, 0 otherwise
-template <typename CopyBytes>
-GtPlan gt_plan(const GemmDesc* d, int n, int tile_m, int tile_n, int slots, int share, CopyBytes&& copy_bytes) {
+// cg_of: CTAs that share a tile of (128 CTAs)^2; cut_from: slabs of k from which a product is cut into shares, of at least `share` slabs each;
+// copy_bytes: of a matrix that is not read as it lies in memory, 0 otherwise.  A problem is planned as if it were alone, so its result does
+// not depend on which others are asked for.
+template <typename CgOf, typename CopyBytes>
+GtPlan gt_plan(const GemmDesc* d, int n, int cut_from, int share, CgOf&& cg_of, CopyBytes&& copy_bytes) {
   GtPlan pl{};
   pl.n = n;
-  long long work = 0;
+  size_t off = 0;
   for (int i = 0; i < n; ++i) {
     const bool dual = d[i].kind == GEMM_GATED;
     GtProblem& q = pl.q[i];
+    const int cg = pl.cg[i] = cg_of(d[i]);
     q.m = (int)d[i].m;
     q.n = d[i].n;
-    q.tiles_n = (int)ceil_div(q.n, tile_n / (dual ? 2 : 1));
-    q.tiles = (int)ceil_div(q.m, tile_m) * q.tiles_n;
+    q.tiles_n = (int)ceil_div(q.n, 128 * cg / (dual ? 2 : 1));
+    q.tiles = (int)ceil_div(q.m, 128 * cg) * q.tiles_n;
     for (int s = 0; s < d[i].n_seg; ++s) {
       const int kb = (int)ceil_div(d[i].k[s], GT_BK);
       q.kb_total += kb;
       if (s == 0) q.kb0 = kb;
     }
-    work += (long long)q.tiles * q.kb_total;
     for (int s = 0; s < 2; ++s)
       for (int is_b = 0; is_b < 2; ++is_b) {
         if (s >= (is_b && dual ? 2 : d[i].n_seg)) continue;
         const Stored o = stored(is_b ? d[i].b[s] : d[i].a[s], is_b ? d[i].n : d[i].m, d[i].k[dual ? 0 : s]);
         (is_b ? q.b_mn : q.a_mn) = o.mn;
         int at = 0;
-        while (at < pl.n_mat && !(pl.mat[at].p == o.p && o.p && pl.mat[at].rows == o.rows && pl.mat[at].cols == o.cols && pl.mat[at].stride == o.stride)) ++at;
+        while (at < pl.n_mat && !(pl.mat[at].p == o.p && pl.mat[at].rows == o.rows && pl.mat[at].cols == o.cols && pl.mat[at].stride == o.stride)) ++at;
         if (at == pl.n_mat) pl.mat[pl.n_mat++] = o;
         (is_b ? q.b : q.a)[s] = (unsigned char)at;
       }
-  }
-  // A share of k for every slot, where that leaves a share worth its start and the pass that adds the shares up.
-  long long ideal = ceil_div(work, slots);
-  if (ideal < share) ideal = share;
-  size_t off = 0;
-  for (int i = 0; i < n; ++i) {
-    GtProblem& q = pl.q[i];
-    const bool plain = gemm_plain(d[i]);
-    const long long least = plain ? ideal : 2 * ideal;
-    long long s = (plain || (n == 1 && d[i].kind == GEMM_LINEAR)) && q.kb_total >= 2 * least ? q.kb_total / least : 1;
+    // a share of k for every slot, where the time that this saves is worth the pass that adds the shares up (4 to 5 us)
+    long long ideal = ceil_div((long long)q.tiles * q.kb_total, sm_count() / cg);
+    if (ideal < share) ideal = share;
+    const long long s = d[i].kind == GEMM_LINEAR && q.kb_total >= cut_from && q.kb_total >= 2 * ideal ? q.kb_total / ideal : 1;
     q.kb_per = (int)ceil_div(q.kb_total, s);
     pl.splits[i] = (int)ceil_div(q.kb_total, q.kb_per);
-    q.unit0 = pl.units;
-    pl.units += q.tiles * pl.splits[i];
+    pl.units[i] = q.tiles * pl.splits[i];
     if (pl.splits[i] > 1) {
       pl.partial[i] = off;
       off += align_up((size_t)pl.splits[i] * q.m * ((q.n + 3) / 4 * 4) * sizeof(float), 256);
@@ -326,7 +322,7 @@ GtPlan gt_plan(const GemmDesc* d, int n, int tile_m, int tile_n, int slots, int 
   return pl;
 }
 // the addresses: where each problem's sums go
-inline void gt_outputs(GtPlan& pl, const GemmDesc* d, void* ws, int operand_dtype) {
+inline void gt_outputs(GtPlan& pl, const GemmDesc* d, void* ws) {
   for (int i = 0; i < pl.n; ++i) {
     GtProblem& q = pl.q[i];
     if (pl.splits[i] > 1) {

@@ -327,8 +327,8 @@ __global__ void __launch_bounds__(256) cut_kernel(const __grid_constant__ CutJob
   }
 }
 
-GtPlan f32_plan(const GemmDesc* d, int n) {
-  return gt_plan(d, n, 128, GF_BN, sm_count(), 4, [](const Stored& o) { return align_up((size_t)o.rows * o.padded() * 2 * GF_PARTS, 256); });
+GtPlan f32_plan(const GemmDesc* d, int n) {  // (a slab of k takes a CTA 1.5 to 1.9 us)
+  return gt_plan(d, n, 6, 2, [](const GemmDesc&) { return 1; }, [](const Stored& o) { return align_up((size_t)o.rows * o.padded() * 2 * GF_PARTS, 256); });
 }
 template <int KIND>
 int run_f32(const GfMaps& maps, const GfParams& p, cudaStream_t st) {
@@ -366,11 +366,7 @@ int launch_gemm_f32(const GemmDesc* d, int n, void* ws, size_t ws_bytes, int* st
   const long long blocks = ceil_div(total, 256), most = 16ll * sm_count();
   cut_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, st>>>(cuts), count_launch();
   LIK_CUDA_OK(cudaGetLastError());
-  gt_outputs(pl, d, ws, LIK_F32);
-  for (int i = 0; i < n; ++i) p.q[i] = pl.q[i];
-  p.n_prob = n;
-  p.units = pl.units;
-  p.raw = n > 1 || pl.any_split();
+  gt_outputs(pl, d, ws);
   p.act = d->act;
   for (int i = 0; i < 2; ++i) {
     p.bias[i] = (const float*)d->bias[i];
@@ -383,8 +379,19 @@ int launch_gemm_f32(const GemmDesc* d, int n, void* ws, size_t ws_bytes, int* st
   p.residual_stride = d->residual_stride;
   p.residual_vec = d->n % 4 == 0 && rows_of_pieces(d->residual, d->residual_stride, LIK_F32);
   p.status = status;
-  if (int rc = d->kind == GEMM_GATED ? run_f32<GEMM_GATED>(maps, p, st) : (d->kind == GEMM_GATED_BWD ? run_f32<GEMM_GATED_BWD>(maps, p, st) : run_f32<GEMM_LINEAR>(maps, p, st)))
-    return rc;
+  for (int i = 0, end; i < n; i = end) {
+    end = pl.group_end(i);
+    p.n_prob = end - i;
+    p.units = 0;
+    for (int k = i; k < end; ++k) {
+      p.q[k - i] = pl.q[k];
+      p.q[k - i].unit0 = p.units;
+      p.units += pl.units[k];
+    }
+    p.raw = p.n_prob > 1 || pl.splits[i] > 1;
+    const int rc = d->kind == GEMM_GATED ? run_f32<GEMM_GATED>(maps, p, st) : (d->kind == GEMM_GATED_BWD ? run_f32<GEMM_GATED_BWD>(maps, p, st) : run_f32<GEMM_LINEAR>(maps, p, st));
+    if (rc) return rc;
+  }
   return launch_sum_splits<float>(pl, d, st);
 }
 

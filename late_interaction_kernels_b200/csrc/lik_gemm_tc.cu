@@ -405,21 +405,14 @@ __global__ void __launch_bounds__(256) repack_kernel(const uint16_t* __restrict_
 }
 
 // Pairs of CTAs take tiles of 256 x 256 where there are enough of them, or enough k to cut into shares, for every pair; else single CTAs
-// tiles of 128 x 128.
+// tiles of 128 x 128.  A slab of k takes a CTA that is alone with its tile 0.2 us.
 GtPlan tc_plan(const GemmDesc* d, int n) {
-  const int sms = sm_count();
-  long long tiles = 0, work = 0;
-  bool cuttable = true;
-  for (int i = 0; i < n; ++i) {
-    const long long t = ceil_div(d[i].m, 256) * ceil_div(d[i].n, d[i].kind == GEMM_GATED ? 128 : 256);
-    tiles += t;
-    work += t * ceil_div(d[i].k[0] + d[i].k[1], GT_BK);
-    cuttable = cuttable && gemm_plain(d[i]) && d[i].m > 128 && d[i].n > 128;
-  }
-  const int cg = tiles * 2 >= sms || (cuttable && work >= 16 * (sms / 2)) ? 2 : 1;
-  GtPlan pl = gt_plan(d, n, 128 * cg, 128 * cg, sms / cg, 16, [](const Stored& o) { return o.aligned() ? (size_t)0 : align_up((size_t)o.rows * o.padded() * 2, 256); });
-  pl.cg = cg;
-  return pl;
+  auto cg = [](const GemmDesc& g) {
+    const long long tiles = ceil_div(g.m, 256) * ceil_div(g.n, g.kind == GEMM_GATED ? 128 : 256), pairs = sm_count() / 2;
+    const bool cuttable = gemm_plain(g) && g.m > 128 && g.n > 128;
+    return tiles >= pairs || (cuttable && tiles * ceil_div(g.k[0] + g.k[1], GT_BK) >= 16 * pairs) ? 2 : 1;
+  };
+  return gt_plan(d, n, 40, 8, cg, [](const Stored& o) { return o.aligned() ? (size_t)0 : align_up((size_t)o.rows * o.padded() * 2, 256); });
 }
 
 template <int CG, int KIND, bool RES, typename T, typename O>
@@ -479,10 +472,7 @@ int launch_gemm_tc(const GemmDesc* d, int n, void* ws, size_t ws_bytes, int* sta
     if (o.rows == 1) o.stride = o.padded();
     if (int rc = make_tmap_rows(&maps.m[i], o.p, d->dtype, o.cols, o.rows, o.stride, GT_BOX)) return rc;
   }
-  gt_outputs(pl, d, ws, d->dtype);
-  for (int i = 0; i < n; ++i) p.q[i] = pl.q[i];
-  p.n_prob = n;
-  p.units = pl.units;
+  gt_outputs(pl, d, ws);
   p.bf16 = d->dtype == LIK_BF16;
   p.act = d->act;
   p.bias_vec = d->n % 8 == 0;
@@ -498,13 +488,20 @@ int launch_gemm_tc(const GemmDesc* d, int n, void* ws, size_t ws_bytes, int* sta
   p.residual_stride = d->residual_stride;
   p.residual_vec = d->n % 8 == 0 && rows_of_pieces(d->residual, d->residual_stride, d->dtype);
   p.status = status;
-  const bool multi = n > 1 || pl.any_split() || d->out_dtype == LIK_F32;
-  if (d->dtype == LIK_F16) {
-    if (int rc = run_tc<__half>(d->kind, multi, pl.cg, maps, p, st)) return rc;
-    return launch_sum_splits<__half>(pl, d, st);
+  for (int i = 0, end; i < n; i = end) {
+    end = pl.group_end(i);
+    p.n_prob = end - i;
+    p.units = 0;
+    for (int k = i; k < end; ++k) {
+      p.q[k - i] = pl.q[k];
+      p.q[k - i].unit0 = p.units;
+      p.units += pl.units[k];
+    }
+    const bool multi = p.n_prob > 1 || pl.splits[i] > 1 || d[i].out_dtype == LIK_F32;
+    const int rc = d->dtype == LIK_F16 ? run_tc<__half>(d->kind, multi, pl.cg[i], maps, p, st) : run_tc<__nv_bfloat16>(d->kind, multi, pl.cg[i], maps, p, st);
+    if (rc) return rc;
   }
-  if (int rc = run_tc<__nv_bfloat16>(d->kind, multi, pl.cg, maps, p, st)) return rc;
-  return launch_sum_splits<__nv_bfloat16>(pl, d, st);
+  return d->dtype == LIK_F16 ? launch_sum_splits<__half>(pl, d, st) : launch_sum_splits<__nv_bfloat16>(pl, d, st);
 }
 
 }  // namespace lik

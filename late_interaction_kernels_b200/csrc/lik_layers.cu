@@ -5,108 +5,139 @@ namespace lik {
 namespace {
 
 // ---------------------------------------------------------------------------------------------
-// out[i] = sum over parts of partial[part][i], in the order of the parts
+// Sums over parts of partial[part][i], in the order of the parts, to up to SUM_OUTS vectors one behind the other
 // ---------------------------------------------------------------------------------------------
-constexpr int SUM_LANES = 8;
+constexpr int SUM_COLS = 8;  // a sector of each part; the block's 32 groups of threads take every 32nd part
 template <typename T>
-__global__ void __launch_bounds__(256) sum_parts_kernel(const float* __restrict__ partial, int parts, long long n, long long split, T* __restrict__ out,
-                                                        T* __restrict__ out2) {
-  __shared__ float s[SUM_LANES][33];
-  const int col = threadIdx.x % 32, lane = threadIdx.x / 32;
-  const long long i = blockIdx.x * 32ll + col;
+__global__ void __launch_bounds__(256) sum_parts_kernel(const float* __restrict__ partial, int parts, const __grid_constant__ SumOuts outs) {
+  __shared__ float s[8][SUM_COLS];
+  const int col = threadIdx.x % SUM_COLS, group = threadIdx.x / SUM_COLS, warp = threadIdx.x / 32;
+  const long long i = blockIdx.x * (long long)SUM_COLS + col, n = outs.end[SUM_OUTS - 1];
   float v = 0.0f;
   if (i < n) {
-#pragma unroll 4
-    for (int q = lane; q < parts; q += SUM_LANES) v += partial[q * n + i];
+#pragma unroll 8
+    for (int q = group; q < parts; q += 32) v += partial[q * n + i];
   }
-  s[lane][col] = v;
+  v += __shfl_xor_sync(0xffffffffu, v, 8);
+  v += __shfl_xor_sync(0xffffffffu, v, 16);
+  if (threadIdx.x % 32 < SUM_COLS) s[warp][col] = v;
   __syncthreads();
-  if (lane == 0 && i < n) {
+  if (group == 0 && i < n) {
 #pragma unroll
-    for (int l = 1; l < SUM_LANES; ++l) v += s[l][col];
-    T* o = i < split ? out : out2;
-    if (o) o[i < split ? i : i - split] = from_f32<T>(v);
+    for (int w = 1; w < 8; ++w) v += s[w][col];
+    outs.put<T>(i, v);
   }
 }
 
 // ---------------------------------------------------------------------------------------------
-// dz = dy * act'(z), and the sums of dz's columns per block of rows.  Memory-bound: each element read once, dz written once.
-// A block takes 32 vectors of columns (a lane's V columns) and ROWS_PER rows, eight at a time.
+// dz = dy * act'(z), and the sums of dz's columns; or the sums of up to SUM_OUTS matrices' columns.  Memory-bound: each element read once, dz
+// written once.  A block takes 32 vectors of columns (a lane's V columns) of a matrix and a share of the rows, eight at a time; with one
+// share the sums are done, else sum_parts_kernel adds them up.
 // ---------------------------------------------------------------------------------------------
 constexpr int SLOPE_LANES = 8;
-struct SlopeParams {
+struct SlopeJob {
   const void *dy, *z;
-  long long dy_stride, z_stride, rows, rows_per;
-  int n;
-  void* dz;  // or NULL: sums only
+  long long dy_stride, z_stride;
+  int n, blocks;  // blocks of columns
+  void* dz;       // or NULL: sums only
   long long dz_stride;
-  float* partial;  // [gridDim.y][n] or NULL
+};
+struct SlopeParams {
+  SlopeJob job[SUM_OUTS];
+  int n_jobs;
+  long long rows, rows_per;
+  float* partial;  // [gridDim.y][columns of all jobs]; NULL: straight to outs
+  bool sums;
+  SumOuts outs;
 };
 template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(32 * SLOPE_LANES) slope_kernel(const SlopeParams p) {
+__global__ void __launch_bounds__(32 * SLOPE_LANES) slope_kernel(const __grid_constant__ SlopeParams p) {
   __shared__ float s[SLOPE_LANES][32 * V + 1];
   const int lane = threadIdx.x % 32, row = threadIdx.x / 32;
-  const int c = (blockIdx.x * 32 + lane) * V;
+  int q = 0, block = blockIdx.x;
+  while (block >= p.job[q].blocks) block -= p.job[q++].blocks;
+  const SlopeJob& j = p.job[q];
+  const int c = (block * 32 + lane) * V;
   float sum[V];
 #pragma unroll
-  for (int j = 0; j < V; ++j) sum[j] = 0.0f;
-  if (c < p.n) {
+  for (int i = 0; i < V; ++i) sum[i] = 0.0f;
+  if (c < j.n) {
     const long long r0 = blockIdx.y * p.rows_per, r1 = r0 + p.rows_per < p.rows ? r0 + p.rows_per : p.rows;
-#pragma unroll 2
+#pragma unroll 4
     for (long long r = r0 + row; r < r1; r += SLOPE_LANES) {
       float g[V], z[V];
-      load_vec<T, V>((const T*)p.dy + r * p.dy_stride + c, g);
+      load_vec<T, V>((const T*)j.dy + r * j.dy_stride + c, g);
       if constexpr (ACT != LIK_ACT_NONE) {
-        load_vec<T, V>((const T*)p.z + r * p.z_stride + c, z);
+        load_vec<T, V>((const T*)j.z + r * j.z_stride + c, z);
 #pragma unroll
-        for (int j = 0; j < V; ++j) g[j] *= act_slope<ACT, sizeof(T) == 4>(z[j], z[j]);
+        for (int i = 0; i < V; ++i) g[i] *= act_slope<ACT, sizeof(T) == 4>(z[i], z[i]);
+        store_vec<T, V>((T*)j.dz + r * j.dz_stride + c, g);
       }
-      if (p.dz) store_vec<T, V>((T*)p.dz + r * p.dz_stride + c, g);
 #pragma unroll
-      for (int j = 0; j < V; ++j) sum[j] += g[j];
+      for (int i = 0; i < V; ++i) sum[i] += g[i];
     }
   }
-  if (!p.partial) return;
+  if (!p.sums) return;
 #pragma unroll
-  for (int j = 0; j < V; ++j) s[row][j * 32 + lane] = sum[j];
+  for (int i = 0; i < V; ++i) s[row][i * 32 + lane] = sum[i];
   __syncthreads();
+  const long long first = q ? p.outs.end[q - 1] : 0, total = p.outs.end[SUM_OUTS - 1];
   for (int i = threadIdx.x; i < 32 * V; i += 32 * SLOPE_LANES) {
     float v = 0.0f;
 #pragma unroll
-    for (int q = 0; q < SLOPE_LANES; ++q) v += s[q][i];
-    const int col = (blockIdx.x * 32 + i % 32) * V + i / 32;
-    if (col < p.n) p.partial[(long long)blockIdx.y * p.n + col] = v;
+    for (int l = 0; l < SLOPE_LANES; ++l) v += s[l][i];
+    const int col = (block * 32 + i % 32) * V + i / 32;
+    if (col < j.n) {
+      if (p.partial) p.partial[blockIdx.y * total + first + col] = v;
+      else p.outs.put<T>(first + col, v);
+    }
   }
 }
-int slope_parts(long long rows, int n, int dtype) {
-  const long long cols = ceil_div(n, 32 * (16 / (int)dtype_size(dtype)));
-  long long want = ceil_div(4ll * sm_count(), cols);
+// (128 rows: a lane's sixteen, in four trips to memory)
+int slope_parts(long long rows, long long cols, int dtype) {
+  if (rows <= 128) return 1;
+  long long want = ceil_div(4ll * sm_count(), ceil_div(cols, 32 * (16 / (int)dtype_size(dtype))));
   if (want > ceil_div(rows, SLOPE_LANES)) want = ceil_div(rows, SLOPE_LANES);
   if (want > 65535) want = 65535;
   return want < 1 ? 1 : (int)want;
 }
+size_t slope_workspace(long long rows, long long cols, int dtype) {
+  const int parts = slope_parts(rows, cols, dtype);
+  return parts == 1 ? 0 : align_up((size_t)parts * cols * sizeof(float), 256);
+}
 template <typename T>
-int run_slope(const SlopeParams& p, int act, bool vec, int parts, cudaStream_t st) {
+int run_slope(SlopeParams& p, int act, bool vec, int parts, cudaStream_t st) {
   constexpr int V = vec_elems<T>();
+  unsigned blocks = 0;
+  for (int i = 0; i < p.n_jobs; ++i) blocks += p.job[i].blocks = (int)ceil_div(p.job[i].n, 32 * (vec ? V : 1));
   with_activation(act, [&](auto a) {
-    if (vec) slope_kernel<T, V, decltype(a)::value><<<dim3((unsigned)ceil_div(p.n, 32 * V), parts), 32 * SLOPE_LANES, 0, st>>>(p), count_launch();
-    else slope_kernel<T, 1, decltype(a)::value><<<dim3((unsigned)ceil_div(p.n, 32), parts), 32 * SLOPE_LANES, 0, st>>>(p), count_launch();
+    if (vec) slope_kernel<T, V, decltype(a)::value><<<dim3(blocks, parts), 32 * SLOPE_LANES, 0, st>>>(p), count_launch();
+    else slope_kernel<T, 1, decltype(a)::value><<<dim3(blocks, parts), 32 * SLOPE_LANES, 0, st>>>(p), count_launch();
   });
   LIK_CUDA_OK(cudaGetLastError());
   return LIK_OK;
 }
-// dz (or NULL) and the columns' sums (sums != NULL: param_dtype [n], with `partial` as scratch)
-size_t slope_workspace(long long rows, int n, int dtype) { return align_up((size_t)slope_parts(rows, n, dtype) * n * sizeof(float), 256); }
-int launch_slope(SlopeParams p, int act, int dtype, void* sums, int sums_dtype, cudaStream_t st) {
-  const int item = (int)dtype_size(dtype), parts = slope_parts(p.rows, p.n, dtype);
+// jobs, rows, partial and the addresses of the sums (of sums_dtype, as the outs say) are filled in
+int launch_slope(SlopeParams& p, int act, int dtype, bool sums, cudaStream_t st) {
+  const int item = (int)dtype_size(dtype);
+  long long cols = 0;
+  bool vec = true;
+  for (int i = 0; i < SUM_OUTS; ++i) {
+    if (i < p.n_jobs) {
+      const SlopeJob& j = p.job[i];
+      cols += j.n;
+      vec = vec && vec_ok(j.dy, j.dy_stride, j.n, item) && (act == LIK_ACT_NONE || (vec_ok(j.z, j.z_stride, j.n, item) && vec_ok(j.dz, j.dz_stride, j.n, item)));
+    }
+    p.outs.end[i] = cols;
+  }
+  const int parts = sums || p.rows > 128 ? slope_parts(p.rows, cols, dtype) : 1;
   p.rows_per = ceil_div(p.rows, parts);
-  if (!sums) p.partial = nullptr;
-  const bool vec = vec_ok(p.dy, p.dy_stride, p.n, item) && (act == LIK_ACT_NONE || vec_ok(p.z, p.z_stride, p.n, item)) &&
-                   (!p.dz || vec_ok(p.dz, p.dz_stride, p.n, item));
+  p.sums = sums;
+  if (parts == 1) p.partial = nullptr;
   int rc = dtype == LIK_F32 ? run_slope<float>(p, act, vec, parts, st)
                             : (dtype == LIK_F16 ? run_slope<__half>(p, act, vec, parts, st) : run_slope<__nv_bfloat16>(p, act, vec, parts, st));
-  if (rc || !sums) return rc;
-  return launch_sum_parts(p.partial, parts, p.n, p.n, sums_dtype, sums, nullptr, st);
+  if (rc || !sums || parts == 1) return rc;
+  return launch_sum_parts(p.partial, parts, p.outs, dtype, st);
 }
 
 // Which kernel a product goes to.  Several products of a pass are plain ones and go to the tensor cores together.
@@ -346,7 +377,8 @@ GatedBwd gated_bwd_layout(const lik_gated_args& a, void* ws) {
     const size_t b = gemm_workspace(&l.dh);
     l.gemm_bytes = b > l.gemm_bytes ? b : l.gemm_bytes;
   }
-  if (a.db_gate || a.db_up || a.db_down) l.partial = c.take<float>(slope_workspace(a.rows, a.hidden > a.out ? a.hidden : a.out, a.dtype) * 2);
+  const long long sums = (a.db_gate ? a.hidden : 0ll) + (a.db_up ? a.hidden : 0ll) + (a.db_down ? a.out : 0ll);
+  if (sums) l.partial = c.take<float>(slope_workspace(a.rows, sums, a.dtype));
   l.gemm = c.take(l.gemm_bytes);
   l.total = c.off;
   return l;
@@ -354,12 +386,12 @@ GatedBwd gated_bwd_layout(const lik_gated_args& a, void* ws) {
 
 }  // namespace
 
-int launch_sum_parts(const float* partial, int parts, long long n, long long split, int dtype, void* out, void* out2, cudaStream_t st) {
-  const long long grid = ceil_div(n, 32);
+int launch_sum_parts(const float* partial, int parts, const SumOuts& outs, int dtype, cudaStream_t st) {
+  const long long grid = ceil_div(outs.end[SUM_OUTS - 1], SUM_COLS);
   LIK_REQUIRE(grid < (1ll << 31), "too many sums");
-  if (dtype == LIK_F32) sum_parts_kernel<float><<<(unsigned)grid, 256, 0, st>>>(partial, parts, n, split, (float*)out, (float*)out2), count_launch();
-  else if (dtype == LIK_F16) sum_parts_kernel<__half><<<(unsigned)grid, 256, 0, st>>>(partial, parts, n, split, (__half*)out, (__half*)out2), count_launch();
-  else sum_parts_kernel<__nv_bfloat16><<<(unsigned)grid, 256, 0, st>>>(partial, parts, n, split, (__nv_bfloat16*)out, (__nv_bfloat16*)out2), count_launch();
+  if (dtype == LIK_F32) sum_parts_kernel<float><<<(unsigned)grid, 256, 0, st>>>(partial, parts, outs), count_launch();
+  else if (dtype == LIK_F16) sum_parts_kernel<__half><<<(unsigned)grid, 256, 0, st>>>(partial, parts, outs), count_launch();
+  else sum_parts_kernel<__nv_bfloat16><<<(unsigned)grid, 256, 0, st>>>(partial, parts, outs), count_launch();
   LIK_CUDA_OK(cudaGetLastError());
   return LIK_OK;
 }
@@ -408,8 +440,14 @@ extern "C" int lik_linear_bwd(const lik_linear_args* args, lik_stream_t stream) 
   const LinearBwd l = linear_bwd_layout(a, a.workspace);
   if (a.workspace_bytes < l.total || (l.total && !a.workspace)) return too_small("lik_linear_bwd");
   if (act || a.dbias) {
-    SlopeParams p{a.dy, a.z, a.dy_stride, a.z_stride, a.rows, 0, a.out, l.dz, l.dz_stride, l.partial};
-    if (int rc = launch_slope(p, a.activation, a.dtype, a.dbias, a.param_dtype, st)) return rc;
+    SlopeParams p{};
+    p.job[0] = {a.dy, a.z, a.dy_stride, a.z_stride, a.out, 0, l.dz, l.dz_stride};
+    p.n_jobs = 1;
+    p.rows = a.rows;
+    p.partial = l.partial;
+    p.outs.out[0] = a.dbias;
+    p.outs.f32 = a.param_dtype == LIK_F32;
+    if (int rc = launch_slope(p, a.activation, a.dtype, a.dbias != nullptr, st)) return rc;
   }
   return launch_gemm(l.grads, l.n_grads, l.gemm, l.gemm_bytes, a.status, st);
 }
@@ -461,12 +499,18 @@ extern "C" int lik_gated_bwd(const lik_gated_args* args, lik_stream_t stream) {
   if (l.dg)
     if (int rc = launch_gemm(&l.dh, 1, l.gemm, l.gemm_bytes, a.status, st)) return rc;
   if (int rc = launch_gemm(l.grads, l.n_grads, l.gemm, l.gemm_bytes, a.status, st)) return rc;
-  auto sums = [&](const void* g, long long stride, int n, void* out) {
-    if (!out) return (int)LIK_OK;
-    SlopeParams p{g, nullptr, stride, 0, a.rows, 0, n, nullptr, 0, l.partial};
-    return launch_slope(p, LIK_ACT_NONE, a.dtype, out, a.param_dtype, st);
+  SlopeParams p{};
+  auto sum = [&](const void* g, long long stride, int n, void* out) {
+    if (!out) return;
+    p.job[p.n_jobs] = {g, nullptr, stride, 0, n, 0, nullptr, 0};
+    p.outs.out[p.n_jobs++] = out;
   };
-  if (int rc = sums(l.dg, l.stride, a.hidden, a.db_gate)) return rc;
-  if (int rc = sums(l.du, l.stride, a.hidden, a.db_up)) return rc;
-  return sums(a.dy, a.dy_stride, a.out, a.db_down);
+  sum(l.dg, l.stride, a.hidden, a.db_gate);
+  sum(l.du, l.stride, a.hidden, a.db_up);
+  sum(a.dy, a.dy_stride, a.out, a.db_down);
+  if (!p.n_jobs) return LIK_OK;
+  p.rows = a.rows;
+  p.partial = l.partial;
+  p.outs.f32 = a.param_dtype == LIK_F32;
+  return launch_slope(p, LIK_ACT_NONE, a.dtype, true, st);
 }

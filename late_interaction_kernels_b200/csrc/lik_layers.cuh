@@ -261,7 +261,21 @@ int launch_gemm_tc(const GemmDesc* d, int n, void* ws, size_t ws_bytes, int* sta
 size_t gemm_f32_workspace(const GemmDesc* d, int n);
 int launch_gemm_f32(const GemmDesc* d, int n, void* ws, size_t ws_bytes, int* status, cudaStream_t st);
 
-// sum over `parts` of partial[part][i], i < n, as dtype: out[i], the second half (i >= split) to out2
-int launch_sum_parts(const float* partial, int parts, long long n, long long split, int dtype, void* out, void* out2, cudaStream_t st);
+// Vectors of sums: element i of all of them, one behind the other, belongs to the first vector whose end is above i.
+constexpr int SUM_OUTS = 3;
+struct SumOuts {
+  void* out[SUM_OUTS];  // of the kernel's T, or fp32; NULL: not wanted
+  long long end[SUM_OUTS];
+  bool f32;
+  template <typename T>
+  __device__ __forceinline__ void put(long long i, float v) const {
+    const int q = i < end[0] ? 0 : (i < end[1] ? 1 : 2);
+    const long long at = i - (q ? end[q - 1] : 0);
+    if (!out[q]) return;
+    if (f32) ((float*)out[q])[at] = v;
+    else ((T*)out[q])[at] = from_f32<T>(v);
+  }
+};
+int launch_sum_parts(const float* partial, int parts, const SumOuts& outs, int dtype, cudaStream_t st);
 
 }  // namespace lik

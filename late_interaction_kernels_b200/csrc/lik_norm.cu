@@ -26,7 +26,7 @@ struct NormParams {
 
 constexpr int NORM_THREADS = 256;
 
-// sums of two numbers over the threads of a row: a warp, or the block
+// sums of two numbers over the threads of a row: a warp, or several, which meet at a barrier of their own
 template <int TPR>
 __device__ __forceinline__ float2 row_sum(float a, float b, float2 (&buf)[2][32], int& turn) {
 #pragma unroll
@@ -34,20 +34,25 @@ __device__ __forceinline__ float2 row_sum(float a, float b, float2 (&buf)[2][32]
     a += __shfl_xor_sync(0xffffffffu, a, o);
     b += __shfl_xor_sync(0xffffffffu, b, o);
   }
-  if (TPR == 32) return make_float2(a, b);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if constexpr (TPR == 32) return make_float2(a, b);
+  else {
+  static_assert(NORM_THREADS / TPR <= 2, "a barrier per row");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = threadIdx.x / TPR;
   // two buffers in turn: nobody is more than one barrier ahead of who still reads
   turn ^= 1;
   if (lane == 0) buf[turn][warp] = make_float2(a, b);
-  __syncthreads();
+  if (TPR == NORM_THREADS) __syncthreads();
+  else if (group == 0) asm volatile("bar.sync 1, %0;" ::"n"(TPR) : "memory");  // (a number in a register would reserve all sixteen barriers)
+  else asm volatile("bar.sync 2, %0;" ::"n"(TPR) : "memory");
   a = b = 0.0f;
 #pragma unroll
   for (int w = 0; w < TPR / 32; ++w) {
-    const float2 f = buf[turn][w];
+    const float2 f = buf[turn][group * (TPR / 32) + w];
     a += f.x;
     b += f.y;
   }
   return make_float2(a, b);
+  }
 }
 
 template <typename T, typename P, int V, int NV, int TPR>
@@ -107,8 +112,33 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_fwd_kernel(const NormParams
   }
 }
 
+// a vector of V elements as it came from memory
+template <typename T, int V>
+struct RawVec {
+  uint4 u;
+  __device__ __forceinline__ void load(const T* p) { u = __ldg(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void get(float (&f)[V]) const {
+    if constexpr (sizeof(T) == 4) {
+      f[0] = __uint_as_float(u.x), f[1] = __uint_as_float(u.y), f[2] = __uint_as_float(u.z), f[3] = __uint_as_float(u.w);
+    } else {
+      unpack2(u.x, f[0], f[1], T());
+      unpack2(u.y, f[2], f[3], T());
+      unpack2(u.z, f[4], f[5], T());
+      unpack2(u.w, f[6], f[7], T());
+    }
+  }
+};
+template <typename T>
+struct RawVec<T, 1> {
+  T e;
+  __device__ __forceinline__ void load(const T* p) { e = *p; }
+  __device__ __forceinline__ void get(float (&f)[1]) const { f[0] = to_f32(e); }
+};
+
+// The next row is fetched while the present one is reduced and written; both stay as they came from memory, since two rows and the columns'
+// sums in fp32 would leave an SM one block.
 template <typename T, typename P, int V, int NV, int TPR, bool PARAMS>
-__global__ void __launch_bounds__(NORM_THREADS) norm_bwd_kernel(const NormParams p) {
+__global__ void __launch_bounds__(NORM_THREADS, NV * V <= 24 ? 2 : 1) norm_bwd_kernel(const NormParams p) {
   __shared__ float2 buf[2][32];
   int turn = 0;
   constexpr int PER_BLOCK = NORM_THREADS / TPR;
@@ -119,52 +149,73 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_bwd_kernel(const NormParams
   for (int i = 0; i < (PARAMS ? NV : 1); ++i)
 #pragma unroll
     for (int j = 0; j < V; ++j) dw[i][j] = db[i][j] = 0.0f;
-  for (long long r = (long long)blockIdx.x * PER_BLOCK + threadIdx.x / TPR; r < p.rows; r += (long long)gridDim.x * PER_BLOCK) {
+  RawVec<T, V> rx[NV], rg[NV];
+  float mean = 0.0f, rstd = 0.0f;
+  auto fetch = [&](long long r) {
+    if (r >= p.rows) return;
     const T* x = (const T*)p.x + r * p.x_stride;
     const T* dy = (const T*)p.dy + r * p.width;
-    const float mean = p.mean[r], rstd = p.rstd[r];
-    float h[NV][V], g[NV][V];
-    float s = 0.0f, t = 0.0f;
+    mean = p.mean[r];
+    rstd = p.rstd[r];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * TPR + lane) * V;
       if (c < p.width) {
-        load_vec<T, V>(x + c, h[i]);
-        load_vec<T, V>(dy + c, g[i]);
+        rx[i].load(x + c);
+        rg[i].load(dy + c);
       }
     }
+  };
+  const long long step = (long long)gridDim.x * PER_BLOCK;
+  long long r = (long long)blockIdx.x * PER_BLOCK + threadIdx.x / TPR;
+  fetch(r);
+  for (; r < p.rows; r += step) {
+    RawVec<T, V> x[NV], y[NV];
+    const float m = mean, s = rstd;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) x[i] = rx[i], y[i] = rg[i];
+    fetch(r + step);
+    float sg = 0.0f, sgh = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * TPR + lane) * V;
       if (c < p.width) {
-        float w[V];
+        float w[V], h[V], g[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) w[j] = 1.0f;
         if (p.w) load_vec<P, V>((const P*)p.w + c, w);
+        x[i].get(h);
+        y[i].get(g);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          h[i][j] = (h[i][j] - mean) * rstd;
+          h[j] = (h[j] - m) * s;
           if (PARAMS) {
-            dw[i][j] = fmaf(g[i][j], h[i][j], dw[i][j]);
-            db[i][j] += g[i][j];
+            dw[i][j] = fmaf(g[j], h[j], dw[i][j]);
+            db[i][j] += g[j];
           }
-          g[i][j] *= w[j];
-          s += g[i][j];
-          t = fmaf(g[i][j], h[i][j], t);
+          g[j] *= w[j];
+          sg += g[j];
+          sgh = fmaf(g[j], h[j], sgh);
         }
       }
     }
     if (p.dx) {
-      const float2 m = row_sum<TPR>(s, t, buf, turn);
-      const float c1 = m.x * inv_n, c2 = m.y * inv_n;
+      const float2 sums = row_sum<TPR>(sg, sgh, buf, turn);
+      const float c1 = sums.x * inv_n, c2 = sums.y * inv_n;
       T* dx = (T*)p.dx + r * p.width;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int c = (i * TPR + lane) * V;
         if (c < p.width) {
+          float w[V], h[V], g[V];
 #pragma unroll
-          for (int j = 0; j < V; ++j) g[i][j] = rstd * (g[i][j] - c1 - h[i][j] * c2);
-          store_vec<T, V>(dx + c, g[i]);
+          for (int j = 0; j < V; ++j) w[j] = 1.0f;
+          if (p.w) load_vec<P, V>((const P*)p.w + c, w);
+          x[i].get(h);
+          y[i].get(g);
+#pragma unroll
+          for (int j = 0; j < V; ++j) g[j] = s * (g[j] * w[j] - c1 - (h[j] - m) * s * c2);
+          store_vec<T, V>(dx + c, g);
         }
       }
     }
@@ -267,42 +318,47 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_dparam_wide_kernel(const No
 
 constexpr int NORM_WIDE_PARTS = 64;
 
-// Which kernel a width goes to: a warp per row as long as its lanes hold the row in 32 (16-bit) or 16 (fp32) registers each, then a
-// block of 256 threads; vectors of 16 bytes where rows and parameters are aligned, else single elements.
+// Which kernel a width goes to: a warp per row, four warps or the block's eight; vectors of 16 bytes where rows and parameters are aligned, else
+// single elements.  The forward keeps a row with a warp up to four vectors per lane.  The backward, which holds a row twice and its columns'
+// sums, keeps a warp per row up to three, at 128 registers: 65536 x 768 bf16 65 us, 102 with four warps per row, of which the fourth has
+// nothing; with four vectors a lane would need 176 (16384 x 1024: 36 us, 31 with four warps per row).
 struct NormPlan {
   bool wide, vec;
   int nv, tpr;
 };
-NormPlan norm_plan(const lik_norm_args& a) {
+NormPlan norm_plan(const lik_norm_args& a, bool bwd) {
   const int item = (int)dtype_size(a.dtype), v = 16 / item;
   NormPlan pl{};
   pl.vec = vec_ok(a.x, a.x_stride, a.width, item) && vec_ok(a.y, a.width, a.width, item) && vec_ok(a.dy, a.width, a.width, item) &&
            vec_ok(a.dx, a.width, a.width, item) && ((uintptr_t)a.weight & 15) == 0 && ((uintptr_t)a.bias & 15) == 0;
-  const int per = pl.vec ? v : 1;
-  const long long vecs = ceil_div(a.width, per);
-  const int warp_most = pl.vec ? 4 : 8, block_most = pl.vec ? 4 : 16;
-  pl.tpr = vecs <= 32 * warp_most ? 32 : 256;
-  pl.nv = (int)ceil_div(vecs, pl.tpr);
-  pl.wide = pl.tpr == 256 && pl.nv > block_most;
-  if (!pl.vec && pl.nv > 1) pl.nv = pl.nv <= 4 ? 4 : (pl.nv <= 8 ? 8 : 16);
-  else if (pl.vec && pl.tpr == 256 && pl.nv == 3) pl.nv = 4;
+  const long long vecs = ceil_div(a.width, pl.vec ? v : 1);
+  if (pl.vec) {
+    pl.tpr = vecs <= (bwd ? 96 : 128) ? 32 : (vecs <= 128 ? 128 : 256);
+    pl.nv = (int)ceil_div(vecs, pl.tpr);
+    if (pl.tpr == 256 && pl.nv == 3) pl.nv = 4;
+    pl.wide = pl.nv > 4;
+  } else {
+    pl.tpr = vecs <= 256 ? 32 : 256;
+    const long long need = ceil_div(vecs, pl.tpr);
+    pl.nv = need == 1 && pl.tpr == 32 ? 1 : (need <= 4 ? 4 : (need <= 8 ? 8 : 16));
+    pl.wide = need > 16;
+  }
   return pl;
 }
 int norm_bwd_blocks(const lik_norm_args& a, const NormPlan& pl) {
   if (pl.wide) return (int)(a.rows < NORM_WIDE_PARTS ? (a.rows ? a.rows : 1) : NORM_WIDE_PARTS);
-  const long long need = ceil_div(a.rows, NORM_THREADS / pl.tpr), most = 2ll * sm_count();
+  const long long need = ceil_div(a.rows, NORM_THREADS / pl.tpr), most = (pl.tpr == 256 && pl.nv <= (pl.vec ? 1 : 4) ? 3ll : 2ll) * sm_count();  // (what an SM holds)
   return (int)(need < most ? (need ? need : 1) : most);
 }
 
 template <typename T, typename P, int V, int NV, int TPR>
 int run_norm(const NormParams& p, bool bwd, bool params, int blocks, cudaStream_t st) {
   if (!bwd) {
-    norm_fwd_kernel<T, P, V, NV, TPR><<<blocks, NORM_THREADS, 0, st>>>(p), count_launch();
-  } else if (params) {
-    const size_t smem = TPR == 32 ? sizeof(float) * 2 * NV * TPR * V : 0;
-    norm_bwd_kernel<T, P, V, NV, TPR, true><<<blocks, NORM_THREADS, smem, st>>>(p), count_launch();
-  } else {
-    norm_bwd_kernel<T, P, V, NV, TPR, false><<<blocks, NORM_THREADS, 0, st>>>(p), count_launch();
+    if constexpr (TPR != 128) norm_fwd_kernel<T, P, V, NV, TPR><<<blocks, NORM_THREADS, 0, st>>>(p), count_launch();
+  } else if constexpr (V == 1 || TPR != 32 || NV <= 3) {
+    const size_t smem = TPR < NORM_THREADS ? sizeof(float) * 2 * NV * TPR * V : 0;
+    if (params) norm_bwd_kernel<T, P, V, NV, TPR, true><<<blocks, NORM_THREADS, smem, st>>>(p), count_launch();
+    else norm_bwd_kernel<T, P, V, NV, TPR, false><<<blocks, NORM_THREADS, 0, st>>>(p), count_launch();
   }
   LIK_CUDA_OK(cudaGetLastError());
   return LIK_OK;
@@ -326,6 +382,7 @@ int run_norm(const NormPlan& pl, const NormParams& p, bool bwd, bool params, int
   LIK_NORM_CASE(V, 2, 32);
   LIK_NORM_CASE(V, 3, 32);
   LIK_NORM_CASE(V, 4, 32);
+  LIK_NORM_CASE(V, 1, 128);
   LIK_NORM_CASE(V, 1, 256);
   LIK_NORM_CASE(V, 2, 256);
   LIK_NORM_CASE(V, 4, 256);
@@ -367,7 +424,7 @@ extern "C" int lik_layer_norm_fwd(const lik_norm_args* args, lik_stream_t stream
   const lik_norm_args& a = *args;
   if (a.rows == 0) return LIK_OK;
   LIK_REQUIRE(a.x && a.y && !a.mean == !a.rstd, "x and y must not be NULL; mean and rstd go together");
-  const NormPlan pl = norm_plan(a);
+  const NormPlan pl = norm_plan(a, false);
   const long long need = ceil_div(a.rows, pl.wide ? 1 : NORM_THREADS / pl.tpr), most = 8ll * sm_count();
   return run_norm(a, pl, norm_params(a), false, false, (int)(need < most ? need : most), (cudaStream_t)stream);
 }
@@ -375,7 +432,7 @@ extern "C" int lik_layer_norm_fwd(const lik_norm_args* args, lik_stream_t stream
 extern "C" size_t lik_layer_norm_bwd_workspace(const lik_norm_args* a) {
   using namespace lik;
   if (check_norm(a) || a->rows == 0 || (!a->dweight && !a->dbias)) return 0;
-  return (size_t)norm_bwd_blocks(*a, norm_plan(*a)) * 2 * a->width * sizeof(float);
+  return (size_t)norm_bwd_blocks(*a, norm_plan(*a, true)) * 2 * a->width * sizeof(float);
 }
 
 extern "C" int lik_layer_norm_bwd(const lik_norm_args* args, lik_stream_t stream) {
@@ -396,10 +453,12 @@ extern "C" int lik_layer_norm_bwd(const lik_norm_args* args, lik_stream_t stream
     set_error("lik_layer_norm_bwd: workspace too small");
     return LIK_ERR_WORKSPACE;
   }
-  const NormPlan pl = norm_plan(a);
+  const NormPlan pl = norm_plan(a, true);
   NormParams p = norm_params(a);
   p.partial = (float*)a.workspace;
   const int blocks = norm_bwd_blocks(a, pl);
   if (int rc = run_norm(a, pl, p, true, params, blocks, st)) return rc;
-  return params ? launch_sum_parts(p.partial, blocks, 2ll * a.width, a.width, a.param_dtype, a.dweight, a.dbias, st) : LIK_OK;
+  if (!params) return LIK_OK;
+  const SumOuts outs{{a.dweight, a.dbias, nullptr}, {a.width, 2ll * a.width, 2ll * a.width}, a.param_dtype == LIK_F32};
+  return launch_sum_parts(p.partial, blocks, outs, a.dtype, st);
 }
