@@ -202,6 +202,7 @@ __device__ __forceinline__ float4 sum_shares(const SumJob& j, long long r, int c
 }
 template <typename T>
 __global__ void __launch_bounds__(256) sum_splits_kernel(const __grid_constant__ SumJobs p) {
+  after_the_kernel_in_front();
   const long long total = p.q[p.n - 1].end;
   for (long long g = blockIdx.x * 256ll + threadIdx.x; g < total; g += gridDim.x * 256ll) {
     int q = 0;
@@ -224,6 +225,7 @@ __global__ void __launch_bounds__(256) sum_splits_kernel(const __grid_constant__
 // ... and what GEMM_LINEAR does to them
 template <typename T>
 __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ SumJob j, const __grid_constant__ GemmDesc d) {
+  after_the_kernel_in_front();
   const int per_row = (j.n + 3) / 4;
   with_activation_dev(d.act, [&](auto act) {
     for (long long i = blockIdx.x * 256ll + threadIdx.x; i < j.end; i += gridDim.x * 256ll) {
@@ -359,10 +361,7 @@ int launch_sum_splits(const GtPlan& pl, const GemmDesc* d, cudaStream_t st) {
   if (!jobs.n) return LIK_OK;
   const long long blocks = ceil_div(total, 256), most = 16ll * sm_count();
   const unsigned grid = (unsigned)(blocks < most ? blocks : most);
-  if (gemm_plain(d[0])) sum_splits_kernel<T><<<grid, 256, 0, st>>>(jobs), count_launch();
-  else finish_kernel<T><<<grid, 256, 0, st>>>(jobs.q[0], d[0]), count_launch();
-  LIK_CUDA_OK(cudaGetLastError());
-  return LIK_OK;
+  return gemm_plain(d[0]) ? launch_after(sum_splits_kernel<T>, grid, 256, 0, st, 1, jobs) : launch_after(finish_kernel<T>, grid, 256, 0, st, 1, jobs.q[0], d[0]);
 }
 // Tensor maps are made by the driver, which wants the device's context to be current: a thread that has made no call of the runtime's
 // yet (autograd's, on the first backward of a process) has none until it says which device it is on.

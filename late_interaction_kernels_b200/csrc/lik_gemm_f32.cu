@@ -70,6 +70,7 @@ __global__ void __launch_bounds__(GF_THREADS, 1) gemm_f32_kernel(const __grid_co
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  after_the_kernel_in_front();
   const uint32_t tmem = ctl->tmem;  // accumulator pair b: a0 b0 in columns [256 b, 256 b + 128), the small products behind
 
   if (warp == GF_PRODUCER) {
@@ -295,6 +296,7 @@ struct CutJobs {
   int n;
 };
 __global__ void __launch_bounds__(256) cut_kernel(const __grid_constant__ CutJobs p) {
+  after_the_kernel_in_front();
   const long long total = p.end[p.n - 1];
   for (long long g = blockIdx.x * 256ll + threadIdx.x; g < total; g += gridDim.x * 256ll) {
     int q = 0;
@@ -333,9 +335,7 @@ GtPlan f32_plan(const GemmDesc* d, int n) {  // (a slab of k takes a CTA 1.5 to 
 template <int KIND>
 int run_f32(const GfMaps& maps, const GfParams& p, cudaStream_t st) {
   LIK_CUDA_OK(allow_smem<gemm_f32_kernel<KIND>>());
-  gemm_f32_kernel<KIND><<<p.units < sm_count() ? p.units : sm_count(), GF_THREADS, 1024 + GF_CTL_AT + sizeof(GfCtl), st>>>(maps, p), count_launch();
-  LIK_CUDA_OK(cudaGetLastError());
-  return LIK_OK;
+  return launch_after(gemm_f32_kernel<KIND>, p.units < sm_count() ? p.units : sm_count(), GF_THREADS, 1024 + GF_CTL_AT + sizeof(GfCtl), st, 1, maps, p);
 }
 
 }  // namespace
@@ -364,8 +364,7 @@ int launch_gemm_f32(const GemmDesc* d, int n, void* ws, size_t ws_bytes, int* st
   }
   cuts.n = pl.n_mat;
   const long long blocks = ceil_div(total, 256), most = 16ll * sm_count();
-  cut_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, st>>>(cuts), count_launch();
-  LIK_CUDA_OK(cudaGetLastError());
+  if (int rc = launch_after(cut_kernel, (unsigned)(blocks < most ? blocks : most), 256, 0, st, 1, cuts)) return rc;
   gt_outputs(pl, d, ws);
   p.act = d->act;
   for (int i = 0; i < 2; ++i) {

@@ -36,6 +36,7 @@ template <typename T, int KIND, int NT, int WARPS>
 __global__ void __launch_bounds__(32 * WARPS) few_mma_kernel(const __grid_constant__ FewParams p) {
   constexpr int DUAL = KIND == GEMM_GATED ? 2 : 1;
   __shared__ float part[WARPS][DUAL][NT][32][4];
+  after_the_kernel_in_front();
   const GemmDesc& d = p.d;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 8 * NT;
@@ -115,6 +116,7 @@ template <typename T, int KIND, int V>
 __global__ void __launch_bounds__(FEW_THREADS) few_fma_kernel(const __grid_constant__ FewParams p) {
   constexpr int DUAL = KIND == GEMM_GATED ? 2 : 1;
   __shared__ float part[DUAL][FEW_WARPS][32];
+  after_the_kernel_in_front();
   const GemmDesc& d = p.d;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n0 = blockIdx.x * FMA_ROWS, m0 = blockIdx.y * FMA_COLS;
@@ -187,14 +189,10 @@ int run_mma(const FewParams& p, cudaStream_t st) {
   // a long k: twice the warps, half the loads one after another (32 rows, 2048 x 768: 8.4 us against 6.2)
   if constexpr (KIND == GEMM_LINEAR) {
     if (d.k[0] >= 1024) {
-      few_mma_kernel<T, KIND, NT, 2 * FEW_WARPS><<<grid, 64 * FEW_WARPS, 0, st>>>(p), count_launch();
-      LIK_CUDA_OK(cudaGetLastError());
-      return LIK_OK;
+      return launch_after(few_mma_kernel<T, KIND, NT, 2 * FEW_WARPS>, grid, 64 * FEW_WARPS, 0, st, 1, p);
     }
   }
-  few_mma_kernel<T, KIND, NT, FEW_WARPS><<<grid, FEW_THREADS, 0, st>>>(p), count_launch();
-  LIK_CUDA_OK(cudaGetLastError());
-  return LIK_OK;
+  return launch_after(few_mma_kernel<T, KIND, NT, FEW_WARPS>, grid, FEW_THREADS, 0, st, 1, p);
 }
 template <typename T, int KIND>
 int run_few(const FewParams& p, cudaStream_t st) {
@@ -205,15 +203,9 @@ int run_few(const FewParams& p, cudaStream_t st) {
   }
   const dim3 grid((unsigned)ceil_div(d.n, FMA_ROWS), (unsigned)ceil_div(d.m, FMA_COLS));
   if constexpr (sizeof(T) == 4) {
-    if (vec) {
-      few_fma_kernel<T, KIND, vec_elems<T>()><<<grid, FEW_THREADS, 0, st>>>(p), count_launch();
-      LIK_CUDA_OK(cudaGetLastError());
-      return LIK_OK;
-    }
+    if (vec) return launch_after(few_fma_kernel<T, KIND, vec_elems<T>()>, grid, FEW_THREADS, 0, st, 1, p);
   }
-  few_fma_kernel<T, KIND, 1><<<grid, FEW_THREADS, 0, st>>>(p), count_launch();
-  LIK_CUDA_OK(cudaGetLastError());
-  return LIK_OK;
+  return launch_after(few_fma_kernel<T, KIND, 1>, grid, FEW_THREADS, 0, st, 1, p);
 }
 template <typename T>
 int run_few(const FewParams& p, cudaStream_t st) {

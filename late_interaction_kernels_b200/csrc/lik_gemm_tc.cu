@@ -154,6 +154,7 @@ __global__ void __launch_bounds__(GtWarps<KIND, !std::is_same<T, O>::value>::THR
   __syncthreads();
   if constexpr (CG == 2) cluster_sync();  // the other CTA's barriers are there
   tc_fence_after();
+  after_the_kernel_in_front();
   const uint32_t tmem = ctl->tmem;
   const int first = blockIdx.x / CG, step = gridDim.x / CG;
 
@@ -392,6 +393,7 @@ __global__ void __launch_bounds__(GtWarps<KIND, !std::is_same<T, O>::value>::THR
 // rows that TMA cannot address, copied to rows of 16 bytes (the columns behind them are zeros)
 __global__ void __launch_bounds__(256) repack_kernel(const uint16_t* __restrict__ src, long long src_stride, long long rows, int cols, uint4* __restrict__ dst,
                                                      int vecs) {
+  after_the_kernel_in_front();
   const long long total = rows * vecs;
   for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
     const long long r = i / vecs;
@@ -419,20 +421,8 @@ template <int CG, int KIND, bool RES, typename T, typename O>
 int run_tc(const GtMaps& maps, const GtParams& p, cudaStream_t st) {
   LIK_CUDA_OK((allow_smem<gemm_tc_kernel<CG, KIND, RES, T, O>>()));
   const int slots = sm_count() / CG;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)((p.units < slots ? p.units : slots) * CG));
-  cfg.blockDim = dim3(GtWarps<KIND, !std::is_same<T, O>::value>::THREADS);
-  cfg.dynamicSmemBytes = 1024 + GT_CTL_AT + sizeof(GtCtl);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CG;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  LIK_CUDA_OK(cudaLaunchKernelEx(&cfg, gemm_tc_kernel<CG, KIND, RES, T, O>, maps, p));
-  count_launch();
-  return LIK_OK;
+  return launch_after(gemm_tc_kernel<CG, KIND, RES, T, O>, (unsigned)((p.units < slots ? p.units : slots) * CG), GtWarps<KIND, !std::is_same<T, O>::value>::THREADS,
+                      1024 + GT_CTL_AT + sizeof(GtCtl), st, CG, maps, p);
 }
 template <int KIND, bool RES, typename T, typename O>
 int run_tc(int cg, const GtMaps& maps, const GtParams& p, cudaStream_t st) {
@@ -464,8 +454,9 @@ int launch_gemm_tc(const GemmDesc* d, int n, void* ws, size_t ws_bytes, int* sta
     if (pl.copied[i]) {
       void* to = (char*)ws + pl.copy[i];
       const long long vecs = o.padded() / 8, blocks = ceil_div(o.rows * vecs, 256), most = 16ll * sm_count();
-      repack_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, st>>>((const uint16_t*)o.p, o.stride, o.rows, (int)o.cols, (uint4*)to, (int)vecs), count_launch();
-      LIK_CUDA_OK(cudaGetLastError());
+      if (int rc = launch_after(repack_kernel, (unsigned)(blocks < most ? blocks : most), 256, 0, st, 1, (const uint16_t*)o.p, o.stride, o.rows, (int)o.cols, (uint4*)to,
+                                (int)vecs))
+        return rc;
       o.p = to;
       o.stride = o.padded();
     }

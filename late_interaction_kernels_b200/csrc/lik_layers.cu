@@ -11,6 +11,7 @@ constexpr int SUM_COLS = 8;  // a sector of each part; the block's 32 groups of 
 template <typename T>
 __global__ void __launch_bounds__(256) sum_parts_kernel(const float* __restrict__ partial, int parts, const __grid_constant__ SumOuts outs) {
   __shared__ float s[8][SUM_COLS];
+  after_the_kernel_in_front();
   const int col = threadIdx.x % SUM_COLS, group = threadIdx.x / SUM_COLS, warp = threadIdx.x / 32;
   const long long i = blockIdx.x * (long long)SUM_COLS + col, n = outs.end[SUM_OUTS - 1];
   float v = 0.0f;
@@ -51,8 +52,9 @@ struct SlopeParams {
   SumOuts outs;
 };
 template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(32 * SLOPE_LANES) slope_kernel(const __grid_constant__ SlopeParams p) {
+__global__ void __launch_bounds__(32 * SLOPE_LANES, 4) slope_kernel(const __grid_constant__ SlopeParams p) {
   __shared__ float s[SLOPE_LANES][32 * V + 1];
+  after_the_kernel_in_front();
   const int lane = threadIdx.x % 32, row = threadIdx.x / 32;
   int q = 0, block = blockIdx.x;
   while (block >= p.job[q].blocks) block -= p.job[q++].blocks;
@@ -63,7 +65,7 @@ __global__ void __launch_bounds__(32 * SLOPE_LANES) slope_kernel(const __grid_co
   for (int i = 0; i < V; ++i) sum[i] = 0.0f;
   if (c < j.n) {
     const long long r0 = blockIdx.y * p.rows_per, r1 = r0 + p.rows_per < p.rows ? r0 + p.rows_per : p.rows;
-#pragma unroll 4
+#pragma unroll 2
     for (long long r = r0 + row; r < r1; r += SLOPE_LANES) {
       float g[V], z[V];
       load_vec<T, V>((const T*)j.dy + r * j.dy_stride + c, g);
@@ -96,7 +98,8 @@ __global__ void __launch_bounds__(32 * SLOPE_LANES) slope_kernel(const __grid_co
 // (128 rows: a lane's sixteen, in four trips to memory)
 int slope_parts(long long rows, long long cols, int dtype) {
   if (rows <= 128) return 1;
-  long long want = ceil_div(4ll * sm_count(), ceil_div(cols, 32 * (16 / (int)dtype_size(dtype))));
+  // four blocks per SM, and none that would wait for one of them to end
+  long long want = 4ll * sm_count() / ceil_div(cols, 32 * (16 / (int)dtype_size(dtype)));
   if (want > ceil_div(rows, SLOPE_LANES)) want = ceil_div(rows, SLOPE_LANES);
   if (want > 65535) want = 65535;
   return want < 1 ? 1 : (int)want;
@@ -110,12 +113,12 @@ int run_slope(SlopeParams& p, int act, bool vec, int parts, cudaStream_t st) {
   constexpr int V = vec_elems<T>();
   unsigned blocks = 0;
   for (int i = 0; i < p.n_jobs; ++i) blocks += p.job[i].blocks = (int)ceil_div(p.job[i].n, 32 * (vec ? V : 1));
+  int rc = LIK_OK;
   with_activation(act, [&](auto a) {
-    if (vec) slope_kernel<T, V, decltype(a)::value><<<dim3(blocks, parts), 32 * SLOPE_LANES, 0, st>>>(p), count_launch();
-    else slope_kernel<T, 1, decltype(a)::value><<<dim3(blocks, parts), 32 * SLOPE_LANES, 0, st>>>(p), count_launch();
+    rc = vec ? launch_after(slope_kernel<T, V, decltype(a)::value>, dim3(blocks, parts), 32 * SLOPE_LANES, 0, st, 1, p)
+             : launch_after(slope_kernel<T, 1, decltype(a)::value>, dim3(blocks, parts), 32 * SLOPE_LANES, 0, st, 1, p);
   });
-  LIK_CUDA_OK(cudaGetLastError());
-  return LIK_OK;
+  return rc;
 }
 // jobs, rows, partial and the addresses of the sums (of sums_dtype, as the outs say) are filled in
 int launch_slope(SlopeParams& p, int act, int dtype, bool sums, cudaStream_t st) {
@@ -389,11 +392,9 @@ GatedBwd gated_bwd_layout(const lik_gated_args& a, void* ws) {
 int launch_sum_parts(const float* partial, int parts, const SumOuts& outs, int dtype, cudaStream_t st) {
   const long long grid = ceil_div(outs.end[SUM_OUTS - 1], SUM_COLS);
   LIK_REQUIRE(grid < (1ll << 31), "too many sums");
-  if (dtype == LIK_F32) sum_parts_kernel<float><<<(unsigned)grid, 256, 0, st>>>(partial, parts, outs), count_launch();
-  else if (dtype == LIK_F16) sum_parts_kernel<__half><<<(unsigned)grid, 256, 0, st>>>(partial, parts, outs), count_launch();
-  else sum_parts_kernel<__nv_bfloat16><<<(unsigned)grid, 256, 0, st>>>(partial, parts, outs), count_launch();
-  LIK_CUDA_OK(cudaGetLastError());
-  return LIK_OK;
+  return dtype == LIK_F32   ? launch_after(sum_parts_kernel<float>, (unsigned)grid, 256, 0, st, 1, partial, parts, outs)
+         : dtype == LIK_F16 ? launch_after(sum_parts_kernel<__half>, (unsigned)grid, 256, 0, st, 1, partial, parts, outs)
+                            : launch_after(sum_parts_kernel<__nv_bfloat16>, (unsigned)grid, 256, 0, st, 1, partial, parts, outs);
 }
 
 }  // namespace lik

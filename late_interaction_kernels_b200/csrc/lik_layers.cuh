@@ -127,6 +127,34 @@ LIK_WITH_ACTIVATION(with_activation_dev, __device__)
 #undef LIK_WITH_ACTIVATION
 
 // ---------------------------------------------------------------------------------------------
+// Launches.  A pass is a chain of short kernels, so each is launched with programmatic stream serialisation: its blocks come to the SMs as those of
+// the kernel in front leave, set themselves up and wait for that kernel's end.  Every kernel here begins with after_the_kernel_in_front(),
+// before which it touches no device memory (a backward pass of 1000 x 768 x 768 in a graph: PDL_BEFORE us without, PDL_AFTER with).
+// ---------------------------------------------------------------------------------------------
+__device__ __forceinline__ void after_the_kernel_in_front() {
+  asm volatile("griddepcontrol.wait;\n\tgriddepcontrol.launch_dependents;" ::: "memory");
+}
+template <typename... P, typename... A>
+int launch_after(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t st, int cluster, const A&... args) {
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  LIK_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, P(args)...));
+  count_launch();
+  return LIK_OK;
+}
+
+// ---------------------------------------------------------------------------------------------
 // Vectors of V elements, V * sizeof(T) = 16 bytes or one element, as fp32
 // ---------------------------------------------------------------------------------------------
 template <typename T>

@@ -58,6 +58,7 @@ __device__ __forceinline__ float2 row_sum(float a, float b, float2 (&buf)[2][32]
 template <typename T, typename P, int V, int NV, int TPR>
 __global__ void __launch_bounds__(NORM_THREADS) norm_fwd_kernel(const NormParams p) {
   __shared__ float2 buf[2][32];
+  after_the_kernel_in_front();
   int turn = 0;
   constexpr int PER_BLOCK = NORM_THREADS / TPR;
   const int lane = threadIdx.x % TPR;
@@ -140,6 +141,7 @@ struct RawVec<T, 1> {
 template <typename T, typename P, int V, int NV, int TPR, bool PARAMS>
 __global__ void __launch_bounds__(NORM_THREADS, NV * V <= 24 ? 2 : 1) norm_bwd_kernel(const NormParams p) {
   __shared__ float2 buf[2][32];
+  after_the_kernel_in_front();
   int turn = 0;
   constexpr int PER_BLOCK = NORM_THREADS / TPR;
   const int lane = threadIdx.x % TPR;
@@ -260,6 +262,7 @@ __global__ void __launch_bounds__(NORM_THREADS, NV * V <= 24 ? 2 : 1) norm_bwd_k
 template <typename T, typename P>
 __global__ void __launch_bounds__(NORM_THREADS) norm_fwd_wide_kernel(const NormParams p) {
   __shared__ float2 buf[2][32];
+  after_the_kernel_in_front();
   int turn = 0;
   const float inv_n = 1.0f / (float)p.width;
   for (long long r = blockIdx.x; r < p.rows; r += gridDim.x) {
@@ -281,6 +284,7 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_fwd_wide_kernel(const NormP
 template <typename T, typename P>
 __global__ void __launch_bounds__(NORM_THREADS) norm_dx_wide_kernel(const NormParams p) {
   __shared__ float2 buf[2][32];
+  after_the_kernel_in_front();
   int turn = 0;
   const float inv_n = 1.0f / (float)p.width;
   for (long long r = blockIdx.x; r < p.rows; r += gridDim.x) {
@@ -303,6 +307,7 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_dx_wide_kernel(const NormPa
 // a thread's column over every gridDim.y-th row
 template <typename T>
 __global__ void __launch_bounds__(NORM_THREADS) norm_dparam_wide_kernel(const NormParams p) {
+  after_the_kernel_in_front();
   const int c = blockIdx.x * NORM_THREADS + threadIdx.x;
   if (c >= p.width) return;
   float dw = 0.0f, db = 0.0f;
@@ -354,27 +359,22 @@ int norm_bwd_blocks(const lik_norm_args& a, const NormPlan& pl) {
 template <typename T, typename P, int V, int NV, int TPR>
 int run_norm(const NormParams& p, bool bwd, bool params, int blocks, cudaStream_t st) {
   if (!bwd) {
-    if constexpr (TPR != 128) norm_fwd_kernel<T, P, V, NV, TPR><<<blocks, NORM_THREADS, 0, st>>>(p), count_launch();
+    if constexpr (TPR != 128) return launch_after(norm_fwd_kernel<T, P, V, NV, TPR>, blocks, NORM_THREADS, 0, st, 1, p);
   } else if constexpr (V == 1 || TPR != 32 || NV <= 3) {
     const size_t smem = TPR < NORM_THREADS ? sizeof(float) * 2 * NV * TPR * V : 0;
-    if (params) norm_bwd_kernel<T, P, V, NV, TPR, true><<<blocks, NORM_THREADS, smem, st>>>(p), count_launch();
-    else norm_bwd_kernel<T, P, V, NV, TPR, false><<<blocks, NORM_THREADS, 0, st>>>(p), count_launch();
+    return params ? launch_after(norm_bwd_kernel<T, P, V, NV, TPR, true>, blocks, NORM_THREADS, smem, st, 1, p)
+                  : launch_after(norm_bwd_kernel<T, P, V, NV, TPR, false>, blocks, NORM_THREADS, 0, st, 1, p);
   }
-  LIK_CUDA_OK(cudaGetLastError());
-  return LIK_OK;
+  return LIK_ERR_UNSUPPORTED;  // (a shape that the plan does not give)
 }
 template <typename T, typename P>
 int run_norm(const NormPlan& pl, const NormParams& p, bool bwd, bool params, int blocks, cudaStream_t st) {
   constexpr int V = vec_elems<T>();
   if (pl.wide) {
-    if (!bwd) {
-      norm_fwd_wide_kernel<T, P><<<blocks, NORM_THREADS, 0, st>>>(p), count_launch();
-    } else {
-      if (p.dx) norm_dx_wide_kernel<T, P><<<(unsigned)(p.rows < 8ll * sm_count() ? p.rows : 8ll * sm_count()), NORM_THREADS, 0, st>>>(p), count_launch();
-      if (params) norm_dparam_wide_kernel<T><<<dim3((unsigned)ceil_div(p.width, NORM_THREADS), blocks), NORM_THREADS, 0, st>>>(p), count_launch();
-    }
-    LIK_CUDA_OK(cudaGetLastError());
-    return LIK_OK;
+    if (!bwd) return launch_after(norm_fwd_wide_kernel<T, P>, blocks, NORM_THREADS, 0, st, 1, p);
+    if (p.dx)
+      if (int rc = launch_after(norm_dx_wide_kernel<T, P>, (unsigned)(p.rows < 8ll * sm_count() ? p.rows : 8ll * sm_count()), NORM_THREADS, 0, st, 1, p)) return rc;
+    return params ? launch_after(norm_dparam_wide_kernel<T>, dim3((unsigned)ceil_div(p.width, NORM_THREADS), blocks), NORM_THREADS, 0, st, 1, p) : LIK_OK;
   }
 #define LIK_NORM_CASE(VV, NN, TT) \
   if ((pl.vec ? V : 1) == VV && pl.nv == NN && pl.tpr == TT) return run_norm<T, P, VV, NN, TT>(p, bwd, params, blocks, st)
