@@ -82,11 +82,12 @@ Tensor as_rows(const Tensor& t, at::ScalarType dt) {
   if (r.dim() == 1) return r.contiguous();
   return rows_of(r);
 }
-// a matrix that kernels write and read again: rows that start on 16 bytes
-Tensor kept_rows(int64_t rows, int64_t cols, const Tensor& like) {
+// matrices that kernels write and read again, one behind the other: rows that start on 16 bytes
+Tensor kept_rows(int64_t n, int64_t rows, int64_t cols, const Tensor& like) {
   const int64_t v = 16 / (int64_t)like.element_size();
-  return at::empty({rows, (cols + v - 1) / v * v}, like.options());
+  return at::empty({n, rows, (cols + v - 1) / v * v}, like.options());
 }
+void* matrix_of(const Tensor& kept, int64_t i) { return kept.numel() ? (char*)kept.data_ptr() + i * kept.stride(0) * kept.element_size() : nullptr; }
 struct Workspace {
   Tensor t;
   void* p = nullptr;
@@ -304,7 +305,7 @@ struct LinearBackward : public torch::autograd::Node {
       a.param_dtype = grad_type;
       const auto popt = X.options().dtype(scalar_of(grad_type));
       a.z = ptr(Z);
-      a.z_stride = Z.defined() ? Z.size(1) : 0;
+      a.z_stride = Z.defined() ? Z.size(2) : 0;
       a.dy = ptr(dy);
       a.dy_stride = row_stride(dy);
       if (need_x) out[0] = at::empty(X.sizes(), X.options());
@@ -353,9 +354,9 @@ Tensor linear(const Tensor& x_, const Tensor& w, const OptTensor& bias_, const s
     y = at::empty({x.size(0), out}, x.options());
     a.y = ptr(y);
     if (grad && act != LIK_ACT_NONE) {
-      z = kept_rows(x.size(0), out, x);
+      z = kept_rows(1, x.size(0), out, x);
       a.z = ptr(z);
-      a.z_stride = z.size(1);
+      a.z_stride = z.size(2);
     }
     const Workspace ws(lik_linear_fwd_workspace(&a), x.device());
     a.workspace = ws.p;
@@ -405,28 +406,26 @@ lik_gated_args gated_args(const Tensor& x, const Tensor& wg, const Tensor& wu, c
 constexpr int N_GATED_PARAMS = 6;  // w_gate, w_up, w_down, b_gate, b_up, b_down
 
 struct GatedFeedForwardBackward : public torch::autograd::Node {
-  SavedVariable x, wg, wu, wd, gate, up, h;
+  SavedVariable x, wg, wu, wd, kept;  // kept: the factors of the gradients of gate and up, and h
   std::array<at::ScalarType, N_GATED_PARAMS> types{};
   int act = LIK_ACT_NONE, grad_type = LIK_F32;
 
   std::string name() const override { return "GatedFeedForwardBackward"; }
   void release_variables() override {
     const std::lock_guard<std::mutex> lock(mutex_);
-    for (SavedVariable* v : {&x, &wg, &wu, &wd, &gate, &up, &h}) v->reset_data();
+    for (SavedVariable* v : {&x, &wg, &wu, &wd, &kept}) v->reset_data();
   }
   variable_list apply(variable_list&& grads) override {
     variable_list out(2 + N_GATED_PARAMS);
     if (!grads[0].defined()) return out;
-    Tensor X, WG, WU, WD, G, U, H;
+    Tensor X, WG, WU, WD, K;
     {
       const std::lock_guard<std::mutex> lock(mutex_);
       X = x.unpack();
       WG = wg.unpack();
       WU = wu.unpack();
       WD = wd.unpack();
-      G = gate.unpack();
-      U = up.unpack();
-      H = h.unpack();
+      K = kept.unpack();
     }
     {
       at::AutoDispatchBelowADInplaceOrView below;
@@ -440,10 +439,10 @@ struct GatedFeedForwardBackward : public torch::autograd::Node {
       lik_gated_args a = gated_args(X, WG, WU, WD, act);
       a.param_dtype = grad_type;
       const auto popt = X.options().dtype(scalar_of(grad_type));
-      a.gate_factor = ptr(G);
-      a.up_factor = ptr(U);
-      a.h = ptr(H);
-      a.kept_stride = G.size(1);
+      a.gate_factor = matrix_of(K, 0);
+      a.up_factor = matrix_of(K, 1);
+      a.h = matrix_of(K, 2);
+      a.kept_stride = K.size(2);
       a.dy = ptr(dy);
       a.dy_stride = row_stride(dy);
       if (task_should_compute_output(0)) out[0] = at::empty(X.sizes(), X.options());
@@ -491,7 +490,7 @@ Tensor gated_feed_forward(const Tensor& x_, const Tensor& wg, const Tensor& wu, 
   const c10::cuda::CUDAGuard guard(x.device());
   const bool grad = wants_grad({&x, &wg, &wu, &wd, &bg, &bu, &bd, &r});
   if (grad) refuse_foreign_accumulators("gated_feed_forward", x.device(), {&x_, &wg, &wu, &wd, &bg, &bu, &bd, &r_});
-  Tensor y, g, u, h, pg, pu, pd;
+  Tensor y, kept, pg, pu, pd;
   {
     at::AutoDispatchBelowADInplaceOrView below;
     pg = as_rows(wg, dt);
@@ -507,13 +506,11 @@ Tensor gated_feed_forward(const Tensor& x_, const Tensor& wg, const Tensor& wu, 
     y = at::empty({x.size(0), out}, x.options());
     a.y = ptr(y);
     if (grad) {
-      g = kept_rows(x.size(0), f, x);
-      u = kept_rows(x.size(0), f, x);
-      h = kept_rows(x.size(0), f, x);
-      a.gate_factor = ptr(g);
-      a.up_factor = ptr(u);
-      a.h = ptr(h);
-      a.kept_stride = g.size(1);
+      kept = kept_rows(3, x.size(0), f, x);
+      a.gate_factor = matrix_of(kept, 0);
+      a.up_factor = matrix_of(kept, 1);
+      a.h = matrix_of(kept, 2);
+      a.kept_stride = kept.size(2);
     }
     const Workspace ws(lik_gated_fwd_workspace(&a), x.device());
     a.workspace = ws.p;
@@ -527,9 +524,7 @@ Tensor gated_feed_forward(const Tensor& x_, const Tensor& wg, const Tensor& wu, 
     node->wg = SavedVariable(wg.scalar_type() == dt ? wg : pg, false);
     node->wu = SavedVariable(wu.scalar_type() == dt ? wu : pu, false);
     node->wd = SavedVariable(wd.scalar_type() == dt ? wd : pd, false);
-    node->gate = SavedVariable(g, false);
-    node->up = SavedVariable(u, false);
-    node->h = SavedVariable(h, false);
+    node->kept = SavedVariable(kept, false);
     const Tensor* const params[N_GATED_PARAMS] = {&wg, &wu, &wd, &bg, &bu, &bd};
     for (int i = 0; i < N_GATED_PARAMS; ++i)
       if (params[i]->defined()) node->types[i] = params[i]->scalar_type();

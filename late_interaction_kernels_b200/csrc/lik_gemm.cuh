@@ -110,7 +110,9 @@ __device__ __forceinline__ void slot_store(const uint8_t* s, int lane, O* p, lon
       if (r < rows && c * PER < cols) *reinterpret_cast<uint4*>(p + r * stride + c * PER) = u;
     }
   } else if (lane < cols) {
-    for (int r = 0; r < rows && r < 32; ++r) p[r * stride + lane] = *reinterpret_cast<const O*>(s + slot_offset<ROW>(r, lane / PER) + (lane % PER) * sizeof(O));
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r)
+      if (r < rows) p[r * stride + lane] = *reinterpret_cast<const O*>(s + slot_offset<ROW>(r, lane / PER) + (lane % PER) * sizeof(O));
   }
 }
 template <typename T>
@@ -126,7 +128,9 @@ __device__ __forceinline__ void slot_fetch(uint8_t* s, int lane, const T* p, lon
                    : "memory");
     }
   } else if (lane < cols) {
-    for (int r = 0; r < rows && r < 32; ++r) *reinterpret_cast<T*>(s + slot_offset<ROW>(r, lane / PER) + (lane % PER) * sizeof(T)) = p[r * stride + lane];
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r)
+      if (r < rows) *reinterpret_cast<T*>(s + slot_offset<ROW>(r, lane / PER) + (lane % PER) * sizeof(T)) = p[r * stride + lane];
   }
 }
 
@@ -142,7 +146,9 @@ __device__ __forceinline__ void slot_store_as(const uint8_t* s, int lane, T* p, 
         *reinterpret_cast<uint4*>(p + r * stride + c * 8) = make_uint4(pack2(x.x, x.y, T()), pack2(x.z, x.w, T()), pack2(y.x, y.y, T()), pack2(y.z, y.w, T()));
     }
   } else if (lane < cols) {
-    for (int r = 0; r < rows && r < 32; ++r) p[r * stride + lane] = from_f32<T>(*reinterpret_cast<const float*>(s + slot_offset<128>(r, lane / 4) + (lane % 4) * 4));
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r)
+      if (r < rows) p[r * stride + lane] = from_f32<T>(*reinterpret_cast<const float*>(s + slot_offset<128>(r, lane / 4) + (lane % 4) * 4));
   }
 }
 

@@ -390,19 +390,40 @@ __global__ void __launch_bounds__(GtWarps<KIND, !std::is_same<T, O>::value>::THR
   if (warp == Warps::ISSUER) gt_dealloc<CG>(tmem, 2 * BN);
 }
 
-// rows that TMA cannot address, copied to rows of 16 bytes (the columns behind them are zeros)
-__global__ void __launch_bounds__(256) repack_kernel(const uint16_t* __restrict__ src, long long src_stride, long long rows, int cols, uint4* __restrict__ dst,
-                                                     int vecs) {
+// Matrices whose rows TMA cannot address, copied to rows of 16 bytes (the columns behind them are zeros).  A lane reads every 32nd element of
+// a row's 512, so that neighbours read neighbours, and the warp puts the pieces together in shared memory.
+constexpr int REPACK_COLS = 512;
+struct RepackJobs {
+  Stored m[GT_MATRICES];
+  void* to[GT_MATRICES];
+  long long end[GT_MATRICES];  // stretches of 512 columns up to and with this matrix
+  int n;
+};
+__global__ void __launch_bounds__(256) repack_kernel(const __grid_constant__ RepackJobs p) {
+  __shared__ __align__(16) uint16_t part[8][REPACK_COLS];
   after_the_kernel_in_front();
-  const long long total = rows * vecs;
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
-    const long long r = i / vecs;
-    const int c = (int)(i - r * vecs) * 8;
-    const uint16_t* s = src + r * src_stride + c;
-    uint32_t e[8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (long long g = blockIdx.x * 8ll + warp; g < p.end[p.n - 1]; g += gridDim.x * 8ll) {
+    int q = 0;
+    while (g >= p.end[q]) ++q;
+    const long long i = q ? g - p.end[q - 1] : g;
+    const int cols = (int)p.m[q].cols, vecs = (cols + 7) / 8, per_row = (vecs * 8 + REPACK_COLS - 1) / REPACK_COLS;
+    const long long r = i / per_row;
+    const int c0 = (int)(i - r * per_row) * REPACK_COLS;
+    const uint16_t* s = (const uint16_t*)p.m[q].p + r * p.m[q].stride + c0;
+    uint4* dst = (uint4*)p.to[q] + r * vecs + c0 / 8;
+    uint16_t e[REPACK_COLS / 32];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) e[j] = c + j < cols ? s[j] : 0;
-    dst[i] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+    for (int j = 0; j < REPACK_COLS / 32; ++j) e[j] = c0 + j * 32 + lane < cols ? s[j * 32 + lane] : (uint16_t)0;
+#pragma unroll
+    for (int j = 0; j < REPACK_COLS / 32; ++j) part[warp][j * 32 + lane] = e[j];
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < REPACK_COLS / 256; ++j) {
+      const int v = j * 32 + lane;
+      if (c0 / 8 + v < vecs) dst[v] = *reinterpret_cast<const uint4*>(&part[warp][v * 8]);
+    }
+    __syncwarp();
   }
 }
 
@@ -449,19 +470,24 @@ int launch_gemm_tc(const GemmDesc* d, int n, void* ws, size_t ws_bytes, int* sta
   if (int rc = make_context_current()) return rc;
   GtMaps maps{};
   GtParams p{};
+  RepackJobs repack{};
   for (int i = 0; i < pl.n_mat; ++i) {
     Stored o = pl.mat[i];
     if (pl.copied[i]) {
       void* to = (char*)ws + pl.copy[i];
-      const long long vecs = o.padded() / 8, blocks = ceil_div(o.rows * vecs, 256), most = 16ll * sm_count();
-      if (int rc = launch_after(repack_kernel, (unsigned)(blocks < most ? blocks : most), 256, 0, st, 1, (const uint16_t*)o.p, o.stride, o.rows, (int)o.cols, (uint4*)to,
-                                (int)vecs))
-        return rc;
+      repack.m[repack.n] = o;
+      repack.to[repack.n] = to;
+      repack.end[repack.n] = (repack.n ? repack.end[repack.n - 1] : 0) + o.rows * ceil_div(o.padded(), REPACK_COLS);
+      ++repack.n;
       o.p = to;
       o.stride = o.padded();
     }
     if (o.rows == 1) o.stride = o.padded();
     if (int rc = make_tmap_rows(&maps.m[i], o.p, d->dtype, o.cols, o.rows, o.stride, GT_BOX)) return rc;
+  }
+  if (repack.n) {
+    const long long blocks = ceil_div(repack.end[repack.n - 1], 8), most = 8ll * sm_count();
+    if (int rc = launch_after(repack_kernel, (unsigned)(blocks < most ? blocks : most), 256, 0, st, 1, repack)) return rc;
   }
   gt_outputs(pl, d, ws);
   p.bf16 = d->dtype == LIK_BF16;

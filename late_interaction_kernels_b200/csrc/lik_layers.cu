@@ -42,6 +42,7 @@ struct SlopeJob {
   int n, blocks;  // blocks of columns
   void* dz;       // or NULL: sums only
   long long dz_stride;
+  bool padded;    // what lies between n and the next 16 bytes belongs to the row
 };
 struct SlopeParams {
   SlopeJob job[SUM_OUTS];
@@ -129,7 +130,7 @@ int launch_slope(SlopeParams& p, int act, int dtype, bool sums, cudaStream_t st)
     if (i < p.n_jobs) {
       const SlopeJob& j = p.job[i];
       cols += j.n;
-      vec = vec && vec_ok(j.dy, j.dy_stride, j.n, item) && (act == LIK_ACT_NONE || (vec_ok(j.z, j.z_stride, j.n, item) && vec_ok(j.dz, j.dz_stride, j.n, item)));
+      vec = vec && vec_ok(j.dy, j.dy_stride, j.padded ? 0 : j.n, item) && (act == LIK_ACT_NONE || (vec_ok(j.z, j.z_stride, j.n, item) && vec_ok(j.dz, j.dz_stride, j.n, item)));
     }
     p.outs.end[i] = cols;
   }
@@ -442,7 +443,7 @@ extern "C" int lik_linear_bwd(const lik_linear_args* args, lik_stream_t stream) 
   if (a.workspace_bytes < l.total || (l.total && !a.workspace)) return too_small("lik_linear_bwd");
   if (act || a.dbias) {
     SlopeParams p{};
-    p.job[0] = {a.dy, a.z, a.dy_stride, a.z_stride, a.out, 0, l.dz, l.dz_stride};
+    p.job[0] = {a.dy, a.z, a.dy_stride, a.z_stride, a.out, 0, l.dz, l.dz_stride, false};
     p.n_jobs = 1;
     p.rows = a.rows;
     p.partial = l.partial;
@@ -501,14 +502,14 @@ extern "C" int lik_gated_bwd(const lik_gated_args* args, lik_stream_t stream) {
     if (int rc = launch_gemm(&l.dh, 1, l.gemm, l.gemm_bytes, a.status, st)) return rc;
   if (int rc = launch_gemm(l.grads, l.n_grads, l.gemm, l.gemm_bytes, a.status, st)) return rc;
   SlopeParams p{};
-  auto sum = [&](const void* g, long long stride, int n, void* out) {
+  auto sum = [&](const void* g, long long stride, int n, void* out, bool padded) {
     if (!out) return;
-    p.job[p.n_jobs] = {g, nullptr, stride, 0, n, 0, nullptr, 0};
+    p.job[p.n_jobs] = {g, nullptr, stride, 0, n, 0, nullptr, 0, padded};
     p.outs.out[p.n_jobs++] = out;
   };
-  sum(l.dg, l.stride, a.hidden, a.db_gate);
-  sum(l.du, l.stride, a.hidden, a.db_up);
-  sum(a.dy, a.dy_stride, a.out, a.db_down);
+  sum(l.dg, l.stride, a.hidden, a.db_gate, true);
+  sum(l.du, l.stride, a.hidden, a.db_up, true);
+  sum(a.dy, a.dy_stride, a.out, a.db_down, false);
   if (!p.n_jobs) return LIK_OK;
   p.rows = a.rows;
   p.partial = l.partial;

@@ -129,7 +129,7 @@ LIK_WITH_ACTIVATION(with_activation_dev, __device__)
 // ---------------------------------------------------------------------------------------------
 // Launches.  A pass is a chain of short kernels, so each is launched with programmatic stream serialisation: its blocks come to the SMs as those of
 // the kernel in front leave, set themselves up and wait for that kernel's end.  Every kernel here begins with after_the_kernel_in_front(),
-// before which it touches no device memory (a backward pass of 1000 x 768 x 768 in a graph: PDL_BEFORE us without, PDL_AFTER with).
+// before which it touches no device memory (a step of 1000 x 768 x 768 in a graph: 26.6 us without this, 23.0 with it).
 // ---------------------------------------------------------------------------------------------
 __device__ __forceinline__ void after_the_kernel_in_front() {
   asm volatile("griddepcontrol.wait;\n\tgriddepcontrol.launch_dependents;" ::: "memory");

@@ -55,6 +55,29 @@ __device__ __forceinline__ float2 row_sum(float a, float b, float2 (&buf)[2][32]
   }
 }
 
+// a vector of V elements as it came from memory
+template <typename T, int V>
+struct RawVec {
+  uint4 u;
+  __device__ __forceinline__ void load(const T* p) { u = __ldg(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void get(float (&f)[V]) const {
+    if constexpr (sizeof(T) == 4) {
+      f[0] = __uint_as_float(u.x), f[1] = __uint_as_float(u.y), f[2] = __uint_as_float(u.z), f[3] = __uint_as_float(u.w);
+    } else {
+      unpack2(u.x, f[0], f[1], T());
+      unpack2(u.y, f[2], f[3], T());
+      unpack2(u.z, f[4], f[5], T());
+      unpack2(u.w, f[6], f[7], T());
+    }
+  }
+};
+template <typename T>
+struct RawVec<T, 1> {
+  T e;
+  __device__ __forceinline__ void load(const T* p) { e = *p; }
+  __device__ __forceinline__ void get(float (&f)[1]) const { f[0] = to_f32(e); }
+};
+
 template <typename T, typename P, int V, int NV, int TPR>
 __global__ void __launch_bounds__(NORM_THREADS) norm_fwd_kernel(const NormParams p) {
   __shared__ float2 buf[2][32];
@@ -63,15 +86,27 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_fwd_kernel(const NormParams
   constexpr int PER_BLOCK = NORM_THREADS / TPR;
   const int lane = threadIdx.x % TPR;
   const float inv_n = 1.0f / (float)p.width;
-  for (long long r = (long long)blockIdx.x * PER_BLOCK + threadIdx.x / TPR; r < p.rows; r += (long long)gridDim.x * PER_BLOCK) {
+  RawVec<T, V> raw[NV];
+  auto fetch = [&](long long r) {  // the next row, while the present one is dealt with
+    if (r >= p.rows) return;
     const T* x = (const T*)p.x + r * p.x_stride;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + lane) * V;
+      if (c < p.width) raw[i].load(x + c);
+    }
+  };
+  const long long step = (long long)gridDim.x * PER_BLOCK;
+  long long r = (long long)blockIdx.x * PER_BLOCK + threadIdx.x / TPR;
+  fetch(r);
+  for (; r < p.rows; r += step) {
     float v[NV][V];
     float s = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * TPR + lane) * V;
       if (c < p.width) {
-        load_vec<T, V>(x + c, v[i]);
+        raw[i].get(v[i]);
       } else {
 #pragma unroll
         for (int j = 0; j < V; ++j) v[i][j] = 0.0f;
@@ -79,6 +114,7 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_fwd_kernel(const NormParams
 #pragma unroll
       for (int j = 0; j < V; ++j) s += v[i][j];
     }
+    fetch(r + step);
     const float mean = row_sum<TPR>(s, 0.0f, buf, turn).x * inv_n;
     float q = 0.0f;
 #pragma unroll
@@ -112,29 +148,6 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_fwd_kernel(const NormParams
     }
   }
 }
-
-// a vector of V elements as it came from memory
-template <typename T, int V>
-struct RawVec {
-  uint4 u;
-  __device__ __forceinline__ void load(const T* p) { u = __ldg(reinterpret_cast<const uint4*>(p)); }
-  __device__ __forceinline__ void get(float (&f)[V]) const {
-    if constexpr (sizeof(T) == 4) {
-      f[0] = __uint_as_float(u.x), f[1] = __uint_as_float(u.y), f[2] = __uint_as_float(u.z), f[3] = __uint_as_float(u.w);
-    } else {
-      unpack2(u.x, f[0], f[1], T());
-      unpack2(u.y, f[2], f[3], T());
-      unpack2(u.z, f[4], f[5], T());
-      unpack2(u.w, f[6], f[7], T());
-    }
-  }
-};
-template <typename T>
-struct RawVec<T, 1> {
-  T e;
-  __device__ __forceinline__ void load(const T* p) { e = *p; }
-  __device__ __forceinline__ void get(float (&f)[1]) const { f[0] = to_f32(e); }
-};
 
 // The next row is fetched while the present one is reduced and written; both stay as they came from memory, since two rows and the columns'
 // sums in fp32 would leave an SM one block.
