@@ -43,11 +43,20 @@ struct Raw16 {
       u[1] = make_uint4(w[4], w[5], w[6], w[7]);
     }
   }
+  // v += these: a multiply-add of 16-bit factors, one of them 1, takes them as they are
   __device__ __forceinline__ void add_to(float (&v)[16]) const {
-    float f[16];
-    get(f);
+    const uint32_t w[8] = {u[0].x, u[0].y, u[0].z, u[0].w, u[1].x, u[1].y, u[1].z, u[1].w};
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] += f[i];
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (std::is_same<T, __half>::value)
+        asm("{\n\t.reg .b16 l, h, one;\n\tmov.b32 {l, h}, %2;\n\tmov.b16 one, 0x3C00;\n\tfma.rn.f32.f16 %0, l, one, %0;\n\tfma.rn.f32.f16 %1, h, one, %1;\n\t}"
+            : "+f"(v[2 * i]), "+f"(v[2 * i + 1])
+            : "r"(w[i]));
+      else
+        asm("{\n\t.reg .b16 l, h, one;\n\tmov.b32 {l, h}, %2;\n\tmov.b16 one, 0x3F80;\n\tfma.rn.f32.bf16 %0, l, one, %0;\n\tfma.rn.f32.bf16 %1, h, one, %1;\n\t}"
+            : "+f"(v[2 * i]), "+f"(v[2 * i + 1])
+            : "r"(w[i]));
+    }
   }
   __device__ __forceinline__ void get(float (&f)[16]) const {
 #pragma unroll
@@ -83,6 +92,11 @@ __device__ __forceinline__ void slot_put(uint8_t* s, int lane, int h, const floa
   }
 }
 template <typename T>
+__device__ __forceinline__ void slot_get_raw(const uint8_t* s, int lane, int h, Raw16<T>& r) {
+#pragma unroll
+  for (int c = 0; c < 2; ++c) r.u[c] = *reinterpret_cast<const uint4*>(s + slot_offset<64>(lane, h * 2 + c));
+}
+template <typename T>
 __device__ __forceinline__ void slot_get(const uint8_t* s, int lane, int h, float (&f)[16]) {
   if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -92,8 +106,7 @@ __device__ __forceinline__ void slot_get(const uint8_t* s, int lane, int h, floa
     }
   } else {
     Raw16<T> r;
-#pragma unroll
-    for (int c = 0; c < 2; ++c) r.u[c] = *reinterpret_cast<const uint4*>(s + slot_offset<64>(lane, h * 2 + c));
+    slot_get_raw(s, lane, h, r);
     r.get(f);
   }
 }

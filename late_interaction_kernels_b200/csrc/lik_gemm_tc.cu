@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(GtWarps<KIND, !std::is_same<T, O>::value>::THR
               float f[16];
               slot_get<T>(to + j * SLOT, lane, h, f);
 #pragma unroll
-              for (int i = 0; i < 16; ++i) f[i] *= v[i];
+              for (int i = 0; i < 16; i += 2) mul2(Pair(f[i], f[i + 1]), Pair(v[i], v[i + 1])).get(f[i], f[i + 1]);
               slot_put<O>(to + j * SLOT, lane, h, f);
             }
           } else {
@@ -337,7 +337,10 @@ __global__ void __launch_bounds__(GtWarps<KIND, !std::is_same<T, O>::value>::THR
                 float f[16];
                 with_activation_dev(p.act, [&](auto act) {
 #pragma unroll
-                  for (int i = 0; i < 16; ++i) f[i] = w[i] * act_slope<decltype(act)::value, false>(v[i], v[i]);
+                  for (int i = 0; i < 16; i += 2) {
+                    act_pair<decltype(act)::value, true>(v[i], v[i + 1], f[i], f[i + 1]);
+                    mul2(Pair(w[i], w[i + 1]), Pair(f[i], f[i + 1])).get(f[i], f[i + 1]);
+                  }
                 });
                 slot_put<O>(to + SLOT, lane, h, f);
                 slot_put<O>(to + (OUT - 1) * SLOT, lane, h, v);
@@ -345,18 +348,17 @@ __global__ void __launch_bounds__(GtWarps<KIND, !std::is_same<T, O>::value>::THR
                 if (!DUAL && p.keep) slot_put<O>(to + (OUT - 1) * SLOT, lane, h, v);
                 with_activation_dev(p.act, [&](auto act) {
 #pragma unroll
-                  for (int i = 0; i < 16; ++i) v[i] = act_value<decltype(act)::value, false>(v[i]);
+                  for (int i = 0; i < 16; i += 2) act_pair<decltype(act)::value, false>(v[i], v[i + 1], v[i], v[i + 1]);
                 });
               }
             }
             if constexpr (DUAL) {
 #pragma unroll
-              for (int i = 0; i < 16; ++i) v[i] *= w[i];
+              for (int i = 0; i < 16; i += 2) mul2(Pair(v[i], v[i + 1]), Pair(w[i], w[i + 1])).get(v[i], v[i + 1]);
             } else if constexpr (RES) {
-              float f[16];
-              slot_get<T>(to, lane, h, f);
-#pragma unroll
-              for (int i = 0; i < 16; ++i) v[i] += f[i];
+              Raw16<T> r;
+              slot_get_raw(to, lane, h, r);
+              r.add_to(v);
             }
             slot_put<O>(to, lane, h, v);
           }

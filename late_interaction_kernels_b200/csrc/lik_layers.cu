@@ -72,8 +72,17 @@ __global__ void __launch_bounds__(32 * SLOPE_LANES, 4) slope_kernel(const __grid
       load_vec<T, V>((const T*)j.dy + r * j.dy_stride + c, g);
       if constexpr (ACT != LIK_ACT_NONE) {
         load_vec<T, V>((const T*)j.z + r * j.z_stride + c, z);
+        if constexpr (sizeof(T) == 4 || V == 1) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) g[i] *= act_slope<ACT, sizeof(T) == 4>(z[i], z[i]);
+          for (int i = 0; i < V; ++i) g[i] *= act_slope<ACT, sizeof(T) == 4>(z[i], z[i]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; i += 2) {
+            float sx, sy;
+            act_pair<ACT, true>(z[i], z[i + 1], sx, sy);
+            mul2(Pair(g[i], g[i + 1]), Pair(sx, sy)).get(g[i], g[i + 1]);
+          }
+        }
         store_vec<T, V>((T*)j.dz + r * j.dz_stride + c, g);
       }
 #pragma unroll

@@ -104,6 +104,82 @@ __device__ __forceinline__ float act_slope(float z, float& value) {
   return 1.0f;
 }
 
+// Two values at a time, for epilogues that are bound by the instructions they issue: additions, products and multiply-adds take one for both, with
+// the bits of the single ones.
+struct Pair {
+  unsigned long long u;
+  __device__ __forceinline__ Pair() {}
+  __device__ __forceinline__ Pair(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(u) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(u)); }
+};
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.u) : "l"(a.u), "l"(b.u));
+  return d;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.u) : "l"(a.u), "l"(b.u));
+  return d;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.u) : "l"(a.u), "l"(b.u), "l"(c.u));
+  return d;
+}
+__device__ __forceinline__ Pair both(float x) { return Pair(x, x); }
+__device__ __forceinline__ Pair exp2_2(Pair p) {
+  float a, b;
+  p.get(a, b);
+  return Pair(fast_exp2(a), fast_exp2(b));
+}
+__device__ __forceinline__ Pair rcp_2(Pair p) {
+  float a, b;
+  p.get(a, b);
+  return Pair(fast_rcp(a), fast_rcp(b));
+}
+__device__ __forceinline__ Pair sigmoid_2(Pair z) { return rcp_2(add2(exp2_2(mul2(z, both(-1.4426950408889634f))), both(1.0f))); }
+// the activation's value of both and, where SLOPE, its derivative (fast functions; see act_value and act_slope)
+template <int ACT, bool SLOPE>
+__device__ __forceinline__ void act_pair(float& x, float& y, float& sx, float& sy) {
+  const Pair z(x, y);
+  if constexpr (ACT == LIK_ACT_SILU || ACT == LIK_ACT_GELU_TANH) {
+    Pair s, q;
+    if constexpr (ACT == LIK_ACT_SILU) {
+      s = sigmoid_2(z);
+    } else {
+      q = mul2(mul2(z, z), both(0.044715f));
+      s = sigmoid_2(mul2(fma2(q, z, z), both(GELU_C)));
+    }
+    mul2(z, s).get(x, y);
+    if constexpr (SLOPE) {
+      const Pair w = ACT == LIK_ACT_SILU ? z : mul2(mul2(z, both(GELU_C)), fma2(q, both(3.0f), both(1.0f)));
+      mul2(s, fma2(w, fma2(s, both(-1.0f), both(1.0f)), both(1.0f))).get(sx, sy);
+    }
+  } else if constexpr (ACT == LIK_ACT_GELU) {
+    const Pair na(-fabsf(x), -fabsf(y)), t = rcp_2(fma2(na, both(-0.3f), both(1.0f))), e = exp2_2(mul2(mul2(z, z), both(-0.72134752f)));
+    Pair r = fma2(t, both(-0.0770966218f), both(0.216034401f));
+    r = fma2(r, t, both(-0.0169447843f));
+    r = fma2(r, t, both(0.144194491f));
+    r = fma2(r, t, both(0.113742429f));
+    r = fma2(r, t, both(0.120074183f));
+    const Pair tail = mul2(mul2(r, t), e);
+    if constexpr (SLOPE) {
+      float a, b, c, d;
+      tail.get(a, b);
+      fma2(tail, both(-1.0f), both(1.0f)).get(c, d);
+      fma2(mul2(z, both(0.3989422804014327f)), e, Pair(x < 0.0f ? a : c, y < 0.0f ? b : d)).get(sx, sy);
+    }
+    fma2(na, tail, Pair(fmaxf(x, 0.0f), fmaxf(y, 0.0f))).get(x, y);
+  } else if constexpr (SLOPE) {
+    sx = act_slope<ACT, false>(x, x);
+    sy = act_slope<ACT, false>(y, y);
+  } else {
+    x = act_value<ACT, false>(x);
+    y = act_value<ACT, false>(y);
+  }
+}
+
 // f(ActConst<activation>): the activation as a compile-time constant, on the host (which kernel) and on the device (which epilogue)
 template <int V>
 struct ActConst {
