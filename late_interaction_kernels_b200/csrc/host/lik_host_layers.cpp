@@ -113,19 +113,18 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
     if (t->defined() && t->requires_grad()) return true;
   return false;
 }
-// A leaf's gradient accumulator belongs to the stream on which the first live graph of that leaf was built.  A backward pass that is
-// being captured would wait for that stream, which is not part of the capture, and CUDA ends the capture in the engine's thread, where
-// the error ends the process; so the call says so before anything is recorded.
-void refuse_foreign_accumulators(const char* op, const at::Device& dev, std::initializer_list<const Tensor*> ts) {
+// A leaf's gradient accumulator belongs to the stream on which the first live graph of that leaf was built.  A backward pass that is being
+// captured waits for that stream and draws it into the capture, which the legacy default stream cannot be: CUDA ends the capture in the
+// engine's thread, where the error ends the process.  So the call says so before anything is recorded.
+void refuse_foreign_accumulators(const char* op, std::initializer_list<const Tensor*> ts) {
   if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
-  const c10::Stream now = c10::cuda::getCurrentCUDAStream(dev.index()).unwrap();
   for (const Tensor* t : ts) {
     if (!t->defined() || !t->requires_grad() || t->grad_fn()) continue;
     const auto acc = torch::autograd::impl::try_get_grad_accumulator(*t);
     const auto made = acc ? acc->stream() : std::nullopt;
-    if (made && *made != now)
-      throw std::runtime_error(std::string(op) + ": a graph of the same leaf tensors, built on another stream, is still alive; drop it (the loss or output that holds it) "
-                               "before this call is captured into a CUDA graph, or capture on the stream it was built on.");
+    if (made && c10::cuda::CUDAStream(*made).stream() == nullptr)
+      throw std::runtime_error(std::string(op) + ": a graph of the same leaf tensors, built on the default stream, is still alive; drop it (the loss or output that holds it) "
+                               "before this call is captured into a CUDA graph.");
   }
 }
 // gradients of gradients do not exist: whoever differentiates the returned gradients is told so
@@ -218,14 +217,14 @@ Tensor layer_norm(const Tensor& x_, const OptTensor& weight_, const OptTensor& b
   const Tensor w = opt(weight_), b = opt(bias_);
   require_layer_inputs("layer_norm", x_, {{"weight", &w}, {"bias", &b}});
   const int64_t width = x_.size(-1);
-  if (width < 1 || width >= (int64_t(1) << 31)) value_error("x must have at least one feature; got " + shape(x_.sizes()));
+  if (width < 1 || width >= (int64_t(1) << 30)) value_error("x must have at least one feature, and less than 2^30; got " + shape(x_.sizes()));
   require_vector("weight", w, width);
   require_vector("bias", b, width);
   if (!(eps >= 0) || eps > 3e38) value_error("eps must be a number that is not negative; got " + std::to_string(eps));
   const Tensor x = rows_of(x_);
   const c10::cuda::CUDAGuard guard(x.device());
   const bool grad = wants_grad({&x, &w, &b});
-  if (grad) refuse_foreign_accumulators("layer_norm", x.device(), {&x_, &w, &b});
+  if (grad) refuse_foreign_accumulators("layer_norm", {&x_, &w, &b});
   Tensor y, stats;
   {
     at::AutoDispatchBelowADInplaceOrView below;
@@ -341,7 +340,7 @@ Tensor linear(const Tensor& x_, const Tensor& w, const OptTensor& bias_, const s
   const Tensor r = r_.defined() ? rows_of(r_.scalar_type() == dt ? r_ : r_.to(dt)) : r_;
   const c10::cuda::CUDAGuard guard(x.device());
   const bool grad = wants_grad({&x, &w, &b, &r});
-  if (grad) refuse_foreign_accumulators("linear", x.device(), {&x_, &w, &b, &r_});
+  if (grad) refuse_foreign_accumulators("linear", {&x_, &w, &b, &r_});
   Tensor y, z, pw;
   {
     at::AutoDispatchBelowADInplaceOrView below;
@@ -489,7 +488,7 @@ Tensor gated_feed_forward(const Tensor& x_, const Tensor& wg, const Tensor& wu, 
   const Tensor r = r_.defined() ? rows_of(r_.scalar_type() == dt ? r_ : r_.to(dt)) : r_;
   const c10::cuda::CUDAGuard guard(x.device());
   const bool grad = wants_grad({&x, &wg, &wu, &wd, &bg, &bu, &bd, &r});
-  if (grad) refuse_foreign_accumulators("gated_feed_forward", x.device(), {&x_, &wg, &wu, &wd, &bg, &bu, &bd, &r_});
+  if (grad) refuse_foreign_accumulators("gated_feed_forward", {&x_, &wg, &wu, &wd, &bg, &bu, &bd, &r_});
   Tensor y, kept, pg, pu, pd;
   {
     at::AutoDispatchBelowADInplaceOrView below;

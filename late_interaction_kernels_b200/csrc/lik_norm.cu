@@ -423,7 +423,7 @@ int check_norm(const lik_norm_args* a) {
   LIK_REQUIRE(a != nullptr, "args is NULL");
   LIK_REQUIRE(a->dtype == LIK_F32 || a->dtype == LIK_F16 || a->dtype == LIK_BF16, "dtype must be fp32, fp16 or bf16");
   LIK_REQUIRE(a->param_dtype == a->dtype || a->param_dtype == LIK_F32, "param_dtype must be dtype or fp32");
-  LIK_REQUIRE(a->rows >= 0 && a->width > 0 && a->x_stride >= a->width, "sizes must be positive, x_stride at least width");
+  LIK_REQUIRE(a->rows >= 0 && a->width > 0 && a->width < (1 << 30) && a->x_stride >= a->width, "sizes must be positive, width below 2^30, x_stride at least width");
   LIK_REQUIRE(a->eps >= 0.0f, "eps must not be negative");
   return LIK_OK;
 }

@@ -235,7 +235,8 @@ def linear_case(m, k, n, dt, act, bias, residual, wdt=None):
 
 SHAPES = [(1, 1, 1), (1, 7, 3), (2, 64, 5), (5, 16, 16), (8, 768, 768), (9, 768, 130), (16, 512, 1024), (17, 512, 1000), (32, 768, 128), (33, 100, 65), (64, 72, 264),
           (128, 128, 128), (129, 255, 257), (255, 264, 248), (300, 768, 520), (700, 1001, 333), (2050, 192, 72), (4096, 64, 64), (20000, 40, 24), (1000, 2048, 136),
-          (2500, 520, 392), (4100, 260, 1030), (30000, 96, 200)]
+          (2500, 520, 392), (4100, 260, 1030), (30000, 96, 200), (40, 1, 1), (300, 1, 5), (5, 300, 1),
+          (300, 4000, 260), (128, 2900, 70), (3000, 2700, 300), (700, 640, 1600)]
 
 
 @pytest.mark.parametrize("dt", [BF16, FP16, FP32])
@@ -380,7 +381,7 @@ def gated_case(m, k, f, o, dt, act, bias, residual, wdt=None):
 
 GATED = [(1, 1, 1, 1), (1, 16, 40, 8), (3, 5, 7, 9), (8, 768, 512, 768), (16, 64, 2048, 64), (17, 384, 1100, 384), (40, 128, 96, 136), (128, 256, 128, 256), (130, 264, 200, 72),
          (257, 65, 129, 33), (600, 768, 512, 768), (2050, 128, 320, 128), (9000, 64, 40, 64),
-         (1500, 300, 700, 260), (3001, 257, 515, 129)]
+         (1500, 300, 700, 260), (3001, 257, 515, 129), (50, 1, 3, 2), (260, 2600, 300, 40), (400, 40, 2800, 136), (5200, 136, 264, 392)]
 
 
 @pytest.mark.parametrize("dt", [BF16, FP16, FP32])
@@ -498,6 +499,73 @@ def test_gradients_are_deterministic_and_only_where_asked(dt):
         assert torch.equal(only, a[i])
     for c in leaves:
         c.requires_grad_(True)
+
+
+def test_steps_on_two_streams_side_by_side():
+    p = head_params(256, 512, BF16)
+    data = [(rand(700, 256, dt=BF16).requires_grad_(), rand(700, 256, dt=BF16)) for _ in range(2)]
+
+    def step(x, d):
+        y = head(x, p)
+        return [y.detach(), *torch.autograd.grad(y, [x, *p.values()], d)]
+
+    want = [step(*d) for d in data]
+    streams = [torch.cuda.Stream() for _ in data]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(step(*data[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for g in got[i]:
+            for a, b in zip(g, want[i]):
+                assert torch.equal(a, b)
+
+
+def test_a_backward_pass_may_run_twice():
+    p = head_params(96, 160, FP32)
+    x, d = rand(333, 96, dt=FP32).requires_grad_(), rand(333, 96, dt=FP32)
+    y = head(x, p)
+    leaves = [x, *p.values()]
+    a = torch.autograd.grad(y, leaves, d, retain_graph=True)
+    b = torch.autograd.grad(y, leaves, d)
+    for s, t in zip(a, b):
+        assert torch.equal(s, t)
+    with pytest.raises(RuntimeError):  # what it kept is gone
+        torch.autograd.grad(y, leaves, d)
+
+
+def test_offsets_beyond_32_bits():
+    """Results of more than 2^31 elements: the last rows are those of a call of their own."""
+    from late_interaction_kernels_b200.token_layers import gated_feed_forward, layer_norm, linear
+
+    if torch.cuda.mem_get_info()[0] < 40e9:
+        pytest.skip("needs 40 GB")
+    m = 530000
+    with torch.no_grad():
+        x, w, b = rand(m, 16, dt=BF16), rand(4096, 16, dt=BF16), rand(4096, dt=BF16)
+        y = linear(x, w, b, activation="silu")
+        assert y.numel() > 2**31
+        tail = linear(x[-5000:], w, b, activation="silu")
+        assert torch.equal(y[-5000:], tail)
+        n = layer_norm(y)
+        assert torch.equal(n[-5000:], layer_norm(tail))
+        del n
+        back = linear(y, rand(24, 4096, dt=BF16).fill_(2**-6))
+        near(back[-64:], *(lambda v, e: (v, e))(*product(tail[-64:].double(), torch.full((24, 4096), 2.0**-6, dtype=torch.float64, device="cuda"))), "back")
+        del y, back
+    x.requires_grad_()
+    wg = rand(4096, 16, dt=BF16)
+    y = gated_feed_forward(x, wg, w, w.t())
+    (dx,) = torch.autograd.grad(y, [x], torch.ones_like(y))
+    few = x.detach()[-5000:].clone().requires_grad_()
+    z = gated_feed_forward(few, wg, w, w.t())
+    # (5000 rows have their sums over 4096 cut into shares: fp32 sums in another order, each element rounded once, so at most a step of 2 u apart)
+    for a, b in ((y[-5000:], z), (dx[-5000:], torch.autograd.grad(z, [few], torch.ones_like(z))[0])):
+        assert float((a.double() - b.double()).norm() / b.double().norm()) < 2 * unit(BF16)
 
 
 def test_a_step_in_a_cuda_graph_and_on_another_stream():

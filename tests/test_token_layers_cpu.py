@@ -58,3 +58,34 @@ def test_c_entries_refuse_before_any_launch(layers):
     assert lib.lik_linear_bwd(C.byref(a), None) == -1 and b"param_dtype" in lib.lik_last_error()
     n = _lib.NormArgs(dtype=2, param_dtype=0, x_stride=8, rows=4, width=8, eps=-1.0)
     assert lib.lik_layer_norm_fwd(C.byref(n), None) == -1 and b"eps" in lib.lik_last_error()
+
+
+def test_workspace_queries_need_no_gpu(layers):
+    """A serving runtime plans its memory ahead: sizes come from the arguments alone, and a larger call needs no less."""
+    from late_interaction_kernels_b200 import _lib
+
+    lib = _lib.load()
+
+    def linear(rows, dtype, odd=0):
+        a = _lib.LinearArgs(x=4096, w=4096, dy=4096, dx=4096, dw=4096, dbias=4096, z=4096, x_stride=768 + odd, w_stride=768 + odd, dy_stride=512, z_stride=512,
+                            rows=rows, out=512, dtype=dtype, param_dtype=dtype, activation=3)
+        setattr(a, "in", 768)
+        return lib.lik_linear_fwd_workspace(C.byref(a)), lib.lik_linear_bwd_workspace(C.byref(a))
+
+    def gated(rows, dtype):
+        a = _lib.GatedArgs(x=4096, w_gate=4096, w_up=8192, w_down=16384, dy=4096, dx=4096, dw_gate=4096, dw_up=4096, dw_down=4096, db_gate=4096, db_up=4096, db_down=4096,
+                           x_stride=768, w_gate_stride=768, w_up_stride=768, w_down_stride=1100, dy_stride=768, kept_stride=1104, rows=rows, hidden=1100, out=768,
+                           dtype=dtype, param_dtype=dtype, activation=2)
+        setattr(a, "in", 768)
+        return lib.lik_gated_fwd_workspace(C.byref(a)), lib.lik_gated_bwd_workspace(C.byref(a))
+
+    for fn in (linear, gated):
+        for dtype in (_lib.LIK_BF16, _lib.LIK_F16, _lib.LIK_F32):
+            assert fn(0, dtype) == (0, 0)
+            sizes = [fn(rows, dtype) for rows in (1, 100, 100_000, 2_000_000_000)]
+            for small, large in zip(sizes, sizes[2:]):
+                assert small[0] <= large[0] and small[1] < large[1]
+    # rows that TMA cannot address ask for room for a copy
+    assert linear(5000, _lib.LIK_BF16, odd=1)[0] >= 5000 * 768 * 2 > linear(5000, _lib.LIK_BF16)[0]
+    a = _lib.NormArgs(dtype=2, param_dtype=2, x_stride=768, rows=10**9, width=768, dweight=4096, eps=1e-5)
+    assert 0 < lib.lik_layer_norm_bwd_workspace(C.byref(a)) < 16 << 20
