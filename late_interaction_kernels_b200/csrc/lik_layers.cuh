@@ -139,6 +139,67 @@ __device__ __forceinline__ Pair rcp_2(Pair p) {
   return Pair(fast_rcp(a), fast_rcp(b));
 }
 __device__ __forceinline__ Pair sigmoid_2(Pair z) { return rcp_2(add2(exp2_2(mul2(z, both(-1.4426950408889634f))), both(1.0f))); }
+// the same on vectors of V elements (one by one where V is 1): v = v * a + b, v = v * a, v = v + a, s += v, s += v * a
+template <int V>
+__device__ __forceinline__ void vec_fma(float (&v)[V], const float (&a)[V], const float (&b)[V]) {
+  if constexpr (V == 1) v[0] = fmaf(v[0], a[0], b[0]);
+  else
+#pragma unroll
+    for (int i = 0; i < V; i += 2) fma2(Pair(v[i], v[i + 1]), Pair(a[i], a[i + 1]), Pair(b[i], b[i + 1])).get(v[i], v[i + 1]);
+}
+template <int V>
+__device__ __forceinline__ void vec_fma(float (&v)[V], float a, float b) {
+  if constexpr (V == 1) v[0] = fmaf(v[0], a, b);
+  else
+#pragma unroll
+    for (int i = 0; i < V; i += 2) fma2(Pair(v[i], v[i + 1]), both(a), both(b)).get(v[i], v[i + 1]);
+}
+template <int V>
+__device__ __forceinline__ void vec_mul(float (&v)[V], const float (&a)[V]) {
+  if constexpr (V == 1) v[0] *= a[0];
+  else
+#pragma unroll
+    for (int i = 0; i < V; i += 2) mul2(Pair(v[i], v[i + 1]), Pair(a[i], a[i + 1])).get(v[i], v[i + 1]);
+}
+template <int V>
+__device__ __forceinline__ void vec_mul(float (&v)[V], float a) {
+  if constexpr (V == 1) v[0] *= a;
+  else
+#pragma unroll
+    for (int i = 0; i < V; i += 2) mul2(Pair(v[i], v[i + 1]), both(a)).get(v[i], v[i + 1]);
+}
+template <int V>
+__device__ __forceinline__ void vec_add(float (&v)[V], const float (&a)[V]) {
+  if constexpr (V == 1) v[0] += a[0];
+  else
+#pragma unroll
+    for (int i = 0; i < V; i += 2) add2(Pair(v[i], v[i + 1]), Pair(a[i], a[i + 1])).get(v[i], v[i + 1]);
+}
+template <int V>
+__device__ __forceinline__ void vec_add(float (&v)[V], float a) {
+  if constexpr (V == 1) v[0] += a;
+  else
+#pragma unroll
+    for (int i = 0; i < V; i += 2) add2(Pair(v[i], v[i + 1]), both(a)).get(v[i], v[i + 1]);
+}
+struct PairSum {  // sums of the even and of the odd elements
+  float a = 0.0f, b = 0.0f;
+  template <int V>
+  __device__ __forceinline__ void add(const float (&v)[V]) {
+    if constexpr (V == 1) a += v[0];
+    else
+#pragma unroll
+      for (int i = 0; i < V; i += 2) add2(Pair(a, b), Pair(v[i], v[i + 1])).get(a, b);
+  }
+  template <int V>
+  __device__ __forceinline__ void dot(const float (&v)[V], const float (&w)[V]) {
+    if constexpr (V == 1) a = fmaf(v[0], w[0], a);
+    else
+#pragma unroll
+      for (int i = 0; i < V; i += 2) fma2(Pair(v[i], v[i + 1]), Pair(w[i], w[i + 1]), Pair(a, b)).get(a, b);
+  }
+  __device__ __forceinline__ float sum() const { return a + b; }
+};
 // the activation's value of both and, where SLOPE, its derivative (fast functions; see act_value and act_slope)
 template <int ACT, bool SLOPE>
 __device__ __forceinline__ void act_pair(float& x, float& y, float& sx, float& sy) {

@@ -5,7 +5,9 @@
 //
 // Everything is bound by memory: a row is read once into registers (a warp's or a block's), and all that is done to it
 // happens there, the variance as a second pass over the registers.  The backward keeps its columns' sums for dw and db in
-// registers from row to row; each block writes them once and a small kernel adds the blocks' sums in their order.
+// registers from row to row; each block writes them once and a small kernel adds the blocks' sums in their order.  With 768 features
+// of 16 bits instruction issue was the bound (82 and 72 %) until two values went through an instruction: 65536 rows forward 34 us = 5.9 TB/s,
+// backward 52 us = 5.8 TB/s, 0.9 of what a copy reaches.
 #include "lik_layers.cuh"
 
 namespace lik {
@@ -101,32 +103,22 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_fwd_kernel(const NormParams
   fetch(r);
   for (; r < p.rows; r += step) {
     float v[NV][V];
-    float s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * TPR + lane) * V;
-      if (c < p.width) {
-        raw[i].get(v[i]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[i][j] = 0.0f;
-      }
-#pragma unroll
-      for (int j = 0; j < V; ++j) s += v[i][j];
-    }
-    fetch(r + step);
-    const float mean = row_sum<TPR>(s, 0.0f, buf, turn).x * inv_n;
-    float q = 0.0f;
+    PairSum s, q;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if ((i * TPR + lane) * V < p.width) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          v[i][j] -= mean;
-          q = fmaf(v[i][j], v[i][j], q);
-        }
+        raw[i].get(v[i]);
+        s.add(v[i]);
       }
-    const float rstd = 1.0f / sqrtf(row_sum<TPR>(q, 0.0f, buf, turn).x * inv_n + p.eps);
+    fetch(r + step);
+    const float mean = row_sum<TPR>(s.sum(), 0.0f, buf, turn).x * inv_n;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if ((i * TPR + lane) * V < p.width) {
+        vec_add(v[i], -mean);
+        q.dot(v[i], v[i]);
+      }
+    const float rstd = 1.0f / sqrtf(row_sum<TPR>(q.sum(), 0.0f, buf, turn).x * inv_n + p.eps);
     if (lane == 0 && p.mean) {
       p.mean[r] = mean;
       p.rstd[r] = rstd;
@@ -137,26 +129,36 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_fwd_kernel(const NormParams
       const int c = (i * TPR + lane) * V;
       if (c < p.width) {
         float w[V], b[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) w[j] = 1.0f, b[j] = 0.0f;
-        if (p.w) load_vec<P, V>((const P*)p.w + c, w);
-        if (p.b) load_vec<P, V>((const P*)p.b + c, b);
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[i][j] = fmaf(v[i][j] * rstd, w[j], b[j]);
+        vec_mul(v[i], rstd);
+        if (p.w) {
+          load_vec<P, V>((const P*)p.w + c, w);
+          if (p.b) {
+            load_vec<P, V>((const P*)p.b + c, b);
+            vec_fma(v[i], w, b);
+          } else {
+            vec_mul(v[i], w);
+          }
+        } else if (p.b) {
+          load_vec<P, V>((const P*)p.b + c, b);
+          vec_add(v[i], b);
+        }
         store_vec<T, V>(y + c, v[i]);
       }
     }
   }
 }
 
+// (blocks of four warps where a warp has its row to itself: three of them, at up to 168 registers a thread, where eight warps at a time would leave
+// an SM one block or spill)
+__host__ __device__ constexpr int norm_bwd_threads(int tpr) { return tpr == 32 ? 128 : NORM_THREADS; }
 // The next row is fetched while the present one is reduced and written; both stay as they came from memory, since two rows and the columns'
 // sums in fp32 would leave an SM one block.
 template <typename T, typename P, int V, int NV, int TPR, bool PARAMS>
-__global__ void __launch_bounds__(NORM_THREADS, NV * V <= 24 ? 2 : 1) norm_bwd_kernel(const NormParams p) {
+__global__ void __launch_bounds__(norm_bwd_threads(TPR), TPR == 32 ? 3 : (NV * V <= 24 ? 2 : 1)) norm_bwd_kernel(const NormParams p) {
   __shared__ float2 buf[2][32];
   after_the_kernel_in_front();
   int turn = 0;
-  constexpr int PER_BLOCK = NORM_THREADS / TPR;
+  constexpr int THREADS = norm_bwd_threads(TPR), PER_BLOCK = THREADS / TPR;
   const int lane = threadIdx.x % TPR;
   const float inv_n = 1.0f / (float)p.width;
   float dw[PARAMS ? NV : 1][V], db[PARAMS ? NV : 1][V];
@@ -190,46 +192,53 @@ __global__ void __launch_bounds__(NORM_THREADS, NV * V <= 24 ? 2 : 1) norm_bwd_k
 #pragma unroll
     for (int i = 0; i < NV; ++i) x[i] = rx[i], y[i] = rg[i];
     fetch(r + step);
-    float sg = 0.0f, sgh = 0.0f;
+    PairSum sg, sgh;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * TPR + lane) * V;
       if (c < p.width) {
         float w[V], h[V], g[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) w[j] = 1.0f;
-        if (p.w) load_vec<P, V>((const P*)p.w + c, w);
         x[i].get(h);
         y[i].get(g);
+        vec_add(h, -m);
+        vec_mul(h, s);
+        if constexpr (PARAMS) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          h[j] = (h[j] - m) * s;
-          if (PARAMS) {
-            dw[i][j] = fmaf(g[j], h[j], dw[i][j]);
-            db[i][j] += g[j];
+          for (int j = 0; j < V; j += V == 1 ? 1 : 2) {
+            if constexpr (V == 1) dw[i][0] = fmaf(g[0], h[0], dw[i][0]);
+            else fma2(Pair(g[j], g[j + 1]), Pair(h[j], h[j + 1]), Pair(dw[i][j], dw[i][j + 1])).get(dw[i][j], dw[i][j + 1]);
           }
-          g[j] *= w[j];
-          sg += g[j];
-          sgh = fmaf(g[j], h[j], sgh);
+          vec_add(db[i], g);
         }
+        if (p.w) {
+          load_vec<P, V>((const P*)p.w + c, w);
+          vec_mul(g, w);
+        }
+        sg.add(g);
+        sgh.dot(g, h);
       }
     }
     if (p.dx) {
-      const float2 sums = row_sum<TPR>(sg, sgh, buf, turn);
-      const float c1 = sums.x * inv_n, c2 = sums.y * inv_n;
+      const float2 sums = row_sum<TPR>(sg.sum(), sgh.sum(), buf, turn);
+      // rstd (g - c1 - h c2), h = (x - mean) rstd
+      const float c1 = -sums.x * inv_n, c2 = -sums.y * inv_n * s;
       T* dx = (T*)p.dx + r * p.width;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int c = (i * TPR + lane) * V;
         if (c < p.width) {
           float w[V], h[V], g[V];
-#pragma unroll
-          for (int j = 0; j < V; ++j) w[j] = 1.0f;
-          if (p.w) load_vec<P, V>((const P*)p.w + c, w);
           x[i].get(h);
           y[i].get(g);
-#pragma unroll
-          for (int j = 0; j < V; ++j) g[j] = s * (g[j] * w[j] - c1 - (h[j] - m) * s * c2);
+          vec_add(h, -m);
+          vec_fma(h, c2, c1);
+          if (p.w) {
+            load_vec<P, V>((const P*)p.w + c, w);
+            vec_fma(g, w, h);
+          } else {
+            vec_add(g, h);
+          }
+          vec_mul(g, s);
           store_vec<T, V>(dx + c, g);
         }
       }
@@ -262,7 +271,7 @@ __global__ void __launch_bounds__(NORM_THREADS, NV * V <= 24 ? 2 : 1) norm_bwd_k
         }
         __syncthreads();
       }
-      for (int c = threadIdx.x; c < COLS; c += NORM_THREADS) {
+      for (int c = threadIdx.x; c < COLS; c += THREADS) {
         // (i, lane, j) of a column
         const int i = c / (TPR * V), l = c / V % TPR, j = c % V, at = (i * V + j) * TPR + l;
         if (c < p.width) out[c] = acc[at], out[p.width + c] = acc[COLS + at];
@@ -337,9 +346,9 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_dparam_wide_kernel(const No
 constexpr int NORM_WIDE_PARTS = 64;
 
 // Which kernel a width goes to: a warp per row, four warps or the block's eight; vectors of 16 bytes where rows and parameters are aligned, else
-// single elements.  The forward keeps a row with a warp up to four vectors per lane.  The backward, which holds a row twice and its columns'
-// sums, keeps a warp per row up to three, at 128 registers: 65536 x 768 bf16 65 us, 102 with four warps per row, of which the fourth has
-// nothing; with four vectors a lane would need 176 (16384 x 1024: 36 us, 31 with four warps per row).
+// single elements (9001 x 1023 fp32, forward and backward: 22 and 23 us by a block per row, 34 and 58 by a warp with 32 elements per lane).  The
+// forward keeps a row with a warp up to four vectors per lane, the backward, which holds a row twice and its columns' sums, up to three:
+// 65536 x 768 bf16 52 us, 102 with four warps per row, of which the fourth has nothing; 16384 x 1024 36 us with a warp per row, 24 with four.
 struct NormPlan {
   bool wide, vec;
   int nv, tpr;
@@ -365,7 +374,7 @@ NormPlan norm_plan(const lik_norm_args& a, bool bwd) {
 }
 int norm_bwd_blocks(const lik_norm_args& a, const NormPlan& pl) {
   if (pl.wide) return (int)(a.rows < NORM_WIDE_PARTS ? (a.rows ? a.rows : 1) : NORM_WIDE_PARTS);
-  const long long need = ceil_div(a.rows, NORM_THREADS / pl.tpr), most = (pl.tpr == 256 && pl.nv <= (pl.vec ? 1 : 4) ? 3ll : 2ll) * sm_count();  // (what an SM holds)
+  const long long need = ceil_div(a.rows, norm_bwd_threads(pl.tpr) / pl.tpr), most = (pl.tpr == 32 || (pl.tpr == 256 && pl.nv <= (pl.vec ? 1 : 4)) ? 3ll : 2ll) * sm_count();  // (what an SM holds)
   return (int)(need < most ? (need ? need : 1) : most);
 }
 
@@ -375,8 +384,8 @@ int run_norm(const NormParams& p, bool bwd, bool params, int blocks, cudaStream_
     if constexpr (TPR != 128) return launch_after(norm_fwd_kernel<T, P, V, NV, TPR>, blocks, NORM_THREADS, 0, st, 1, p);
   } else if constexpr (V == 1 || TPR != 32 || NV <= 3) {
     const size_t smem = TPR < NORM_THREADS ? sizeof(float) * 2 * NV * TPR * V : 0;
-    return params ? launch_after(norm_bwd_kernel<T, P, V, NV, TPR, true>, blocks, NORM_THREADS, smem, st, 1, p)
-                  : launch_after(norm_bwd_kernel<T, P, V, NV, TPR, false>, blocks, NORM_THREADS, 0, st, 1, p);
+    return params ? launch_after(norm_bwd_kernel<T, P, V, NV, TPR, true>, blocks, norm_bwd_threads(TPR), smem, st, 1, p)
+                  : launch_after(norm_bwd_kernel<T, P, V, NV, TPR, false>, blocks, norm_bwd_threads(TPR), 0, st, 1, p);
   }
   return LIK_ERR_UNSUPPORTED;  // (a shape that the plan does not give)
 }
