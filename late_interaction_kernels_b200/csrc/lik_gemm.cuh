@@ -254,7 +254,16 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Sum
       const float f[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        if (c + k < j.n) gemm_element<T, T, GEMM_LINEAR, decltype(act)::value>(d, r, c + k, f[k], 0.0f);
+        if (c + k < j.n) {
+          bool above = true;
+          if constexpr (decltype(act)::value == LIK_ACT_RELU) {
+            const float z = d.bias[0] ? f[k] + to_f32(((const T*)d.bias[0])[c + k]) : f[k];
+            above = z > 0.0f;
+            if (sizeof(T) == 2 && d.kept[0] && fabsf(z) < kink_bound(fmaxf(fmaxf(fabsf(f[0]), fabsf(f[1])), fmaxf(fabsf(f[2]), fabsf(f[3]))), d.k[0]))
+              above = above_zero<T>(d, r, c + k);
+          }
+          gemm_element<T, T, GEMM_LINEAR, decltype(act)::value>(d, r, c + k, f[k], 0.0f, above);
+        }
     }
   });
 }

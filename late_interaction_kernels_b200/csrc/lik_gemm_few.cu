@@ -98,14 +98,22 @@ __global__ void __launch_bounds__(32 * WARPS) few_mma_kernel(const __grid_consta
     // neighbouring threads: neighbouring rows of b, which are neighbours in the result
     for (int e = threadIdx.x; e < NT * 128; e += 32 * WARPS) {
       const int r = e % 16, in = e / 16, i = in / 8, col = in % 8, m = m0 + in;
-      if (m < d.m && n0 + r < d.n) {
-        float v[2] = {0.0f, 0.0f};
+      const bool there = m < d.m && n0 + r < d.n;
+      float v[2] = {0.0f, 0.0f};
 #pragma unroll
-        for (int q = 0; q < DUAL; ++q)
+      for (int q = 0; q < DUAL; ++q)
 #pragma unroll
-          for (int s = 0; s < WARPS; ++s) v[q] += part[s][q][i][(r % 8) * 4 + col / 2][(r / 8) * 2 + col % 2];
-        gemm_element<T, T, KIND, decltype(act)::value>(d, m, n0 + r, v[0], v[1]);
+        for (int s = 0; s < WARPS; ++s) v[q] += part[s][q][i][(r % 8) * 4 + col / 2][(r / 8) * 2 + col % 2];
+      bool above = true;
+      if constexpr (decltype(act)::value == LIK_ACT_RELU) {  // (whole warps come here)
+        const float z = there && d.bias[0] ? v[0] + to_f32(((const T*)d.bias[0])[n0 + r]) : v[0];
+        float largest = fabsf(z);
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+        above = z > 0.0f;
+        if (there && d.kept[0] && fabsf(z) < kink_bound(largest, d.k[0])) above = above_zero<T>(d, m, n0 + r);
       }
+      if (there) gemm_element<T, T, KIND, decltype(act)::value>(d, m, n0 + r, v[0], v[1], above);
     }
   });
 }
@@ -171,7 +179,11 @@ __global__ void __launch_bounds__(FEW_THREADS) few_fma_kernel(const __grid_const
       for (int q = 0; q < DUAL; ++q)
 #pragma unroll
         for (int w = 0; w < FEW_WARPS; ++w) v[q] += part[q][w][at];
-      with_activation_dev(d.act, [&](auto act) { gemm_element<T, T, KIND, decltype(act)::value>(d, m, n0 + r, v[0], v[1]); });
+      with_activation_dev(d.act, [&](auto act) {
+        // (sums of fp32 multiply-adds, rounded: relu's argument has the sign that they have)
+        const float z = d.bias[0] ? v[0] + to_f32(((const T*)d.bias[0])[n0 + r]) : v[0];
+        gemm_element<T, T, KIND, decltype(act)::value>(d, m, n0 + r, v[0], v[1], z > 0.0f);
+      });
     }
   }
 }

@@ -41,6 +41,8 @@ struct GtParams {
   void *out2, *kept[2];  // kept: written, or read by GEMM_GATED_BWD
   long long residual_stride, kept_stride;
   bool bias_vec, residual_vec, keep;  // *_vec: rows of whole 16-byte pieces
+  const void *a, *b;                  // the operands of z as the caller has them, k contiguous
+  long long a_stride, b_stride, k;
   int* status;
 };
 struct GtCtl {
@@ -120,8 +122,35 @@ __device__ __forceinline__ bool gt_chunk(const GtParams& p, int u, int c, int ra
   return row0 < p.q[0].m && col < p.q[0].n;
 }
 
-// RES: with a residual (GEMM_LINEAR).  O fp32: plain products, several of them, in fp32 or T, or shares of one.
-template <int CG, int KIND, bool RES, typename T, typename O>
+// Which of 16 z, columns of the lane's row, are above 0 (bit i: column col + i): those near relu's kink are taken by the warp's lanes together.
+template <typename T>
+__device__ __forceinline__ uint32_t above_kink(const GtParams& p, int row0, int col, int lane, const float (&v)[16]) {
+  float largest = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) largest = fmaxf(largest, fabsf(v[i]));
+  const float bound = kink_bound(largest, p.k);
+  uint32_t above = 0, unsure = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    above |= (v[i] > 0.0f ? 1u : 0u) << i;
+    unsure |= (fabsf(v[i]) < bound && row0 + lane < p.q[0].m && col + i < p.q[0].n ? 1u : 0u) << i;
+  }
+  for (uint32_t lanes = __ballot_sync(0xffffffffu, unsure != 0); lanes; lanes &= lanes - 1) {
+    const int l = __ffs(lanes) - 1;
+    for (uint32_t cols = __shfl_sync(0xffffffffu, unsure, l); cols; cols &= cols - 1) {
+      const int c = __ffs(cols) - 1;
+      double z = exact_part((const T*)p.a + (row0 + l) * p.a_stride, (const T*)p.b + (col + c) * p.b_stride, p.k, lane, 32);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+      if (p.bias[0]) z += (double)to_f32(((const T*)p.bias[0])[col + c]);
+      if (lane == l) above = z > 0.0 ? above | 1u << c : above & ~(1u << c);
+    }
+  }
+  return above;
+}
+
+// RES: with a residual (GEMM_LINEAR).  KINK: relu, for a backward pass.  O fp32: plain products, several of them, in fp32 or T, or shares of one.
+template <int CG, int KIND, bool RES, bool KINK, typename T, typename O>
 __global__ void __launch_bounds__(GtWarps<KIND, !std::is_same<T, O>::value>::THREADS, 1) gemm_tc_kernel(const __grid_constant__ GtMaps maps,
                                                                                                        const __grid_constant__ GtParams p) {
   using Warps = GtWarps<KIND, !std::is_same<T, O>::value>;
@@ -333,7 +362,20 @@ __global__ void __launch_bounds__(GtWarps<KIND, !std::is_same<T, O>::value>::THR
               if (p.bias[1]) bias[1].add_to(w);
             }
             if constexpr (!MULTI) {
-              if (DUAL && p.keep) {
+              if constexpr (KINK) {
+                const uint32_t above = above_kink<T>(p, row0, col + 16 * h, lane, v);
+                float f[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                  const bool up = above >> i & 1u;
+                  if constexpr (DUAL) f[i] = up ? w[i] : 0.0f;
+                  else f[i] = keep_side<T>(v[i], up);
+                }
+                slot_put<O>(to + SLOT, lane, h, f);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) v[i] = act_value<LIK_ACT_RELU, false>(v[i]);
+                if constexpr (DUAL) slot_put<O>(to + (OUT - 1) * SLOT, lane, h, v);
+              } else if (DUAL && p.keep) {
                 float f[16];
                 with_activation_dev(p.act, [&](auto act) {
 #pragma unroll
@@ -440,23 +482,25 @@ GtPlan tc_plan(const GemmDesc* d, int n) {
   return gt_plan(d, n, 40, 8, cg, [](const Stored& o) { return o.aligned() ? (size_t)0 : align_up((size_t)o.rows * o.padded() * 2, 256); });
 }
 
-template <int CG, int KIND, bool RES, typename T, typename O>
+template <int CG, int KIND, bool RES, bool KINK, typename T, typename O>
 int run_tc(const GtMaps& maps, const GtParams& p, cudaStream_t st) {
-  LIK_CUDA_OK((allow_smem<gemm_tc_kernel<CG, KIND, RES, T, O>>()));
+  LIK_CUDA_OK((allow_smem<gemm_tc_kernel<CG, KIND, RES, KINK, T, O>>()));
   const int slots = sm_count() / CG;
-  return launch_after(gemm_tc_kernel<CG, KIND, RES, T, O>, (unsigned)((p.units < slots ? p.units : slots) * CG), GtWarps<KIND, !std::is_same<T, O>::value>::THREADS,
+  return launch_after(gemm_tc_kernel<CG, KIND, RES, KINK, T, O>, (unsigned)((p.units < slots ? p.units : slots) * CG), GtWarps<KIND, !std::is_same<T, O>::value>::THREADS,
                       1024 + GT_CTL_AT + sizeof(GtCtl), st, CG, maps, p);
 }
-template <int KIND, bool RES, typename T, typename O>
+template <int KIND, bool RES, bool KINK, typename T, typename O>
 int run_tc(int cg, const GtMaps& maps, const GtParams& p, cudaStream_t st) {
-  return cg == 2 ? run_tc<2, KIND, RES, T, O>(maps, p, st) : run_tc<1, KIND, RES, T, O>(maps, p, st);
+  return cg == 2 ? run_tc<2, KIND, RES, KINK, T, O>(maps, p, st) : run_tc<1, KIND, RES, KINK, T, O>(maps, p, st);
 }
 template <typename T>
 int run_tc(int kind, bool multi, int cg, const GtMaps& maps, const GtParams& p, cudaStream_t st) {
-  if (kind == GEMM_GATED) return run_tc<GEMM_GATED, false, T, T>(cg, maps, p, st);
-  if (kind == GEMM_GATED_BWD) return run_tc<GEMM_GATED_BWD, false, T, T>(cg, maps, p, st);
-  if (multi) return run_tc<GEMM_LINEAR, false, T, float>(cg, maps, p, st);
-  return p.residual ? run_tc<GEMM_LINEAR, true, T, T>(cg, maps, p, st) : run_tc<GEMM_LINEAR, false, T, T>(cg, maps, p, st);
+  const bool kink = p.keep && p.act == LIK_ACT_RELU;
+  if (kind == GEMM_GATED_BWD) return run_tc<GEMM_GATED_BWD, false, false, T, T>(cg, maps, p, st);
+  if (kind == GEMM_GATED) return kink ? run_tc<GEMM_GATED, false, true, T, T>(cg, maps, p, st) : run_tc<GEMM_GATED, false, false, T, T>(cg, maps, p, st);
+  if (multi) return run_tc<GEMM_LINEAR, false, false, T, float>(cg, maps, p, st);
+  if (p.residual) return kink ? run_tc<GEMM_LINEAR, true, true, T, T>(cg, maps, p, st) : run_tc<GEMM_LINEAR, true, false, T, T>(cg, maps, p, st);
+  return kink ? run_tc<GEMM_LINEAR, false, true, T, T>(cg, maps, p, st) : run_tc<GEMM_LINEAR, false, false, T, T>(cg, maps, p, st);
 }
 
 }  // namespace
@@ -502,6 +546,11 @@ int launch_gemm_tc(const GemmDesc* d, int n, void* ws, size_t ws_bytes, int* sta
   }
   p.out2 = d->out[1];
   p.keep = d->kind != GEMM_GATED_BWD && d->kept[0];
+  p.a = d->a[0].p;
+  p.b = d->b[0].p;
+  p.a_stride = d->a[0].row;
+  p.b_stride = d->b[0].row;
+  p.k = d->k[0];
   p.kept_stride = d->kept_stride;
   p.residual = d->residual;
   p.residual_stride = d->residual_stride;

@@ -384,9 +384,34 @@ struct GemmDesc {
   void* kept[2] = {nullptr, nullptr};  // the factors of the backward: written, or read by GEMM_GATED_BWD; rows of 16 bytes
   long long kept_stride = 0;
 };
-// one element of the result, from the sums c0 and (GEMM_GATED) c1
+// The kink of relu.  Its slope goes by the sign of z, and the tensor core's sums, which are cut off at every 16 products, have a wrong sign for a z
+// within some 1e-6 of its neighbours: a few in a million, each a whole gradient off.  So where z is that much smaller than the largest of
+// its 16 neighbours and a backward pass will look at its sign, it is taken again from the operands, in 64 bits.
+__device__ __forceinline__ float kink_bound(float largest, long long k) { return largest * (1e-5f + 1e-8f * (float)k); }
+// products of 16-bit values are exact in fp32
+template <typename T>
+__device__ __forceinline__ double exact_part(const T* a, const T* b, long long k, long long first, long long step) {
+  double s = 0.0;
+#pragma unroll 8
+  for (long long i = first; i < k; i += step) s += (double)(to_f32(a[i]) * to_f32(b[i]));
+  return s;
+}
+// whether z of element (m, n) is above 0, by one thread
+template <typename T>
+__device__ __noinline__ bool above_zero(const GemmDesc& d, long long m, int n) {
+  const double z = exact_part((const T*)d.a[0].p + m * d.a[0].row, (const T*)d.b[0].p + n * d.b[0].row, d.k[0], 0, 1);
+  return (d.bias[0] ? z + (double)to_f32(((const T*)d.bias[0])[n]) : z) > 0.0;
+}
+// z as it is kept for relu's backward pass, which looks at its sign: above 0 also in its type where it is, and not where it is not
+template <typename T>
+__device__ __forceinline__ float keep_side(float z, bool above) {
+  const float least = std::is_same<T, __half>::value ? 5.9604644775390625e-8f : 1.1754943508222875e-38f;
+  return above ? fmaxf(z, least) : (z > 0.0f ? 0.0f : z);
+}
+
+// one element of the result, from the sums c0 and (GEMM_GATED) c1; above: whether relu's argument is above 0, as far as it is kept
 template <typename T, typename O, int KIND, int ACT>
-__device__ __forceinline__ void gemm_element(const GemmDesc& d, long long m, int n, float c0, float c1) {
+__device__ __forceinline__ void gemm_element(const GemmDesc& d, long long m, int n, float c0, float c1, bool above) {
   constexpr bool PRECISE = sizeof(T) == 4;
   const long long ki = m * d.kept_stride + n, oi = m * d.out_stride + n;
   if constexpr (KIND == GEMM_GATED_BWD) {
@@ -397,7 +422,8 @@ __device__ __forceinline__ void gemm_element(const GemmDesc& d, long long m, int
   if (d.bias[0]) c0 += to_f32(((const T*)d.bias[0])[n]);
   float v;
   if constexpr (KIND == GEMM_GATED) {
-    const float slope = act_slope<ACT, PRECISE>(c0, v);
+    float slope = act_slope<ACT, PRECISE>(c0, v);
+    if constexpr (ACT == LIK_ACT_RELU) slope = above ? 1.0f : 0.0f;
     if (d.bias[1]) c1 += to_f32(((const T*)d.bias[1])[n]);
     if (d.kept[0]) {
       ((T*)d.kept[0])[ki] = from_f32<T>(c1 * slope);
@@ -406,7 +432,7 @@ __device__ __forceinline__ void gemm_element(const GemmDesc& d, long long m, int
     v *= c1;
   } else {
     v = act_value<ACT, PRECISE>(c0);
-    if (d.kept[0]) ((T*)d.kept[0])[ki] = from_f32<T>(c0);
+    if (d.kept[0]) ((T*)d.kept[0])[ki] = from_f32<T>(ACT == LIK_ACT_RELU ? keep_side<T>(c0, above) : c0);
     if (d.residual) v += to_f32(((const T*)d.residual)[m * d.residual_stride + n]);
   }
   ((O*)d.out[0])[oi] = from_f32<O>(v);

@@ -280,6 +280,43 @@ def test_activations_over_their_range():
             assert (off <= 0).all(), (dt, act, float(x.flatten()[off.argmax()]), float(off.max()))
 
 
+@pytest.mark.parametrize("dt", [BF16, FP16])
+@pytest.mark.parametrize("m", [3, 40, 700, 5000])
+def test_relu_near_its_kink(dt, m):
+    """z that is next to nothing beside the products that it is a sum of, as sums that cut off what they shift out get wrong: half the products
+    cancel the other half (in another order, so that partial sums are large), what is left is +-2^-20, and the slope is its sign."""
+    from late_interaction_kernels_b200.token_layers import gated_feed_forward, linear
+
+    h, n = 496, 200
+    a, b = rand(m, h, dt=dt), rand(n, h, dt=dt)
+    perm = torch.randperm(h, device="cuda")
+    tiny = torch.where(torch.rand(m, 1, device="cuda") < 0.5, -1.0, 1.0) * 2.0**-10
+    x = torch.cat([a, a[:, perm], tiny.to(dt).expand(m, 8)], 1)
+    w = torch.cat([b, -b[:, perm], torch.full((n, 8), 2.0**-13, device="cuda").to(dt)], 1)
+    big = rand(n, x.shape[1], dt=dt)  # (neighbours of the usual size)
+    w[::2] = big[::2]
+    bias = torch.zeros(n, device="cuda", dtype=dt)
+    for bi in (None, bias):
+        x1 = x.clone().requires_grad_()
+        y = linear(x1, w, bi, activation="relu")
+        (dx,) = torch.autograd.grad(y, [x1], torch.ones_like(y))
+        z = x.double() @ w.double().t()
+        assert float(z[:, 1::2].abs().max()) == 2.0**-20
+        want = (z > 0).double() @ w.double()
+        near(dx, want, 2 * n * E * ((z > 0).double() @ w.double().abs()), "dx")
+    # the gate of a block: only odd features get through to the result, as 1 where the gate is open
+    wd = torch.zeros(8, n, device="cuda", dtype=dt)
+    wd[:, 1::2] = 1
+    up = torch.zeros_like(w)
+    up1 = torch.ones(n, device="cuda", dtype=dt)
+    x1 = x.clone().requires_grad_()
+    g1 = w.clone().requires_grad_()
+    y = gated_feed_forward(x1, g1, up, wd, b_up=up1, activation="relu")
+    (dg,) = torch.autograd.grad(y, [g1], torch.ones_like(y))
+    open_ = (z[:, 1::2] > 0).double()
+    near(dg[1::2], 8 * open_.t() @ x.double(), 2 * m * E * 8 * open_.t() @ x.double().abs(), "dw_gate")
+
+
 def test_linear_strides():
     """Rows that do not follow one another, start off 16 bytes, overlap or lie across: the kernels differ, the numbers are held to the same bounds."""
     from late_interaction_kernels_b200.token_layers import linear
