@@ -479,7 +479,7 @@ GtPlan tc_plan(const GemmDesc* d, int n) {
     const bool cuttable = gemm_plain(g) && g.m > 128 && g.n > 128;
     return tiles >= pairs || (cuttable && tiles * ceil_div(g.k[0] + g.k[1], GT_BK) >= 16 * pairs) ? 2 : 1;
   };
-  return gt_plan(d, n, 40, 8, cg, [](const Stored& o) { return o.aligned() ? (size_t)0 : align_up((size_t)o.rows * o.padded() * 2, 256); });
+  return gt_plan(d, n, {40, 96}, 8, cg, [](const Stored& o) { return o.aligned() ? (size_t)0 : align_up((size_t)o.rows * o.padded() * 2, 256); });
 }
 
 template <int CG, int KIND, bool RES, bool KINK, typename T, typename O>

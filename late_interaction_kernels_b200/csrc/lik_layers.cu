@@ -385,6 +385,7 @@ GatedBwd gated_bwd_layout(const lik_gated_args& a, void* ws) {
     d.a[1] = {l.du, l.stride, 1};
     d.b[1] = {a.w_up, 1, a.w_up_stride};
   }
+  for (int i = 0; i < l.n_grads; ++i) l.grads[i].several = true;
   l.gemm_bytes = gemm_workspace(l.grads, l.n_grads);
   if (inner) {
     const size_t b = gemm_workspace(&l.dh);

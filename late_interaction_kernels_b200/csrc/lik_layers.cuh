@@ -370,6 +370,7 @@ struct GemmOperand {
 };
 struct GemmDesc {
   int kind = GEMM_LINEAR, act = LIK_ACT_NONE, dtype = 0;
+  bool several = false;       // one of up to four products that may share a launch
   long long m = 0;
   int n = 0;
   int n_seg = 1;              // segments of the sum (GEMM_LINEAR) ...
@@ -392,7 +393,7 @@ __device__ __forceinline__ float kink_bound(float largest, long long k) { return
 template <typename T>
 __device__ __forceinline__ double exact_part(const T* a, const T* b, long long k, long long first, long long step) {
   double s = 0.0;
-#pragma unroll 8
+#pragma unroll 16
   for (long long i = first; i < k; i += step) s += (double)(to_f32(a[i]) * to_f32(b[i]));
   return s;
 }

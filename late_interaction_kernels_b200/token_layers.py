@@ -13,7 +13,9 @@ bfloat16; sums, statistics and activations are fp32 and results are rounded once
 weights beside bf16 activations) are brought to ``x``'s type for the products - a layer norm reads fp32 weights as they are - and get
 gradients of their own type, rounded from fp32.  Gradients are deterministic.  Backward passes keep what they need: the input, in ``x``'s
 type the values in front of an activation or, of a gated block, the factors of its gradients, and a row's mean and inverse deviation in fp32.  Everything runs
-on the current stream and may be captured into a CUDA graph.  (No counterpart in the reference, which starts at the hidden states.)
+on the current stream and may be captured into a CUDA graph.  With 16-bit operands ``relu``'s
+gradient goes by the sign of the exact sum where that sum is small beside its neighbours.  An infinity among fp32
+operands of a product gives infinities or NaN in its row.  (No counterpart in the reference, which starts at the hidden states.)
 """
 
 from __future__ import annotations
