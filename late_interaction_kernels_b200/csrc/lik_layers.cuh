@@ -415,11 +415,6 @@ template <typename T, typename O, int KIND, int ACT>
 __device__ __forceinline__ void gemm_element(const GemmDesc& d, long long m, int n, float c0, float c1, bool above) {
   constexpr bool PRECISE = sizeof(T) == 4;
   const long long ki = m * d.kept_stride + n, oi = m * d.out_stride + n;
-  if constexpr (KIND == GEMM_GATED_BWD) {
-    ((T*)d.out[0])[oi] = from_f32<T>(c0 * to_f32(((const T*)d.kept[0])[ki]));
-    ((T*)d.out[1])[oi] = from_f32<T>(c0 * to_f32(((const T*)d.kept[1])[ki]));
-    return;
-  }
   if (d.bias[0]) c0 += to_f32(((const T*)d.bias[0])[n]);
   float v;
   if constexpr (KIND == GEMM_GATED) {
