@@ -50,7 +50,12 @@ void require_layer_inputs(const char* op, const Tensor& x, Named others) {
 void require_vector(const char* name, const Tensor& t, int64_t n) {
   if (t.defined() && (t.dim() != 1 || t.size(0) != n)) value_error(std::string(name) + " must be [" + std::to_string(n) + "]; got " + shape(t.sizes()));
 }
+constexpr int64_t FEATURES_END = int64_t(1) << 30;  // (the kernels count features in 32 bits)
+void require_features(const Tensor& x) {
+  if (x.size(-1) < 1 || x.size(-1) >= FEATURES_END) value_error("x must have at least one feature, and less than 2^30; got " + shape(x.sizes()));
+}
 void require_matrix(const char* name, const Tensor& t, int64_t rows, const char* cols_name, int64_t cols) {
+  if (t.dim() == 2 && t.size(0) >= FEATURES_END) value_error(std::string(name) + " must have less than 2^30 rows; got " + shape(t.sizes()));
   if (t.dim() != 2 || t.size(1) != cols || (rows >= 0 && t.size(0) != rows) || t.size(0) < 1)
     value_error(std::string(name) + " must be [" + (rows >= 0 ? std::to_string(rows) : "features >= 1") + ", " + cols_name + "=" + std::to_string(cols) + "]; got " + shape(t.sizes()));
 }
@@ -217,7 +222,7 @@ Tensor layer_norm(const Tensor& x_, const OptTensor& weight_, const OptTensor& b
   const Tensor w = opt(weight_), b = opt(bias_);
   require_layer_inputs("layer_norm", x_, {{"weight", &w}, {"bias", &b}});
   const int64_t width = x_.size(-1);
-  if (width < 1 || width >= (int64_t(1) << 30)) value_error("x must have at least one feature, and less than 2^30; got " + shape(x_.sizes()));
+  require_features(x_);
   require_vector("weight", w, width);
   require_vector("bias", b, width);
   if (!(eps >= 0) || eps > 3e38) value_error("eps must be a number that is not negative; got " + std::to_string(eps));
@@ -329,7 +334,7 @@ Tensor linear(const Tensor& x_, const Tensor& w, const OptTensor& bias_, const s
   const Tensor b = opt(bias_), r_ = opt(residual_);
   require_layer_inputs("linear", x_, {{"weight", &w}, {"bias", &b}, {"residual", &r_}});
   const int64_t in = x_.size(-1);
-  if (in < 1) value_error("x must have at least one feature; got " + shape(x_.sizes()));
+  require_features(x_);
   require_matrix("weight", w, -1, "in_features", in);
   const int64_t out = w.size(0);
   require_vector("bias", b, out);
@@ -472,7 +477,7 @@ Tensor gated_feed_forward(const Tensor& x_, const Tensor& wg, const Tensor& wu, 
   require_layer_inputs("gated_feed_forward", x_,
                        {{"w_gate", &wg}, {"w_up", &wu}, {"w_down", &wd}, {"b_gate", &bg}, {"b_up", &bu}, {"b_down", &bd}, {"residual", &r_}});
   const int64_t in = x_.size(-1);
-  if (in < 1) value_error("x must have at least one feature; got " + shape(x_.sizes()));
+  require_features(x_);
   require_matrix("w_gate", wg, -1, "in_features", in);
   const int64_t f = wg.size(0);
   require_matrix("w_up", wu, f, "in_features", in);

@@ -562,6 +562,45 @@ def test_steps_on_two_streams_side_by_side():
                 assert torch.equal(a, b)
 
 
+def test_steps_from_two_threads():
+    from concurrent.futures import ThreadPoolExecutor
+
+    p = head_params(160, 320, BF16)
+    data = [(rand(n, 160, dt=BF16).requires_grad_(), rand(n, 160, dt=BF16)) for n in (5, 900)]
+
+    def steps(i):
+        x, d = data[i]
+        with torch.cuda.stream(torch.cuda.Stream()):
+            out = []
+            for _ in range(10):
+                y = head(x, p)
+                out.append([y.detach(), *torch.autograd.grad(y, [x, *p.values()], d)])
+            torch.cuda.current_stream().synchronize()
+        return out
+
+    torch.cuda.synchronize()
+    want = [steps(i)[0] for i in range(2)]
+    with ThreadPoolExecutor(2) as pool:
+        got = list(pool.map(steps, range(2)))
+    for i in range(2):
+        for g in got[i]:
+            for a, b in zip(g, want[i]):
+                assert torch.equal(a, b)
+
+
+def test_what_is_kept_may_wait_on_the_host():
+    p = head_params(96, 160, BF16)
+    x, d = rand(70, 96, dt=BF16).requires_grad_(), rand(70, 96, dt=BF16)
+    leaves = [x, *p.values()]
+    want = torch.autograd.grad(head(x, p), leaves, d)
+    with torch.autograd.graph.save_on_cpu():
+        y = head(x, p)
+    for a, b in zip(torch.autograd.grad(y, leaves, d), want):
+        assert torch.equal(a, b)
+    with torch.inference_mode():
+        assert torch.equal(head(x, p), y)
+
+
 def test_a_backward_pass_may_run_twice():
     p = head_params(96, 160, FP32)
     x, d = rand(333, 96, dt=FP32).requires_grad_(), rand(333, 96, dt=FP32)
@@ -725,6 +764,7 @@ def test_refusals():
 
     x, w, b = rand(4, 8, dt=BF16), rand(6, 8, dt=BF16), rand(6, dt=BF16)
     wd = rand(8, 6, dt=BF16)
+    one = rand(1, 1, dt=BF16)
     bad = [
         (lambda: layer_norm(x, b), r"weight must be \[8\]"), (lambda: layer_norm(x, None, b), r"bias must be \[8\]"), (lambda: layer_norm(x, eps=-1.0), "eps"),
         (lambda: layer_norm(x, eps=float("nan")), "eps"), (lambda: layer_norm(x.to(torch.float64)), "not supported"), (lambda: layer_norm(x[:, :0]), "at least one feature"),
@@ -736,6 +776,10 @@ def test_refusals():
         (lambda: gated_feed_forward(x, w, w[:5], wd), "w_up must be"), (lambda: gated_feed_forward(x, w, w, wd[:, :5]), "w_down must be"),
         (lambda: gated_feed_forward(x, w, w, wd, b_down=b), r"b_down must be \[8\]"), (lambda: gated_feed_forward(x, w, w, wd, residual=x[:3]), "residual must have"),
         (lambda: gated_feed_forward(x, w, w, wd, activation="x"), "activation must be"),
+        # sizes beyond what the kernels count with
+        (lambda: linear(one.expand(1, 2**32 + 8), one.expand(1, 2**32 + 8)), "less than 2"), (lambda: linear(one, one.expand(2**32 + 8, 1)), "less than 2"),
+        (lambda: gated_feed_forward(one, one.expand(2**32, 1), one.expand(2**32, 1), one.expand(1, 2**32)), "less than 2"),
+        (lambda: gated_feed_forward(one, one, one, one.expand(2**32, 1)), "less than 2"),
     ]
     for fn, text in bad:
         with pytest.raises(ValueError, match=text):
