@@ -299,13 +299,13 @@ struct GtPlan {
     return end;
   }
 };
-// cg_of: CTAs that share a tile of (128 CTAs)^2; cut_from: slabs of k from which a product is cut into shares, of at least `share` slabs each;
-// copy_bytes: of a matrix that is not read as it lies in memory, 0 otherwise.  cut_from[1] is for one of up to four products, which share a
-// launch if they are not cut: a step of 3500 x 768 through a gated block of 2048 took 154 us cut from 40 slabs on, 119 from 96 on; with the
-// two products of a linear layer it is the other way round, 41 and 45 us.  A problem is planned as if it were alone, so its result does not
-// depend on which others are asked for.
+// cg_of: CTAs that share a tile of (128 CTAs)^2; cut_from: slabs of k from which a product is cut into shares, of at least `share` slabs each, if
+// that spares a CTA `spare` of them; copy_bytes: of a matrix that is not read as it lies in memory, 0 otherwise.  cut_from[1] is for one of up to
+// four products, which share a launch if they are not cut: a step of 3500 x 768 through a gated block of 2048 took 154 us cut from 40 slabs on, 119
+// from 96 on; with the two products of a linear layer it is the other way round, 41 and 45 us.  A problem is planned as if it were alone, so its
+// result does not depend on which others are asked for.
 template <typename CgOf, typename CopyBytes>
-GtPlan gt_plan(const GemmDesc* d, int n, const int (&cut_from)[2], int share, CgOf&& cg_of, CopyBytes&& copy_bytes) {
+GtPlan gt_plan(const GemmDesc* d, int n, const int (&cut_from)[2], int share, int spare, CgOf&& cg_of, CopyBytes&& copy_bytes) {
   GtPlan pl{};
   pl.n = n;
   size_t off = 0;
@@ -332,10 +332,10 @@ GtPlan gt_plan(const GemmDesc* d, int n, const int (&cut_from)[2], int share, Cg
         if (at == pl.n_mat) pl.mat[pl.n_mat++] = o;
         (is_b ? q.b : q.a)[s] = (unsigned char)at;
       }
-    // a share of k for every slot, where the time that this saves is worth the pass that adds the shares up (4 to 5 us)
+    // a share of k for every slot, where the time that this saves is worth the pass that adds the shares up (2.5 us)
     long long ideal = ceil_div((long long)q.tiles * q.kb_total, sm_count() / cg);
     if (ideal < share) ideal = share;
-    const long long s = d[i].kind == GEMM_LINEAR && q.kb_total >= cut_from[d[i].several] && q.kb_total >= 2 * ideal ? q.kb_total / ideal : 1;
+    const long long s = d[i].kind == GEMM_LINEAR && q.kb_total >= cut_from[d[i].several] && q.kb_total >= 2 * ideal && q.kb_total - ideal >= spare ? q.kb_total / ideal : 1;
     q.kb_per = (int)ceil_div(q.kb_total, s);
     pl.splits[i] = (int)ceil_div(q.kb_total, q.kb_per);
     pl.units[i] = q.tiles * pl.splits[i];

@@ -226,16 +226,23 @@ int run_few(const FewParams& p, cudaStream_t st) {
 
 }  // namespace
 
-// By the blocks that there are for an SM.  A block's time grows little with k; the tensor-core kernels have a start of their own of 6 us
-// (fp32: 10 with the cuts) and one CTA's loads per 128 columns.  Measured on both sides of either limit, few rows against tensor cores in
-// us, by blocks per SM: 16-bit 768 x 2048, 96 rows (2.6) 6.2 / 8.2, 128 rows (3.5) 9.8 / 8.4; 2048 x 2048, 96 rows (2.6) 10.1 / 12.3, 128 rows
-// (3.5) 17 / 12.5; fp32 768 x 768, 32 rows (5.2) 9.0 / 13.1, 64 rows (10.4) 16 / 13.4.
+// By the blocks that there are for an SM, and from k = 1024 on, where a block's 512 threads have an SM to themselves, by the k that an SM goes through
+// one after another; the tensor-core kernels have a start of their own of 6 us (fp32: 10 with the cuts) and can cut a long k.  Measured on both
+// sides of each limit, few rows against tensor cores in us: 16-bit 768 x 768, 256 rows (2.6 blocks) 6.5 / 8.0; 768 x 2048, 128 rows (3.5) 9.8 / 8.0;
+// k = 1024, 96 rows of 1024 (two of 1024) 6.4 / 6.8, 192 (three) 9.4 / 7.4; k = 2048, 96 rows of 768 (one) 6.0 / 7.0, 128 (two) 10.5 / 7.4;
+// k = 4096, 32 rows (one) 9.1 / 7.7, 16 rows 6.8 / 7.4; k = 8192, 16 rows 11.2 / 8.2, 8 rows 6.8 / 8.3; k = 16384, 8 rows 11.4 / 9.9; fp32 768 x 768, 32 rows
+// (5.2 blocks) 9.6 / 11.5, 64 rows (10.4) 16 / 11.3.
 bool gemm_few_pays(const GemmDesc& d) {
   if (d.kind == GEMM_GATED_BWD || d.n_seg != 1 || d.a[0].k != 1 || d.b[0].k != 1 || d.out_dtype != d.dtype || d.k[0] >= (1ll << 31) - 4096) return false;
   const long long sms = sm_count(), dual = d.kind == GEMM_GATED ? 2 : 1;
   if (d.dtype != LIK_F32 && few_vec(d)) {
     const long long rows = d.m <= 8 ? 8 : (d.m <= 16 ? 16 : 32);
-    return dual * ceil_div(d.n, 16) * ceil_div(d.m, rows) * 5 <= 13 * sms * (32 / rows);
+    const long long blocks = dual * ceil_div(d.n, 16) * ceil_div(d.m, rows);
+    if (d.kind == GEMM_LINEAR && d.k[0] >= 1024) {
+      const long long in_turn = rows == 8 ? d.k[0] : ceil_div(blocks, sms) * d.k[0];
+      if (in_turn > (rows == 8 ? 12000 : (rows == 16 ? 5000 : 2500))) return false;
+    }
+    return blocks * 5 <= 13 * sms * (32 / rows);
   }
   return dual * ceil_div(d.n, FMA_ROWS) * ceil_div(d.m, FMA_COLS) <= 8 * sms;
 }

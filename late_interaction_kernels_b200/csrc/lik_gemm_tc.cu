@@ -472,14 +472,16 @@ __global__ void __launch_bounds__(256) repack_kernel(const __grid_constant__ Rep
 }
 
 // Pairs of CTAs take tiles of 256 x 256 where there are enough of them, or enough k to cut into shares, for every pair; else single CTAs
-// tiles of 128 x 128.  A slab of k takes a CTA that is alone with its tile 0.2 us.
+// tiles of 128 x 128.  A slab of k takes a CTA that is alone with its tile 0.2 us, so shares pay from 12 slabs spared on: 512 rows, 2048 x 768 (6 of 32
+// slabs each) 12.3 us whole, 9.0 cut; 1024 rows, 1024 x 1024 (7 of 16) 9.4 and 10.3.  (Four CTAs of a cluster that add their sums up in shared
+// memory, without the pass: 10.4 and 9.9; their start costs what the pass does.)
 GtPlan tc_plan(const GemmDesc* d, int n) {
   auto cg = [](const GemmDesc& g) {
     const long long tiles = ceil_div(g.m, 256) * ceil_div(g.n, g.kind == GEMM_GATED ? 128 : 256), pairs = sm_count() / 2;
     const bool cuttable = gemm_plain(g) && g.m > 128 && g.n > 128;
     return tiles >= pairs || (cuttable && tiles * ceil_div(g.k[0] + g.k[1], GT_BK) >= 16 * pairs) ? 2 : 1;
   };
-  return gt_plan(d, n, {40, 96}, 8, cg, [](const Stored& o) { return o.aligned() ? (size_t)0 : align_up((size_t)o.rows * o.padded() * 2, 256); });
+  return gt_plan(d, n, {16, 96}, 4, 12, cg, [](const Stored& o) { return o.aligned() ? (size_t)0 : align_up((size_t)o.rows * o.padded() * 2, 256); });
 }
 
 template <int CG, int KIND, bool RES, bool KINK, typename T, typename O>

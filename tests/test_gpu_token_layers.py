@@ -236,7 +236,7 @@ def linear_case(m, k, n, dt, act, bias, residual, wdt=None):
 SHAPES = [(1, 1, 1), (1, 7, 3), (2, 64, 5), (5, 16, 16), (8, 768, 768), (9, 768, 130), (16, 512, 1024), (17, 512, 1000), (32, 768, 128), (33, 100, 65), (64, 72, 264),
           (128, 128, 128), (129, 255, 257), (255, 264, 248), (300, 768, 520), (700, 1001, 333), (2050, 192, 72), (4096, 64, 64), (20000, 40, 24), (1000, 2048, 136),
           (2500, 520, 392), (4100, 260, 1030), (30000, 96, 200), (40, 1, 1), (300, 1, 5), (5, 300, 1),
-          (300, 4000, 260), (128, 2900, 70), (3000, 2700, 300), (700, 640, 1600)]
+          (300, 4000, 260), (128, 2900, 70), (3000, 2700, 300), (700, 640, 1600), (200, 1500, 136), (16, 5200, 24), (6, 12300, 40)]
 
 
 @pytest.mark.parametrize("dt", [BF16, FP16, FP32])
