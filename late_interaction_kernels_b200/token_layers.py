@@ -32,7 +32,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
 
 
 def linear(x, weight, bias=None, activation=None, residual=None):
-    """``act(x @ weight.T + bias) + residual`` in one kernel; autograd-aware in all four tensors.
+    """``act(x @ weight.T + bias) + residual``; autograd-aware in all four tensors.  Nothing between the product and the result goes through memory,
+    but for the shares of a long sum with few rows.
 
     ``x [..., in]``, ``weight [out, in]``, ``bias [out]`` or None, ``activation`` None, ``"relu"``, ``"silu"``, ``"gelu"`` (with the
     normal distribution), ``"gelu_tanh"`` (its approximation), ``"tanh"`` or ``"sigmoid"``, ``residual [..., out]`` or None."""
