@@ -272,14 +272,20 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Sum
 struct Stored {
   const void* p;
   long long rows, cols, stride;
-  bool mn;  // rows are k
   // as TMA wants 16-bit rows
   bool aligned() const { return ((uintptr_t)p & 15) == 0 && (rows == 1 || stride % 8 == 0); }
   long long padded() const { return (cols + 7) / 8 * 8; }
 };
-inline Stored stored(const GemmOperand& o, long long rows, long long k) {
-  if (o.k == 1) return {o.p, rows, k, o.row, false};
-  return {o.p, k, rows, o.k, true};
+// mn: its rows are k
+inline Stored stored(const GemmOperand& o, long long rows, long long k, bool mn) {
+  return mn ? Stored{o.p, k, rows, o.k} : Stored{o.p, rows, k, o.row};
+}
+// Whether k runs along the rows in memory: one answer for all `n` operands of a side, since a unit's MMAs read them the same way.  Where a matrix is
+// a single column wide, both of its steps may be 1, or that of k alone may not be (a column of a wider matrix): across fits either.
+inline bool stored_across(const GemmOperand* o, int n) {
+  for (int i = 0; i < n; ++i)
+    if (o[i].k != 1) return true;
+  return false;
 }
 inline bool rows_of_pieces(const void* p, long long stride, int dtype) { return ((uintptr_t)p & 15) == 0 && stride * (long long)dtype_size(dtype) % 16 == 0; }
 
@@ -322,11 +328,12 @@ GtPlan gt_plan(const GemmDesc* d, int n, const int (&cut_from)[2], int share, in
       q.kb_total += kb;
       if (s == 0) q.kb0 = kb;
     }
+    q.a_mn = stored_across(d[i].a, d[i].n_seg);
+    q.b_mn = stored_across(d[i].b, dual ? 2 : d[i].n_seg);
     for (int s = 0; s < 2; ++s)
       for (int is_b = 0; is_b < 2; ++is_b) {
         if (s >= (is_b && dual ? 2 : d[i].n_seg)) continue;
-        const Stored o = stored(is_b ? d[i].b[s] : d[i].a[s], is_b ? d[i].n : d[i].m, d[i].k[dual ? 0 : s]);
-        (is_b ? q.b_mn : q.a_mn) = o.mn;
+        const Stored o = is_b ? stored(d[i].b[s], d[i].n, d[i].k[dual ? 0 : s], q.b_mn) : stored(d[i].a[s], d[i].m, d[i].k[s], q.a_mn);
         int at = 0;
         while (at < pl.n_mat && !(pl.mat[at].p == o.p && pl.mat[at].rows == o.rows && pl.mat[at].cols == o.cols && pl.mat[at].stride == o.stride)) ++at;
         if (at == pl.n_mat) pl.mat[pl.n_mat++] = o;

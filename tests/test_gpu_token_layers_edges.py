@@ -1,0 +1,38 @@
+"""The layers in front of the document head where they can go wrong: operands that lie in memory in unlike ways.
+
+Bounds as in test_gpu_token_layers: every rounding counted at its most."""
+
+import pytest
+import torch
+
+from test_gpu_token_layers import BF16, E, FP16, FP32, floor, near, rand, unit
+
+pytestmark = pytest.mark.gpu
+
+
+# ----------------------------------------------------------------------------- operands that lie in memory in unlike ways
+@pytest.mark.parametrize("dt", [BF16, FP16, FP32])
+@pytest.mark.parametrize("m, k, f", [(300, 1, 200), (5, 1, 200), (2000, 1, 40), (300, 24, 200), (700, 1, 1)])
+def test_gated_weights_of_differing_strides(dt, m, k, f):
+    """With one input feature a contiguous weight has its features next to one another, a slice of a wider one has not."""
+    from late_interaction_kernels_b200.token_layers import gated_feed_forward
+
+    o = 16
+    x, dy = rand(m, k, dt=dt), rand(m, o, dt=dt)
+    plain, wide, across = rand(f, k, dt=dt), rand(f, k + 4, dt=dt)[:, 2 : 2 + k], rand(k, f, dt=dt).t()
+    down, down_wide, down_across = rand(o, f, dt=dt), rand(o, 2 * f + 1, dt=dt)[:, f + 1 :], rand(f, o, dt=dt).t()
+    for wg, wu, wd in ((plain, wide, down), (wide, plain, down_wide), (across, wide, down_across), (wide, across, down), (plain, across, down_wide)):
+        leaves = [t.detach().requires_grad_() for t in (x, wg, wu, wd)]
+        y = gated_feed_forward(*leaves, activation=None)
+        dx, dg_w, du_w, dd_w = torch.autograd.grad(y, leaves, dy)
+        X, G, U, D, d = (t.double() for t in (x, wg, wu, wd, dy))
+        g, u, dh = X @ G.t(), X @ U.t(), d @ D
+        gs, us, dhs = X.abs() @ G.abs().t(), X.abs() @ U.abs().t(), d.abs() @ D.abs()
+        # a factor is rounded, and its product with dh; products of k, o, f and m terms, the magnitudes of sums in place of the sums; a rounding
+        # among subnormal numbers is off by `low`, the factor's times dh
+        rel, low = 3 * unit(dt) + 4 * (k + o + f + m) * E, floor(dt) * (dhs + 1)
+        near(y.detach(), (g * u) @ D.t(), (rel * gs * us + floor(dt)) @ D.abs().t(), "y")
+        near(dx, (dh * u) @ G + (dh * g) @ U, (rel * dhs * us + low) @ G.abs() + (rel * dhs * gs + low) @ U.abs(), "dx")
+        near(dg_w, (dh * u).t() @ X, (rel * dhs * us + low).t() @ X.abs(), "dw_gate")
+        near(du_w, (dh * g).t() @ X, (rel * dhs * gs + low).t() @ X.abs(), "dw_up")
+        near(dd_w, d.t() @ (g * u), d.abs().t() @ (rel * gs * us + floor(dt)), "dw_down")
