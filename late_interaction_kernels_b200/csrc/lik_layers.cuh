@@ -45,6 +45,15 @@ __device__ __forceinline__ float normal_tail(float z, float& e) {
   r = fmaf(r, t, 0.120074183f);
   return r * t * e;
 }
+// gelu from the tail: z - z tail above 0, z tail below.  As a product with 0 or 1 the first term is infinite for z = inf and NaN for z = -inf, as z Phi(z)
+// is; the second one's factor stays finite, since a tail of 0 has to make it 0.
+__device__ __forceinline__ float above0(float z) {
+  float r;
+  asm("set.gt.f32.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(z));
+  return r;
+}
+__device__ __forceinline__ float minus_abs(float z) { return fmaxf(-fabsf(z), -1e30f); }
+__device__ __forceinline__ float gelu_from(float z, float tail) { return fmaf(minus_abs(z), tail, z * above0(z)); }
 constexpr float GELU_C = 1.5957691216057308f;  // 2 sqrt(2 / pi): (1 + tanh(y)) / 2 = sigmoid(2 y)
 
 template <int ACT, bool PRECISE>
@@ -55,7 +64,7 @@ __device__ __forceinline__ float act_value(float z) {
     if constexpr (PRECISE) return 0.5f * z * erfcf(-0.70710678118654752f * z);
     float e;
     const float tail = normal_tail(z, e);
-    return fmaf(-fabsf(z), tail, fmaxf(z, 0.0f));  // z - z tail above 0, z tail below
+    return gelu_from(z, tail);
   }
   if constexpr (ACT == LIK_ACT_GELU_TANH) return z * sigmoid_f<PRECISE>(GELU_C * fmaf(0.044715f * z * z, z, z));
   if constexpr (ACT == LIK_ACT_TANH) return tanh_f<PRECISE>(z);
@@ -83,7 +92,7 @@ __device__ __forceinline__ float act_slope(float z, float& value) {
     } else {
       const float tail = normal_tail(z, e);
       cdf = z < 0.0f ? tail : 1.0f - tail;
-      value = fmaf(-fabsf(z), tail, fmaxf(z, 0.0f));
+      value = gelu_from(z, tail);
     }
     return fmaf(0.3989422804014327f * z, e, cdf);
   }
@@ -218,7 +227,7 @@ __device__ __forceinline__ void act_pair(float& x, float& y, float& sx, float& s
       mul2(s, fma2(w, fma2(s, both(-1.0f), both(1.0f)), both(1.0f))).get(sx, sy);
     }
   } else if constexpr (ACT == LIK_ACT_GELU) {
-    const Pair na(-fabsf(x), -fabsf(y)), t = rcp_2(fma2(na, both(-0.3f), both(1.0f))), e = exp2_2(mul2(mul2(z, z), both(-0.72134752f)));
+    const Pair na(minus_abs(x), minus_abs(y)), t = rcp_2(fma2(na, both(-0.3f), both(1.0f))), e = exp2_2(mul2(mul2(z, z), both(-0.72134752f)));
     Pair r = fma2(t, both(-0.0770966218f), both(0.216034401f));
     r = fma2(r, t, both(-0.0169447843f));
     r = fma2(r, t, both(0.144194491f));
@@ -231,7 +240,7 @@ __device__ __forceinline__ void act_pair(float& x, float& y, float& sx, float& s
       fma2(tail, both(-1.0f), both(1.0f)).get(c, d);
       fma2(mul2(z, both(0.3989422804014327f)), e, Pair(x < 0.0f ? a : c, y < 0.0f ? b : d)).get(sx, sy);
     }
-    fma2(na, tail, Pair(fmaxf(x, 0.0f), fmaxf(y, 0.0f))).get(x, y);
+    fma2(na, tail, mul2(z, Pair(above0(x), above0(y)))).get(x, y);  // (gelu_from)
   } else if constexpr (SLOPE) {
     sx = act_slope<ACT, false>(x, x);
     sy = act_slope<ACT, false>(y, y);

@@ -1,11 +1,11 @@
-"""The layers in front of the document head where they can go wrong: operands that lie in memory in unlike ways.
+"""The layers in front of the document head where they can go wrong: operands that lie in memory in unlike ways, infinities.
 
 Bounds as in test_gpu_token_layers: every rounding counted at its most."""
 
 import pytest
 import torch
 
-from test_gpu_token_layers import BF16, E, FP16, FP32, floor, near, rand, unit
+from test_gpu_token_layers import ACTS, BF16, E, FP16, FP32, floor, near, rand, unit
 
 pytestmark = pytest.mark.gpu
 
@@ -36,3 +36,33 @@ def test_gated_weights_of_differing_strides(dt, m, k, f):
         near(dg_w, (dh * u).t() @ X, (rel * dhs * us + low).t() @ X.abs(), "dw_gate")
         near(du_w, (dh * g).t() @ X, (rel * dhs * gs + low).t() @ X.abs(), "dw_up")
         near(dd_w, d.t() @ (g * u), d.abs().t() @ (rel * gs * us + floor(dt)), "dw_down")
+
+
+# ----------------------------------------------------------------------------- infinities, and values beyond the type
+# rows, features in and out: few rows, few rows of odd width, single CTAs, pairs, a product that is cut along k
+KERNELS = [(3, 64, 72), (3, 63, 71), (300, 64, 72), (300, 63, 71), (9000, 64, 520), (300, 4000, 264)]
+
+
+@pytest.mark.parametrize("dt", [BF16, FP16, FP32])
+@pytest.mark.parametrize("m, k, n", KERNELS)
+def test_activations_of_infinity(dt, m, k, n):
+    from late_interaction_kernels_b200.token_layers import gated_feed_forward, linear
+
+    inf = float("inf")
+    x, w, b = rand(m, k, dt=dt), rand(n, k, dt=dt, scale=k**-0.5), torch.zeros(n, device="cuda", dtype=dt)
+    b[1], b[n - 2] = inf, -inf
+    ones, up = torch.zeros_like(w), torch.ones(n, device="cuda", dtype=dt)
+    down = torch.zeros(2, n, device="cuda", dtype=dt)
+    for act in ACTS[1:]:
+        y = linear(x, w, b, activation=act)
+        assert (y[:, 1] == (1 if act in ("tanh", "sigmoid") else inf)).all(), act
+        if act in ("relu", "tanh", "sigmoid"):
+            assert (y[:, n - 2] == (-1 if act == "tanh" else 0)).all(), act
+        rest = [i for i in range(n) if i not in (1, n - 2)]
+        assert torch.equal(y[:, rest], linear(x, w, torch.zeros_like(b), activation=act)[:, rest])
+        bg = b.clone()
+        bg[n - 2] = 0
+        down[:, 1] = 1
+        h = gated_feed_forward(x, w, ones, down[:, :n], b_gate=bg, b_up=up, activation=act)
+        if act not in ("tanh", "sigmoid") and dt != FP32:  # (an fp32 infinity gives NaN or infinities in the second product)
+            assert not torch.isfinite(h).any() and not torch.isfinite(h[:, 0]).any()
