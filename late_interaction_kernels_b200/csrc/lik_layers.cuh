@@ -54,6 +54,8 @@ __device__ __forceinline__ float above0(float z) {
 }
 __device__ __forceinline__ float minus_abs(float z) { return fmaxf(-fabsf(z), -1e30f); }
 __device__ __forceinline__ float gelu_from(float z, float tail) { return fmaf(minus_abs(z), tail, z * above0(z)); }
+// A factor beside one that is exactly 0 once z is far from zero: from |z| of 1e13 on the polynomial in gelu_tanh's slope is infinite.  (The factor that may be 0 keeps a NaN.)
+__device__ __forceinline__ float bounded(float w) { return fminf(fmaxf(w, -1e30f), 1e30f); }
 constexpr float GELU_C = 1.5957691216057308f;  // 2 sqrt(2 / pi): (1 + tanh(y)) / 2 = sigmoid(2 y)
 
 template <int ACT, bool PRECISE>
@@ -99,7 +101,7 @@ __device__ __forceinline__ float act_slope(float z, float& value) {
   if constexpr (ACT == LIK_ACT_GELU_TANH) {
     const float q = 0.044715f * z * z, s = sigmoid_f<PRECISE>(GELU_C * fmaf(q, z, z));
     value = z * s;
-    return s * fmaf(GELU_C * z * fmaf(3.0f, q, 1.0f), 1.0f - s, 1.0f);
+    return s * fmaf(bounded(GELU_C * z * fmaf(3.0f, q, 1.0f)), 1.0f - s, 1.0f);
   }
   if constexpr (ACT == LIK_ACT_TANH) {
     value = tanh_f<PRECISE>(z);
@@ -146,6 +148,11 @@ __device__ __forceinline__ Pair rcp_2(Pair p) {
   float a, b;
   p.get(a, b);
   return Pair(fast_rcp(a), fast_rcp(b));
+}
+__device__ __forceinline__ Pair bounded_2(Pair p) {
+  float a, b;
+  p.get(a, b);
+  return Pair(bounded(a), bounded(b));
 }
 __device__ __forceinline__ Pair sigmoid_2(Pair z) { return rcp_2(add2(exp2_2(mul2(z, both(-1.4426950408889634f))), both(1.0f))); }
 // the same on vectors of V elements (one by one where V is 1): v = v * a + b, v = v * a, v = v + a, s += v, s += v * a
@@ -223,7 +230,7 @@ __device__ __forceinline__ void act_pair(float& x, float& y, float& sx, float& s
     }
     mul2(z, s).get(x, y);
     if constexpr (SLOPE) {
-      const Pair w = ACT == LIK_ACT_SILU ? z : mul2(mul2(z, both(GELU_C)), fma2(q, both(3.0f), both(1.0f)));
+      const Pair w = ACT == LIK_ACT_SILU ? z : bounded_2(mul2(mul2(z, both(GELU_C)), fma2(q, both(3.0f), both(1.0f))));
       mul2(s, fma2(w, fma2(s, both(-1.0f), both(1.0f)), both(1.0f))).get(sx, sy);
     }
   } else if constexpr (ACT == LIK_ACT_GELU) {

@@ -1,4 +1,5 @@
-"""The layers in front of the document head where they can go wrong: operands that lie in memory in unlike ways, infinities.
+"""The layers in front of the document head where they can go wrong: operands that lie in memory in unlike ways, infinities and
+large values.
 
 Bounds as in test_gpu_token_layers: every rounding counted at its most."""
 
@@ -66,3 +67,25 @@ def test_activations_of_infinity(dt, m, k, n):
         h = gated_feed_forward(x, w, ones, down[:, :n], b_gate=bg, b_up=up, activation=act)
         if act not in ("tanh", "sigmoid") and dt != FP32:  # (an fp32 infinity gives NaN or infinities in the second product)
             assert not torch.isfinite(h).any() and not torch.isfinite(h[:, 0]).any()
+
+
+@pytest.mark.parametrize("dt", [BF16, FP32])
+@pytest.mark.parametrize("m", [3, 300, 9000])
+def test_slopes_of_large_values(dt, m):
+    """Far from zero a slope is 0 or 1, up to the largest finite value; at -50, the nearest, silu's is off by 49 exp(-50) = 9.5e-21."""
+    from late_interaction_kernels_b200.token_layers import gated_feed_forward, linear
+
+    n = 64
+    mags = torch.tensor([50.0, 1e4, 1e8, 1e12, 2e13, 1e16, 1e20, 1e30], device="cuda").repeat(n // 8)
+    z = (mags * torch.where(torch.rand(m, n, device="cuda") < 0.5, -1.0, 1.0)).to(dt)
+    dy = rand(m, n, dt=dt)
+    eye = torch.eye(n, device="cuda", dtype=dt)
+    one = torch.ones(n, device="cuda", dtype=dt)
+    for act in ACTS[1:]:
+        want = dy * (z > 0) if act not in ("tanh", "sigmoid") else torch.zeros_like(dy)
+        x = z.clone().requires_grad_()
+        (dx,) = torch.autograd.grad(linear(x, eye, activation=act), [x], dy)
+        assert ((dx - want).abs() <= 1e-20 * dy.abs()).all(), act
+        x = z.clone().requires_grad_()
+        (dx,) = torch.autograd.grad(gated_feed_forward(x, eye, torch.zeros_like(eye), eye, b_up=one, activation=act), [x], dy)
+        assert ((dx - want).abs() <= 1e-20 * dy.abs()).all(), act
