@@ -54,7 +54,8 @@ __device__ __forceinline__ float above0(float z) {
 }
 __device__ __forceinline__ float minus_abs(float z) { return fmaxf(-fabsf(z), -1e30f); }
 __device__ __forceinline__ float gelu_from(float z, float tail) { return fmaf(minus_abs(z), tail, z * above0(z)); }
-// A factor beside one that is exactly 0 once z is far from zero: from |z| of 1e13 on the polynomial in gelu_tanh's slope is infinite.  (The factor that may be 0 keeps a NaN.)
+// A factor beside one that is exactly 0 once z is far from zero: z itself, which a linear layer keeps in its type (infinite beyond fp16's 65504 although
+// the sum was finite), and the polynomial in gelu_tanh's slope, infinite from |z| of 1e13 on.  (The factor that may be 0 keeps a NaN.)
 __device__ __forceinline__ float bounded(float w) { return fminf(fmaxf(w, -1e30f), 1e30f); }
 constexpr float GELU_C = 1.5957691216057308f;  // 2 sqrt(2 / pi): (1 + tanh(y)) / 2 = sigmoid(2 y)
 
@@ -83,7 +84,7 @@ __device__ __forceinline__ float act_slope(float z, float& value) {
   if constexpr (ACT == LIK_ACT_SILU) {
     const float s = sigmoid_f<PRECISE>(z);
     value = z * s;
-    return s * fmaf(z, 1.0f - s, 1.0f);
+    return s * fmaf(bounded(z), 1.0f - s, 1.0f);
   }
   if constexpr (ACT == LIK_ACT_GELU) {
     float cdf, e;
@@ -96,7 +97,7 @@ __device__ __forceinline__ float act_slope(float z, float& value) {
       cdf = z < 0.0f ? tail : 1.0f - tail;
       value = gelu_from(z, tail);
     }
-    return fmaf(0.3989422804014327f * z, e, cdf);
+    return fmaf(0.3989422804014327f * bounded(z), e, cdf);
   }
   if constexpr (ACT == LIK_ACT_GELU_TANH) {
     const float q = 0.044715f * z * z, s = sigmoid_f<PRECISE>(GELU_C * fmaf(q, z, z));
@@ -230,7 +231,7 @@ __device__ __forceinline__ void act_pair(float& x, float& y, float& sx, float& s
     }
     mul2(z, s).get(x, y);
     if constexpr (SLOPE) {
-      const Pair w = ACT == LIK_ACT_SILU ? z : bounded_2(mul2(mul2(z, both(GELU_C)), fma2(q, both(3.0f), both(1.0f))));
+      const Pair w = bounded_2(ACT == LIK_ACT_SILU ? z : mul2(mul2(z, both(GELU_C)), fma2(q, both(3.0f), both(1.0f))));
       mul2(s, fma2(w, fma2(s, both(-1.0f), both(1.0f)), both(1.0f))).get(sx, sy);
     }
   } else if constexpr (ACT == LIK_ACT_GELU) {
@@ -245,7 +246,7 @@ __device__ __forceinline__ void act_pair(float& x, float& y, float& sx, float& s
       float a, b, c, d;
       tail.get(a, b);
       fma2(tail, both(-1.0f), both(1.0f)).get(c, d);
-      fma2(mul2(z, both(0.3989422804014327f)), e, Pair(x < 0.0f ? a : c, y < 0.0f ? b : d)).get(sx, sy);
+      fma2(mul2(bounded_2(z), both(0.3989422804014327f)), e, Pair(x < 0.0f ? a : c, y < 0.0f ? b : d)).get(sx, sy);
     }
     fma2(na, tail, mul2(z, Pair(above0(x), above0(y)))).get(x, y);  // (gelu_from)
   } else if constexpr (SLOPE) {

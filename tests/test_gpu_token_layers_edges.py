@@ -1,12 +1,12 @@
 """The layers in front of the document head where they can go wrong: operands that lie in memory in unlike ways, infinities and
-large values.
+values beyond the type.
 
 Bounds as in test_gpu_token_layers: every rounding counted at its most."""
 
 import pytest
 import torch
 
-from test_gpu_token_layers import ACTS, BF16, E, FP16, FP32, floor, near, rand, unit
+from test_gpu_token_layers import ACTS, BF16, E, FP16, FP32, floor, near, product, rand, unit
 
 pytestmark = pytest.mark.gpu
 
@@ -89,3 +89,26 @@ def test_slopes_of_large_values(dt, m):
         x = z.clone().requires_grad_()
         (dx,) = torch.autograd.grad(gated_feed_forward(x, eye, torch.zeros_like(eye), eye, b_up=one, activation=act), [x], dy)
         assert ((dx - want).abs() <= 1e-20 * dy.abs()).all(), act
+
+
+@pytest.mark.parametrize("dt", [FP16, BF16, FP32])
+@pytest.mark.parametrize("m, k, n", KERNELS)
+def test_slopes_where_what_is_kept_is_beyond_its_type(dt, m, k, n):
+    """z of +-131072 is finite in the sums and the result, +-infinity where it is kept in fp16; its slope is 0 or 1 all the same."""
+    from late_interaction_kernels_b200.token_layers import linear
+
+    x, w = rand(m, k, dt=dt, scale=0.1), rand(n, k, dt=dt, scale=0.1)
+    x[:, 0] = 256
+    w[:, 0] = torch.where(torch.rand(n, device="cuda") < 0.5, -512.0, 512.0).to(dt)
+    dy = rand(m, n, dt=dt, scale=2.0**-6)
+    b = torch.zeros(n, device="cuda", dtype=dt)
+    for act in ACTS[1:]:
+        leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+        y = linear(*leaves, activation=act)
+        dx, dw, db = torch.autograd.grad(y, leaves, dy)
+        open_ = (w[:, 0] > 0).double() if act not in ("tanh", "sigmoid") else torch.zeros(n, device="cuda", dtype=torch.float64)
+        assert torch.isfinite(y[:, w[:, 0] < 0]).all(), act
+        dz = dy.double() * open_
+        for got, (want, err), name in ((dx, product(dz, w.double().t()), "dx"), (dw, product(dz.t(), x.double().t()), "dw")):
+            near(got, want, err, f"{act} {name}")
+        near(db, dz.sum(0), 2 * m * E * dz.abs().sum(0), f"{act} db")
