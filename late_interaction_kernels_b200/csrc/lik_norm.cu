@@ -6,8 +6,8 @@
 // Everything is bound by memory: a row is read once into registers (a warp's or a block's), and all that is done to it
 // happens there, the variance as a second pass over the registers.  The backward keeps its columns' sums for dw and db in
 // registers from row to row; each block writes them once and a small kernel adds the blocks' sums in their order.  With 768 features
-// of 16 bits instruction issue was the bound (82 and 72 %) until two values went through an instruction: 65536 rows forward 34 us = 5.9 TB/s,
-// backward 52 us = 5.8 TB/s, 0.9 of what a copy reaches.
+// of 16 bits instruction issue was the bound (82 and 72 %) until two values went through an instruction: 65536 rows forward 35 us = 5.7 TB/s,
+// backward 52 us = 5.8 TB/s, 0.9 of what a copy reaches; rows of 768 in fp32 forward 64 us = 6.3 TB/s.
 #include "lik_layers.cuh"
 
 namespace lik {
@@ -28,32 +28,41 @@ struct NormParams {
 
 constexpr int NORM_THREADS = 256;
 
-// sums of two numbers over the threads of a row: a warp, or several, which meet at a barrier of their own
-template <int TPR>
-__device__ __forceinline__ float2 row_sum(float a, float b, float2 (&buf)[2][32], int& turn) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    a += __shfl_xor_sync(0xffffffffu, a, o);
-    b += __shfl_xor_sync(0xffffffffu, b, o);
-  }
-  if constexpr (TPR == 32) return make_float2(a, b);
-  else {
-  static_assert(NORM_THREADS / TPR <= 2, "a barrier per row");
+// Sums of one or two numbers over the threads of a row: a warp, or several, which meet at a barrier of their own.  Of two numbers the lower lanes go on
+// with the first and the upper ones with the second after the first exchange: five exchanges, or six with the way back, instead of ten.
+struct RowBuf {
+  float4 sum[2][2][NORM_THREADS / 128];  // [turn][which sum], a float per warp
+};
+template <int TPR, bool TWO>
+__device__ __forceinline__ float2 row_sum(float a, float b, RowBuf& buf, int& turn) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = threadIdx.x / TPR;
-  // two buffers in turn: nobody is more than one barrier ahead of who still reads
-  turn ^= 1;
-  if (lane == 0) buf[turn][warp] = make_float2(a, b);
-  if (TPR == NORM_THREADS) __syncthreads();
-  else if (group == 0) asm volatile("bar.sync 1, %0;" ::"n"(TPR) : "memory");  // (a number in a register would reserve all sixteen barriers)
-  else asm volatile("bar.sync 2, %0;" ::"n"(TPR) : "memory");
-  a = b = 0.0f;
-#pragma unroll
-  for (int w = 0; w < TPR / 32; ++w) {
-    const float2 f = buf[turn][group * (TPR / 32) + w];
-    a += f.x;
-    b += f.y;
+  if constexpr (TWO) {
+    const bool up = lane & 16;
+    a = (up ? b : a) + __shfl_xor_sync(0xffffffffu, up ? a : b, 16);
+  } else {
+    a += __shfl_xor_sync(0xffffffffu, a, 16);
   }
-  return make_float2(a, b);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+  if constexpr (TPR == 32) {
+    if constexpr (!TWO) return make_float2(a, 0.0f);
+    b = __shfl_xor_sync(0xffffffffu, a, 16);
+    return lane & 16 ? make_float2(b, a) : make_float2(a, b);
+  } else {
+    static_assert(NORM_THREADS / TPR <= 2, "a barrier per row");
+    // two buffers in turn: nobody is more than one barrier ahead of who still reads
+    turn ^= 1;
+    if (TWO ? lane % 16 == 0 : lane == 0) reinterpret_cast<float*>(buf.sum[turn][lane / 16])[warp] = a;
+    if (TPR == NORM_THREADS) __syncthreads();
+    else if (group == 0) asm volatile("bar.sync 1, %0;" ::"n"(TPR) : "memory");  // (a number in a register would reserve all sixteen barriers)
+    else asm volatile("bar.sync 2, %0;" ::"n"(TPR) : "memory");
+    auto add_up = [&](const float4* f) {
+      float s = 0.0f;
+#pragma unroll
+      for (int w = 0; w < TPR / 128; ++w) s = (((s + f[w].x) + f[w].y) + f[w].z) + f[w].w;
+      return s;
+    };
+    return make_float2(add_up(&buf.sum[turn][0][group * (TPR / 128)]), TWO ? add_up(&buf.sum[turn][1][group * (TPR / 128)]) : 0.0f);
   }
 }
 
@@ -80,9 +89,23 @@ struct RawVec<T, 1> {
   __device__ __forceinline__ void get(float (&f)[1]) const { f[0] = to_f32(e); }
 };
 
+// A row's statistics from the sums of the differences' squares and of the differences from its mean.  That mean is rounded - a step of a value far
+// from zero may be more than the row's deviation, and 1 / N is rounded too - but the differences are all but exact, so their own mean says by how
+// much it is off: a row of one value comes out as zeros, and one around 1e4 as exact as one around 0.  (What is within a rounding of the
+// deviation is itself the rounding of these sums, and is left alone.)
+struct NormStats {
+  float off, rstd;
+  __device__ __forceinline__ NormStats(float2 sums, float inv_n, float eps) : off(sums.y * inv_n) {
+    float var = fmaf(-off, off, sums.x * inv_n);
+    var = (var < 0.0f ? 0.0f : var) + eps;  // (a NaN stays one)
+    if (!(off * off > 1.4210854715202004e-14f * var)) off = 0.0f;
+    rstd = 1.0f / sqrtf(var);
+  }
+};
+
 template <typename T, typename P, int V, int NV, int TPR>
 __global__ void __launch_bounds__(NORM_THREADS) norm_fwd_kernel(const NormParams p) {
-  __shared__ float2 buf[2][32];
+  __shared__ RowBuf buf;
   after_the_kernel_in_front();
   int turn = 0;
   constexpr int PER_BLOCK = NORM_THREADS / TPR;
@@ -103,7 +126,7 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_fwd_kernel(const NormParams
   fetch(r);
   for (; r < p.rows; r += step) {
     float v[NV][V];
-    PairSum s, q;
+    PairSum s, t, q;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if ((i * TPR + lane) * V < p.width) {
@@ -111,17 +134,18 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_fwd_kernel(const NormParams
         s.add(v[i]);
       }
     fetch(r + step);
-    const float mean = row_sum<TPR>(s.sum(), 0.0f, buf, turn).x * inv_n;
+    const float mean = row_sum<TPR, false>(s.sum(), 0.0f, buf, turn).x * inv_n;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if ((i * TPR + lane) * V < p.width) {
         vec_add(v[i], -mean);
+        t.add(v[i]);
         q.dot(v[i], v[i]);
       }
-    const float rstd = 1.0f / sqrtf(row_sum<TPR>(q.sum(), 0.0f, buf, turn).x * inv_n + p.eps);
+    const NormStats st(row_sum<TPR, true>(q.sum(), t.sum(), buf, turn), inv_n, p.eps);
     if (lane == 0 && p.mean) {
-      p.mean[r] = mean;
-      p.rstd[r] = rstd;
+      p.mean[r] = mean + st.off;
+      p.rstd[r] = st.rstd;
     }
     T* y = (T*)p.y + r * p.width;
 #pragma unroll
@@ -129,7 +153,7 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_fwd_kernel(const NormParams
       const int c = (i * TPR + lane) * V;
       if (c < p.width) {
         float w[V], b[V];
-        vec_mul(v[i], rstd);
+        vec_fma(v[i], st.rstd, -st.off * st.rstd);
         if (p.w) {
           load_vec<P, V>((const P*)p.w + c, w);
           if (p.b) {
@@ -155,7 +179,7 @@ __host__ __device__ constexpr int norm_bwd_threads(int tpr) { return tpr == 32 ?
 // sums in fp32 would leave an SM one block.
 template <typename T, typename P, int V, int NV, int TPR, bool PARAMS>
 __global__ void __launch_bounds__(norm_bwd_threads(TPR), TPR == 32 ? 3 : (NV * V <= 24 ? 2 : 1)) norm_bwd_kernel(const NormParams p) {
-  __shared__ float2 buf[2][32];
+  __shared__ RowBuf buf;
   after_the_kernel_in_front();
   int turn = 0;
   constexpr int THREADS = norm_bwd_threads(TPR), PER_BLOCK = THREADS / TPR;
@@ -219,7 +243,7 @@ __global__ void __launch_bounds__(norm_bwd_threads(TPR), TPR == 32 ? 3 : (NV * V
       }
     }
     if (p.dx) {
-      const float2 sums = row_sum<TPR>(sg.sum(), sgh.sum(), buf, turn);
+      const float2 sums = row_sum<TPR, true>(sg.sum(), sgh.sum(), buf, turn);
       // rstd (g - c1 - h c2), h = (x - mean) rstd
       const float c1 = -sums.x * inv_n, c2 = -sums.y * inv_n * s;
       T* dx = (T*)p.dx + r * p.width;
@@ -283,29 +307,30 @@ __global__ void __launch_bounds__(norm_bwd_threads(TPR), TPR == 32 ? 3 : (NV * V
 // Rows that no block holds in registers: a block goes through its row three times, the later ones out of L2.
 template <typename T, typename P>
 __global__ void __launch_bounds__(NORM_THREADS) norm_fwd_wide_kernel(const NormParams p) {
-  __shared__ float2 buf[2][32];
+  __shared__ RowBuf buf;
   after_the_kernel_in_front();
   int turn = 0;
   const float inv_n = 1.0f / (float)p.width;
   for (long long r = blockIdx.x; r < p.rows; r += gridDim.x) {
     const T* x = (const T*)p.x + r * p.x_stride;
-    float s = 0.0f, q = 0.0f;
+    float s = 0.0f, t = 0.0f, q = 0.0f;
     for (int c = threadIdx.x; c < p.width; c += NORM_THREADS) s += to_f32(x[c]);
-    const float mean = row_sum<NORM_THREADS>(s, 0.0f, buf, turn).x * inv_n;
+    const float mean = row_sum<NORM_THREADS, false>(s, 0.0f, buf, turn).x * inv_n;
     for (int c = threadIdx.x; c < p.width; c += NORM_THREADS) {
       const float d = to_f32(x[c]) - mean;
+      t += d;
       q = fmaf(d, d, q);
     }
-    const float rstd = 1.0f / sqrtf(row_sum<NORM_THREADS>(q, 0.0f, buf, turn).x * inv_n + p.eps);
-    if (threadIdx.x == 0 && p.mean) p.mean[r] = mean, p.rstd[r] = rstd;
+    const NormStats st(row_sum<NORM_THREADS, true>(q, t, buf, turn), inv_n, p.eps);
+    if (threadIdx.x == 0 && p.mean) p.mean[r] = mean + st.off, p.rstd[r] = st.rstd;
     for (int c = threadIdx.x; c < p.width; c += NORM_THREADS)
       ((T*)p.y)[r * p.width + c] =
-          from_f32<T>(fmaf((to_f32(x[c]) - mean) * rstd, p.w ? to_f32(((const P*)p.w)[c]) : 1.0f, p.b ? to_f32(((const P*)p.b)[c]) : 0.0f));
+          from_f32<T>(fmaf((to_f32(x[c]) - mean - st.off) * st.rstd, p.w ? to_f32(((const P*)p.w)[c]) : 1.0f, p.b ? to_f32(((const P*)p.b)[c]) : 0.0f));
   }
 }
 template <typename T, typename P>
 __global__ void __launch_bounds__(NORM_THREADS) norm_dx_wide_kernel(const NormParams p) {
-  __shared__ float2 buf[2][32];
+  __shared__ RowBuf buf;
   after_the_kernel_in_front();
   int turn = 0;
   const float inv_n = 1.0f / (float)p.width;
@@ -318,7 +343,7 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_dx_wide_kernel(const NormPa
       s += g;
       t = fmaf(g, (to_f32(x[c]) - mean) * rstd, t);
     }
-    const float2 m = row_sum<NORM_THREADS>(s, t, buf, turn);
+    const float2 m = row_sum<NORM_THREADS, true>(s, t, buf, turn);
     const float c1 = m.x * inv_n, c2 = m.y * inv_n;
     for (int c = threadIdx.x; c < p.width; c += NORM_THREADS) {
       const float g = to_f32(dy[c]) * (p.w ? to_f32(((const P*)p.w)[c]) : 1.0f);
@@ -346,9 +371,9 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_dparam_wide_kernel(const No
 constexpr int NORM_WIDE_PARTS = 64;
 
 // Which kernel a width goes to: a warp per row, four warps or the block's eight; vectors of 16 bytes where rows and parameters are aligned, else
-// single elements (9001 x 1023 fp32, forward and backward: 22 and 23 us by a block per row, 34 and 58 by a warp with 32 elements per lane).  The
-// forward keeps a row with a warp up to four vectors per lane, the backward, which holds a row twice and its columns' sums, up to three:
-// 65536 x 768 bf16 52 us, 102 with four warps per row, of which the fourth has nothing; 16384 x 1024 36 us with a warp per row, 24 with four.
+// single elements (9001 x 1023 fp32: forward 16 us by four warps per row, 20 by a block; backward 23 by a block, 58 by a warp with 32 elements per lane).  The
+// forward keeps a row with a warp up to 1024 features (65536 x 768 fp32: 64 us; 110 by a block per row, of which each warp adds the row's sums up
+// for itself), the backward, which holds a row twice and its columns' sums, up to three vectors per lane: 65536 x 768 bf16 52 us, 102 with four warps per row, of which the fourth has nothing; 16384 x 1024 36 us with a warp per row, 24 with four.
 struct NormPlan {
   bool wide, vec;
   int nv, tpr;
@@ -360,12 +385,13 @@ NormPlan norm_plan(const lik_norm_args& a, bool bwd) {
            vec_ok(a.dx, a.width, a.width, item) && ((uintptr_t)a.weight & 15) == 0 && ((uintptr_t)a.bias & 15) == 0;
   const long long vecs = ceil_div(a.width, pl.vec ? v : 1);
   if (pl.vec) {
-    pl.tpr = vecs <= (bwd ? 96 : 128) ? 32 : (vecs <= 128 ? 128 : 256);
+    pl.tpr = vecs <= (bwd ? 96 : 1024 / v) ? 32 : (vecs <= 128 ? 128 : 256);
     pl.nv = (int)ceil_div(vecs, pl.tpr);
     if (pl.tpr == 256 && pl.nv == 3) pl.nv = 4;
-    pl.wide = pl.nv > 4;
+    if (pl.tpr == 32 && pl.nv > 4) pl.nv = (pl.nv + 1) / 2 * 2;
+    pl.wide = pl.tpr == 256 && pl.nv > 4;
   } else {
-    pl.tpr = vecs <= 256 ? 32 : 256;
+    pl.tpr = vecs <= 256 ? 32 : (!bwd && vecs <= 1024 ? 128 : 256);
     const long long need = ceil_div(vecs, pl.tpr);
     pl.nv = need == 1 && pl.tpr == 32 ? 1 : (need <= 4 ? 4 : (need <= 8 ? 8 : 16));
     pl.wide = need > 16;
@@ -381,8 +407,8 @@ int norm_bwd_blocks(const lik_norm_args& a, const NormPlan& pl) {
 template <typename T, typename P, int V, int NV, int TPR>
 int run_norm(const NormParams& p, bool bwd, bool params, int blocks, cudaStream_t st) {
   if (!bwd) {
-    if constexpr (TPR != 128) return launch_after(norm_fwd_kernel<T, P, V, NV, TPR>, blocks, NORM_THREADS, 0, st, 1, p);
-  } else if constexpr (V == 1 || TPR != 32 || NV <= 3) {
+    if constexpr (V == 1 || (TPR != 128 && (TPR != 32 || NV * V <= 32))) return launch_after(norm_fwd_kernel<T, P, V, NV, TPR>, blocks, NORM_THREADS, 0, st, 1, p);
+  } else if constexpr (V == 1 ? TPR != 128 : TPR != 32 || NV <= 3) {
     const size_t smem = TPR < NORM_THREADS ? sizeof(float) * 2 * NV * TPR * V : 0;
     return params ? launch_after(norm_bwd_kernel<T, P, V, NV, TPR, true>, blocks, norm_bwd_threads(TPR), smem, st, 1, p)
                   : launch_after(norm_bwd_kernel<T, P, V, NV, TPR, false>, blocks, norm_bwd_threads(TPR), 0, st, 1, p);
@@ -404,6 +430,8 @@ int run_norm(const NormPlan& pl, const NormParams& p, bool bwd, bool params, int
   LIK_NORM_CASE(V, 2, 32);
   LIK_NORM_CASE(V, 3, 32);
   LIK_NORM_CASE(V, 4, 32);
+  LIK_NORM_CASE(V, 6, 32);
+  LIK_NORM_CASE(V, 8, 32);
   LIK_NORM_CASE(V, 1, 128);
   LIK_NORM_CASE(V, 1, 256);
   LIK_NORM_CASE(V, 2, 256);
@@ -411,6 +439,8 @@ int run_norm(const NormPlan& pl, const NormParams& p, bool bwd, bool params, int
   LIK_NORM_CASE(1, 1, 32);
   LIK_NORM_CASE(1, 4, 32);
   LIK_NORM_CASE(1, 8, 32);
+  LIK_NORM_CASE(1, 4, 128);
+  LIK_NORM_CASE(1, 8, 128);
   LIK_NORM_CASE(1, 4, 256);
   LIK_NORM_CASE(1, 8, 256);
   LIK_NORM_CASE(1, 16, 256);

@@ -1,5 +1,5 @@
 """The layers in front of the document head where they can go wrong: operands that lie in memory in unlike ways, infinities and
-values beyond the type.
+values beyond the type, rows far from zero.
 
 Bounds as in test_gpu_token_layers: every rounding counted at its most."""
 
@@ -112,3 +112,45 @@ def test_slopes_where_what_is_kept_is_beyond_its_type(dt, m, k, n):
         for got, (want, err), name in ((dx, product(dz, w.double().t()), "dx"), (dw, product(dz.t(), x.double().t()), "dw")):
             near(got, want, err, f"{act} {name}")
         near(db, dz.sum(0), 2 * m * E * dz.abs().sum(0), f"{act} db")
+
+
+# ----------------------------------------------------------------------------- rows far from zero
+FAR_WIDTHS = [7, 100, 300, 768, 1000, 1001, 1023, 1500, 3000, 5000, 9001, 16385, 20000]
+
+
+@pytest.mark.parametrize("dt", [BF16, FP16, FP32])
+@pytest.mark.parametrize("width", FAR_WIDTHS)
+def test_layer_norm_of_constant_rows(dt, width):
+    """A row of one value is its own mean: what is left is zero, whatever the width's reciprocal and the sum of the row round to."""
+    from late_interaction_kernels_b200.token_layers import layer_norm
+
+    values = torch.tensor([3.25, 7.0, 0.1, 100.0, 1000.0, 1001.0, -999.0, 0.0], device="cuda").to(dt)
+    x = values[:, None].expand(8, width).contiguous().requires_grad_()
+    y = layer_norm(x)
+    # the mean is off by a rounding of its sum's steps, what corrects it by as much of that again
+    steps = min(width, 64) + 16
+    bound = (2 * steps * E) ** 2 * values.double().abs()[:, None] * 1e-5**-0.5
+    near(y.detach(), torch.zeros(8, width, dtype=torch.float64, device="cuda"), bound.expand(8, width), "y")
+    dy = rand(8, width, dt=dt)
+    (dx,) = torch.autograd.grad(y, [x], dy)
+    d = dy.double()
+    # the mean that is kept is the value itself, or its nearest neighbour: h is at most a step of the value over the deviation
+    h = 2 * E * values.double().abs()[:, None] * 1e-5**-0.5
+    s = d.abs().mean(1, keepdim=True)
+    near(dx, 1e-5**-0.5 * (d - d.mean(1, keepdim=True)), 1e-5**-0.5 * (8 * steps * E * (d.abs() + s) + h * h * s + 2 * h * h * (d.abs() + s)), "dx")
+
+
+@pytest.mark.parametrize("width", FAR_WIDTHS)
+def test_layer_norm_far_from_zero(width):
+    """fp32 rows whose mean is ten thousand times their deviation: the result is as near to 64 bits as that of rows around zero."""
+    from late_interaction_kernels_b200.token_layers import layer_norm
+
+    for shift in (1e4, -3e4):
+        x = rand(9, width, dt=FP32, shift=shift)
+        v = x.double()
+        mean, var = v.mean(1, keepdim=True), v.var(1, correction=0, keepdim=True)
+        hat = (v - mean) / (var + 1e-5).sqrt()
+        steps = min(width, 64) + 16
+        # differences from the rounded mean are exact to a rounding; their mean and that of their squares are sums of `steps`
+        off = steps * E * (abs(shift) * E * steps / var.sqrt() + hat.abs().mean(1, keepdim=True))
+        near(layer_norm(x), hat, off + hat.abs() * (2 * steps + 8) * E + 4 * E, "y")
