@@ -245,25 +245,26 @@ __global__ void __launch_bounds__(256) sum_splits_kernel(const __grid_constant__
 template <typename T>
 __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ SumJob j, const __grid_constant__ GemmDesc d) {
   after_the_kernel_in_front();
-  const int per_row = (j.n + 3) / 4;
+  const int per_row = (j.n + 3) / 4, lane = threadIdx.x & 31;
   with_activation_dev(d.act, [&](auto act) {
-    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < j.end; i += gridDim.x * 256ll) {
-      const long long r = i / per_row;
+    for (long long first = blockIdx.x * 256ll + threadIdx.x - lane; first < j.end; first += gridDim.x * 256ll) {  // (whole warps)
+      const long long i = first + lane < j.end ? first + lane : j.end - 1, r = i / per_row;
       const int c = (int)(i - r * per_row) * 4;
       const float4 v = sum_shares(j, r, c);
       const float f[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (c + k < j.n) {
-          bool above = true;
-          if constexpr (decltype(act)::value == LIK_ACT_RELU) {
-            const float z = d.bias[0] ? f[k] + to_f32(((const T*)d.bias[0])[c + k]) : f[k];
-            above = z > 0.0f;
-            if (sizeof(T) == 2 && d.kept[0] && fabsf(z) < kink_bound(fmaxf(fmaxf(fabsf(f[0]), fabsf(f[1])), fmaxf(fabsf(f[2]), fabsf(f[3]))), d.k[0]))
-              above = above_zero<T>(d, r, c + k);
+      for (int k = 0; k < 4; ++k) {
+        const bool there = first + lane < j.end && c + k < j.n;
+        bool above = true;
+        if constexpr (decltype(act)::value == LIK_ACT_RELU) {
+          const float z = there && d.bias[0] ? f[k] + to_f32(((const T*)d.bias[0])[c + k]) : f[k];
+          above = z > 0.0f;
+          if constexpr (sizeof(T) == 2) {
+            if (d.norm_a) above = above_zero<T>(d, r, there ? c + k : 0, z, there, lane);
           }
-          gemm_element<T, T, GEMM_LINEAR, decltype(act)::value>(d, r, c + k, f[k], 0.0f, above);
         }
+        if (there) gemm_element<T, T, GEMM_LINEAR, decltype(act)::value>(d, r, c + k, f[k], 0.0f, above);
+      }
     }
   });
 }

@@ -2,7 +2,7 @@
 //
 // What there is to do is to read b once, so the work is cut for loads in flight: a block of eight warps owns 16 rows of b (MMA) or four
 // (multiply-add), each warp an eighth of k, and the warps' sums meet in shared memory in a fixed order.  The rows of a come out of L1
-// and L2.  One launch, no workspace.
+// and L2.  One launch.
 //   16-bit, rows of whole 16-byte pieces: mma.sync, b's rows as its 16 rows and up to 32 rows of a as its columns, eight at a time.  A sum
 //     may be taken in any order of k, so a lane's fragments are 16 consecutive bytes of either operand as they lie in memory: no shared memory
 //     and no shuffles before the end.  (tcgen05 would take its operands by way of shared memory, in tiles of 128 rows of b, of which
@@ -107,11 +107,7 @@ __global__ void __launch_bounds__(32 * WARPS) few_mma_kernel(const __grid_consta
       bool above = true;
       if constexpr (decltype(act)::value == LIK_ACT_RELU) {  // (whole warps come here)
         const float z = there && d.bias[0] ? v[0] + to_f32(((const T*)d.bias[0])[n0 + r]) : v[0];
-        float largest = fabsf(z);
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
-        above = z > 0.0f;
-        if (there && d.kept[0] && fabsf(z) < kink_bound(largest, d.k[0])) above = above_zero<T>(d, m, n0 + r);
+        above = d.norm_a ? above_zero<T>(d, there ? m : 0, there ? n0 + r : 0, z, there, lane) : z > 0.0f;
       }
       if (there) gemm_element<T, T, KIND, decltype(act)::value>(d, m, n0 + r, v[0], v[1], above);
     }
@@ -173,18 +169,23 @@ __global__ void __launch_bounds__(FEW_THREADS) few_fma_kernel(const __grid_const
   __syncthreads();
   if (warp == 0) {
     const int m = m0 + lane / FMA_ROWS, r = lane % FMA_ROWS, at = r * FMA_COLS + lane / FMA_ROWS;
-    if (m < d.m && n0 + r < d.n) {
-      float v[2] = {0.0f, 0.0f};
+    const bool there = m < d.m && n0 + r < d.n;
+    float v[2] = {0.0f, 0.0f};
 #pragma unroll
-      for (int q = 0; q < DUAL; ++q)
+    for (int q = 0; q < DUAL; ++q)
 #pragma unroll
-        for (int w = 0; w < FEW_WARPS; ++w) v[q] += part[q][w][at];
-      with_activation_dev(d.act, [&](auto act) {
-        // (sums of fp32 multiply-adds, rounded: relu's argument has the sign that they have)
-        const float z = d.bias[0] ? v[0] + to_f32(((const T*)d.bias[0])[n0 + r]) : v[0];
-        gemm_element<T, T, KIND, decltype(act)::value>(d, m, n0 + r, v[0], v[1], z > 0.0f);
-      });
-    }
+      for (int w = 0; w < FEW_WARPS; ++w) v[q] += part[q][w][at];
+    with_activation_dev(d.act, [&](auto act) {
+      bool above = true;
+      if constexpr (decltype(act)::value == LIK_ACT_RELU) {
+        const float z = there && d.bias[0] ? v[0] + to_f32(((const T*)d.bias[0])[n0 + r]) : v[0];
+        above = z > 0.0f;
+        if constexpr (sizeof(T) == 2) {
+          if (d.norm_a) above = above_zero<T>(d, there ? m : 0, there ? n0 + r : 0, z, there, lane);
+        }
+      }
+      if (there) gemm_element<T, T, KIND, decltype(act)::value>(d, m, n0 + r, v[0], v[1], above);
+    });
   }
 }
 

@@ -41,8 +41,9 @@ struct GtParams {
   void *out2, *kept[2];  // kept: written, or read by GEMM_GATED_BWD
   long long residual_stride, kept_stride;
   bool bias_vec, residual_vec, keep;  // *_vec: rows of whole 16-byte pieces
-  const void *a, *b;                  // the operands of z as the caller has them, k contiguous
+  const void *a, *b;                  // the operands of z as the caller has them, k contiguous, and their rows' lengths
   long long a_stride, b_stride, k;
+  const float *norm_a, *norm_b;
   int* status;
 };
 struct GtCtl {
@@ -125,23 +126,23 @@ __device__ __forceinline__ bool gt_chunk(const GtParams& p, int u, int c, int ra
 // Which of 16 z, columns of the lane's row, are above 0 (bit i: column col + i): those near relu's kink are taken by the warp's lanes together.
 template <typename T>
 __device__ __forceinline__ uint32_t above_kink(const GtParams& p, int row0, int col, int lane, const float (&v)[16]) {
-  float largest = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) largest = fmaxf(largest, fabsf(v[i]));
-  const float bound = kink_bound(largest, p.k);
   uint32_t above = 0, unsure = 0;
+  const float norm = row0 + lane < p.q[0].m ? __ldg(p.norm_a + row0 + lane) : 0.0f;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    above |= (v[i] > 0.0f ? 1u : 0u) << i;
-    unsure |= (fabsf(v[i]) < bound && row0 + lane < p.q[0].m && col + i < p.q[0].n ? 1u : 0u) << i;
+  for (int i = 0; i < 16; i += 4) {  // (there is room for whole vectors behind the lengths)
+    const float4 n = __ldg(reinterpret_cast<const float4*>(p.norm_b + col + i));
+    const float ns[4] = {n.x, n.y, n.z, n.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      above |= (v[i + j] > 0.0f ? 1u : 0u) << (i + j);
+      unsure |= (fabsf(v[i + j]) < kink_bound(norm, ns[j], p.k) && col + i + j < p.q[0].n ? 1u : 0u) << (i + j);
+    }
   }
   for (uint32_t lanes = __ballot_sync(0xffffffffu, unsure != 0); lanes; lanes &= lanes - 1) {
     const int l = __ffs(lanes) - 1;
     for (uint32_t cols = __shfl_sync(0xffffffffu, unsure, l); cols; cols &= cols - 1) {
       const int c = __ffs(cols) - 1;
-      double z = exact_part((const T*)p.a + (row0 + l) * p.a_stride, (const T*)p.b + (col + c) * p.b_stride, p.k, lane, 32);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+      double z = exact_sum((const T*)p.a + (row0 + l) * p.a_stride, (const T*)p.b + (col + c) * p.b_stride, p.k, lane);
       if (p.bias[0]) z += (double)to_f32(((const T*)p.bias[0])[col + c]);
       if (lane == l) above = z > 0.0 ? above | 1u << c : above & ~(1u << c);
     }
@@ -553,6 +554,8 @@ int launch_gemm_tc(const GemmDesc* d, int n, void* ws, size_t ws_bytes, int* sta
   p.a_stride = d->a[0].row;
   p.b_stride = d->b[0].row;
   p.k = d->k[0];
+  p.norm_a = d->norm_a;
+  p.norm_b = d->norm_b;
   p.kept_stride = d->kept_stride;
   p.residual = d->residual;
   p.residual_stride = d->residual_stride;

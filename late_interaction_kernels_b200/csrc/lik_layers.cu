@@ -153,6 +153,57 @@ int launch_slope(SlopeParams& p, int act, int dtype, bool sums, cudaStream_t st)
   return launch_sum_parts(p.partial, parts, p.outs, dtype, st);
 }
 
+// ---------------------------------------------------------------------------------------------
+// Lengths of the rows of two matrices (kink_bound), a warp per row.  Bound by memory: each element read once.
+// ---------------------------------------------------------------------------------------------
+struct KinkNorms {
+  const void* p[2];
+  long long stride[2], rows[2];
+  long long k;
+  float* norm[2];
+};
+template <typename T>
+__global__ void __launch_bounds__(256) kink_norms_kernel(const __grid_constant__ KinkNorms p) {
+  after_the_kernel_in_front();
+  const int lane = threadIdx.x & 31;
+  for (long long g = blockIdx.x * 8ll + threadIdx.x / 32; g < p.rows[0] + p.rows[1]; g += gridDim.x * 8ll) {
+    const int q = g < p.rows[0] ? 0 : 1;
+    const long long r = q ? g - p.rows[0] : g;
+    const T* x = (const T*)p.p[q] + r * p.stride[q];
+    float s = 0.0f, largest = 0.0f;
+    auto take = [&](float v) {
+      s = fmaf(v, v, s);
+      largest = fmaxf(largest, fabsf(v));
+    };
+    long long done = 0;
+    if (((uintptr_t)x & 15) == 0) {
+      done = p.k & ~7ll;
+#pragma unroll 4
+      for (long long i = lane * 8; i < done; i += 256) {
+        float v[8];
+        load_vec<T, 8>(x + i, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) take(v[j]);
+      }
+    }
+#pragma unroll 8
+    for (long long i = done + lane; i < p.k; i += 32) take(to_f32(x[i]));
+    s = warp_sum(s);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+    // (where squares would leave fp32's range: the bound by the largest; a NaN is no bound, and its row's sums have no sign)
+    if (lane == 0) p.norm[q][r] = largest < 1e-15f || largest > 1e15f ? (s != s ? s : largest * sqrtf((float)p.k)) : sqrtf(s);
+  }
+}
+bool keeps_side(const GemmDesc& d) { return d.dtype != LIK_F32 && d.act == LIK_ACT_RELU && d.kept[0]; }
+int launch_kink_norms(const GemmDesc& d, cudaStream_t st) {
+  if (!d.norm_a) return LIK_OK;
+  const KinkNorms p{{d.a[0].p, d.b[0].p}, {d.a[0].row, d.b[0].row}, {d.m, d.n}, d.k[0], {(float*)d.norm_a, (float*)d.norm_b}};
+  const long long need = ceil_div(d.m + d.n, 8), most = 16ll * sm_count();
+  const unsigned grid = (unsigned)(need < most ? need : most);
+  return d.dtype == LIK_F16 ? launch_after(kink_norms_kernel<__half>, grid, 256, 0, st, 1, p) : launch_after(kink_norms_kernel<__nv_bfloat16>, grid, 256, 0, st, 1, p);
+}
+
 // Which kernel a product goes to.  Several products of a pass are plain ones and go to the tensor cores together.
 size_t gemm_workspace(const GemmDesc* d, int n = 1) {
   if (n == 0 || (n == 1 && gemm_few_pays(*d))) return 0;
@@ -186,6 +237,13 @@ struct Carve {
   }
 };
 
+// room for the lengths of the rows that a kept side of relu asks for
+void take_norms(GemmDesc& d, Carve& c) {
+  if (!keeps_side(d)) return;
+  d.norm_a = c.take<float>((size_t)d.m * sizeof(float));
+  d.norm_b = c.take<float>((size_t)d.n * sizeof(float));
+}
+
 // units of the products are counted in 32 bits, shares of k included
 bool tiles_fit(long long m, long long n) { return ceil_div(m, 128) * ceil_div(n, 64) < (1ll << 30); }
 
@@ -217,6 +275,20 @@ GemmDesc linear_fwd_desc(const lik_linear_args& a) {
   d.kept[0] = a.activation == LIK_ACT_NONE ? nullptr : a.z;
   d.kept_stride = a.z_stride;
   return d;
+}
+struct LinearFwd {
+  GemmDesc d;
+  void* gemm;
+  size_t gemm_bytes, total;
+};
+LinearFwd linear_fwd_layout(const lik_linear_args& a, void* ws) {
+  LinearFwd l{linear_fwd_desc(a)};
+  Carve c(ws);
+  take_norms(l.d, c);
+  l.gemm_bytes = gemm_workspace(&l.d);
+  l.gemm = c.take(l.gemm_bytes);
+  l.total = c.off;
+  return l;
 }
 // dx = dz w and dw = dz^T x
 GemmDesc grad_x_desc(int dtype, long long rows, int out, int in, const void* dz, long long dz_stride, const void* w, long long w_stride, void* dx) {
@@ -325,6 +397,7 @@ GatedFwd gated_fwd_layout(const lik_gated_args& a, void* ws) {
   u.kept[0] = a.gate_factor;
   u.kept[1] = a.up_factor;
   u.kept_stride = a.kept_stride;
+  take_norms(u, c);
   GemmDesc& d = l.down;
   d.dtype = d.out_dtype = a.dtype;
   d.m = a.rows;
@@ -413,8 +486,7 @@ int launch_sum_parts(const float* partial, int parts, const SumOuts& outs, int d
 extern "C" size_t lik_linear_fwd_workspace(const lik_linear_args* a) {
   using namespace lik;
   if (check_linear(a) || a->rows == 0) return 0;
-  const GemmDesc d = linear_fwd_desc(*a);
-  return gemm_workspace(&d);
+  return linear_fwd_layout(*a, nullptr).total;
 }
 extern "C" int lik_linear_fwd(const lik_linear_args* args, lik_stream_t stream) {
   using namespace lik;
@@ -424,9 +496,10 @@ extern "C" int lik_linear_fwd(const lik_linear_args* args, lik_stream_t stream) 
   LIK_REQUIRE(a.x && a.w && a.y, "x, w and y must not be NULL");
   LIK_REQUIRE(!a.z || (a.z_stride >= a.out && a.z_stride * dtype_size(a.dtype) % 16 == 0 && ((uintptr_t)a.z & 15) == 0), "z must have 16-byte rows");
   LIK_REQUIRE(!a.residual || a.residual_stride >= a.out, "residual_stride must be at least out");
-  const GemmDesc d = linear_fwd_desc(a);
-  if (a.workspace_bytes < gemm_workspace(&d)) return too_small("lik_linear_fwd");
-  return launch_gemm(&d, 1, a.workspace, a.workspace_bytes, a.status, (cudaStream_t)stream);
+  const LinearFwd l = linear_fwd_layout(a, a.workspace);
+  if (a.workspace_bytes < l.total || (l.total && !a.workspace)) return too_small("lik_linear_fwd");
+  if (int rc = launch_kink_norms(l.d, (cudaStream_t)stream)) return rc;
+  return launch_gemm(&l.d, 1, l.gemm, l.gemm_bytes, a.status, (cudaStream_t)stream);
 }
 
 extern "C" size_t lik_linear_bwd_workspace(const lik_linear_args* a) {
@@ -481,6 +554,7 @@ extern "C" int lik_gated_fwd(const lik_gated_args* args, lik_stream_t stream) {
   LIK_REQUIRE(!a.residual || a.residual_stride >= a.out, "residual_stride must be at least out");
   const GatedFwd l = gated_fwd_layout(a, a.workspace);
   if (a.workspace_bytes < l.total || (l.total && !a.workspace)) return too_small("lik_gated_fwd");
+  if (int rc = launch_kink_norms(l.up, (cudaStream_t)stream)) return rc;
   if (int rc = launch_gemm(&l.up, 1, l.gemm, l.gemm_bytes, a.status, (cudaStream_t)stream)) return rc;
   return launch_gemm(&l.down, 1, l.gemm, l.gemm_bytes, a.status, (cudaStream_t)stream);
 }

@@ -401,24 +401,82 @@ struct GemmDesc {
   int out_dtype = 0;                   // dtype, or LIK_F32 for products without anything else to them
   void* kept[2] = {nullptr, nullptr};  // the factors of the backward: written, or read by GEMM_GATED_BWD; rows of 16 bytes
   long long kept_stride = 0;
+  const float *norm_a = nullptr, *norm_b = nullptr;  // of a's rows and of (the gate's) b's, where relu's side is kept from 16-bit operands
 };
-// The kink of relu.  Its slope goes by the sign of z, and the tensor core's sums, which are cut off at every 16 products, have a wrong sign for a z
-// within some 1e-6 of its neighbours: a few in a million, each a whole gradient off.  So where z is that much smaller than the largest of
-// its 16 neighbours and a backward pass will look at its sign, it is taken again from the operands, in 64 bits.
-__device__ __forceinline__ float kink_bound(float largest, long long k) { return largest * (1e-5f + 1e-8f * (float)k); }
-// products of 16-bit values are exact in fp32
+// The kink of relu.  Its slope goes by the sign of z, and the tensor core's sums, which cut off what they shift out at every 16 products, have a wrong
+// sign for a z that is next to nothing beside what it is a sum of: a few in a million, each a whole gradient off.  An addition of 16 products loses
+// up to four steps (2^-23; 1.6 on average) of the largest number in it.  Partial sums of a z near 0 are at most half of |a| |b|, the product of
+// the rows' lengths: what comes first is bounded by the lengths of its parts, and so is what comes after and cancels it.  So where z is within
+// kink_bound and a backward pass will look at its sign, it is taken again from the operands, in 64 bits, by a warp.  The lengths come from a
+// pass over the operands (kink_norms): nothing at hand says as much about a sum that came out small.  (The largest of z's neighbours, asked before, is
+// small too where a whole row cancels, and beside a feature that is switched off or dead it made every z look small: 65536 x 768 x 768 went from 105
+// us to 4 100 with one feature at -1e9 and to 5 400 with a tenth of the features dead; a zero row has length 0 and z of it is sure.)
+// A z that is 0 because the operands have no nonzero place in common is taken again like any other.
+__device__ __forceinline__ float kink_bound(float norm_a, float norm_b, long long k) { return norm_a * (2.384185791015625e-7f * (float)(k / 16 + 2)) * norm_b; }
+// sum over k of a b by a warp, in all lanes; products of 16-bit values are exact in fp32.  (Not inline: it is rarely called, and its loads, all
+// of 1024 k at once, would take the registers of the epilogue around it.)
 template <typename T>
-__device__ __forceinline__ double exact_part(const T* a, const T* b, long long k, long long first, long long step) {
-  double s = 0.0;
-#pragma unroll 16
-  for (long long i = first; i < k; i += step) s += (double)(to_f32(a[i]) * to_f32(b[i]));
-  return s;
+__device__ __noinline__ double exact_sum(const T* a, const T* b, long long k, int lane) {
+  double s[2] = {0.0, 0.0};
+  long long done = 0;
+  if ((((uintptr_t)a | (uintptr_t)b) & 15) == 0) {
+    done = k & ~7ll;
+#pragma unroll 1
+    for (long long first = 0; first < done; first += 1024) {
+      uint4 u[4], w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const long long i = first + j * 256 + lane * 8;
+        const bool there = i < done;
+        u[j] = there ? *reinterpret_cast<const uint4*>(a + i) : make_uint4(0u, 0u, 0u, 0u);
+        w[j] = there ? *reinterpret_cast<const uint4*>(b + i) : make_uint4(0u, 0u, 0u, 0u);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t x[4] = {u[j].x, u[j].y, u[j].z, u[j].w}, y[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float xl, xh, yl, yh;
+          unpack2(x[e], xl, xh, T());
+          unpack2(y[e], yl, yh, T());
+          s[0] += (double)(xl * yl);
+          s[1] += (double)(xh * yh);
+        }
+      }
+    }
+  }
+#pragma unroll 1
+  for (long long first = done; first < k; first += 512) {
+    T x[16], y[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const long long i = first + j * 32 + lane;
+      const bool there = i < k;
+      x[j] = there ? a[i] : from_f32<T>(0.0f);
+      y[j] = there ? b[i] : from_f32<T>(0.0f);
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) s[j & 1] += (double)(to_f32(x[j]) * to_f32(y[j]));
+  }
+  double sum = s[0] + s[1];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return sum;
 }
-// whether z of element (m, n) is above 0, by one thread
+// Whether z of element (m, n), a lane's own, is above 0; whole warps come here.
 template <typename T>
-__device__ __noinline__ bool above_zero(const GemmDesc& d, long long m, int n) {
-  const double z = exact_part((const T*)d.a[0].p + m * d.a[0].row, (const T*)d.b[0].p + n * d.b[0].row, d.k[0], 0, 1);
-  return (d.bias[0] ? z + (double)to_f32(((const T*)d.bias[0])[n]) : z) > 0.0;
+__device__ __forceinline__ bool above_zero(const GemmDesc& d, long long m, int n, float z, bool there, int lane) {
+  bool above = z > 0.0f;
+  const bool unsure = there && fabsf(z) < kink_bound(d.norm_a[m], d.norm_b[n], d.k[0]);
+  for (uint32_t lanes = __ballot_sync(0xffffffffu, unsure); lanes; lanes &= lanes - 1) {
+    const int l = __ffs(lanes) - 1;
+    const long long lm = __shfl_sync(0xffffffffu, m, l);
+    const int ln = __shfl_sync(0xffffffffu, n, l);
+    double e = exact_sum((const T*)d.a[0].p + lm * d.a[0].row, (const T*)d.b[0].p + ln * d.b[0].row, d.k[0], lane);
+    if (d.bias[0]) e += (double)to_f32(((const T*)d.bias[0])[ln]);
+    if (lane == l) above = e > 0.0;
+  }
+  return above;
 }
 // z as it is kept for relu's backward pass, which looks at its sign: above 0 also in its type where it is, and not where it is not
 template <typename T>

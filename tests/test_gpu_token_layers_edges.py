@@ -1,5 +1,5 @@
 """The layers in front of the document head where they can go wrong: operands that lie in memory in unlike ways, infinities and
-values beyond the type, rows far from zero.
+values beyond the type, rows far from zero, relu near its kink.
 
 Bounds as in test_gpu_token_layers: every rounding counted at its most."""
 
@@ -154,3 +154,63 @@ def test_layer_norm_far_from_zero(width):
         # differences from the rounded mean are exact to a rounding; their mean and that of their squares are sums of `steps`
         off = steps * E * (abs(shift) * E * steps / var.sqrt() + hat.abs().mean(1, keepdim=True))
         near(layer_norm(x), hat, off + hat.abs() * (2 * steps + 8) * E + 4 * E, "y")
+
+
+# ----------------------------------------------------------------------------- relu near its kink
+def cancelling(m, h, n, dt):
+    """Rows and features whose products cancel to +-2^-20 in another order than they come in."""
+    a, b = rand(m, h, dt=dt), rand(n, h, dt=dt)
+    perm = torch.randperm(h, device="cuda")
+    tiny = torch.where(torch.rand(m, 1, device="cuda") < 0.5, -1.0, 1.0) * 2.0**-10
+    return torch.cat([a, a[:, perm], tiny.to(dt)], 1), torch.cat([b, -b[:, perm], torch.full((n, 1), 2.0**-10, device="cuda", dtype=dt)], 1)
+
+
+@pytest.mark.parametrize("dt", [BF16, FP16])
+@pytest.mark.parametrize("m, pad", [(3, 7), (3, 0), (40, 7), (700, 7), (700, 0), (5000, 7)])
+@pytest.mark.parametrize("h", [496, 2000])
+def test_relu_where_all_neighbours_are_near_its_kink(dt, m, pad, h):
+    from late_interaction_kernels_b200.token_layers import gated_feed_forward, linear
+
+    n = 200
+    x, w = cancelling(m, h, n, dt)
+    zero = lambda t: torch.cat([t, torch.zeros(t.shape[0], pad, device="cuda", dtype=dt)], 1)
+    x, w = zero(x), zero(w)
+    z = x.double() @ w.double().t()
+    assert float((z.abs() - 2.0**-20).abs().max()) < 2.0**-30
+    open_ = (z > 0).double()
+    for bias in (None, torch.zeros(n, device="cuda", dtype=dt)):
+        x1 = x.clone().requires_grad_()
+        (dx,) = torch.autograd.grad(linear(x1, w, bias, activation="relu"), [x1], torch.ones(m, n, device="cuda", dtype=dt))
+        near(dx, open_ @ w.double(), 2 * n * E * (open_ @ w.double().abs()), "dx")
+    g1 = w.clone().requires_grad_()
+    y = gated_feed_forward(x, g1, torch.zeros_like(w), torch.ones(8, n, device="cuda", dtype=dt), b_up=torch.ones(n, device="cuda", dtype=dt), activation="relu")
+    (dg,) = torch.autograd.grad(y, [g1], torch.ones_like(y))
+    near(dg, 8 * open_.t() @ x.double(), 2 * m * E * 8 * open_.t() @ x.double().abs(), "dw_gate")
+
+
+@pytest.mark.parametrize("dt", [BF16, FP16])
+@pytest.mark.parametrize("m", [3, 300, 9000])
+def test_relu_beside_features_that_are_off_zero_or_infinite(dt, m):
+    """One feature switched off by its bias, a dead one, one with an infinite weight and rows of padding: the others' gradients are as without."""
+    from late_interaction_kernels_b200.token_layers import linear
+
+    k, n = 128, 96
+    x, w, b = rand(m, k, dt=dt), rand(n, k, dt=dt, scale=k**-0.5), rand(n, dt=dt)
+    x[m // 2 :] = 0
+    dy = rand(m, n, dt=dt)
+    w[5], b[5] = 0, 0
+    b[3], b[40] = -60000, 60000
+    want = torch.where(z_of(x, w, b) > 0, dy.double(), 0)
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+    dx, dw, db = torch.autograd.grad(linear(*leaves, activation="relu"), leaves, dy)
+    near(dx, want @ w.double(), 2 * n * E * want.abs() @ w.double().abs(), "dx")
+    near(dw, want.t() @ x.double(), 2 * m * E * want.abs().t() @ x.double().abs(), "dw")
+    near(db, want.sum(0), 2 * m * E * want.abs().sum(0), "db")
+    leaves[1].data[60, 7] = float("inf")
+    rest = [i for i in range(n) if i != 60]
+    dw2 = torch.autograd.grad(linear(*leaves, activation="relu"), leaves, dy)[1]
+    assert torch.equal(dw2[rest], dw[rest])
+
+
+def z_of(x, w, b):
+    return x.double() @ w.double().t() + b.double()
