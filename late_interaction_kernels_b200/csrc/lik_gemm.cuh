@@ -310,9 +310,9 @@ struct GtPlan {
 // that spares a CTA `spare` of them; copy_bytes: of a matrix that is not read as it lies in memory, 0 otherwise.  cut_from[1] is for one of up to
 // four products, which share a launch if they are not cut: a step of 3500 x 768 through a gated block of 2048 took 154 us cut from 40 slabs on, 119
 // from 96 on; with the two products of a linear layer it is the other way round, 41 and 45 us.  A problem is planned as if it were alone, so its
-// result does not depend on which others are asked for.
-template <typename CgOf, typename CopyBytes>
-GtPlan gt_plan(const GemmDesc* d, int n, const int (&cut_from)[2], int share, int spare, CgOf&& cg_of, CopyBytes&& copy_bytes) {
+// result does not depend on which others are asked for.  slabs_of: slabs that one accumulator may go through, for the accuracy's sake.
+template <typename CgOf, typename CopyBytes, typename SlabsOf>
+GtPlan gt_plan(const GemmDesc* d, int n, const int (&cut_from)[2], int share, int spare, CgOf&& cg_of, CopyBytes&& copy_bytes, SlabsOf&& slabs_of) {
   GtPlan pl{};
   pl.n = n;
   size_t off = 0;
@@ -343,7 +343,12 @@ GtPlan gt_plan(const GemmDesc* d, int n, const int (&cut_from)[2], int share, in
     // a share of k for every slot, where the time that this saves is worth the pass that adds the shares up (2.5 us)
     long long ideal = ceil_div((long long)q.tiles * q.kb_total, sm_count() / cg);
     if (ideal < share) ideal = share;
-    const long long s = d[i].kind == GEMM_LINEAR && q.kb_total >= cut_from[d[i].several] && q.kb_total >= 2 * ideal && q.kb_total - ideal >= spare ? q.kb_total / ideal : 1;
+    long long s = d[i].kind == GEMM_LINEAR && q.kb_total >= cut_from[d[i].several] && q.kb_total >= 2 * ideal && q.kb_total - ideal >= spare ? q.kb_total / ideal : 1;
+    if (d[i].kind == GEMM_LINEAR) {
+      long long least = ceil_div(q.kb_total, slabs_of(d[i]));
+      if (least > (1 << 30) / q.tiles) least = (1 << 30) / q.tiles;  // (units are counted in 32 bits)
+      if (s < least) s = least;
+    }
     q.kb_per = (int)ceil_div(q.kb_total, s);
     pl.splits[i] = (int)ceil_div(q.kb_total, q.kb_per);
     pl.units[i] = q.tiles * pl.splits[i];

@@ -330,7 +330,8 @@ __global__ void __launch_bounds__(256) cut_kernel(const __grid_constant__ CutJob
 }
 
 GtPlan f32_plan(const GemmDesc* d, int n) {  // (a slab of k takes a CTA 1.5 to 1.9 us)
-  return gt_plan(d, n, {6, 12}, 2, 0, [](const GemmDesc&) { return 1; }, [](const Stored& o) { return align_up((size_t)o.rows * o.padded() * 2 * GF_PARTS, 256); });
+  return gt_plan(d, n, {6, 12}, 2, 0, [](const GemmDesc&) { return 1; }, [](const Stored& o) { return align_up((size_t)o.rows * o.padded() * 2 * GF_PARTS, 256); },
+                 [](const GemmDesc&) { return 1 << 30; });
 }
 template <int KIND>
 int run_f32(const GfMaps& maps, const GfParams& p, cudaStream_t st) {

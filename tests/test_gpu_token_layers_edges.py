@@ -1,5 +1,5 @@
 """The layers in front of the document head where they can go wrong: operands that lie in memory in unlike ways, infinities and
-values beyond the type, rows far from zero, relu near its kink.
+values beyond the type, rows far from zero, relu near its kink, long sums.
 
 Bounds as in test_gpu_token_layers: every rounding counted at its most."""
 
@@ -214,3 +214,21 @@ def test_relu_beside_features_that_are_off_zero_or_infinite(dt, m):
 
 def z_of(x, w, b):
     return x.double() @ w.double().t() + b.double()
+
+
+# ----------------------------------------------------------------------------- long sums
+@pytest.mark.parametrize("dt", [BF16, FP16])
+@pytest.mark.parametrize("n, k", [(1024, 1024), (4096, 1024), (128, 128)])
+def test_fp32_gradients_of_many_tokens(dt, n, k):
+    """Terms of one sign: an addition of 16 products cuts off up to four steps of what has been summed.  One accumulator goes over 8192 tokens at most:
+    512 additions, with half of the whole sum on average, so 1024 steps of 2^-23 of the result."""
+    from late_interaction_kernels_b200.token_layers import linear
+
+    m = 65536
+    x, dy = rand(m, k, dt=dt).abs() + 0.5, rand(m, n, dt=dt).abs() + 0.5
+    w = torch.zeros(n, k, device="cuda", dtype=FP32).requires_grad_()
+    (dw,) = torch.autograd.grad(linear(x, w), [w], dy)
+    want = torch.zeros(n, k, device="cuda", dtype=torch.float64)
+    for i in range(0, m, 8192):
+        want += dy[i : i + 8192].double().t() @ x[i : i + 8192].double()
+    assert float(((dw.double() - want).abs() / want).max()) < 1024 * 2.0**-23 + 16 * E
