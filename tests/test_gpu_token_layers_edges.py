@@ -217,6 +217,35 @@ def z_of(x, w, b):
 
 
 # ----------------------------------------------------------------------------- long sums
+LONG = [(20000, 40, 24), (30000, 96, 200), (30001, 95, 200), (66011, 72, 40), (65600, 264, 520), (140000, 16, 8), (70001, 8, 300)]
+
+
+@pytest.mark.parametrize("dt", [BF16, FP16, FP32])
+@pytest.mark.parametrize("m, k, n", LONG)
+def test_long_sums_of_whole_numbers_are_exact(dt, m, k, n):
+    """Sums over many tokens whose every partial sum is a whole number below 2^24: in any order and with any adder of 24 bits they are exact, and a
+    token, a slab or a share that is left out or taken twice shows."""
+    from late_interaction_kernels_b200.token_layers import gated_feed_forward, linear
+
+    ints = lambda *shape: torch.randint(-3, 4, shape, device="cuda").to(dt)
+    x, dy = ints(m, k), ints(m, n)
+    w, b = torch.zeros(n, k, device="cuda", dtype=FP32).requires_grad_(), torch.zeros(n, device="cuda", dtype=FP32).requires_grad_()
+    dw, db = torch.autograd.grad(linear(x, w, b), [w, b], dy)
+    assert dw.dtype == FP32 and torch.equal(dw.double(), dy.double().t() @ x.double()) and torch.equal(db.double(), dy.double().sum(0))
+    # a gated block whose gate is 1 everywhere and whose up projection picks a feature of x: its factors and gradients are whole numbers of a few bits
+    pick = torch.zeros(n, k, device="cuda", dtype=FP32)
+    pick[torch.arange(n), torch.arange(n) % k] = 1
+    pick.requires_grad_()
+    wg, wd = torch.zeros(n, k, device="cuda", dtype=FP32).requires_grad_(), torch.zeros(8, n, device="cuda", dtype=FP32)
+    wd[torch.arange(n) % 8, torch.arange(n)] = 1
+    wd.requires_grad_()
+    bg, d = torch.ones(n, device="cuda", dtype=FP32).requires_grad_(), ints(m, 8)
+    got = torch.autograd.grad(gated_feed_forward(x, wg, pick, wd, b_gate=bg, activation=None), [wg, pick, wd, bg], d)
+    X, u, dh = x.double(), x.double() @ pick.detach().double().t(), d.double() @ wd.detach().double()
+    for g, want in zip(got, ((dh * u).t() @ X, dh.t() @ X, d.double().t() @ u, (dh * u).sum(0))):
+        assert g.dtype == FP32 and torch.equal(g.double(), want)
+
+
 @pytest.mark.parametrize("dt", [BF16, FP16])
 @pytest.mark.parametrize("n, k", [(1024, 1024), (4096, 1024), (128, 128)])
 def test_fp32_gradients_of_many_tokens(dt, n, k):
