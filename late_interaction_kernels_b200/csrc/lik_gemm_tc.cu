@@ -476,9 +476,10 @@ __global__ void __launch_bounds__(256) repack_kernel(const __grid_constant__ Rep
 // tiles of 128 x 128.  A slab of k takes a CTA that is alone with its tile 0.2 us, so shares pay from 12 slabs spared on: 512 rows, 2048 x 768 (6 of 32
 // slabs each) 12.3 us whole, 9.0 cut; 1024 rows, 1024 x 1024 (7 of 16) 9.4 and 10.3.  (Four CTAs of a cluster that add their sums up in shared
 // memory, without the pass: 10.4 and 9.9; their start costs what the pass does.)
-// An addition of 16 products cuts off 1.6 steps (2^-23) of the accumulator on average, one-sided: 4e-4 of a sum of 65536 terms of one sign, 5e-5 of 8192.  So
-// one accumulator goes through so much of k that this is a tenth of what the result's rounding may be off, and through 8192 for fp32 results, which
-// have no rounding that would hide it; the shares' sums are added in fp32 with rounding.
+// An addition of 16 products cuts off some 1.6 steps (2^-23) of the accumulator, one-sided: of 65536 terms of one sign 4e-4 of their sum was missing, of 8192
+// it is 2e-5.  So fp32 results, which have no rounding that would hide it, are sums of shares of at most 8192 of k, added with rounding (1024 x 1024
+// of 65536 tokens: 1.9e-5, where a library's fp32 product is off by up to 1.7e-5); for 16-bit results one accumulator goes through so much of k that a
+// tenth or so of what their own rounding may be off comes of it.
 GtPlan tc_plan(const GemmDesc* d, int n) {
   auto cg = [](const GemmDesc& g) {
     const long long tiles = ceil_div(g.m, 256) * ceil_div(g.n, g.kind == GEMM_GATED ? 128 : 256), pairs = sm_count() / 2;
@@ -486,7 +487,7 @@ GtPlan tc_plan(const GemmDesc* d, int n) {
     return tiles >= pairs || (cuttable && tiles * ceil_div(g.k[0] + g.k[1], GT_BK) >= 16 * pairs) ? 2 : 1;
   };
   return gt_plan(d, n, {16, 96}, 4, 12, cg, [](const Stored& o) { return o.aligned() ? (size_t)0 : align_up((size_t)o.rows * o.padded() * 2, 256); },
-                 [](const GemmDesc& g) { return (g.out_dtype == LIK_BF16 ? 65536 : 8192) / GT_BK; });
+                 [](const GemmDesc& g) { return (g.out_dtype == LIK_F32 ? 8192 : (g.out_dtype == LIK_F16 ? 16384 : 65536)) / GT_BK; });
 }
 
 template <int CG, int KIND, bool RES, bool KINK, typename T, typename O>

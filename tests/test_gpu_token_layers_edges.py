@@ -6,7 +6,7 @@ Bounds as in test_gpu_token_layers: every rounding counted at its most."""
 import pytest
 import torch
 
-from test_gpu_token_layers import ACTS, BF16, E, FP16, FP32, floor, near, product, rand, unit
+from test_gpu_token_layers import ACTS, BF16, E, FP16, FP32, floor, linear_case, near, product, rand, unit
 
 pytestmark = pytest.mark.gpu
 
@@ -140,6 +140,17 @@ def test_layer_norm_of_constant_rows(dt, width):
     near(dx, 1e-5**-0.5 * (d - d.mean(1, keepdim=True)), 1e-5**-0.5 * (8 * steps * E * (d.abs() + s) + h * h * s + 2 * h * h * (d.abs() + s)), "dx")
 
 
+@pytest.mark.parametrize("dt", [BF16, FP32])
+@pytest.mark.parametrize("width", FAR_WIDTHS)
+def test_layer_norm_of_rows_beyond_the_squares_of_fp32(dt, width):
+    """Squares of differences beyond 3e38 leave no deviation to divide by but infinity: the row is zeros, not NaN."""
+    from late_interaction_kernels_b200.token_layers import layer_norm
+
+    x = torch.tensor([1e30, -3e33, 7e25, 1e20], device="cuda").to(dt)[:, None].expand(4, width).contiguous()
+    assert torch.isfinite(layer_norm(x)).all()
+    assert torch.equal(layer_norm(rand(5, width, dt=dt) * 1e30), torch.zeros(5, width, device="cuda", dtype=dt))
+
+
 @pytest.mark.parametrize("width", FAR_WIDTHS)
 def test_layer_norm_far_from_zero(width):
     """fp32 rows whose mean is ten thousand times their deviation: the result is as near to 64 bits as that of rows around zero."""
@@ -218,6 +229,7 @@ def z_of(x, w, b):
 
 # ----------------------------------------------------------------------------- long sums
 LONG = [(20000, 40, 24), (30000, 96, 200), (30001, 95, 200), (66011, 72, 40), (65600, 264, 520), (140000, 16, 8), (70001, 8, 300)]
+LONG_K = [(700, 33000, 260), (5200, 17000, 1100), (40, 66000, 72), (2600, 70000, 264)]
 
 
 @pytest.mark.parametrize("dt", [BF16, FP16, FP32])
@@ -244,6 +256,13 @@ def test_long_sums_of_whole_numbers_are_exact(dt, m, k, n):
     X, u, dh = x.double(), x.double() @ pick.detach().double().t(), d.double() @ wd.detach().double()
     for g, want in zip(got, ((dh * u).t() @ X, dh.t() @ X, d.double().t() @ u, (dh * u).sum(0))):
         assert g.dtype == FP32 and torch.equal(g.double(), want)
+
+
+@pytest.mark.parametrize("dt", [BF16, FP16, FP32])
+@pytest.mark.parametrize("i", range(len(LONG_K)))
+def test_linear_of_many_features(dt, i):
+    """Products with a bias, an activation and a residual whose sums are cut for their length alone."""
+    linear_case(*LONG_K[i], dt, ACTS[1 + i], True, True)
 
 
 @pytest.mark.parametrize("dt", [BF16, FP16])
