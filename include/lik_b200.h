@@ -468,7 +468,7 @@ typedef struct lik_gated_args {
   int32_t param_dtype;
   void* y;               /* forward: [rows, out] */
   void* gate_factor;     /* u act'(g), act(g) and h for the backward, [rows, hidden] with kept_stride (a multiple of 16 bytes): */
-  void* up_factor;       /* written by the forward unless NULL (all three or none), read by the backward */
+  void* up_factor;       /* written by the forward unless NULL (all three or none), read by the backward unless db_down alone is asked for */
   void* h;
   int64_t kept_stride;
   const void* dy;        /* backward: [rows, out] */

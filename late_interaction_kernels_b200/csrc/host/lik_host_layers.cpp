@@ -357,7 +357,7 @@ Tensor linear(const Tensor& x_, const Tensor& w, const OptTensor& bias_, const s
     a.residual_stride = r.defined() ? row_stride(r) : 0;
     y = at::empty({x.size(0), out}, x.options());
     a.y = ptr(y);
-    if (grad && act != LIK_ACT_NONE) {
+    if (act != LIK_ACT_NONE && wants_grad({&x, &w, &b})) {  // (a residual's gradient is dy)
       z = kept_rows(1, x.size(0), out, x);
       a.z = ptr(z);
       a.z_stride = z.size(2);
@@ -443,10 +443,12 @@ struct GatedFeedForwardBackward : public torch::autograd::Node {
       lik_gated_args a = gated_args(X, WG, WU, WD, act);
       a.param_dtype = grad_type;
       const auto popt = X.options().dtype(scalar_of(grad_type));
-      a.gate_factor = matrix_of(K, 0);
-      a.up_factor = matrix_of(K, 1);
-      a.h = matrix_of(K, 2);
-      a.kept_stride = K.size(2);
+      if (K.defined()) {
+        a.gate_factor = matrix_of(K, 0);
+        a.up_factor = matrix_of(K, 1);
+        a.h = matrix_of(K, 2);
+        a.kept_stride = K.size(2);
+      }
       a.dy = ptr(dy);
       a.dy_stride = row_stride(dy);
       if (task_should_compute_output(0)) out[0] = at::empty(X.sizes(), X.options());
@@ -509,7 +511,7 @@ Tensor gated_feed_forward(const Tensor& x_, const Tensor& wg, const Tensor& wu, 
     a.residual_stride = r.defined() ? row_stride(r) : 0;
     y = at::empty({x.size(0), out}, x.options());
     a.y = ptr(y);
-    if (grad) {
+    if (wants_grad({&x, &wg, &wu, &wd, &bg, &bu})) {  // (b_down's and a residual's gradients are made of dy alone)
       kept = kept_rows(3, x.size(0), f, x);
       a.gate_factor = matrix_of(kept, 0);
       a.up_factor = matrix_of(kept, 1);

@@ -578,8 +578,9 @@ extern "C" int lik_gated_bwd(const lik_gated_args* args, lik_stream_t stream) {
     return LIK_OK;
   }
   LIK_REQUIRE(a.x && a.w_gate && a.w_up && a.w_down && a.dy && a.dy_stride >= a.out, "x, the weights and dy must not be NULL, dy_stride at least out");
-  LIK_REQUIRE(a.gate_factor && a.up_factor && a.h && a.kept_stride >= a.hidden && a.kept_stride * dtype_size(a.dtype) % 16 == 0 &&
-                  (((uintptr_t)a.gate_factor | (uintptr_t)a.up_factor | (uintptr_t)a.h) & 15) == 0, "gate_factor, up_factor and h must be there, with 16-byte rows");
+  const bool kept = a.dx || a.dw_gate || a.dw_up || a.dw_down || a.db_gate || a.db_up;  // (db_down is made of dy alone)
+  LIK_REQUIRE(!kept || (a.gate_factor && a.up_factor && a.h && a.kept_stride >= a.hidden && a.kept_stride * dtype_size(a.dtype) % 16 == 0 &&
+                        (((uintptr_t)a.gate_factor | (uintptr_t)a.up_factor | (uintptr_t)a.h) & 15) == 0), "gate_factor, up_factor and h must be there, with 16-byte rows");
   const GatedBwd l = gated_bwd_layout(a, a.workspace);
   if (a.workspace_bytes < l.total || (l.total && !a.workspace)) return too_small("lik_gated_bwd");
   if (l.dg)

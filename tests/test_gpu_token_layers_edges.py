@@ -1,5 +1,5 @@
 """The layers in front of the document head where they can go wrong: operands that lie in memory in unlike ways, infinities and
-values beyond the type, rows far from zero, relu near its kink, long sums.
+values beyond the type, rows far from zero, relu near its kink, long sums, what is kept.
 
 Bounds as in test_gpu_token_layers: every rounding counted at its most."""
 
@@ -280,3 +280,26 @@ def test_fp32_gradients_of_many_tokens(dt, n, k):
     for i in range(0, m, 8192):
         want += dy[i : i + 8192].double().t() @ x[i : i + 8192].double()
     assert float(((dw.double() - want).abs() / want).max()) < 1024 * 2.0**-23 + 16 * E
+
+
+# ----------------------------------------------------------------------------- what is kept
+def test_nothing_is_kept_for_gradients_that_are_made_of_dy_alone():
+    """With everything frozen but a residual, or the bias behind a gated block's last product, the call holds its result and no more."""
+    from late_interaction_kernels_b200.token_layers import gated_feed_forward, linear
+
+    m, k, f = 4096, 256, 1024
+    x, w, wg, wd, r, d = rand(m, k, dt=BF16), rand(k, k, dt=BF16), rand(f, k, dt=BF16), rand(k, f, dt=BF16), rand(m, k, dt=BF16), rand(m, k, dt=BF16)
+    b = rand(k, dt=BF16)
+    for fn in (lambda r, b: linear(x, w, activation="gelu", residual=r), lambda r, b: gated_feed_forward(x, wg, wg, wd, b_down=b, residual=r)):
+        leaves = [t.clone().requires_grad_() for t in (r, b)]
+        fn(*leaves)
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        y = fn(*leaves)
+        torch.cuda.synchronize()
+        assert torch.cuda.memory_allocated() - before <= y.numel() * y.element_size() + 4096
+        dr, db = torch.autograd.grad(y, leaves, d, allow_unused=True)
+        assert torch.equal(dr, d)
+        if db is not None:
+            near(db, d.double().sum(0), 2 * m * E * d.double().abs().sum(0), "db_down")
+        assert torch.equal(y, fn(*(t.detach() for t in leaves)))
