@@ -5,7 +5,7 @@
 // instead of rounding it, a shift of some 0.3 last places towards zero per 16 products; so a0 b0 and the five small products have
 // an accumulator each - cutting off the small one's sums is 2^-8 as bad - and after 128 k both are added to sums in registers, which are
 // rounded.  What remains is below 2e-7 of a sum of 768 Gaussian products, less than fp32 multiply-adds in a row leave.
-// An operand that is infinite gives NaN or infinities, as inf * 0 is among its products of parts.
+// Infinities and NaN come out as fp32 products would have them (cut3).
 //
 // Roles as in the 16-bit kernel: a persistent CTA per SM, tiles of 128 x 128; a stage is 64 k of three parts of either operand (96 KB,
 // 24 MMAs), and there are two.  Bound by shared memory, which the MMAs read at 128 bytes per cycle while TMA writes half as much.
@@ -275,18 +275,23 @@ __global__ void __launch_bounds__(GF_THREADS, 1) gemm_f32_kernel(const __grid_co
   if (warp == GF_ISSUER) tmem_dealloc(tmem, 512);
 }
 
-// x = p0 + p1 + p2 in bf16, each the nearest to what the ones before leave.  A value that bf16 would round to infinity is cut off instead,
-// and one that is not finite has no further parts.
+// x = p0 + p1 + p2 in bf16, each the nearest to what the ones before leave.  A value that bf16 would round to infinity is cut off instead.  Of an infinite
+// one the last part is infinite, which meets p0 of the other operand alone - in the first place it would meet that one's small parts, of any
+// sign, and 0 - and p0 is its sign, for where that one is infinite too.  A NaN has no further parts.
 __device__ __forceinline__ void cut3(float x, uint32_t (&p)[3]) {
-  __nv_bfloat16 h = __float2bfloat16_rn(x);
-  if (fabsf(x) > 3.3895e38f) h = __float2bfloat16_rz(x);
-  const bool finite = fabsf(x) <= 3.402823466e38f;
-  p[0] = __bfloat16_as_ushort(h);
-  float r = finite ? x - __bfloat162float(h) : 0.0f;
-  h = __float2bfloat16_rn(r);
-  p[1] = __bfloat16_as_ushort(h);
-  r -= __bfloat162float(h);
-  p[2] = __bfloat16_as_ushort(__float2bfloat16_rn(r));
+  if (fabsf(x) <= 3.402823466e38f) {
+    __nv_bfloat16 h = fabsf(x) > 3.3895e38f ? __float2bfloat16_rz(x) : __float2bfloat16_rn(x);
+    p[0] = __bfloat16_as_ushort(h);
+    float r = x - __bfloat162float(h);
+    h = __float2bfloat16_rn(r);
+    p[1] = __bfloat16_as_ushort(h);
+    p[2] = __bfloat16_as_ushort(__float2bfloat16_rn(r - __bfloat162float(h)));
+  } else {
+    const uint32_t sign = __float_as_uint(x) >> 16 & 0x8000u;
+    p[0] = x != x ? 0x7FC0u : sign | 0x3F80u;
+    p[1] = 0u;
+    p[2] = x != x ? 0u : sign | 0x7F80u;
+  }
 }
 // matrices in their three parts, rows of whole 16-byte pieces (zeros behind the columns).  Bound by memory: 4 bytes in and 6 out per value.
 struct CutJobs {

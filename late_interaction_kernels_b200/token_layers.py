@@ -14,8 +14,8 @@ weights beside bf16 activations) are brought to ``x``'s type for the products - 
 gradients of their own type, rounded from fp32.  Gradients are deterministic.  Backward passes keep what they need: the input, in ``x``'s
 type the values in front of an activation or, of a gated block, the factors of its gradients, and a row's mean and inverse deviation in fp32.  Everything runs
 on the current stream and may be captured into a CUDA graph.  With 16-bit operands ``relu``'s
-gradient goes by the sign of the exact sum where that sum is next to nothing beside the lengths of the rows that it is a product of.  An infinity among fp32
-operands of a product gives infinities or NaN in its row.  (No counterpart in the reference, which starts at the hidden states.)
+gradient goes by the sign of the exact sum where that sum is next to nothing beside the lengths of the rows that it is a product of.
+(No counterpart in the reference, which starts at the hidden states.)
 """
 
 from __future__ import annotations

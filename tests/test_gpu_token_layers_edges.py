@@ -69,6 +69,32 @@ def test_activations_of_infinity(dt, m, k, n):
             assert not torch.isfinite(h).any() and not torch.isfinite(h[:, 0]).any()
 
 
+def same_kind(got, want):
+    """NaN, infinities of either sign and finite numbers in the same places."""
+    want = want.to(torch.float64)
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(torch.isposinf(got), torch.isposinf(want)) and torch.equal(torch.isneginf(got), torch.isneginf(want))
+
+
+@pytest.mark.parametrize("dt", [BF16, FP16, FP32])
+@pytest.mark.parametrize("m, k, n", KERNELS)
+def test_infinite_operands(dt, m, k, n):
+    """An infinity gives infinities of its factors' signs, NaN where it meets 0 or another of the other sign, in every kernel and direction."""
+    from late_interaction_kernels_b200.token_layers import linear
+
+    inf = float("inf")
+    x, w, dy = rand(m, k, dt=dt), rand(n, k, dt=dt), rand(m, n, dt=dt)
+    x[0, 3], x[1, 5], x[1, 7], x[2, k - 1] = inf, -inf, inf, inf
+    w[4, 3], w[5, 9], w[6, k - 1], w[7, 3] = -inf, inf, inf, 0
+    dy[2, 8], dy[m - 1, 0] = -inf, inf
+    x, w = x.requires_grad_(), w.requires_grad_()
+    y = linear(x, w)
+    dx, dw = torch.autograd.grad(y, [x, w], dy)
+    X, W, D = x.detach().double(), w.detach().double(), dy.double()
+    for got, want in ((y.detach(), X @ W.t()), (dx, D @ W), (dw, D.t() @ X)):
+        same_kind(got, want)
+
+
 @pytest.mark.parametrize("dt", [BF16, FP32])
 @pytest.mark.parametrize("m", [3, 300, 9000])
 def test_slopes_of_large_values(dt, m):
