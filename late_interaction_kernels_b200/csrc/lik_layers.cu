@@ -175,19 +175,17 @@ __global__ void __launch_bounds__(256) kink_norms_kernel(const __grid_constant__
       s = fmaf(v, v, s);
       largest = fmaxf(largest, fabsf(v));
     };
-    long long done = 0;
-    if (((uintptr_t)x & 15) == 0) {
-      done = p.k & ~7ll;
+    // (up to the first 16-byte boundary element by element, and behind the last)
+    const long long head = min((long long)((16 - ((uintptr_t)x & 15)) % 16 / sizeof(T)), p.k), end = head + ((p.k - head) & ~7ll);
+    if (lane < head) take(to_f32(x[lane]));
+    if (end + lane < p.k) take(to_f32(x[end + lane]));
 #pragma unroll 4
-      for (long long i = lane * 8; i < done; i += 256) {
-        float v[8];
-        load_vec<T, 8>(x + i, v);
+    for (long long i = head + lane * 8; i < end; i += 256) {
+      float v[8];
+      load_vec<T, 8>(x + i, v);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) take(v[j]);
-      }
+      for (int j = 0; j < 8; ++j) take(v[j]);
     }
-#pragma unroll 8
-    for (long long i = done + lane; i < p.k; i += 32) take(to_f32(x[i]));
     s = warp_sum(s);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
