@@ -1,5 +1,5 @@
-"""The layers in front of the document head where they can go wrong: operands that lie in memory in unlike ways, infinities and
-values beyond the type, rows far from zero, relu near its kink, long sums, what is kept.
+"""The layers in front of the document head where they can go wrong: operands that lie in memory in unlike ways, infinities and values beyond the
+type, rows far from zero, relu near its kink, long sums, what is kept, calls side by side.
 
 Bounds as in test_gpu_token_layers: every rounding counted at its most."""
 
@@ -329,3 +329,42 @@ def test_nothing_is_kept_for_gradients_that_are_made_of_dy_alone():
         if db is not None:
             near(db, d.double().sum(0), 2 * m * E * d.double().abs().sum(0), "db_down")
         assert torch.equal(y, fn(*(t.detach() for t in leaves)))
+
+
+# ----------------------------------------------------------------------------- captured, and beside another stream
+@pytest.mark.parametrize("wdt", [BF16, FP32])
+def test_relu_steps_in_two_graphs_and_on_two_streams(wdt):
+    """The lengths for relu's kink and the shares of long sums are workspaces of a call's own."""
+    from late_interaction_kernels_b200 import check_device_status
+    from late_interaction_kernels_b200.token_layers import gated_feed_forward, linear
+
+    k = 192
+    data = [(rand(m, k, dt=BF16).requires_grad_(), rand(m, k, dt=BF16)) for m in (20000, 700)]
+    p = [rand(*s, dt=wdt, scale=k**-0.5).requires_grad_() for s in ((k, k), (2 * k, k), (2 * k, k), (k, 2 * k))]
+
+    def step(x, d):
+        y = gated_feed_forward(linear(x, p[0], activation="relu", residual=x), *p[1:], activation="relu")
+        return [y.detach(), *torch.autograd.grad(y, [x, *p], d)]
+
+    want = [step(*d) for d in data]
+    graphs = []
+    for d in data:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step(*d)
+        graphs.append((g, out))
+    streams = [torch.cuda.Stream() for _ in data]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                graphs[i][0].replay()
+                got[i].append([t.clone() for t in graphs[i][1]])
+                got[1 - i].append(step(*data[1 - i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for g in got[i]:
+            for a, b in zip(g, want[i]):
+                assert torch.equal(a, b)
+    check_device_status()

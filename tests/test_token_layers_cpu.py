@@ -89,3 +89,32 @@ def test_workspace_queries_need_no_gpu(layers):
     assert linear(5000, _lib.LIK_BF16, odd=1)[0] >= 5000 * 768 * 2 > linear(5000, _lib.LIK_BF16)[0]
     a = _lib.NormArgs(dtype=2, param_dtype=2, x_stride=768, rows=10**9, width=768, dweight=4096, eps=1e-5)
     assert 0 < lib.lik_layer_norm_bwd_workspace(C.byref(a)) < 16 << 20
+
+
+def test_a_kept_side_of_relu_asks_for_workspace_and_says_so(layers):
+    """relu's forward pass takes its rows' lengths first where a backward pass follows: a call without the room for them is refused before any launch."""
+    from late_interaction_kernels_b200 import _lib
+
+    lib = _lib.load()
+    for rows in (3, 5000):
+        a = _lib.LinearArgs(x=4096, w=4096, y=4096, x_stride=768, w_stride=768, z_stride=512, rows=rows, out=512, dtype=_lib.LIK_BF16, param_dtype=_lib.LIK_BF16, activation=1)
+        setattr(a, "in", 768)
+        without = lib.lik_linear_fwd_workspace(C.byref(a))
+        a.z = 4096
+        assert lib.lik_linear_fwd_workspace(C.byref(a)) >= without + 4 * (rows + 512)
+        a.workspace_bytes = without
+        assert lib.lik_linear_fwd(C.byref(a), None) != 0 and b"workspace" in lib.lik_last_error()
+        a.activation = 3
+        assert lib.lik_linear_fwd_workspace(C.byref(a)) == without
+
+
+def test_only_what_is_made_of_dy_needs_nothing_kept(layers):
+    from late_interaction_kernels_b200 import _lib
+
+    lib = _lib.load()
+    a = _lib.GatedArgs(x=4096, w_gate=4096, w_up=8192, w_down=16384, dy=4096, db_down=4096, x_stride=64, w_gate_stride=64, w_up_stride=64, w_down_stride=128, dy_stride=64,
+                       rows=300, hidden=128, out=64, dtype=_lib.LIK_BF16, param_dtype=_lib.LIK_BF16, activation=2)
+    setattr(a, "in", 64)
+    assert lib.lik_gated_bwd(C.byref(a), None) != 0 and b"workspace" in lib.lik_last_error()  # (past the check of what is kept)
+    a.dw_down = 4096
+    assert lib.lik_gated_bwd(C.byref(a), None) == -1 and b"must be there" in lib.lik_last_error()
