@@ -80,7 +80,8 @@ Tensor rows_of(const Tensor& t) {
   return (r.size(1) > 1 && r.stride(1) != 1) || (r.size(0) > 1 && r.stride(0) < r.size(1)) ? r.contiguous() : r;
 }
 int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? std::max(t.stride(0), t.size(1)) : t.size(1); }
-// as the kernels read it: in the call's type, unit stride inside rows that do not overlap
+// as the kernels read it: in the call's type (fp32 weights have to be, as the tensor core's operands; biases and residuals are with them, so that a call
+// has one type and one epilogue: half a step of a term that is added to a sum which is rounded to the same type), unit stride inside rows that do not overlap
 Tensor as_rows(const Tensor& t, at::ScalarType dt) {
   if (!t.defined()) return t;
   Tensor r = t.scalar_type() == dt ? t : t.to(dt);

@@ -9,9 +9,9 @@
 //                  descriptors say which (K-major or MN-major, 128-byte swizzle).  Rows and k behind the ends arrive as zeros.
 //   issuer warp    (of the pair's first CTA) four MMAs of 16 k per slab, one elected lane issuing; two accumulators in tensor memory, so
 //                  that the next unit's product runs while this unit's accumulator is read.
-//   8 epilogue warps  32 rows x half of the columns each, 32 columns at a time: tensor memory -> registers, bias, activation,
-//                  residual in fp32, one rounding, a swizzled slot in shared memory, a TMA store (which leaves out what lies behind the
-//                  matrix).  Rows that TMA cannot address (not multiples of 16 bytes) are written from the slot by plain stores.
+//   16 epilogue warps (8 where one needs more registers)  32 rows x a quarter (a half) of the columns each, 32 columns at a time: tensor memory ->
+//                  registers, bias, activation, residual in fp32, one rounding, a swizzled slot in shared memory, and plain stores from there,
+//                  neighbouring lanes on neighbouring pieces of a row (element by element where rows are not whole 16-byte pieces).
 // The gated block's two projections are one unit: half of its columns are the gate's, half are up's.
 // Products with few tiles and a long k are cut along k; the shares' fp32 sums go to the workspace and are added in their order.
 #include "lik_gemm.cuh"
@@ -246,7 +246,7 @@ __global__ void __launch_bounds__(GtWarps<KIND, !std::is_same<T, O>::value>::THR
       const uint32_t hi = (uint32_t)(smem_desc_sw128(0) >> 32);
       for (int u = first; u < p.units && ok; u += step, ++it) {
         const GtUnit t = gt_unit<MULTI>(p.q, p.n_prob, u);
-      const GtProblem& q = p.q[t.q];
+        const GtProblem& q = p.q[t.q];
         const uint32_t a_lbo = (q.a_mn ? GT_BOX_BYTES >> 4 : 1) << 16, b_lbo = (q.b_mn ? GT_BOX_BYTES >> 4 : 1) << 16;
         const uint32_t a_step = q.a_mn ? 128 : 2, b_step = q.b_mn ? 128 : 2;
         const uint32_t idesc = (1u << 4) | ((p.bf16 ? 1u : 0u) << 7) | ((p.bf16 ? 1u : 0u) << 10) | ((q.a_mn ? 1u : 0u) << 15) | ((q.b_mn ? 1u : 0u) << 16) |
@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(GtWarps<KIND, !std::is_same<T, O>::value>::THR
             __syncwarp();
             if (lane == 0) CG == 2 ? arrive_remote(release) : mbar_arrive(release);
           }
-          if constexpr (KIND == GEMM_GATED_BWD) {
+          if constexpr (KIND == GEMM_GATED_BWD) {  // (rounded to T: they are the operands of the next products, which take 16 bits)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               float f[16];
@@ -363,6 +363,8 @@ __global__ void __launch_bounds__(GtWarps<KIND, !std::is_same<T, O>::value>::THR
               if (p.bias[1]) bias[1].add_to(w);
             }
             if constexpr (!MULTI) {
+              // what the backward pass reads is rounded to T, as what autograd keeps between two 16-bit layers is: z, or both factors and h (a gradient
+              // is off by its own rounding and one of these, of a gated block two; fp32 would be twice the bytes of what is kept, written and read again)
               if constexpr (KINK) {
                 const uint32_t above = above_kink<T>(p, row0, col + 16 * h, lane, v);
                 float f[16];

@@ -31,7 +31,7 @@ __global__ void __launch_bounds__(256) sum_parts_kernel(const float* __restrict_
 }
 
 // ---------------------------------------------------------------------------------------------
-// dz = dy * act'(z), and the sums of dz's columns; or the sums of up to SUM_OUTS matrices' columns.  Memory-bound: each element read once, dz
+// dz = dy * act'(z), rounded to T as the operand of two products, and the sums of its columns before that rounding; or the sums of up to SUM_OUTS matrices' columns.  Memory-bound: each element read once, dz
 // written once.  A block takes 32 vectors of columns (a lane's V columns) of a matrix and a share of the rows, eight at a time; with one
 // share the sums are done, else sum_parts_kernel adds them up.
 // ---------------------------------------------------------------------------------------------
@@ -590,6 +590,8 @@ extern "C" int lik_gated_bwd(const lik_gated_args* args, lik_stream_t stream) {
     p.job[p.n_jobs] = {g, nullptr, stride, 0, n, 0, nullptr, 0, padded};
     p.outs.out[p.n_jobs++] = out;
   };
+  // (of dg and du as they were rounded for the products: before that they are in an epilogue that has each column in pieces, and over many rows what
+  // the roundings add up to is small beside one rounding of the sum)
   sum(l.dg, l.stride, a.hidden, a.db_gate, true);
   sum(l.du, l.stride, a.hidden, a.db_up, true);
   sum(a.dy, a.dy_stride, a.out, a.db_down, false);

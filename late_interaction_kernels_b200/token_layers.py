@@ -10,9 +10,10 @@ trained without leaving the package::
 
 All three take tensors of any number of leading dimensions, with any strides, and compute in ``x``'s type: float32, float16 or
 bfloat16; sums, statistics and activations are fp32 and results are rounded once.  Parameters of another type (fp32 master
-weights beside bf16 activations) are brought to ``x``'s type for the products - a layer norm reads fp32 weights as they are - and get
-gradients of their own type, rounded from fp32.  Gradients are deterministic.  Backward passes keep what they need: the input, in ``x``'s
-type the values in front of an activation or, of a gated block, the factors of its gradients, and a row's mean and inverse deviation in fp32.  Everything runs
+weights beside bf16 activations, and biases with them) and a residual of another type are brought to ``x``'s - a layer norm reads fp32 weights as they
+are - and parameters get gradients of their own type, rounded from fp32 sums.  Gradients are deterministic.  Backward passes keep what they need: the input, in ``x``'s
+type the values in front of an activation or, of a gated block, the factors of its gradients, and a row's mean and inverse deviation in fp32 (so the
+backward pass of rows far from zero sees them off by a step of their mean; the forward does not).  Everything runs
 on the current stream and may be captured into a CUDA graph.  With 16-bit operands ``relu``'s
 gradient goes by the sign of the exact sum where that sum is next to nothing beside the lengths of the rows that it is a product of.
 (No counterpart in the reference, which starts at the hidden states.)
