@@ -411,7 +411,8 @@ struct GemmDesc {
 // pass over the operands (kink_norms): nothing at hand says as much about a sum that came out small.  (The largest of z's neighbours, asked before, is
 // small too where a whole row cancels, and beside a feature that is switched off or dead it made every z look small: 65536 x 768 x 768 went from 105
 // us to 4 100 with one feature at -1e9 and to 5 400 with a tenth of the features dead; a zero row has length 0 and z of it is sure.)
-// A z that is 0 because the operands have no nonzero place in common is taken again like any other.
+// What remains is data whose sums are 0 for their own sake, which are taken again like any other: half of x 0 costs nothing, but where a twentieth of x and a
+// tenth of the weights are not 0 (2 % of z are 0) that forward takes 690 us, and 9.9 ms with a hundredth of x (46 %).
 __device__ __forceinline__ float kink_bound(float norm_a, float norm_b, long long k) { return norm_a * (2.384185791015625e-7f * (float)(k / 16 + 2)) * norm_b; }
 // sum over k of a b by a warp, in all lanes; products of 16-bit values are exact in fp32.  (Not inline: it is rarely called, and its loads, all
 // of 1024 k at once, would take the registers of the epilogue around it.)
